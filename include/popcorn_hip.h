@@ -555,6 +555,83 @@ popcorn_status_t popcorn_kernel_embedding_gather_quantized(const popcorn_tensor_
                                                            const popcorn_affine_quantized_tensor_t *table,
                                                            const popcorn_tensor_t *out, popcorn_kernel_t *kernel);
 
+/* ---- a batch of requests over a paged cache ------------------------------
+ * No counterpart in the reference, which serves one sequence over contiguous
+ * caches (KVCacheWrite.swift, FlashAttention.swift) and picks tokens with
+ * Argmax. A cache is [pages, Nkv, page_size, Hd]; slot s is row s % page_size
+ * of page s / page_size. Row r of page_tables (i32 [R, columns]) names the
+ * pages that hold request r's keys, page_size keys each, in order. All lengths
+ * are read on the GPU, so a step captured into a graph is replayed with the
+ * lengths that its tensors hold then. */
+
+/* The tables of one step. past_lens[r] keys of request r are in the cache
+ * already, new_lens[r] tokens come (i32 [R]; a negative length counts as 0).
+ * The tokens of all requests are numbered in a row, request by request:
+ *   query_starts i32 [R + 1]: each request's first token, then their number (at most T);
+ *   key_lens i32 [R]: past + new;
+ *   positions, slots i32 [T]: each token's position in its request and its
+ *     slot; 0 and -1 behind the last token;
+ *   page_tables: the entries of pages that the new tokens begin are written,
+ *     with pages taken from free_pages (i32 [F]) from the front, in request
+ *     order; entries of pages that hold past keys are read; others stay;
+ *   counts i32 [2]: tokens and free pages that the step needs.
+ * T is positions' length. Where the free pages or the table's columns run out
+ * the entry becomes -1 and the tokens' slots -1; tokens past T are left out.
+ * Both show in counts. The outputs must not overlap the inputs. */
+popcorn_status_t popcorn_kernel_page_tables(const popcorn_tensor_t *past_lens, const popcorn_tensor_t *new_lens,
+                                            const popcorn_tensor_t *free_pages, const popcorn_tensor_t *page_tables,
+                                            int64_t page_size, const popcorn_tensor_t *query_starts,
+                                            const popcorn_tensor_t *key_lens, const popcorn_tensor_t *positions,
+                                            const popcorn_tensor_t *slots, const popcorn_tensor_t *counts,
+                                            popcorn_kernel_t *kernel);
+
+/* The new tokens' rows k, v [T, Nkv, Hd] into their slots (i32 [T]) of k_cache
+ * and v_cache [pages, Nkv, page_size, Hd]; a slot outside the cache (-1) is
+ * skipped. (row, cache) dtypes as for KVCacheWrite: (f32, f32), (f16, f16),
+ * (bf16, bf16) or (f32, bf16). Of two tokens with one slot either one's
+ * values may be left, element by element. */
+popcorn_status_t popcorn_kernel_paged_kv_cache_write(const popcorn_tensor_t *k, const popcorn_tensor_t *v,
+                                                     const popcorn_tensor_t *slots, const popcorn_tensor_t *k_cache,
+                                                     const popcorn_tensor_t *v_cache, popcorn_kernel_t *kernel);
+
+/* Attention of every request's new tokens over its pages: q and out [T, Nq, Hd]
+ * hold the tokens in a row, request r's at rows query_starts[r] ..
+ * query_starts[r + 1] - 1 (i32 [R + 1], ascending), the last of its key_lens[r]
+ * (i32 [R]) keys. mask as for FlashAttention; under a sliding window the first
+ * `sinks` keys stay visible too (to rows at or behind them). Keys that a row
+ * does not see, and rows of the pages behind the last key, may hold anything. A key whose
+ * table entry names no page of the cache is left out. A row that sees no key
+ * is 0; rows outside the requests' ranges are left as they were.
+ * q, the caches and out share one dtype (f32, f16, bf16); page_size is a
+ * multiple of 16, Hd at most 512. max_query_len (0: unknown) is the longest
+ * request's number of new tokens; the kernels are chosen for it, the result
+ * does not depend on it. */
+popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
+                                                const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
+                                                const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens,
+                                                const popcorn_tensor_t *out, float scale, popcorn_attention_mask_t mask,
+                                                int64_t sinks, int64_t max_query_len, popcorn_kernel_t *kernel);
+
+/* One token (i32 [rows]) of each row of logits [rows, vocab] (f32, f16, bf16),
+ * drawn with the row's uniform random number (f32 [rows], in [0, 1)). Tokens
+ * rank by logit, ties by index. Of the first top_k[row] of them (i32) are kept
+ * those before which less than top_p[row] (f32) of their weight lies (the first always), and of
+ * these the ones of at least min_p[row] (f32) times the first's weight; the
+ * token is drawn among them by weight, in index order.
+ * A token's weight is the whole number rint(2^40 exp((logit - highest) /
+ * temperature[row])), the sums are exact, and the token is the first kept index
+ * whose running weight passes floor(uniform x weight kept), the uniform and top_p taken to 31 bits:
+ * the result depends on no order of summation, and two calls agree. Each
+ * option may be NULL (off), as are top_k <= 0, top_p >= 1 and min_p <= 0; NULL
+ * is temperature 1. A temperature of 0 (or less, or NaN) takes the highest
+ * logit, the lowest index of several. A NaN logit is never drawn, nor is
+ * -infinity; a row without any other gives -1. Infinite logits share the
+ * draw among them. */
+popcorn_status_t popcorn_kernel_sample(const popcorn_tensor_t *logits, const popcorn_tensor_t *uniforms,
+                                       const popcorn_tensor_t *temperature, const popcorn_tensor_t *top_k,
+                                       const popcorn_tensor_t *top_p, const popcorn_tensor_t *min_p,
+                                       const popcorn_tensor_t *tokens, popcorn_kernel_t *kernel);
+
 /* A DispatchKernel built by the caller (Kernel.swift:54-70): function name,
  * bound tensors with their access (1 read, 2 write, 3 both), constants blocks,
  * and the launch geometry in blocks/threads. */

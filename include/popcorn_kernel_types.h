@@ -410,6 +410,59 @@ typedef struct {
     uint32_t cols;
 } Transpose2DConstants;
 
+/* ---- a batch of requests over a paged cache (no counterpart in the reference,
+ * whose caches are one contiguous block per sequence) ----
+ * A cache is [pages, Nkv, pageSize, Hd]; slot s is row s % pageSize of page
+ * s / pageSize. Row r of the page tables [R, columns] names the pages of
+ * request r's keys in order. */
+
+/* page_tables. T: tokens that positions and slots hold; F: free pages. */
+typedef struct {
+    uint32_t R;
+    uint32_t columns;
+    uint32_t F;
+    uint32_t T;
+    uint32_t pageSize;
+} PageTablesConstants;
+
+/* paged_kv_write_*: rows [T, Nkv, Hd] of K and V into the slots. */
+typedef struct {
+    uint32_t T;
+    uint32_t Nkv;
+    uint32_t Hd;
+    uint32_t pageSize;
+    uint32_t pages;
+} PagedKVWriteConstants;
+
+/* paged_attention_*: q and out [T, Nq, Hd]; request r's new tokens are rows
+ * queryStarts[r] .. queryStarts[r + 1] - 1, the last of its keyLens[r] keys.
+ * maskKind as for FlashAttention; with 1 (sliding window) keys below `sinks`
+ * stay visible. */
+typedef struct {
+    uint32_t T;
+    uint32_t R;
+    uint32_t Nq;
+    uint32_t Nkv;
+    uint32_t Hd;
+    uint32_t pageSize;
+    uint32_t pages;
+    uint32_t columns;
+    uint32_t maskKind;
+    int32_t slidingWindow;
+    uint32_t sinks;
+    float scale;
+} PagedAttentionConstants;
+
+/* sample_*: one token of each row of logits [rows, vocab]. */
+typedef struct {
+    uint32_t rows;
+    uint32_t vocab;
+    uint32_t hasTemperature;
+    uint32_t hasTopK;
+    uint32_t hasTopP;
+    uint32_t hasMinP;
+} SampleConstants;
+
 #ifdef __cplusplus
 }
 #endif

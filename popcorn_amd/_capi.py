@@ -186,6 +186,11 @@ PROTOTYPES = {
     "popcorn_kernel_matmul_quantized": (_st, [_T, C.POINTER(AffineQuantizedDesc), _T, _K]),
     "popcorn_kernel_embedding_gather_quantized": (_st, [_T, C.POINTER(AffineQuantizedDesc), _T, _K]),
     "popcorn_kernel_argmax": (_st, [_T, _T, _K]),
+    "popcorn_kernel_page_tables": (_st, [_T, _T, _T, _T, C.c_int64, _T, _T, _T, _T, _T, _K]),
+    "popcorn_kernel_paged_kv_cache_write": (_st, [_T, _T, _T, _T, _T, _K]),
+    "popcorn_kernel_paged_attention": (_st, [_T, _T, _T, _T, _T, _T, _T, C.c_float, AttentionMaskDesc, C.c_int64,
+                                             C.c_int64, _K]),
+    "popcorn_kernel_sample": (_st, [_T, _T, _T, _T, _T, _T, _T, _K]),
     "popcorn_kernel_custom": (_st, [C.c_char_p, _T, C.POINTER(C.c_uint8), C.c_int32, C.POINTER(C.c_void_p),
                                     C.POINTER(C.c_size_t), C.c_int32, C.POINTER(C.c_uint32),
                                     C.POINTER(C.c_uint32), _K]),

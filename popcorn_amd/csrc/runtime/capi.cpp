@@ -814,6 +814,55 @@ popcorn_status_t popcorn_kernel_argmax(const popcorn_tensor_t *x, const popcorn_
     return guarded([&] { emit(kernel, Kernels::Argmax(T(x, "x"), T(indices, "indices"))); });
 }
 
+popcorn_status_t popcorn_kernel_page_tables(const popcorn_tensor_t *past_lens, const popcorn_tensor_t *new_lens,
+                                            const popcorn_tensor_t *free_pages, const popcorn_tensor_t *page_tables,
+                                            int64_t page_size, const popcorn_tensor_t *query_starts,
+                                            const popcorn_tensor_t *key_lens, const popcorn_tensor_t *positions,
+                                            const popcorn_tensor_t *slots, const popcorn_tensor_t *counts,
+                                            popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::PageTables(T(past_lens, "past_lens"), T(new_lens, "new_lens"), T(free_pages, "free_pages"),
+                                         T(page_tables, "page_tables"), page_size, T(query_starts, "query_starts"),
+                                         T(key_lens, "key_lens"), T(positions, "positions"), T(slots, "slots"),
+                                         T(counts, "counts")));
+    });
+}
+
+popcorn_status_t popcorn_kernel_paged_kv_cache_write(const popcorn_tensor_t *k, const popcorn_tensor_t *v,
+                                                     const popcorn_tensor_t *slots, const popcorn_tensor_t *k_cache,
+                                                     const popcorn_tensor_t *v_cache, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::PagedKVCacheWrite(T(k, "k"), T(v, "v"), T(slots, "slots"), T(k_cache, "k_cache"), T(v_cache, "v_cache")));
+    });
+}
+
+popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
+                                                const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
+                                                const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens,
+                                                const popcorn_tensor_t *out, float scale, popcorn_attention_mask_t mask,
+                                                int64_t sinks, int64_t max_query_len, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::PagedAttention(T(q, "q"), T(k_cache, "k_cache"), T(v_cache, "v_cache"), T(page_tables, "page_tables"),
+                                             T(query_starts, "query_starts"), T(key_lens, "key_lens"), T(out, "out"), scale,
+                                             AttentionMask{mask.kind, mask.window}, sinks, max_query_len));
+    });
+}
+
+popcorn_status_t popcorn_kernel_sample(const popcorn_tensor_t *logits, const popcorn_tensor_t *uniforms,
+                                       const popcorn_tensor_t *temperature, const popcorn_tensor_t *top_k,
+                                       const popcorn_tensor_t *top_p, const popcorn_tensor_t *min_p,
+                                       const popcorn_tensor_t *tokens, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        Tensor opt[4];
+        const popcorn_tensor_t *in[4] = {temperature, top_k, top_p, min_p};
+        for (int i = 0; i < 4; ++i)
+            if (in[i]) opt[i] = Tensor::fromC(*in[i]);
+        emit(kernel, Kernels::Sample(T(logits, "logits"), T(uniforms, "uniforms"), in[0] ? &opt[0] : nullptr,
+                                     in[1] ? &opt[1] : nullptr, in[2] ? &opt[2] : nullptr, in[3] ? &opt[3] : nullptr,
+                                     T(tokens, "tokens")));
+    });
+}
+
 popcorn_status_t popcorn_kernel_custom(const char *function_name, const popcorn_tensor_t *tensors, const uint8_t *access,
                                        int32_t ntensors, const void *const *constants, const size_t *constant_sizes,
                                        int32_t nconstants, const uint32_t grid[3], const uint32_t block[3],

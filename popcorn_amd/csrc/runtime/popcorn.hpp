@@ -458,6 +458,18 @@ std::unique_ptr<Kernel> Matmul(const Tensor &a, const AffineQuantizedTensor &b, 
 std::unique_ptr<Kernel> EmbeddingGather(const Tensor &ids, const AffineQuantizedTensor &table, const Tensor &out);
 std::unique_ptr<Kernel> Argmax(const Tensor &x, const Tensor &indices);
 
+// A batch of requests over a paged cache (serving.cpp; popcorn_hip.h says what each does).
+std::unique_ptr<Kernel> PageTables(const Tensor &pastLens, const Tensor &newLens, const Tensor &freePages,
+                                   const Tensor &pageTables, int64_t pageSize, const Tensor &queryStarts,
+                                   const Tensor &keyLens, const Tensor &positions, const Tensor &slots, const Tensor &counts);
+std::unique_ptr<Kernel> PagedKVCacheWrite(const Tensor &k, const Tensor &v, const Tensor &slots, const Tensor &kCache,
+                                          const Tensor &vCache);
+std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
+                                       const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, float scale,
+                                       AttentionMask mask, int64_t sinks, int64_t maxQueryLen);
+std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK,
+                               const Tensor *topP, const Tensor *minP, const Tensor &tokens);
+
 std::unique_ptr<Kernel> Custom(const std::string &functionName, std::vector<Binding> tensors,
                                std::vector<std::vector<uint8_t>> constants, dim3 grid, dim3 block);
 // The same with `dynamicLds` bytes of dynamic LDS per block.

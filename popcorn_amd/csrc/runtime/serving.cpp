@@ -1,0 +1,182 @@
+// Kernels.* descriptors of a batch of requests over a paged cache: page tables,
+// the paged cache write, paged attention, and the draw of the next token.
+// No counterparts in the reference; validation and errors are as for its own
+// operations (kernels.cpp).
+#include <algorithm>
+
+#include "popcorn.hpp"
+
+namespace popcorn {
+namespace {
+
+int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool isFloat(DataType t) { return t == DataType::f32 || t == DataType::f16 || t == DataType::bf16; }
+bool aligned(const void *p, int bytes) { return reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes == 0; }
+
+void requireRank(const Tensor &t, int rank) {
+    if (t.shape.rank() != rank) throw Error::tensorInvalidRank(rank, t.shape.rank());
+}
+
+// Every size below 2^31 (the kernels count in 32 bits), the bytes below 2^62, and the data's place.
+void requireTensor(const Tensor &t, const std::string &what) {
+    int64_t bytes = stride(t.dataType);
+    for (int64_t d : t.shape.dims) {
+        if (d >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch(what + " dimensions must be below 2^31; got " + t.shape.str() + ".");
+        if (__builtin_mul_overflow(bytes, d, &bytes) || bytes >= (int64_t{1} << 62))
+            throw Error::tensorShapeMismatch(what + " is too large: " + t.shape.str() + ".");
+    }
+    if (bytes > 0 && !t.data) throw Error::invalidArgument(what + ": null data pointer");
+    if (!aligned(t.data, stride(t.dataType))) throw Error::invalidArgument(what + ": data is not aligned to its elements");
+}
+
+void requireShape(const Tensor &t, DataType type, std::initializer_list<int64_t> dims, const std::string &what) {
+    if (t.dataType != type)
+        throw Error::unsupportedDataTypeCombination(what + " must be " + name(type) + "; got " + name(t.dataType) + ".");
+    const Shape want(dims);
+    requireRank(t, want.rank());
+    if (t.shape != want) throw Error::tensorShapeMismatch(what + " must have shape " + want.str() + "; got " + t.shape.str() + ".");
+    requireTensor(t, what);
+}
+
+// The caches [pages, Nkv, page size, Hd] of one shape and dtype.
+void requireCaches(const Tensor &k, const Tensor &v, const std::string &op) {
+    requireRank(k, 4);
+    if (v.shape != k.shape) throw Error::tensorShapeMismatch(op + " caches must share a shape; got " + k.shape.str() + " and " + v.shape.str() + ".");
+    requireTensor(k, op + " k_cache");
+    requireTensor(v, op + " v_cache");
+    if (k.shape[2] <= 0) throw Error::tensorShapeMismatch(op + " page size must be positive; got " + k.shape.str() + ".");
+    if (k.shape[0] * k.shape[2] >= (int64_t{1} << 31))
+        throw Error::tensorShapeMismatch(op + " cache must hold fewer than 2^31 slots; got " + k.shape.str() + ".");
+}
+
+std::unique_ptr<Kernel> fixed(const std::string &fn, std::vector<Binding> b, std::vector<uint8_t> c, dim3 grid, unsigned block) {
+    return Kernels::Custom(fn, std::move(b), {std::move(c)}, grid, dim3(block, 1, 1));
+}
+
+}  // namespace
+
+namespace Kernels {
+
+std::unique_ptr<Kernel> PageTables(const Tensor &pastLens, const Tensor &newLens, const Tensor &freePages,
+                                   const Tensor &pageTables, int64_t pageSize, const Tensor &queryStarts,
+                                   const Tensor &keyLens, const Tensor &positions, const Tensor &slots, const Tensor &counts) {
+    using D = DataType;
+    requireRank(pastLens, 1);
+    requireRank(freePages, 1);
+    requireRank(pageTables, 2);
+    requireRank(positions, 1);
+    const int64_t R = pastLens.shape[0], F = freePages.shape[0], M = pageTables.shape[1], T = positions.shape[0];
+    if (pageSize <= 0 || pageSize >= (int64_t{1} << 31)) throw Error::invalidArgument("PageTables page size must be positive and below 2^31.");
+    if (R >= (int64_t{1} << 31) - 1) throw Error::tensorShapeMismatch("PageTables takes fewer than 2^31 - 1 requests.");
+    requireShape(pastLens, D::i32, {R}, "PageTables past_lens");
+    requireShape(newLens, D::i32, {R}, "PageTables new_lens");
+    requireShape(freePages, D::i32, {F}, "PageTables free_pages");
+    requireShape(pageTables, D::i32, {R, M}, "PageTables page_tables");
+    requireShape(queryStarts, D::i32, {R + 1}, "PageTables query_starts");
+    requireShape(keyLens, D::i32, {R}, "PageTables key_lens");
+    requireShape(positions, D::i32, {T}, "PageTables positions");
+    requireShape(slots, D::i32, {T}, "PageTables slots");
+    requireShape(counts, D::i32, {2}, "PageTables counts");
+    const PageTablesConstants pc{(uint32_t)R, (uint32_t)M, (uint32_t)F, (uint32_t)T, (uint32_t)pageSize};
+    const int64_t blocks = std::clamp<int64_t>(cdiv(T, 256), 1, 256);
+    return fixed("page_tables",
+                 {{pastLens, kRead}, {newLens, kRead}, {freePages, kRead}, {pageTables, kReadWrite}, {queryStarts, kWrite},
+                  {keyLens, kWrite}, {positions, kWrite}, {slots, kWrite}, {counts, kWrite}},
+                 bytesOf(pc), dim3((unsigned)blocks, 1, 1), 256);
+}
+
+std::unique_ptr<Kernel> PagedKVCacheWrite(const Tensor &k, const Tensor &v, const Tensor &slots, const Tensor &kCache,
+                                          const Tensor &vCache) {
+    using D = DataType;
+    const D s = k.dataType, c = kCache.dataType;
+    const char *fn = s == D::f32 && c == D::f32    ? "paged_kv_write_f32"
+                     : s == D::f16 && c == D::f16   ? "paged_kv_write_f16"
+                     : s == D::bf16 && c == D::bf16 ? "paged_kv_write_bf16"
+                     : s == D::f32 && c == D::bf16  ? "paged_kv_write_f32_to_bf16"
+                                                    : nullptr;
+    if (!fn || v.dataType != s || vCache.dataType != c)
+        throw Error::unsupportedDataTypeCombination(std::string("Unsupported paged KV cache data type combination: ") + name(s) + ", " +
+                                                    name(v.dataType) + ", " + name(c) + ", " + name(vCache.dataType) + ".");
+    requireCaches(kCache, vCache, "PagedKVCacheWrite");
+    requireRank(k, 3);
+    const int64_t T = k.shape[0], Nkv = kCache.shape[1], page = kCache.shape[2], Hd = kCache.shape[3];
+    requireShape(k, s, {T, Nkv, Hd}, "PagedKVCacheWrite k");
+    requireShape(v, s, {T, Nkv, Hd}, "PagedKVCacheWrite v");
+    requireShape(slots, D::i32, {T}, "PagedKVCacheWrite slots");
+    const int64_t run = 16 / stride(s), perToken = Nkv * cdiv(Hd, run);
+    if (perToken >= (int64_t{1} << 30)) throw Error::tensorShapeMismatch("PagedKVCacheWrite rows are too long: " + k.shape.str() + ".");
+    const int64_t blocks = cdiv(T * perToken, 1024);
+    if (blocks >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("PagedKVCacheWrite holds too many rows: " + k.shape.str() + ".");
+    const PagedKVWriteConstants pc{(uint32_t)T, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page, (uint32_t)kCache.shape[0]};
+    return fixed(fn, {{k, kRead}, {v, kRead}, {slots, kRead}, {kCache, kWrite}, {vCache, kWrite}}, bytesOf(pc),
+                 dim3((unsigned)blocks, blocks ? 2 : 0, 1), 256);
+}
+
+std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
+                                       const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, float scale,
+                                       AttentionMask mask, int64_t sinks, int64_t maxQueryLen) {
+    using D = DataType;
+    const D t = q.dataType;
+    if (!isFloat(t) || kCache.dataType != t || vCache.dataType != t || out.dataType != t)
+        throw Error::unsupportedDataTypeCombination(std::string("PagedAttention needs one floating dtype for q, the caches and out; got ") +
+                                                    name(t) + ", " + name(kCache.dataType) + ", " + name(vCache.dataType) + ", " +
+                                                    name(out.dataType) + ".");
+    if (mask.kind > 2) throw Error::invalidArgument("unknown attention mask kind");
+    if (sinks < 0 || sinks >= (int64_t{1} << 31)) throw Error::invalidArgument("PagedAttention sinks must be at least 0 and below 2^31.");
+    if (sinks > 0 && mask.kind != 1) throw Error::invalidArgument("PagedAttention sinks go with a sliding window.");
+    if (maxQueryLen < 0) throw Error::invalidArgument("PagedAttention max_query_len must not be negative.");
+    requireCaches(kCache, vCache, "PagedAttention");
+    requireRank(q, 3);
+    requireRank(pageTables, 2);
+    const int64_t T = q.shape[0], Nq = q.shape[1], Hd = q.shape[2], Nkv = kCache.shape[1], page = kCache.shape[2];
+    const int64_t R = pageTables.shape[0], M = pageTables.shape[1];
+    if (Nkv <= 0 || Nq <= 0 || Nq % Nkv != 0)
+        throw Error::tensorShapeMismatch("PagedAttention query heads must be divisible by KV heads; got " + std::to_string(Nq) + " and " +
+                                         std::to_string(Nkv) + ".");
+    if (Hd <= 0 || Hd > 512)
+        throw Error::tensorShapeMismatch("PagedAttention head dim must be 1 to 512 (kernel limit); got " + std::to_string(Hd) + ".");
+    if (kCache.shape[3] != Hd)
+        throw Error::tensorShapeMismatch("PagedAttention caches must have q's head dim; got " + q.shape.str() + " and " + kCache.shape.str() + ".");
+    if (page % 16 != 0)
+        throw Error::tensorShapeMismatch("PagedAttention page size must be a multiple of 16; got " + std::to_string(page) + ".");
+    requireShape(q, t, {T, Nq, Hd}, "PagedAttention q");
+    requireShape(out, t, {T, Nq, Hd}, "PagedAttention out");
+    requireShape(pageTables, D::i32, {R, M}, "PagedAttention page_tables");
+    requireShape(queryStarts, D::i32, {R + 1}, "PagedAttention query_starts");
+    requireShape(keyLens, D::i32, {R}, "PagedAttention key_lens");
+    if (T * Nq >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("PagedAttention takes fewer than 2^31 query rows; got " + q.shape.str() + ".");
+    const PagedAttentionConstants pc{(uint32_t)T, (uint32_t)R, (uint32_t)Nq, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page,
+                                     (uint32_t)kCache.shape[0], (uint32_t)M, mask.kind, mask.window, (uint32_t)sinks, scale};
+    std::string fn = std::string("paged_attention_plain_") + name(t);
+    const int run = 4 * stride(t);
+    if (Hd % 4 || !aligned(kCache.data, run) || !aligned(vCache.data, run)) fn += "_any";
+    return fixed(fn, {{q, kRead}, {kCache, kRead}, {vCache, kRead}, {pageTables, kRead}, {queryStarts, kRead}, {keyLens, kRead}, {out, kWrite}},
+                 bytesOf(pc), dim3((unsigned)(R ? cdiv(T * Nq, 16) : 0), 1, 1), 256);
+}
+
+std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK,
+                               const Tensor *topP, const Tensor *minP, const Tensor &tokens) {
+    using D = DataType;
+    if (!isFloat(logits.dataType))
+        throw Error::unsupportedDataTypeCombination(std::string("Sample logits must be f32, f16 or bf16; got ") + name(logits.dataType) + ".");
+    requireRank(logits, 2);
+    const int64_t rows = logits.shape[0], vocab = logits.shape[1];
+    if (vocab <= 0 || vocab > (int64_t{1} << 22))
+        throw Error::tensorShapeMismatch("Sample takes 1 to 2^22 logits a row; got " + std::to_string(vocab) + ".");
+    requireTensor(logits, "Sample logits");
+    requireShape(uniforms, D::f32, {rows}, "Sample uniforms");
+    requireShape(tokens, D::i32, {rows}, "Sample tokens");
+    if (temperature) requireShape(*temperature, D::f32, {rows}, "Sample temperature");
+    if (topK) requireShape(*topK, D::i32, {rows}, "Sample top_k");
+    if (topP) requireShape(*topP, D::f32, {rows}, "Sample top_p");
+    if (minP) requireShape(*minP, D::f32, {rows}, "Sample min_p");
+    const SampleConstants sc{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr};
+    const Tensor &none = uniforms;  // bound where an option is absent, and not read
+    return fixed(std::string("sample_") + name(logits.dataType),
+                 {{logits, kRead}, {uniforms, kRead}, {temperature ? *temperature : none, kRead}, {topK ? *topK : none, kRead},
+                  {topP ? *topP : none, kRead}, {minP ? *minP : none, kRead}, {tokens, kWrite}},
+                 bytesOf(sc), dim3((unsigned)rows, 1, 1), 1024);
+}
+
+}  // namespace Kernels
+}  // namespace popcorn

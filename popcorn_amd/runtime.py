@@ -704,6 +704,40 @@ class Kernels:
         return _make(lib().popcorn_kernel_argmax, _d(x), _d(indices), refs=(x, indices))
 
     @staticmethod
+    def PageTables(past_lens: Tensor, new_lens: Tensor, free_pages: Tensor, page_tables: Tensor, *, page_size: int,
+                   query_starts: Tensor, key_lens: Tensor, positions: Tensor, slots: Tensor, counts: Tensor) -> Kernel:
+        """A step's tables from the requests' lengths (popcorn_kernel_page_tables): page_tables [R, columns]
+        takes pages from the front of free_pages; each new token gets its position and slot."""
+        ts = (past_lens, new_lens, free_pages, page_tables, query_starts, key_lens, positions, slots, counts)
+        d = [_d(t) for t in ts]
+        return _make(lib().popcorn_kernel_page_tables, *d[:4], page_size, *d[4:], refs=ts)
+
+    @staticmethod
+    def PagedKVCacheWrite(k: Tensor, v: Tensor, slots: Tensor, k_cache: Tensor, v_cache: Tensor) -> Kernel:
+        """k, v [T, Nkv, Hd] into their slots of the caches [pages, Nkv, page_size, Hd]
+        (popcorn_kernel_paged_kv_cache_write)."""
+        ts = (k, v, slots, k_cache, v_cache)
+        return _make(lib().popcorn_kernel_paged_kv_cache_write, *[_d(t) for t in ts], refs=ts)
+
+    @staticmethod
+    def PagedAttention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_tables: Tensor, query_starts: Tensor,
+                       key_lens: Tensor, into: Tensor, *, scale: float, mask: AttentionMask = AttentionMask(0),
+                       sinks: int = 0, max_query_len: int = 0) -> Kernel:
+        """Attention of every request's new tokens q [T, Nq, Hd] over its pages (popcorn_kernel_paged_attention);
+        max_query_len, the longest request's number of new tokens, chooses the kernels."""
+        ts = (q, k_cache, v_cache, page_tables, query_starts, key_lens, into)
+        return _make(lib().popcorn_kernel_paged_attention, *[_d(t) for t in ts], scale, mask.desc(), sinks,
+                     max_query_len, refs=ts)
+
+    @staticmethod
+    def Sample(logits: Tensor, uniforms: Tensor, into: Tensor, *, temperature: Optional[Tensor] = None,
+               top_k: Optional[Tensor] = None, top_p: Optional[Tensor] = None,
+               min_p: Optional[Tensor] = None) -> Kernel:
+        """One token of each row of logits, drawn with the row's uniform random number (popcorn_kernel_sample)."""
+        ts = (logits, uniforms, temperature, top_k, top_p, min_p, into)
+        return _make(lib().popcorn_kernel_sample, *[_d(t) for t in ts], refs=ts)
+
+    @staticmethod
     def Custom(function_name: str, tensors: Sequence[Tensor], access: Sequence[int], constants: Sequence[bytes],
                grid, block) -> Kernel:
         """A caller-built DispatchKernel (Kernel.swift:54-70); access 1 read, 2 write, 3 both."""
