@@ -453,6 +453,21 @@ typedef struct {
     float scale;
 } PagedAttentionConstants;
 
+/* The work of a paged attention launch, laid out by paged_plan. A request's
+ * rows (token, head of a KV head's group) are cut into tiles of `rows`, a
+ * tile's visible keys into steps of `stepKeys`; the (tile, KV head) units of
+ * steps in a row are dealt to `workers` blocks in equal stretches of at least
+ * minSteps. A launch takes the requests of fewRows < rows <= manyRows. */
+typedef struct {
+    uint32_t rows;
+    uint32_t stepKeys;
+    uint32_t fewRows;
+    uint32_t manyRows;
+    uint32_t maxTiles;
+    uint32_t workers;
+    uint32_t minSteps;
+} PagedWorkConstants;
+
 /* sample_*: one token of each row of logits [rows, vocab]. */
 typedef struct {
     uint32_t rows;

@@ -59,4 +59,44 @@ PAGED_FN bool paged_sees(int32_t pos, int32_t key, const PagedAttentionConstants
     return (p.maskKind == 2u) | ((key <= pos) & ((p.maskKind == 0u) | ((int64_t)pos - key < p.slidingWindow) | ((uint32_t)key < p.sinks)));
 }
 
+// The plan of a launch: entry 0 holds the steps of all tiles (of one KV head)
+// and the number of tiles, entry 1 + i tile i with the steps before it.
+struct PagedTile {
+    uint64_t before;
+    uint32_t request, tile;
+};
+
+// Tile `tile` of request r: rows r0 .. r1 - 1 of its n * G, and its steps: sink
+// steps from key 0, then the others from step `first`. A tile without a visible key has one
+// step, so that its rows are written.
+struct PagedSteps {
+    uint32_t r0, r1, sinks, first, n;
+};
+
+PAGED_FN PagedSteps paged_steps(const PagedRequest &r, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    const uint32_t G = p.Nq / p.Nkv, rows = (uint32_t)r.n * G;
+    PagedSteps s;
+    s.r0 = tile * w.rows;
+    s.r1 = rows - s.r0 < w.rows ? rows : s.r0 + w.rows;
+    const PagedSpan k = paged_span(r.pos0 + (int32_t)(s.r0 / G), r.pos0 + (int32_t)((s.r1 - 1) / G), r.keys, p);
+    const uint32_t step = w.stepKeys;
+    s.sinks = ((uint32_t)k.sinkEnd + step - 1) / step;
+    s.first = (uint32_t)k.lo / step > s.sinks ? (uint32_t)k.lo / step : s.sinks;
+    const uint32_t end = k.hi > k.lo ? ((uint32_t)k.hi + step - 1) / step : 0u;
+    s.n = s.sinks + (end > s.first ? end - s.first : 0u);
+    if (s.n == 0) s.n = 1;
+    return s;
+}
+
+// First key of step `step` of a tile.
+PAGED_FN uint32_t paged_step_key(const PagedSteps &s, uint32_t step, const PagedWorkConstants &w) {
+    return (step < s.sinks ? step : step - s.sinks + s.first) * w.stepKeys;
+}
+
+// Steps per worker, for `total` steps of all units.
+PAGED_FN uint64_t paged_share(uint64_t total, const PagedWorkConstants &w) {
+    const uint64_t q = (total + w.workers - 1) / w.workers;
+    return q > w.minSteps ? q : w.minSteps;
+}
+
 }  // namespace pk

@@ -2,6 +2,8 @@
 // [pages, Nkv, pageSize, Hd]: out = softmax(scale q K^T | visible keys) V per
 // request, query heads in groups per KV head, with the lengths and the pages
 // read on the GPU.
+#include <type_traits>
+
 #include "mfma.hpp"
 #include "paged.hpp"
 
@@ -72,6 +74,530 @@ __device__ inline void paged_row(const pk::f32x4 (&q)[NJ], const typename T::sto
     }
 }
 
+
+// ---- the plan ----------------------------------------------------------------------
+
+constexpr uint32_t kPlanThreads = 1024;
+
+// Inclusive sum of v over the block (`sums`: one entry per wave), and the total.
+__device__ inline uint64_t block_scan(uint64_t v, uint64_t *sums, uint64_t &total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint64_t x = __shfl_up((unsigned long long)v, d);
+        if (lane >= d) v += x;
+    }
+    __syncthreads();
+    if (lane == 63) sums[wave] = v;
+    __syncthreads();
+    total = 0;
+    uint64_t before = 0;
+    for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
+        if (w == wave) before = total;
+        total += sums[w];
+    }
+    return before + v;
+}
+
+}  // namespace
+
+// One block: the tiles of every request, in request order.
+POPCORN_KERNEL void __launch_bounds__(1024)
+    paged_plan(const int32_t *starts, const int32_t *keyLens, pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants w) {
+    __shared__ uint64_t sSums[kPlanThreads / 64];
+    __shared__ uint32_t sTile[kPlanThreads + 1];
+    __shared__ pk::PagedRequest sReq[kPlanThreads];
+    const uint32_t tid = threadIdx.x, G = p.Nq / p.Nkv;
+    uint64_t steps = 0;
+    uint32_t tiles = 0;
+    for (uint32_t base = 0; base < p.R; base += kPlanThreads) {
+        const uint32_t r = base + tid;
+        pk::PagedRequest q{0, 0, 0, 0};
+        if (r < p.R) q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
+        const uint32_t rows = (uint32_t)q.n * G;
+        const uint32_t mine = rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
+        uint64_t total;
+        const uint64_t upto = block_scan(mine, sSums, total);
+        // overlapping ranges of requests could hold more rows than there are: what passes the plan's room is left out
+        const uint32_t here = (uint32_t)min(total, (uint64_t)(w.maxTiles - tiles));
+        sTile[tid] = (uint32_t)min(upto - mine, (uint64_t)here);
+        sReq[tid] = q;
+        if (tid == 0) sTile[kPlanThreads] = here;
+        __syncthreads();
+        for (uint32_t t0 = 0; t0 < here; t0 += kPlanThreads) {
+            const uint32_t t = t0 + tid;
+            uint32_t i = 0, n = 0;
+            if (t < here) {
+#pragma unroll
+                for (uint32_t d = kPlanThreads / 2; d; d >>= 1)
+                    if (sTile[i + d] <= t) i += d;
+                n = pk::paged_steps(sReq[i], t - sTile[i], p, w).n;
+            }
+            uint64_t sum;
+            const uint64_t end = block_scan(n, sSums, sum);
+            if (t < here) plan[1 + tiles + t] = pk::PagedTile{steps + end - n, base + i, t - sTile[i]};
+            steps += sum;
+        }
+        tiles += here;
+        __syncthreads();
+    }
+    if (tid == 0) plan[0] = pk::PagedTile{steps, tiles, 0};
+}
+
+namespace {
+
+// ---- a few rows per KV head: decode and drafts ------------------------------------------------
+
+constexpr int kWaves = 4;
+constexpr float kRescaleGap = 8.0f * kLog2e;  // log2 units, as the maxima
+constexpr int kOutOfRange = (int)0x80000000u;  // past every page: zeros
+
+typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+using pk::u32x2;
+using pk::u32x4;
+
+__device__ inline float quad16_max(float v) { return pk::pair32_max(pk::pair16_max(v)); }
+__device__ inline float quad16_sum(float v) { return pk::pair32_sum(pk::pair16_sum(v)); }
+
+template <int N>
+__device__ inline void wait_vmcnt() {
+    static_assert(N >= 0 && N < 64, "vmcnt range");
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+__device__ inline uint32_t first_lane(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline uint64_t first_lane64(uint64_t v) {
+    return (uint64_t)first_lane((uint32_t)(v >> 32)) << 32 | first_lane((uint32_t)v);
+}
+
+// The tile whose units hold step x: the last with before * Nkv <= x. A wave's
+// lanes look at 64 entries at once.
+__device__ inline uint32_t find_tile(const pk::PagedTile *plan, uint32_t tiles, uint64_t x, uint32_t Nkv) {
+    const uint64_t at = x / Nkv;
+    uint32_t lo = 0, n = tiles;
+    while (n > 1) {
+        const uint32_t stride = (n + 63) / 64, i = (threadIdx.x & 63) * stride;
+        const bool in = i < n && plan[1 + lo + i].before <= at;
+        const uint32_t last = 63 - __clzll(__ballot(in));  // lane 0's entry is always at or before x
+        const uint32_t from = last * stride;
+        n = min(stride, n - from);
+        lo += from;
+    }
+    return first_lane(lo);
+}
+
+// A stretch of one unit's steps.
+struct Piece {
+    pk::PagedRequest req;
+    pk::PagedSteps steps;
+    uint32_t request, hkv, lo, hi;
+};
+
+// The piece that begins at step x of all units and ends before `end`; `i` is x's tile, and moves on with x.
+__device__ inline Piece next_piece(const pk::PagedTile *plan, uint32_t &i, uint64_t &x, uint64_t end, const int32_t *starts,
+                                   const int32_t *keyLens, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    const pk::PagedTile t = plan[1 + i];
+    Piece c;
+    c.request = first_lane(t.request);
+    c.req = pk::paged_request(starts[c.request], starts[c.request + 1], keyLens[c.request], p);
+    c.steps = pk::paged_steps(c.req, first_lane(t.tile), p, w);
+    const uint64_t in = x - first_lane64(t.before) * p.Nkv;
+    c.hkv = (uint32_t)(in / c.steps.n);
+    c.lo = (uint32_t)(in - (uint64_t)c.hkv * c.steps.n);
+    c.hi = (uint32_t)min((uint64_t)c.steps.n, c.lo + (end - x));
+    x += c.hi - c.lo;
+    if (c.hi == c.steps.n && c.hkv + 1 == p.Nkv) ++i;
+    return c;
+}
+
+// The result of one row's lane of 4 dims, rounded.
+template <typename T>
+__device__ inline void store4(typename T::storage *dst, const pk::f32x4 &o, float l) {
+    pk::f32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = l != 0.0f ? o[i] / l : 0.0f;
+    if constexpr (sizeof(typename T::storage) == 4) {
+        *reinterpret_cast<pk::f32x4 *>(dst) = v;
+    } else {
+        *reinterpret_cast<u32x2 *>(dst) = u32x2{pk::bits16<T>(v[0]) | pk::bits16<T>(v[1]) << 16, pk::bits16<T>(v[2]) | pk::bits16<T>(v[3]) << 16};
+    }
+}
+
+// A piece's partial state goes to one of its worker's two slots: 2 w + 1 if
+// the piece begins its unit, else 2 w.
+template <typename T, int HD, int RT>
+__device__ void paged_few(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
+                          const typename T::storage *__restrict__ V, const int32_t *__restrict__ tables,
+                          const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                          const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
+                          typename T::storage *__restrict__ out, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    using S = typename T::storage;
+    constexpr bool kWide = sizeof(S) == 4;
+    constexpr int KM = kWide ? 1 : 2;          // 16-key groups per step
+    constexpr int BKV = 16 * KM, E = 16 / sizeof(S);
+    constexpr int KS = HD / (4 * E);           // 16-byte pieces of a lane's K and Q rows
+    constexpr int DT = HD / 16;                // 16-row tiles of O^T
+    constexpr int CH = HD / E;                 // 16-byte chunks per row
+    constexpr int kRowsPer = CH > 64 ? 1 : 64 / CH;  // V rows per copy instruction
+    constexpr int kHalves = CH > 64 ? CH / 64 : 1;   // copy instructions per row
+    constexpr int kParts = kWide ? 1 : 2;
+    constexpr float kLead = std::is_same<T, pk::F16>::value ? 4.0f : 0.0f;  // max over reference when it moves
+    constexpr int LDO = HD + 4;                // merged-state row, in floats
+    constexpr int kStage = kWaves * BKV * HD * (int)sizeof(S), kMerge = kWaves * 16 * LDO * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kStage > kMerge ? kStage : kMerge];
+    __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
+    __shared__ uint32_t sm_bad;
+
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
+    const uint32_t wave = first_lane(threadIdx.x >> 6);
+    const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
+    const float c2 = p.scale * kLog2e;
+    const uint64_t total = plan[0].before * p.Nkv, share = pk::paged_share(total, w);
+    uint64_t x = first_lane64(blockIdx.x * share);
+    const uint64_t end = first_lane64(min(x + share, total));
+    if (x >= end) return;
+    uint32_t tile = find_tile(plan, plan[0].request, x, p.Nkv);
+
+    while (x < end) {
+        const Piece c = next_piece(plan, tile, x, end, starts, keyLens, p, w);
+        const int32_t *table = tables + (uint64_t)c.request * p.columns;
+        const uint32_t keys = (uint32_t)c.req.keys;
+        auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
+
+        // rows past the tile's last repeat it and are not stored
+        u32x4 qf[RT][KS];
+        int posQ[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const uint32_t r = min(c.steps.r0 + rt * 16 + c16, c.steps.r1 - 1);
+            posQ[rt] = c.req.pos0 + (int)(r / G);
+            const S *row = Q + q_row(r) * D + g * E;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                qf[rt][s] = s * 4 * E + g * E < D ? *reinterpret_cast<const u32x4 *>(row + s * 4 * E) : u32x4{0u, 0u, 0u, 0u};
+        }
+
+        // The wave's steps are c.lo + wave + kWaves i. Lane l holds page and row in it
+        // of group l % KM of the wave's step `page0` + l / KM; a group that no
+        // page holds has none (-1): its keys are left out and read as zeros.
+        constexpr uint32_t kHeld = 64 / KM;
+        uint32_t page0 = 0, heldPage = 0, heldRow = 0;
+        auto hold = [&](uint32_t i) {
+            const uint32_t step = c.lo + wave + kWaves * (i + lane / KM);
+            page0 = i;
+            heldPage = ~0u;
+            heldRow = 0;
+            if (step < c.hi) {
+                const uint32_t key = pk::paged_step_key(c.steps, step, w) + lane % KM * 16, column = key / p.pageSize;
+                if (key < keys) {
+                    heldPage = (uint32_t)table[column];
+                    heldRow = key - column * p.pageSize;
+                }
+            }
+        };
+        struct Group {
+            __amdgpu_buffer_rsrc_t k, v;
+            bool ok;
+        };
+        auto group = [&](uint32_t i, int mt, uint32_t key) {
+            const uint32_t at = (i - page0) * KM + mt;
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)at);
+            const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)heldRow, (int)at);
+            Group gr;
+            gr.ok = page < p.pages;
+            const uint64_t off = gr.ok ? (((uint64_t)page * p.Nkv + c.hkv) * p.pageSize + row) * D : 0;
+            const int bytes = gr.ok ? (int)(min(16u, keys - key) * D * (uint32_t)sizeof(S)) : 0;
+            gr.k = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(K + off), 0, bytes, 0x00020000);
+            gr.v = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(V + off), 0, bytes, 0x00020000);
+            return gr;
+        };
+
+        u32x4 kf[KM][KS];
+        Group gr[KM];
+        auto loadK = [&](uint32_t i, uint32_t step) {
+            const uint32_t key = step < c.hi ? pk::paged_step_key(c.steps, step, w) : keys;
+#pragma unroll
+            for (int mt = 0; mt < KM; ++mt) {
+                gr[mt] = group(i, mt, key + mt * 16);
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const uint32_t d = s * 4 * E + g * E;
+                    const int off = d < D ? (int)((c16 * D + d) * sizeof(S)) : kOutOfRange;
+                    kf[mt][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(gr[mt].k, off, 0, 0));
+                }
+            }
+        };
+        // V goes row-major into the wave's own tile, 16-byte chunks swizzled by the row (`swz`)
+        uint8_t *sV = smem + wave * (BKV * HD * sizeof(S));
+        auto swz = [](uint32_t row) { return kWide ? ((row >> 2) & 3u) << 2 : 2u * (row % 8u) % CH; };
+        auto copyV = [&](const Group *from) {
+#pragma unroll
+            for (int mt = 0; mt < KM; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16 / kRowsPer * kHalves; ++i) {
+                    const uint32_t row = i / kHalves * kRowsPer + (kHalves > 1 ? 0u : lane / CH);
+                    const uint32_t chunk = ((i % kHalves) * 64 + lane % CH) ^ swz(row);
+                    const int off = chunk * E < D ? (int)((row * D + chunk * E) * sizeof(S)) : kOutOfRange;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(from[mt].v, (lds_void *)(sV + (mt * 16 / kRowsPer * kHalves + i) * 1024), 16, off, 0, 0, 0);
+                }
+        };
+
+        pk::f32x4 acc[RT][DT];
+        float m[RT], l[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            m[rt] = -INFINITY;
+            l[rt] = 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[rt][dt] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+
+        hold(0);
+        uint32_t i = 0;
+        loadK(0, c.lo + wave);
+        for (uint32_t step = c.lo + wave; step < c.hi; step += kWaves, ++i) {
+            const uint32_t k0 = pk::paged_step_key(c.steps, step, w);
+            bool ok[KM];
+#pragma unroll
+            for (int mt = 0; mt < KM; ++mt) ok[mt] = gr[mt].ok;
+            copyV(gr);
+            pk::f32x4 st[RT][KM];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int mt = 0; mt < KM; ++mt) {
+                    st[rt][mt] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        if constexpr (kWide) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                st[rt][mt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[mt][s][e]), __uint_as_float(qf[rt][s][e]),
+                                                                                  st[rt][mt], 0, 0, 0);
+                        } else {
+                            st[rt][mt] = pk::Mma16<T>::run(kf[mt][s], qf[rt][s], st[rt][mt]);
+                        }
+                    }
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 - page0 == kHeld) hold(i + 1);
+            loadK(i + 1, step + kWaves);
+            __builtin_amdgcn_sched_barrier(0);
+            float pw[RT][4 * KM];
+            u32x4 pf[RT][kParts];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                float mx = -INFINITY, ps = 0.0f, alpha = 1.0f;
+#pragma unroll
+                for (int j = 0; j < 4 * KM; ++j) {
+                    const int key = (int)k0 + (j / 4) * 16 + (int)g * 4 + j % 4;
+                    const bool seen = ok[j / 4] & (key < (int)keys) & pk::paged_sees(posQ[rt], key, p);
+                    pw[rt][j] = seen ? st[rt][j / 4][j % 4] * c2 : -INFINITY;
+                    mx = fmaxf(mx, pw[rt][j]);
+                }
+                mx = quad16_max(mx);
+                const bool move = mx > m[rt] + (kRescaleGap + kLead);
+                if (move) {
+                    alpha = __builtin_amdgcn_exp2f(m[rt] - (mx - kLead));
+                    m[rt] = mx - kLead;
+                }
+                if (__ballot(move)) {
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt) acc[rt][dt] *= alpha;
+                }
+                // a row that has seen no key yet: every weight 0
+                const float mref = m[rt] == -INFINITY ? 0.0f : m[rt];
+#pragma unroll
+                for (int j = 0; j < 4 * KM; ++j) {
+                    pw[rt][j] = __builtin_amdgcn_exp2f(pw[rt][j] - mref);
+                    ps += pw[rt][j];
+                }
+                if constexpr (!kWide) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < kParts; ++e) {
+                            const uint32_t v = pk::pack2<T>(pw[rt][2 * j], pw[rt][2 * j + 1]);
+                            pf[rt][e][j] = v;
+                            pw[rt][2 * j] -= pk::from_bits16<T>(v & 0xffffu);  // exact
+                            pw[rt][2 * j + 1] -= pk::from_bits16<T>(v >> 16);
+                        }
+                }
+                l[rt] = l[rt] * alpha + quad16_sum(ps);
+            }
+            wait_vmcnt<(KM * KS < 63 ? KM * KS : 63)>();  // the V copies; the next step's K loads stay in flight
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                if constexpr (kWide) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t key = 4 * g + e, chunk = (dt * 4 + c16 / 4) ^ swz(key);
+                        const float va = *reinterpret_cast<const float *>(sV + (key * CH + chunk) * 16 + c16 % 4 * 4);
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(va, pw[rt][e], acc[rt][dt], 0, 0, 0);
+                    }
+                } else {
+                    auto readV = [&](uint32_t key) {
+                        const uint32_t chunk = (2 * dt + (c16 & 3) / 2) ^ swz(key);
+                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sV + (key * CH + chunk) * 16 + (c16 & 1) * 8));
+                        return __builtin_bit_cast(u32x2, v);
+                    };
+                    const u32x2 a = readV(4 * g + c16 / 4), b = readV(16 + 4 * g + c16 / 4);
+                    const u32x4 va = {a.x, a.y, b.x, b.y};
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                        for (int e = 0; e < kParts; ++e) acc[rt][dt] = pk::Mma16<T>::run(va, pf[rt][e], acc[rt][dt]);
+                }
+            }
+            __builtin_amdgcn_s_waitcnt(0xC07F);  // this wave's reads of its V tile are done before it is overwritten
+            asm volatile("" ::: "memory");
+        }
+        wait_vmcnt<0>();  // the last K loads (zeros), before their registers go
+
+        // merge the waves' states, one tile of 16 rows at a time: O through LDS,
+        // thread t takes row t / 16, dims 4 (t % 16) + 64 j
+        if (g == 0) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                sm_m[wave][rt * 16 + c16] = m[rt];
+                sm_l[wave][rt * 16 + c16] = l[rt];
+            }
+        }
+        if (threadIdx.x == 0) sm_bad = 0;
+        float *sO = reinterpret_cast<float *>(smem);
+        const uint32_t tr = threadIdx.x / 16, td = threadIdx.x % 16 * 4;
+        const bool whole = c.lo == 0 && c.hi == c.steps.n;
+        const uint64_t slot = (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * (RT * 16);
+        auto store = [&](uint32_t r, uint32_t d, const pk::f32x4 &o, float L) {
+            if (whole) store4<T>(out + q_row(r) * D + d, o, L);
+            else *reinterpret_cast<pk::f32x4 *>(pO + (slot + r - c.steps.r0) * HD + d) = o;
+        };
+        auto storeML = [&](uint32_t r, float M, float L) {
+            if (!whole && td == 0) *reinterpret_cast<float2 *>(pML + 2 * (slot + r - c.steps.r0)) = float2{M, L};
+        };
+        bool bad = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            __syncthreads();  // V tiles and the previous tile's state are read
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+                *reinterpret_cast<pk::f32x4 *>(&sO[(wave * 16 + c16) * LDO + dt * 16 + g * 4]) = acc[rt][dt];
+            __syncthreads();
+            const uint32_t r = c.steps.r0 + rt * 16 + tr;
+            if (r >= c.steps.r1) continue;
+            float M = -INFINITY, wt[kWaves], L = 0.0f;
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sm_m[v][rt * 16 + tr]);
+#pragma unroll
+            for (int v = 0; v < kWaves; ++v) {
+                const float mv = sm_m[v][rt * 16 + tr];
+                wt[v] = mv == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mv - M);
+                L += wt[v] * sm_l[v][rt * 16 + tr];
+            }
+            bad |= !(fabsf(L) < INFINITY);
+            for (uint32_t d = td; d < D; d += 64) {
+                pk::f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int v = 0; v < kWaves; ++v) o += *reinterpret_cast<const pk::f32x4 *>(&sO[(v * 16 + tr) * LDO + d]) * wt[v];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[e]) < INFINITY);
+                store(r, d, o, L);
+            }
+            storeML(r, M, L);
+        }
+        if (bad) sm_bad = 1;
+        __syncthreads();
+        if (sm_bad) {
+            // A matrix product adds 0 x V for a key that a row does not see, which an infinity or
+            // NaN in V turns into NaN: the rows again, over the keys that each sees.
+            const uint32_t s0 = min(c.lo, c.steps.sinks), s1 = min(c.hi, c.steps.sinks);
+            const uint32_t t0 = max(c.lo, c.steps.sinks), t1 = max(c.hi, c.steps.sinks);
+            auto key_at = [&](uint32_t k) { return (int)min(k * w.stepKeys, keys); };
+            for (uint32_t r = c.steps.r0 + tr; r < c.steps.r1; r += 16) {
+                constexpr int NJ = HD / 64;
+                pk::f32x4 qv[NJ], o[NJ];
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    o[j] = qv[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    if (td + 64 * j < D)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) qv[j][e] = T::load(Q[q_row(r) * D + td + 64 * j + e]);
+                }
+                const int pos = c.req.pos0 + (int)(r / G);
+                paged_row<T, NJ, true>(qv, K, V, table, c.hkv, pos, key_at(s0), key_at(s1), p, o, M, L);
+                paged_row<T, NJ, true>(qv, K, V, table, c.hkv, pos, key_at(t0 - c.steps.sinks + c.steps.first),
+                                       key_at(t1 - c.steps.sinks + c.steps.first), p, o, M, L);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (td + 64 * j < D) store(r, td + 64 * j, o[j], L);
+                storeML(r, M, L);
+            }
+        }
+        __syncthreads();  // the state is read before the next piece's V tiles
+    }
+}
+
+// The units that several workers shared: the worker whose last piece begins a
+// unit and does not end it merges that unit's pieces, its own from slot 2 w + 1
+// and the following workers' from their slots 2 w'.
+template <typename T, int HD>
+__device__ void paged_merge(const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                            const pk::PagedTile *__restrict__ plan, const float *__restrict__ pO, const float *__restrict__ pML,
+                            typename T::storage *__restrict__ out, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    constexpr int NJ = HD / 64;
+    const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
+    const uint64_t total = plan[0].before * p.Nkv, share = pk::paged_share(total, w);
+    const uint64_t lo = first_lane64(blockIdx.x * share), hi = first_lane64(min(lo + share, total));
+    if (lo >= hi || hi == total) return;  // (nothing goes on behind the last step)
+    uint64_t x = hi - 1;
+    uint32_t tile = find_tile(plan, plan[0].request, x, p.Nkv);
+    const Piece c = next_piece(plan, tile, x, hi, starts, keyLens, p, w);
+    const uint64_t begin = hi - 1 - c.lo, after = begin + c.steps.n;  // the unit's steps
+    if (begin < lo || after <= hi) return;
+    const uint32_t pieces = (uint32_t)((after - 1) / share - blockIdx.x) + 1;
+    const uint32_t td = threadIdx.x % 16 * 4;
+    for (uint32_t r = c.steps.r0 + blockIdx.y * 16 + threadIdx.x / 16; r < c.steps.r1; r += 16 * gridDim.y) {
+        const uint32_t in = r - c.steps.r0;
+        pk::f32x4 o[NJ];
+        float m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr uint32_t U = NJ > 4 ? 2 : 4;  // pieces in flight
+        for (uint32_t i0 = 0; i0 < pieces; i0 += U) {
+            float2 ml[U];
+            pk::f32x4 v[U][NJ];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                const uint32_t i = min(i0 + u, pieces - 1);
+                const uint64_t row = (2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * w.rows + in;
+                ml[u] = *reinterpret_cast<const float2 *>(pML + 2 * row);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    if (td + 64 * j < D) v[u][j] = *reinterpret_cast<const pk::f32x4 *>(pO + row * HD + td + 64 * j);
+            }
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) {
+                if (i0 + u >= pieces || (ml[u].x == -INFINITY && ml[u].y == 0.0f)) continue;
+                const float mn = fmaxf(m, ml[u].x);
+                const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(ml[u].x - mn);
+                l = l * a + ml[u].y * b;
+                m = mn;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[j] = o[j] * a + v[u][j] * b;
+            }
+        }
+        const uint64_t row = ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+            if (td + 64 * j < D) store4<T>(out + row * D + td + 64 * j, o[j], l);
+    }
+}
+
 // Any head dim up to 512 and any alignment: 16 rows per block, row b * 16 + i
 // of the T * Nq (token, head) pairs.
 template <typename T, bool VEC>
@@ -136,3 +662,33 @@ PAGED_PLAIN(paged_attention_plain_bf16, BF16, true)
 PAGED_PLAIN(paged_attention_plain_f32_any, F32, false)
 PAGED_PLAIN(paged_attention_plain_f16_any, F16, false)
 PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
+
+#define PAGED_FEW(name, T, HD, RT, PER_CU)                                                                                \
+    POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                    \
+        name(const T::storage *q, const T::storage *k, const T::storage *v, const int32_t *tables, const int32_t *starts, \
+             const int32_t *keyLens, const pk::PagedTile *plan, float *pO, float *pML, T::storage *out,                   \
+             PagedAttentionConstants p, PagedWorkConstants w) {                                                           \
+        paged_few<T, HD, RT>(q, k, v, tables, starts, keyLens, plan, pO, pML, out, p, w);                                 \
+    }
+#define PAGED_MERGE(name, T, HD)                                                                                            \
+    POPCORN_KERNEL void __launch_bounds__(256)                                                                              \
+        name(const int32_t *starts, const int32_t *keyLens, const pk::PagedTile *plan, const float *pO, const float *pML, \
+             T::storage *out, PagedAttentionConstants p, PagedWorkConstants w) {                                            \
+        paged_merge<T, HD>(starts, keyLens, plan, pO, pML, out, p, w);                                                      \
+    }
+#define PAGED_FEW_D(t, T, PER256)                                   \
+    PAGED_FEW(paged_attention_few_##t##_d64_r1, T, 64, 1, 4)   \
+    PAGED_FEW(paged_attention_few_##t##_d64_r2, T, 64, 2, 3)   \
+    PAGED_FEW(paged_attention_few_##t##_d128_r1, T, 128, 1, 3) \
+    PAGED_FEW(paged_attention_few_##t##_d128_r2, T, 128, 2, 2) \
+    PAGED_FEW(paged_attention_few_##t##_d256_r1, T, 256, 1, PER256) \
+    PAGED_FEW(paged_attention_few_##t##_d256_r2, T, 256, 2, 1) \
+    PAGED_FEW(paged_attention_few_##t##_d512_r1, T, 512, 1, 1) \
+    PAGED_MERGE(paged_attention_merge_##t##_d64, T, 64)        \
+    PAGED_MERGE(paged_attention_merge_##t##_d128, T, 128)      \
+    PAGED_MERGE(paged_attention_merge_##t##_d256, T, 256)      \
+    PAGED_MERGE(paged_attention_merge_##t##_d512, T, 512)
+
+PAGED_FEW_D(f32, F32, 1)
+PAGED_FEW_D(f16, F16, 2)
+PAGED_FEW_D(bf16, BF16, 2)

@@ -53,6 +53,80 @@ std::unique_ptr<Kernel> fixed(const std::string &fn, std::vector<Binding> b, std
     return Kernels::Custom(fn, std::move(b), {std::move(c)}, grid, dim3(block, 1, 1));
 }
 
+int deviceCUs() {
+    static thread_local int cachedDev = -1, cachedCUs = 256;
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess) {
+        (void)hipGetLastError();
+        return cachedCUs;
+    }
+    if (dev != cachedDev) {
+        int cus = 0;
+        if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) == hipSuccess && cus > 0) cachedCUs = cus;
+        (void)hipGetLastError();
+        cachedDev = dev;
+    }
+    return cachedCUs;
+}
+
+// PagedAttention on the matrix cores (paged_attention.hip): a plan of tiles,
+// the pieces of work, and the merge of what several blocks shared.
+class PagedAttentionKernel : public Kernel {
+public:
+    PagedAttentionKernel(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &tables, const Tensor &starts, const Tensor &lens,
+                         const Tensor &out, const PagedAttentionConstants &pc, int64_t maxQueryLen)
+        : q_(q), k_(k), v_(v), tables_(tables), starts_(starts), lens_(lens), out_(out), pc_(pc) {
+        const int64_t G = pc.Nq / pc.Nkv, R = pc.R, T = pc.T;
+        hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
+        const int rt = hdp_ == 512 || (maxQueryLen > 0 && maxQueryLen * G <= 16) ? 1 : 2;
+        const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
+        fn_ = "paged_attention_few_" + type + hd + "_r" + std::to_string(rt);
+        merge_ = "paged_attention_merge_" + type + hd;
+        w_.rows = 16 * (uint32_t)rt;
+        w_.stepKeys = q.dataType == DataType::f32 ? 16 : 32;
+        w_.fewRows = 0;
+        w_.manyRows = UINT32_MAX;
+        w_.maxTiles = (uint32_t)(cdiv(T * G, w_.rows) + std::min(R, T));
+        w_.minSteps = 4;
+        // as many as run at once (the kernels' registers)
+        const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && q.dataType != DataType::f32 ? 2 : 1;
+        // no more workers than the longest requests that the tables can name could give work to
+        const double steps = (double)w_.maxTiles * pc.Nkv * (double)cdiv((int64_t)pc.columns * pc.pageSize + w_.stepKeys, w_.stepKeys);
+        w_.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps / w_.minSteps + 1));
+    }
+    std::vector<Binding> tensors() const override {
+        return {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {out_, kWrite}};
+    }
+    std::string describe() const override { return "paged_plan," + fn_ + "," + merge_; }
+    void encode(KernelCommandEncoder &enc) const override {
+        const int64_t slots = 2 * (int64_t)w_.workers * w_.rows;
+        enc.withTemporaryTensor(ScratchSpec{{(int64_t)w_.maxTiles + 1, 4}, DataType::u32}, [&](Tensor plan) {
+            enc.withTemporaryTensor(ScratchSpec{{slots, hdp_}, DataType::f32}, [&](Tensor pO) {
+                enc.withTemporaryTensor(ScratchSpec{{slots, 2}, DataType::f32}, [&](Tensor pML) {
+                    launch(enc, "paged_plan", {{starts_, kRead}, {lens_, kRead}, {plan, kWrite}}, dim3(1, 1, 1), 1024);
+                    launch(enc, fn_,
+                           {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {plan, kRead},
+                            {pO, kWrite}, {pML, kWrite}, {out_, kWrite}},
+                           dim3(w_.workers, 1, 1), 256);
+                    launch(enc, merge_, {{starts_, kRead}, {lens_, kRead}, {plan, kRead}, {pO, kRead}, {pML, kRead}, {out_, kWrite}},
+                           dim3(w_.workers, w_.rows / 16, 1), 256);
+                });
+            });
+        });
+    }
+
+private:
+    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, dim3 grid, unsigned block) const {
+        enc.encode(*Kernels::Custom(fn, std::move(b), {bytesOf(pc_), bytesOf(w_)}, grid, dim3(block, 1, 1)));
+    }
+
+    Tensor q_, k_, v_, tables_, starts_, lens_, out_;
+    PagedAttentionConstants pc_;
+    PagedWorkConstants w_{};
+    std::string fn_, merge_;
+    int64_t hdp_ = 0;
+};
+
 }  // namespace
 
 namespace Kernels {
@@ -147,6 +221,9 @@ std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, co
     if (T * Nq >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("PagedAttention takes fewer than 2^31 query rows; got " + q.shape.str() + ".");
     const PagedAttentionConstants pc{(uint32_t)T, (uint32_t)R, (uint32_t)Nq, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page,
                                      (uint32_t)kCache.shape[0], (uint32_t)M, mask.kind, mask.window, (uint32_t)sinks, scale};
+    // 16-byte rows: the matrix cores
+    if (R && T && Hd % (16 / stride(t)) == 0 && aligned(q.data, 16) && aligned(kCache.data, 16) && aligned(vCache.data, 16) && aligned(out.data, 16))
+        return std::make_unique<PagedAttentionKernel>(q, kCache, vCache, pageTables, queryStarts, keyLens, out, pc, maxQueryLen);
     std::string fn = std::string("paged_attention_plain_") + name(t);
     const int run = 4 * stride(t);
     if (Hd % 4 || !aligned(kCache.data, run) || !aligned(vCache.data, run)) fn += "_any";
