@@ -453,11 +453,14 @@ typedef struct {
     float scale;
 } PagedAttentionConstants;
 
-/* The work of a paged attention launch, laid out by paged_plan. A request's
- * rows (token, head of a KV head's group) are cut into tiles of `rows`, a
- * tile's visible keys into steps of `stepKeys`; the (tile, KV head) units of
- * steps in a row are dealt to `workers` blocks in equal stretches of at least
- * minSteps. A launch takes the requests of fewRows < rows <= manyRows. */
+/* The work of a paged attention launch. A request's rows (token, head of a KV
+ * head's group) are cut into tiles of `rows`, a tile's visible keys into steps
+ * of `stepKeys`; the (tile, KV head) units of steps in a row are dealt to
+ * `workers` blocks in equal stretches of at least minSteps, a unit counted as
+ * unitSteps more than it has (what a unit costs beside its steps). A launch
+ * takes the requests of fewRows < rows <= manyRows. ownPlan: every block lays
+ * the tiles out by itself (at most 1024, all their steps below 2^31), else
+ * paged_plan has. */
 typedef struct {
     uint32_t rows;
     uint32_t stepKeys;
@@ -466,6 +469,8 @@ typedef struct {
     uint32_t maxTiles;
     uint32_t workers;
     uint32_t minSteps;
+    uint32_t unitSteps;
+    uint32_t ownPlan;
 } PagedWorkConstants;
 
 /* sample_*: one token of each row of logits [rows, vocab]. */

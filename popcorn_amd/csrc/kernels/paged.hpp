@@ -59,8 +59,8 @@ PAGED_FN bool paged_sees(int32_t pos, int32_t key, const PagedAttentionConstants
     return (p.maskKind == 2u) | ((key <= pos) & ((p.maskKind == 0u) | ((int64_t)pos - key < p.slidingWindow) | ((uint32_t)key < p.sinks)));
 }
 
-// The plan of a launch: entry 0 holds the steps of all tiles (of one KV head)
-// and the number of tiles, entry 1 + i tile i with the steps before it.
+// The plan of a launch: entry 0 holds the counted steps of all tiles (of one
+// KV head) and the number of tiles, entry 1 + i tile i with those before it.
 struct PagedTile {
     uint64_t before;
     uint32_t request, tile;

@@ -77,21 +77,25 @@ __device__ inline void paged_row(const pk::f32x4 (&q)[NJ], const typename T::sto
 
 // ---- the plan ----------------------------------------------------------------------
 
-constexpr uint32_t kPlanThreads = 1024;
+__device__ inline uint32_t first_lane(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ inline uint64_t first_lane64(uint64_t v) {
+    return (uint64_t)first_lane((uint32_t)(v >> 32)) << 32 | first_lane((uint32_t)v);
+}
 
 // Inclusive sum of v over the block (`sums`: one entry per wave), and the total.
-__device__ inline uint64_t block_scan(uint64_t v, uint64_t *sums, uint64_t &total) {
+template <typename U>
+__device__ inline U block_scan(U v, U *sums, U &total) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint64_t x = __shfl_up((unsigned long long)v, d);
+        const U x = __shfl_up(v, d);
         if (lane >= d) v += x;
     }
     __syncthreads();
     if (lane == 63) sums[wave] = v;
     __syncthreads();
     total = 0;
-    uint64_t before = 0;
+    U before = 0;
     for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
         if (w == wave) before = total;
         total += sums[w];
@@ -99,49 +103,65 @@ __device__ inline uint64_t block_scan(uint64_t v, uint64_t *sums, uint64_t &tota
     return before + v;
 }
 
-}  // namespace
+template <uint32_t N, typename U>
+struct PlanSpace {  // of a block of N threads
+    U sums[N / 64];
+    uint32_t tile[N];
+    pk::PagedRequest req[N];
+};
 
-// One block: the tiles of every request, in request order.
-POPCORN_KERNEL void __launch_bounds__(1024)
-    paged_plan(const int32_t *starts, const int32_t *keyLens, pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants w) {
-    __shared__ uint64_t sSums[kPlanThreads / 64];
-    __shared__ uint32_t sTile[kPlanThreads + 1];
-    __shared__ pk::PagedRequest sReq[kPlanThreads];
+// The tiles of every request, in request order: put(tile, steps before, request, tile of it).
+template <uint32_t N, typename U, typename Put>
+__device__ inline void lay_tiles(const int32_t *starts, const int32_t *keyLens, PlanSpace<N, U> &sp, const PagedAttentionConstants &p,
+                                 const PagedWorkConstants &w, U &steps, uint32_t &tiles, Put &&put) {
     const uint32_t tid = threadIdx.x, G = p.Nq / p.Nkv;
-    uint64_t steps = 0;
-    uint32_t tiles = 0;
-    for (uint32_t base = 0; base < p.R; base += kPlanThreads) {
+    steps = 0;
+    tiles = 0;
+    for (uint32_t base = 0; base < p.R; base += N) {
         const uint32_t r = base + tid;
         pk::PagedRequest q{0, 0, 0, 0};
         if (r < p.R) q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
         const uint32_t rows = (uint32_t)q.n * G;
         const uint32_t mine = rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
-        uint64_t total;
-        const uint64_t upto = block_scan(mine, sSums, total);
+        U total;
+        const U upto = block_scan((U)mine, sp.sums, total);
         // overlapping ranges of requests could hold more rows than there are: what passes the plan's room is left out
-        const uint32_t here = (uint32_t)min(total, (uint64_t)(w.maxTiles - tiles));
-        sTile[tid] = (uint32_t)min(upto - mine, (uint64_t)here);
-        sReq[tid] = q;
-        if (tid == 0) sTile[kPlanThreads] = here;
+        const uint32_t here = (uint32_t)min(total, (U)(w.maxTiles - tiles));
+        sp.tile[tid] = (uint32_t)min(upto - mine, (U)here);
+        sp.req[tid] = q;
         __syncthreads();
-        for (uint32_t t0 = 0; t0 < here; t0 += kPlanThreads) {
+        for (uint32_t t0 = 0; t0 < here; t0 += N) {
             const uint32_t t = t0 + tid;
             uint32_t i = 0, n = 0;
             if (t < here) {
 #pragma unroll
-                for (uint32_t d = kPlanThreads / 2; d; d >>= 1)
-                    if (sTile[i + d] <= t) i += d;
-                n = pk::paged_steps(sReq[i], t - sTile[i], p, w).n;
+                for (uint32_t d = N / 2; d; d >>= 1)
+                    if (sp.tile[i + d] <= t) i += d;
+                n = pk::paged_steps(sp.req[i], t - sp.tile[i], p, w).n + w.unitSteps;
             }
-            uint64_t sum;
-            const uint64_t end = block_scan(n, sSums, sum);
-            if (t < here) plan[1 + tiles + t] = pk::PagedTile{steps + end - n, base + i, t - sTile[i]};
+            U sum;
+            const U end = block_scan((U)n, sp.sums, sum);
+            if (t < here) put(tiles + t, steps + end - n, base + i, t - sp.tile[i]);
             steps += sum;
         }
         tiles += here;
         __syncthreads();
     }
-    if (tid == 0) plan[0] = pk::PagedTile{steps, tiles, 0};
+}
+
+typedef unsigned long long u64;
+
+}  // namespace
+
+POPCORN_KERNEL void __launch_bounds__(1024)
+    paged_plan(const int32_t *starts, const int32_t *keyLens, pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants w) {
+    __shared__ PlanSpace<1024, u64> space;
+    u64 steps;
+    uint32_t tiles;
+    lay_tiles<1024, u64>(starts, keyLens, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) {
+        plan[1 + at] = pk::PagedTile{before, request, tile};
+    });
+    if (threadIdx.x == 0) plan[0] = pk::PagedTile{steps, tiles, 0};
 }
 
 namespace {
@@ -167,19 +187,20 @@ __device__ inline void wait_vmcnt() {
     __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
 }
 
-__device__ inline uint32_t first_lane(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ inline uint64_t first_lane64(uint64_t v) {
-    return (uint64_t)first_lane((uint32_t)(v >> 32)) << 32 | first_lane((uint32_t)v);
-}
+// Tiles that a block lays out by itself, in LDS.
+constexpr uint32_t kOwnTiles = 1024;
+struct OwnTile {
+    uint32_t before, place;  // request << 16 | tile
+};
 
 // The tile whose units hold step x: the last with before * Nkv <= x. A wave's
 // lanes look at 64 entries at once.
-__device__ inline uint32_t find_tile(const pk::PagedTile *plan, uint32_t tiles, uint64_t x, uint32_t Nkv) {
-    const uint64_t at = x / Nkv;
+template <typename Before>
+__device__ inline uint32_t find_tile(uint32_t tiles, uint64_t at, Before &&before) {
     uint32_t lo = 0, n = tiles;
     while (n > 1) {
         const uint32_t stride = (n + 63) / 64, i = (threadIdx.x & 63) * stride;
-        const bool in = i < n && plan[1 + lo + i].before <= at;
+        const bool in = i < n && before(lo + i) <= at;
         const uint32_t last = 63 - __clzll(__ballot(in));  // lane 0's entry is always at or before x
         const uint32_t from = last * stride;
         n = min(stride, n - from);
@@ -188,29 +209,19 @@ __device__ inline uint32_t find_tile(const pk::PagedTile *plan, uint32_t tiles, 
     return first_lane(lo);
 }
 
-// A stretch of one unit's steps.
+// A stretch [lo, hi) of one unit's steps, empty where it is of the unit's extra
+// count only.
 struct Piece {
     pk::PagedRequest req;
     pk::PagedSteps steps;
     uint32_t request, hkv, lo, hi;
 };
 
-// The piece that begins at step x of all units and ends before `end`; `i` is x's tile, and moves on with x.
-__device__ inline Piece next_piece(const pk::PagedTile *plan, uint32_t &i, uint64_t &x, uint64_t end, const int32_t *starts,
-                                   const int32_t *keyLens, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
-    const pk::PagedTile t = plan[1 + i];
-    Piece c;
-    c.request = first_lane(t.request);
-    c.req = pk::paged_request(starts[c.request], starts[c.request + 1], keyLens[c.request], p);
-    c.steps = pk::paged_steps(c.req, first_lane(t.tile), p, w);
-    const uint64_t in = x - first_lane64(t.before) * p.Nkv;
-    c.hkv = (uint32_t)(in / c.steps.n);
-    c.lo = (uint32_t)(in - (uint64_t)c.hkv * c.steps.n);
-    c.hi = (uint32_t)min((uint64_t)c.steps.n, c.lo + (end - x));
-    x += c.hi - c.lo;
-    if (c.hi == c.steps.n && c.hkv + 1 == p.Nkv) ++i;
-    return c;
-}
+// What a worker's last piece leaves to the merge: nothing (pieces 0), or the
+// rows r0 .. r1 - 1 of a unit that it begins and `pieces` workers share.
+struct Shared {
+    uint32_t pieces, start, hkv, r0, r1, pad[3];
+};
 
 // The result of one row's lane of 4 dims, rounded.
 template <typename T>
@@ -232,7 +243,8 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
                           const typename T::storage *__restrict__ V, const int32_t *__restrict__ tables,
                           const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
                           const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
-                          typename T::storage *__restrict__ out, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+                          Shared *__restrict__ shared, typename T::storage *__restrict__ out, const PagedAttentionConstants &p,
+                          const PagedWorkConstants &w) {
     using S = typename T::storage;
     constexpr bool kWide = sizeof(S) == 4;
     constexpr int KM = kWide ? 1 : 2;          // 16-key groups per step
@@ -248,20 +260,67 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     constexpr int kStage = kWaves * BKV * HD * (int)sizeof(S), kMerge = kWaves * 16 * LDO * 4;
     __shared__ __attribute__((aligned(16))) uint8_t smem[kStage > kMerge ? kStage : kMerge];
     __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
+    __shared__ OwnTile sm_plan[kOwnTiles];
     __shared__ uint32_t sm_bad;
+    static_assert(sizeof(PlanSpace<64 * kWaves, uint32_t>) <= sizeof(smem), "the plan is laid out where V goes");
 
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
     const uint32_t wave = first_lane(threadIdx.x >> 6);
     const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
     const float c2 = p.scale * kLog2e;
-    const uint64_t total = plan[0].before * p.Nkv, share = pk::paged_share(total, w);
+    uint32_t tiles;
+    uint64_t total;
+    if (w.ownPlan) {
+        uint32_t steps;
+        lay_tiles<64 * kWaves, uint32_t>(starts, keyLens, *reinterpret_cast<PlanSpace<64 * kWaves, uint32_t> *>(smem), p, w, steps, tiles,
+                                         [&](uint32_t at, uint32_t before, uint32_t request, uint32_t tile) {
+                                             sm_plan[at] = OwnTile{before, request << 16 | tile};
+                                         });
+        total = (uint64_t)first_lane(steps) * p.Nkv;
+        tiles = first_lane(tiles);
+    } else {
+        total = plan[0].before * p.Nkv;
+        tiles = plan[0].request;
+    }
+    const uint64_t share = pk::paged_share(total, w);
     uint64_t x = first_lane64(blockIdx.x * share);
     const uint64_t end = first_lane64(min(x + share, total));
-    if (x >= end) return;
-    uint32_t tile = find_tile(plan, plan[0].request, x, p.Nkv);
+    if (x >= end) {
+        if (threadIdx.x == 0) shared[blockIdx.x].pieces = 0;
+        return;
+    }
+    uint32_t tile = w.ownPlan ? find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return sm_plan[i].before; })
+                              : find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
 
     while (x < end) {
-        const Piece c = next_piece(plan, tile, x, end, starts, keyLens, p, w);
+        Piece c;
+        {
+            pk::PagedTile t;
+            if (w.ownPlan) {
+                const OwnTile o = sm_plan[tile];
+                t = pk::PagedTile{first_lane(o.before), first_lane(o.place >> 16), first_lane(o.place & 0xffffu)};
+            } else {
+                t = plan[1 + tile];
+                t = pk::PagedTile{first_lane64(t.before), first_lane(t.request), first_lane(t.tile)};
+            }
+            c.request = t.request;
+            c.req = pk::paged_request(starts[t.request], starts[t.request + 1], keyLens[t.request], p);
+            c.steps = pk::paged_steps(c.req, t.tile, p, w);
+            const uint64_t in = x - t.before * p.Nkv;  // counted steps before x of this tile's units
+            const uint32_t n = c.steps.n + w.unitSteps;
+            c.hkv = (uint32_t)(in / n);
+            const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * n), hi = (uint32_t)min((uint64_t)n, lo + (end - x));
+            c.lo = max(lo, w.unitSteps) - w.unitSteps;
+            c.hi = max(hi, w.unitSteps) - w.unitSteps;
+            x += hi - lo;
+            if (hi == n && c.hkv + 1 == p.Nkv) ++tile;
+            if (x == end && threadIdx.x == 0) {
+                Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, {0, 0, 0}};
+                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = (uint32_t)((end + (n - hi) - 1) / share - blockIdx.x) + 1;
+                shared[blockIdx.x] = sh;
+            }
+            if (c.lo == c.hi) continue;
+        }
         const int32_t *table = tables + (uint64_t)c.request * p.columns;
         const uint32_t keys = (uint32_t)c.req.keys;
         auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
@@ -542,60 +601,75 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     }
 }
 
-// The units that several workers shared: the worker whose last piece begins a
-// unit and does not end it merges that unit's pieces, its own from slot 2 w + 1
-// and the following workers' from their slots 2 w'.
+// The units that several workers shared: the first one's state is in its slot
+// 2 w + 1, the following ones' in theirs 2 w'. 16 lanes take a row's dims; with
+// fewer than 16 rows, several groups of lanes share a row's pieces.
 template <typename T, int HD>
-__device__ void paged_merge(const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
-                            const pk::PagedTile *__restrict__ plan, const float *__restrict__ pO, const float *__restrict__ pML,
+__device__ void paged_merge(const float *__restrict__ pO, const float *__restrict__ pML, const Shared *__restrict__ shared,
                             typename T::storage *__restrict__ out, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
     constexpr int NJ = HD / 64;
+    __shared__ __attribute__((aligned(16))) float sO[16][HD];
+    __shared__ float sM[16], sL[16];
     const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
-    const uint64_t total = plan[0].before * p.Nkv, share = pk::paged_share(total, w);
-    const uint64_t lo = first_lane64(blockIdx.x * share), hi = first_lane64(min(lo + share, total));
-    if (lo >= hi || hi == total) return;  // (nothing goes on behind the last step)
-    uint64_t x = hi - 1;
-    uint32_t tile = find_tile(plan, plan[0].request, x, p.Nkv);
-    const Piece c = next_piece(plan, tile, x, hi, starts, keyLens, p, w);
-    const uint64_t begin = hi - 1 - c.lo, after = begin + c.steps.n;  // the unit's steps
-    if (begin < lo || after <= hi) return;
-    const uint32_t pieces = (uint32_t)((after - 1) / share - blockIdx.x) + 1;
-    const uint32_t td = threadIdx.x % 16 * 4;
-    for (uint32_t r = c.steps.r0 + blockIdx.y * 16 + threadIdx.x / 16; r < c.steps.r1; r += 16 * gridDim.y) {
-        const uint32_t in = r - c.steps.r0;
-        pk::f32x4 o[NJ];
-        float m = -INFINITY, l = 0.0f;
+    const Shared c = shared[blockIdx.x];
+    if (c.pieces == 0) return;
+    const uint32_t r0 = c.r0 + blockIdx.y * 16;
+    if (r0 >= c.r1) return;
+    const uint32_t rows = min(c.r1 - r0, 16u), each = rows <= 8 ? 16u >> (32 - __clz(rows - 1)) : 1u;  // groups per row
+    const uint32_t td = threadIdx.x % 16 * 4, group = threadIdx.x / 16, in = group / each, sub = group % each;
+    const uint32_t r = r0 + in;
+    const bool live = in < rows;
+    pk::f32x4 o[NJ];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) o[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr uint32_t U = NJ > 4 ? 2 : 4;  // pieces in flight
-        for (uint32_t i0 = 0; i0 < pieces; i0 += U) {
+    for (int j = 0; j < NJ; ++j) o[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto add = [&](float mi, float li, const pk::f32x4 (&v)[NJ]) {
+        if (mi == -INFINITY && li == 0.0f) return;  // no key seen
+        const float mn = fmaxf(m, mi);
+        const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(mi - mn);
+        l = l * a + li * b;
+        m = mn;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = o[j] * a + v[j] * b;
+    };
+    constexpr uint32_t U = NJ > 4 ? 2 : 4;  // pieces in flight
+    if (live)
+        for (uint32_t i0 = sub; i0 < c.pieces; i0 += U * each) {
             float2 ml[U];
             pk::f32x4 v[U][NJ];
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
-                const uint32_t i = min(i0 + u, pieces - 1);
-                const uint64_t row = (2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * w.rows + in;
+                const uint32_t i = min(i0 + u * each, c.pieces - 1);
+                const uint64_t row = (2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * w.rows + (r - c.r0);
                 ml[u] = *reinterpret_cast<const float2 *>(pML + 2 * row);
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
-                    if (td + 64 * j < D) v[u][j] = *reinterpret_cast<const pk::f32x4 *>(pO + row * HD + td + 64 * j);
+                for (int j = 0; j < NJ; ++j) v[u][j] = td + 64 * j < D ? *reinterpret_cast<const pk::f32x4 *>(pO + row * HD + td + 64 * j) : o[j];
             }
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u) {
-                if (i0 + u >= pieces || (ml[u].x == -INFINITY && ml[u].y == 0.0f)) continue;
-                const float mn = fmaxf(m, ml[u].x);
-                const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), b = __builtin_amdgcn_exp2f(ml[u].x - mn);
-                l = l * a + ml[u].y * b;
-                m = mn;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) o[j] = o[j] * a + v[u][j] * b;
-            }
+            for (uint32_t u = 0; u < U; ++u)
+                if (i0 + u * each < c.pieces) add(ml[u].x, ml[u].y, v[u]);
         }
-        const uint64_t row = ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G;
+    if (each > 1) {
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-            if (td + 64 * j < D) store4<T>(out + row * D + td + 64 * j, o[j], l);
+        for (int j = 0; j < NJ; ++j) *reinterpret_cast<pk::f32x4 *>(&sO[group][td + 64 * j]) = o[j];
+        if (td == 0) {
+            sM[group] = m;
+            sL[group] = l;
+        }
+        __syncthreads();
+        if (sub != 0) return;
+        for (uint32_t e = 1; e < each; ++e) {
+            pk::f32x4 v[NJ];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) v[j] = *reinterpret_cast<const pk::f32x4 *>(&sO[group + e][td + 64 * j]);
+            add(sM[group + e], sL[group + e], v);
+        }
     }
+    if (!live) return;
+    const uint64_t row = ((uint64_t)c.start + r / G) * p.Nq + c.hkv * G + r % G;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+        if (td + 64 * j < D) store4<T>(out + row * D + td + 64 * j, o[j], l);
 }
 
 // Any head dim up to 512 and any alignment: 16 rows per block, row b * 16 + i
@@ -666,15 +740,14 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
 #define PAGED_FEW(name, T, HD, RT, PER_CU)                                                                                \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                    \
         name(const T::storage *q, const T::storage *k, const T::storage *v, const int32_t *tables, const int32_t *starts, \
-             const int32_t *keyLens, const pk::PagedTile *plan, float *pO, float *pML, T::storage *out,                   \
+             const int32_t *keyLens, const pk::PagedTile *plan, float *pO, float *pML, Shared *shared, T::storage *out,   \
              PagedAttentionConstants p, PagedWorkConstants w) {                                                           \
-        paged_few<T, HD, RT>(q, k, v, tables, starts, keyLens, plan, pO, pML, out, p, w);                                 \
+        paged_few<T, HD, RT>(q, k, v, tables, starts, keyLens, plan, pO, pML, shared, out, p, w);                         \
     }
-#define PAGED_MERGE(name, T, HD)                                                                                            \
-    POPCORN_KERNEL void __launch_bounds__(256)                                                                              \
-        name(const int32_t *starts, const int32_t *keyLens, const pk::PagedTile *plan, const float *pO, const float *pML, \
-             T::storage *out, PagedAttentionConstants p, PagedWorkConstants w) {                                            \
-        paged_merge<T, HD>(starts, keyLens, plan, pO, pML, out, p, w);                                                      \
+#define PAGED_MERGE(name, T, HD)                                                                                          \
+    POPCORN_KERNEL void __launch_bounds__(256) name(const float *pO, const float *pML, const Shared *shared, T::storage *out, \
+                                                    PagedAttentionConstants p, PagedWorkConstants w) {                    \
+        paged_merge<T, HD>(pO, pML, shared, out, p, w);                                                                   \
     }
 #define PAGED_FEW_D(t, T, PER256)                                   \
     PAGED_FEW(paged_attention_few_##t##_d64_r1, T, 64, 1, 4)   \

@@ -90,28 +90,31 @@ public:
         w_.minSteps = 4;
         // as many as run at once (the kernels' registers)
         const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && q.dataType != DataType::f32 ? 2 : 1;
+        w_.unitSteps = 12;
         // no more workers than the longest requests that the tables can name could give work to
-        const double steps = (double)w_.maxTiles * pc.Nkv * (double)cdiv((int64_t)pc.columns * pc.pageSize + w_.stepKeys, w_.stepKeys);
-        w_.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps / w_.minSteps + 1));
+        const double tileSteps = (double)cdiv((int64_t)pc.columns * pc.pageSize + w_.stepKeys, w_.stepKeys) + w_.unitSteps;
+        const double steps = (double)w_.maxTiles * tileSteps;
+        w_.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc.Nkv / w_.minSteps + 1));
+        w_.ownPlan = w_.maxTiles <= 1024 && R <= 1024 && steps < 2147483648.0;
     }
     std::vector<Binding> tensors() const override {
         return {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {out_, kWrite}};
     }
-    std::string describe() const override { return "paged_plan," + fn_ + "," + merge_; }
+    std::string describe() const override { return (w_.ownPlan ? "" : "paged_plan,") + fn_ + "," + merge_; }
     void encode(KernelCommandEncoder &enc) const override {
-        const int64_t slots = 2 * (int64_t)w_.workers * w_.rows;
-        enc.withTemporaryTensor(ScratchSpec{{(int64_t)w_.maxTiles + 1, 4}, DataType::u32}, [&](Tensor plan) {
-            enc.withTemporaryTensor(ScratchSpec{{slots, hdp_}, DataType::f32}, [&](Tensor pO) {
-                enc.withTemporaryTensor(ScratchSpec{{slots, 2}, DataType::f32}, [&](Tensor pML) {
-                    launch(enc, "paged_plan", {{starts_, kRead}, {lens_, kRead}, {plan, kWrite}}, dim3(1, 1, 1), 1024);
-                    launch(enc, fn_,
-                           {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {plan, kRead},
-                            {pO, kWrite}, {pML, kWrite}, {out_, kWrite}},
-                           dim3(w_.workers, 1, 1), 256);
-                    launch(enc, merge_, {{starts_, kRead}, {lens_, kRead}, {plan, kRead}, {pO, kRead}, {pML, kRead}, {out_, kWrite}},
-                           dim3(w_.workers, w_.rows / 16, 1), 256);
-                });
-            });
+        // one buffer: the states' O, their m and l, what is shared, the plan
+        const int64_t states = 2 * (int64_t)w_.workers * w_.rows;
+        const int64_t o = states * hdp_ * 4, ml = states * 8, shared = (int64_t)w_.workers * 32;
+        const int64_t plan = w_.ownPlan ? 0 : ((int64_t)w_.maxTiles + 1) * 16;
+        enc.withTemporaryTensor(ScratchSpec{{o + ml + shared + plan}, DataType::u8}, [&](Tensor scratch) {
+            auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
+            const Tensor pO = part(0, o), pML = part(o, ml), sh = part(o + ml, shared), pl = part(o + ml + shared, plan);
+            if (!w_.ownPlan) launch(enc, "paged_plan", {{starts_, kRead}, {lens_, kRead}, {pl, kWrite}}, dim3(1, 1, 1), 1024);
+            launch(enc, fn_,
+                   {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {pl, kRead}, {pO, kWrite},
+                    {pML, kWrite}, {sh, kWrite}, {out_, kWrite}},
+                   dim3(w_.workers, 1, 1), 256);
+            launch(enc, merge_, {{pO, kRead}, {pML, kRead}, {sh, kRead}, {out_, kWrite}}, dim3(w_.workers, w_.rows / 16, 1), 256);
         });
     }
 

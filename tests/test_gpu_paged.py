@@ -368,3 +368,11 @@ def test_attention_cache_past_4_gib(env):
             x[j // page, :, j % page] = r[j]
     want, parts = R.attention(q, *small, np.array([[0, 1, 2]]), [0, 3], [40], np.zeros((3, nq, hd)), np.float32(0.088))
     assert (np.abs(download(out, stream) - want) <= R.attention_bound(want, parts, "bf16", hd)).all()
+
+
+def test_attention_many_requests(env):
+    # more tiles than a block lays out by itself
+    g = np.random.default_rng(14)
+    lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 60, 1500), g.integers(0, 3, 1500))]
+    for dtype in ("bf16", "f32"):
+        Batch(lens, 4, 2, 64, dtype, 16, seed=15, pad=2).check(env)
