@@ -130,6 +130,76 @@ private:
     int64_t hdp_ = 0;
 };
 
+// Sample (sample.hip): a row of up to SAMPLE_CANDIDATES logits by one block,
+// a longer one in slices.
+class SampleKernel : public Kernel {
+public:
+    SampleKernel(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK, const Tensor *topP,
+                 const Tensor *minP, const Tensor &tokens)
+        : logits_(logits), tokens_(tokens), type_(name(logits.dataType)) {
+        const int64_t rows = logits.shape[0], vocab = logits.shape[1];
+        options_ = {uniforms};
+        for (const Tensor *t : {temperature, topK, topP, minP}) options_.push_back(t ? *t : uniforms);  // (not read where absent)
+        sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab, 1};
+        small_ = vocab <= SAMPLE_CANDIDATES;
+        if (small_ || rows == 0) return;
+        // slices of 2048 logits or more, about 4 blocks per CU
+        const int64_t slices = std::clamp<int64_t>(cdiv(4 * deviceCUs(), rows), 1, std::min<int64_t>(SAMPLE_MAX_SLICES, cdiv(vocab, 2048)));
+        sc_.sliceLen = (uint32_t)cdiv(cdiv(vocab, slices), 8) * 8;
+        sc_.slices = (uint32_t)cdiv(vocab, sc_.sliceLen);
+        sc_.histBlocks = (uint32_t)std::clamp<int64_t>(cdiv(2 * deviceCUs(), rows), 1, sc_.slices);
+        if (rows * sc_.slices >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("Sample takes fewer rows; got " + logits.shape.str() + ".");
+    }
+    std::vector<Binding> tensors() const override {
+        std::vector<Binding> b = options({{logits_, kRead}});
+        b.push_back({tokens_, kWrite});
+        return b;
+    }
+    std::string describe() const override {
+        if (small_) return "sample_small_" + type_;
+        return "sample_top_" + type_ + (cuts() ? ",sample_hist_" + type_ : "") + ",sample_gather_" + type_ + ",sample_finish_" + type_;
+    }
+    void encode(KernelCommandEncoder &enc) const override {
+        if (sc_.rows == 0) return;
+        if (small_) {
+            std::vector<Binding> b = options({{logits_, kRead}});
+            b.push_back({tokens_, kWrite});
+            launch(enc, "sample_small_", std::move(b), sc_.rows, 1024);
+            return;
+        }
+        enc.withTemporaryTensor(ScratchSpec{{(int64_t)sc_.rows * (int64_t)sizeof(SampleRow)}, DataType::u8}, [&](Tensor rows) {
+            launch(enc, "sample_top_", {{logits_, kRead}, {rows, kWrite}}, sc_.rows * sc_.slices, 256);
+            auto with = [&](Access a) {
+                std::vector<Binding> b = options({{logits_, kRead}});
+                b.push_back({rows, (uint8_t)a});
+                return b;
+            };
+            if (cuts()) launch(enc, "sample_hist_", with(kReadWrite), sc_.rows * sc_.histBlocks, 256);
+            launch(enc, "sample_gather_", with(kReadWrite), sc_.rows * sc_.slices, 256);
+            std::vector<Binding> b = with(kRead);
+            b.push_back({tokens_, kWrite});
+            launch(enc, "sample_finish_", std::move(b), sc_.rows, 1024);
+        });
+    }
+
+private:
+    // A row may be cut: by top-k, by top-p, or by a temperature of 0.
+    bool cuts() const { return sc_.hasTemperature || sc_.hasTopK || sc_.hasTopP; }
+    std::vector<Binding> options(std::vector<Binding> b) const {
+        for (const Tensor &t : options_) b.push_back({t, kRead});
+        return b;
+    }
+    void launch(KernelCommandEncoder &enc, const char *fn, std::vector<Binding> b, uint32_t blocks, unsigned threads) const {
+        enc.encode(*Kernels::Custom(fn + type_, std::move(b), {bytesOf(sc_)}, dim3(blocks, 1, 1), dim3(threads, 1, 1)));
+    }
+
+    Tensor logits_, tokens_;
+    std::vector<Tensor> options_;
+    std::string type_;
+    SampleConstants sc_{};
+    bool small_ = false;
+};
+
 }  // namespace
 
 namespace Kernels {
@@ -250,12 +320,7 @@ std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, con
     if (topK) requireShape(*topK, D::i32, {rows}, "Sample top_k");
     if (topP) requireShape(*topP, D::f32, {rows}, "Sample top_p");
     if (minP) requireShape(*minP, D::f32, {rows}, "Sample min_p");
-    const SampleConstants sc{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr};
-    const Tensor &none = uniforms;  // bound where an option is absent, and not read
-    return fixed(std::string("sample_") + name(logits.dataType),
-                 {{logits, kRead}, {uniforms, kRead}, {temperature ? *temperature : none, kRead}, {topK ? *topK : none, kRead},
-                  {topP ? *topP : none, kRead}, {minP ? *minP : none, kRead}, {tokens, kWrite}},
-                 bytesOf(sc), dim3((unsigned)rows, 1, 1), 1024);
+    return std::make_unique<SampleKernel>(logits, uniforms, temperature, topK, topP, minP, tokens);
 }
 
 }  // namespace Kernels
