@@ -474,8 +474,7 @@ typedef struct {
 } PagedWorkConstants;
 
 /* sample_*: one token of each row of logits [rows, vocab]; a row is cut into
- * `slices` slices of `sliceLen` logits, and histograms are made by
- * `histBlocks` blocks. */
+ * `slices` slices of `sliceLen` logits. */
 typedef struct {
     uint32_t rows;
     uint32_t vocab;
@@ -485,27 +484,28 @@ typedef struct {
     uint32_t hasMinP;
     uint32_t slices;
     uint32_t sliceLen;
-    uint32_t histBlocks;
 } SampleConstants;
 
-/* What the sample_* launches hand on of one row. A logit's bin is its distance
- * from the highest in 72nds of the temperature. */
+/* What the sample_* launches hand on of one row; beside it, the weight of each
+ * slice's bins (uint64_t [rows, slices, SAMPLE_BINS]). A logit's bin is its
+ * distance from the highest in 72nds of the temperature. */
 #define SAMPLE_BINS 2048
 #define SAMPLE_CANDIDATES 4096
-#define SAMPLE_MAX_SLICES 256
+#define SAMPLE_MAX_SLICES 64
 typedef struct {
-    uint64_t weight[SAMPLE_BINS];        /* of each bin */
+    uint64_t weight[SAMPLE_BINS];          /* of each bin; of each slice where neither top-k nor top-p cuts */
     uint64_t candidate[SAMPLE_CANDIDATES]; /* rank key << 32 | ~index, of the bins where a cut may fall */
-    uint64_t sliceWeight[SAMPLE_MAX_SLICES]; /* of what is kept whatever the cut */
-    uint64_t aboveK;                     /* weight of the bins before top-k's */
-    uint64_t aboveP;                     /* weight of the bins before the first where top-p may cut */
-    uint64_t total;                      /* weight of the row */
-    uint32_t count[SAMPLE_BINS];         /* tokens of each bin */
-    uint32_t sliceTop[SAMPLE_MAX_SLICES]; /* highest rank key */
+    uint64_t aboveK;                       /* weight of the bins before top-k's */
+    uint64_t aboveP;                       /* weight of the bins before the first where top-p may cut */
+    uint64_t total;                        /* weight of the row */
+    uint32_t count[SAMPLE_BINS];           /* tokens of each bin */
+    uint32_t sliceTop[SAMPLE_MAX_SLICES];  /* highest rank key */
     uint32_t candidates;
-    uint32_t binK;                       /* top-k's bin; SAMPLE_BINS: top-k keeps all */
-    uint32_t needK;                      /* tokens of binK that top-k keeps */
-    uint32_t lastP;                      /* last bin where top-p may cut */
+    uint32_t first;                        /* first bin where top-p, or else top-k, may cut */
+    uint32_t binK;                         /* top-k's bin; SAMPLE_BINS: top-k keeps all */
+    uint32_t needK;                        /* tokens of binK that top-k keeps */
+    uint32_t lastP;                        /* last bin where top-p may cut */
+    uint32_t pad;
 } SampleRow;
 
 #ifdef __cplusplus

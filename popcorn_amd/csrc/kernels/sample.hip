@@ -7,14 +7,16 @@
 // what is kept is one cut (a logit and an index) and a least weight.
 //
 // Sorting the row is not needed to find the cut. Four launches, a row cut into slices:
-//  1. sample_top: each slice's highest logit;
-//  2. sample_hist (top-k, top-p): number and weight of the tokens in 2048
-//     bins of the distance from the highest;
+//  1. sample_top: the highest logit;
+//  2. sample_hist: number and weight of the tokens of each slice in 2048
+//     bins of the distance from the highest, and their sums over the row;
 //  3. sample_gather: the bins in which the cuts must fall, from the bins'
 //     running sums; their tokens (the candidates, a few hundred of a large
-//     vocabulary) go to a list, the weight before them is summed by slice;
+//     vocabulary) go to a list;
 //  4. sample_finish: sorts the candidates, finds the cuts among them, the
 //     slice where the running weight passes the draw, and the token in it.
+// Only the second evaluates the whole row's weights. A row that neither top-k
+// nor top-p cuts has its slices' weights summed by the third instead.
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
 // More candidates than the list holds (thousands of equal logits at the cut)
 // are counted digit by digit of their logits instead (cut_by_digits).
@@ -22,12 +24,12 @@
 
 namespace {
 
-constexpr uint32_t kSlice = 256;                        // threads of a slice's block
-constexpr uint32_t kRow = 1024, kRowWaves = kRow / 64;  // threads of a row's block
+constexpr uint32_t kThreads = 1024, kWaves = kThreads / 64;
 constexpr uint32_t E = 8;                               // consecutive logits per thread and step
 constexpr double kOne = 1099511627776.0;                // 2^40
 constexpr uint32_t kBins = SAMPLE_BINS, kList = SAMPLE_CANDIDATES;
-constexpr uint32_t kPerThread = kBins / kSlice;
+constexpr uint32_t kPerThread = kBins / kThreads;
+constexpr uint32_t kFound = 1024;                       // candidates that a block of sample_gather collects
 typedef unsigned long long u64;
 
 // A logit's place in the ranking: greater for greater logits, 0 for NaN, equal
@@ -113,232 +115,306 @@ __device__ inline u64 limit_of(float p, u64 z) {
     return max(s + more, (u64)1);
 }
 
-__device__ inline uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-    return v;
+// v of the lane that kCtrl names, 0 where there is none or kRows leaves the row out.
+template <int kCtrl, int kRows = 0xf>
+__device__ inline uint32_t moved(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, false);
 }
-__device__ inline u64 wave_sum64(u64 v) {
-#pragma unroll
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
+template <int kCtrl, int kRows = 0xf>
+__device__ inline u64 moved(u64 v) {
+    return (u64)moved<kCtrl, kRows>((uint32_t)(v >> 32)) << 32 | moved<kCtrl, kRows>((uint32_t)v);
+}
+__device__ inline uint32_t of_lane(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
+__device__ inline u64 of_lane(u64 v, uint32_t lane) { return (u64)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane); }
+
+// Inclusive sums over a row of 16 lanes, and over the wave, in registers.
+template <typename U>
+__device__ inline U row_scan(U v) {
+    v += moved<0x111>(v);  // row_shr:1, 2, 4, 8
+    v += moved<0x112>(v);
+    v += moved<0x114>(v);
+    return v + moved<0x118>(v);
+}
+template <typename U>
+__device__ inline U wave_scan(U v) {
+    v = row_scan(v);
+    v += moved<0x142, 0xa>(v);         // lane 15 of a row to the odd row behind it
+    return v + moved<0x143, 0xc>(v);   // lane 31 to the upper half
+}
+__device__ inline u64 wave_sum64(u64 v) { return of_lane(wave_scan(v), 63); }
+__device__ inline uint32_t wave_max_u32(uint32_t v) {  // (0 is the least)
+    v = max(v, moved<0x111>(v));
+    v = max(v, moved<0x112>(v));
+    v = max(v, moved<0x114>(v));
+    v = max(v, moved<0x118>(v));
+    v = max(v, moved<0x142, 0xa>(v));
+    return of_lane(max(v, moved<0x143, 0xc>(v)), 63);
 }
 
-// Inclusive sums over the block of NT threads, and the total.
-template <uint32_t NT, typename U>
-__device__ inline U block_scan(U v, U *sums, U &total) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const U x = __shfl_up(v, d);
-        if (lane >= d) v += x;
-    }
+template <typename U>
+struct Scan {
+    U upto, total;
+};
+// Inclusive sums over the block of 16 waves, and the total.
+template <typename U>
+__device__ inline Scan<U> block_scan(U v, U *sums) {
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    static_assert(kWaves == 16, "one row of lanes");
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) sums[wave] = v;
     __syncthreads();
-    U before = 0;
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < NT / 64; ++w) {
-        if (w == wave) before = total;
-        total += sums[w];
-    }
-    return before + v;
+    const U run = row_scan(sums[lane & 15]);
+    return {(wave ? of_lane(run, wave - 1) : 0) + v, of_lane(run, 15)};
 }
 
-// f(index, logit) for this thread's logits of [lo, hi), eight in a row at a time.
-template <typename T, uint32_t NT, typename F>
+// f(index, its place among the eight, logit) for this thread's logits of [lo, hi), eight in a row at a time.
+template <typename T, typename F>
 __device__ inline void each_logit(const typename T::storage *__restrict__ x, uint32_t lo, uint32_t hi, F &&f) {
     struct Eight {
         typename T::storage v[E];
     };
-    for (uint32_t i = lo + threadIdx.x * E; i < hi; i += NT * E) {
+#pragma unroll 1
+    for (uint32_t i = lo + threadIdx.x * E; i < hi; i += kThreads * E) {
         if (i + E <= hi) {
             Eight e;
             __builtin_memcpy(&e, x + i, sizeof(e));
 #pragma unroll
-            for (uint32_t j = 0; j < E; ++j) f(i + j, T::load(e.v[j]));
+            for (uint32_t j = 0; j < E; ++j) f(i + j, j, T::load(e.v[j]));
         } else {
-            for (uint32_t j = i; j < hi; ++j) f(j, T::load(x[j]));
+#pragma unroll 1
+            for (uint32_t j = i; j < hi; ++j) f(j, j - i, T::load(x[j]));
         }
     }
 }
 
-template <typename T>
-__device__ void sample_top(const typename T::storage *__restrict__ logits, SampleRow *__restrict__ rows, const SampleConstants &c) {
-    __shared__ uint32_t sTop[kSlice / 64];
-    const uint32_t r = blockIdx.x / c.slices, slice = blockIdx.x % c.slices;
-    SampleRow &row = rows[r];
-    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
-    uint32_t best = 0;
-    each_logit<T, kSlice>(logits + (uint64_t)r * c.vocab, lo, hi, [&](uint32_t, float v) { best = max(best, rank_key(v)); });
-    best = wave_max_u32(best);
-    if ((threadIdx.x & 63) == 0) sTop[threadIdx.x >> 6] = best;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (uint32_t w = 1; w < kSlice / 64; ++w) best = max(best, sTop[w]);
-        row.sliceTop[slice] = best;
-        if (slice == 0) row.candidates = 0;
-    }
-    // the next launch adds to these
-    for (uint32_t b = slice * kSlice + threadIdx.x; b < kBins; b += c.slices * kSlice) {
+// Clears what the launches after it add to.
+__device__ inline void clear_row(SampleRow &row, uint32_t at, uint32_t step) {
+    for (uint32_t b = at; b < kBins; b += step) {
         row.weight[b] = 0;
         row.count[b] = 0;
     }
+    if (at == 0) row.candidates = 0;
 }
 
-// The row's highest logit, of up to 256 slices.
-template <uint32_t NT>
-__device__ inline uint32_t top_of(const SampleRow &row, uint32_t slices, uint32_t *shared) {
-    const uint32_t best = wave_max_u32(threadIdx.x < slices ? row.sliceTop[threadIdx.x] : 0u);
-    if ((threadIdx.x & 63) == 0 && threadIdx.x < 256) shared[threadIdx.x >> 6] = best;
+template <typename T>
+__device__ void sample_top(const typename T::storage *__restrict__ logits, SampleRow *__restrict__ rows, const SampleConstants &c) {
+    __shared__ uint32_t sTop[kWaves];
+    const uint32_t r = blockIdx.x / c.slices, slice = blockIdx.x % c.slices;
+    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
+    uint32_t best = 0;
+    each_logit<T>(logits + (uint64_t)r * c.vocab, lo, hi, [&](uint32_t, uint32_t, float v) { best = max(best, rank_key(v)); });
+    best = wave_max_u32(best);
+    if ((threadIdx.x & 63) == 0) sTop[threadIdx.x >> 6] = best;
     __syncthreads();
-    return max(max(shared[0], shared[1]), max(shared[2], shared[3]));
+    if (threadIdx.x < 64) {
+        best = wave_max_u32(threadIdx.x < kWaves ? sTop[threadIdx.x] : 0u);
+        if (threadIdx.x == 0) rows[r].sliceTop[slice] = best;
+    }
+    clear_row(rows[r], slice * kThreads + threadIdx.x, c.slices * kThreads);
+}
+
+// The row's highest logit, of up to 64 slices: each wave by itself.
+__device__ inline uint32_t top_of(const SampleRow &row, uint32_t slices) {
+    const uint32_t lane = threadIdx.x & 63;
+    return wave_max_u32(lane < slices ? row.sliceTop[lane] : 0u);
 }
 
 template <typename T>
 __device__ void sample_hist(const typename T::storage *__restrict__ logits, const Options &o, SampleRow *__restrict__ rows,
-                            const SampleConstants &c) {
+                            uint64_t *__restrict__ bins, const SampleConstants &c) {
     __shared__ u64 sWeight[kBins];
-    __shared__ uint32_t sCount[kBins], sTop[4];
-    const uint32_t r = blockIdx.x / c.histBlocks, part = blockIdx.x % c.histBlocks;
+    __shared__ uint32_t sCount[kBins];
+    const uint32_t r = blockIdx.x / c.slices, slice = blockIdx.x % c.slices;
     SampleRow &row = rows[r];
-    const Row w = row_of(o, r, top_of<kSlice>(row, c.slices, sTop), c);
+    const Row w = row_of(o, r, top_of(row, c.slices), c);
     if (!w.live || !(w.useK || w.useP)) return;
-    for (uint32_t b = threadIdx.x; b < kBins; b += kSlice) {
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
         sWeight[b] = 0;
         sCount[b] = 0;
     }
     __syncthreads();
-    const uint32_t per = (c.slices + c.histBlocks - 1) / c.histBlocks * c.sliceLen;
-    const uint32_t lo = min(part * per, c.vocab), hi = min(lo + per, c.vocab);
-    each_logit<T, kSlice>(logits + (uint64_t)r * c.vocab, lo, hi, [&](uint32_t, float v) {
+    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
+    each_logit<T>(logits + (uint64_t)r * c.vocab, lo, hi, [&](uint32_t, uint32_t, float v) {
         const u64 u = w.weight(v);
         if (u == 0) return;
         const uint32_t b = w.bin(v);
-        if (w.useP) atomicAdd(&sWeight[b], u);
+        atomicAdd(&sWeight[b], u);
         if (w.useK) atomicAdd(&sCount[b], 1u);
     });
     __syncthreads();
-    for (uint32_t b = threadIdx.x; b < kBins; b += kSlice) {
+    uint64_t *mine = bins + (uint64_t)blockIdx.x * kBins;
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
+        mine[b] = sWeight[b];
         if (sWeight[b]) atomicAdd(reinterpret_cast<u64 *>(&row.weight[b]), sWeight[b]);
         if (sCount[b]) atomicAdd(&row.count[b], sCount[b]);
     }
 }
 
+// Whether min-p may cut in a bin: the last bins with weights of at least
+// `least`, one to either side for the roundings of bin and weight (a bin's
+// weights span 1.4%).
+__device__ inline bool least_bin(const Row &w, uint32_t b, float at) {
+    return (w.least != 0) & (fabsf((float)b + 0.5f - at) < 2.0f);
+}
+__device__ inline float least_at(const Row &w) {
+    return w.least ? (40.0f - __log2f((float)w.least)) * (72.0f * 0.69314718f) : 1e9f;
+}
+
 template <typename T>
 __device__ void sample_gather(const typename T::storage *__restrict__ logits, const Options &o, SampleRow *__restrict__ rows,
                               const SampleConstants &c) {
-    __shared__ u64 sSums[kSlice / 64], sAbove[2];
-    __shared__ uint32_t sCounts[kSlice / 64], sTop[4], sBin[3], sNeed;
+    __shared__ u64 sSums[kWaves], sAbove[2], sWith, sList[kFound];
+    __shared__ uint32_t sCounts[kWaves], sBin[3], sNeed, sFound, sBase;
     const uint32_t r = blockIdx.x / c.slices, slice = blockIdx.x % c.slices;
     SampleRow &row = rows[r];
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
-    const Row w = row_of(o, r, top_of<kSlice>(row, c.slices, sTop), c);
+    const uint32_t tid = threadIdx.x;
+    const Row w = row_of(o, r, top_of(row, c.slices), c);
     if (!w.live) return;
+    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
+    const typename T::storage *x = logits + (uint64_t)r * c.vocab;
+    if (!(w.useK || w.useP)) {
+        u64 sum = 0;
+        each_logit<T>(x, lo, hi, [&](uint32_t, uint32_t, float v) {
+            const u64 u = w.weight(v);
+            sum += u >= w.least ? u : 0;
+        });
+        sum = block_scan(sum, sSums).total;
+        if (tid == 0) row.weight[slice] = sum;
+        return;
+    }
     // bins before `first` are kept; candidates are the bins first .. lastP and binK
-    uint32_t first = kBins, lastP = 0, binK = kBins;
-    if (w.useK || w.useP) {
-        u64 bw[kPerThread], mine = 0, total;
-        uint32_t bc[kPerThread], here = 0, counted;
+    u64 bw[kPerThread], mine = 0;
+    uint32_t bc[kPerThread], here = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kPerThread; ++j) {
+        bw[j] = row.weight[tid * kPerThread + j];
+        bc[j] = row.count[tid * kPerThread + j];
+        mine += bw[j];
+        here += bc[j];
+    }
+    const Scan<u64> weights = block_scan(mine, sSums);
+    const u64 wend = weights.upto, total = weights.total;
+    const uint32_t cend = block_scan(here, sCounts).upto;
+    if (tid == 0) {
+        sFound = 0;
+        sBin[0] = sBin[1] = sBin[2] = kBins;
+        sAbove[0] = sAbove[1] = 0;
+        sNeed = 0;
+    }
+    __syncthreads();
+    // calls at(bin, weight before it, with it, tokens before it) for the one bin of this thread's that `in` names
+    auto find = [&](auto &&in, auto &&at) {
+        u64 before = wend - mine;
+        uint32_t cb = cend - here;
 #pragma unroll
         for (uint32_t j = 0; j < kPerThread; ++j) {
-            bw[j] = row.weight[tid * kPerThread + j];
-            bc[j] = row.count[tid * kPerThread + j];
-            mine += bw[j];
-            here += bc[j];
+            if (in(before, before + bw[j], cb, cb + bc[j])) at(tid * kPerThread + j, before, before + bw[j], cb);
+            before += bw[j];
+            cb += bc[j];
         }
-        const u64 wend = block_scan<kSlice>(mine, sSums, total);
-        const uint32_t cend = block_scan<kSlice>(here, sCounts, counted);
-        if (tid == 0) {
-            sBin[0] = sBin[1] = sBin[2] = kBins;
-            sAbove[0] = sAbove[1] = 0;
-            sNeed = 0;
-        }
+    };
+    u64 zLo = total, zHi = total;
+    uint32_t first, lastP, binK = kBins;
+    if (w.useK) {
+        find([&](u64, u64, uint32_t a, uint32_t b) { return a < w.k && w.k <= b; },
+             [&](uint32_t b, u64 before, u64 with, uint32_t cb) {
+                 sBin[0] = b;
+                 sAbove[0] = before;
+                 sWith = with;
+                 sNeed = w.k - cb;
+             });
         __syncthreads();
-        // calls at(bin, weight before it) for the one bin of this thread's that `in(before, with)` names
-        auto find = [&](auto &&in, auto &&at) {
-            u64 before = wend - mine;
-            uint32_t cb = cend - here;
-#pragma unroll
-            for (uint32_t j = 0; j < kPerThread; ++j) {
-                if (in(before, before + bw[j], cb, cb + bc[j])) at(tid * kPerThread + j, before, cb);
-                before += bw[j];
-                cb += bc[j];
-            }
-        };
-        u64 zLo = total, zHi = total;
-        if (w.useK) {
-            find([&](u64, u64, uint32_t a, uint32_t b) { return a < w.k && w.k <= b; },
-                 [&](uint32_t b, u64 before, uint32_t cb) {
-                     sBin[0] = b;
-                     sAbove[0] = before;
-                     sNeed = w.k - cb;
-                 });
-            __syncthreads();
-            binK = sBin[0];
-            if (binK < kBins) {
-                zLo = sAbove[0];
-                zHi = zLo + row.weight[binK];
-            }
-        }
-        if (w.useP) {
-            // top-p's share is of a weight between zLo and zHi
-            const u64 lo = limit_of(w.p, zLo), hi = limit_of(w.p, zHi);
-            find([&](u64 a, u64 b, uint32_t, uint32_t) { return a < lo && lo <= b; },
-                 [&](uint32_t b, u64 before, uint32_t) {
-                     sBin[1] = b;
-                     sAbove[1] = before;
-                 });
-            find([&](u64 a, u64 b, uint32_t, uint32_t) { return a < hi && hi <= b; }, [&](uint32_t b, u64, uint32_t) { sBin[2] = b; });
-            __syncthreads();
-            first = sBin[1];
-            lastP = sBin[2];
-        } else {
-            first = lastP = binK;
-        }
-        if (slice == 0 && tid == 0) {
-            row.binK = binK;
-            row.needK = sNeed;
-            row.aboveK = sAbove[0];
-            row.aboveP = sAbove[1];
-            row.total = total;
-            row.lastP = lastP;
+        binK = sBin[0];
+        if (binK < kBins) {
+            zLo = sAbove[0];
+            zHi = sWith;
         }
     }
-    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
-    u64 sum = 0;
-    each_logit<T, kSlice>(logits + (uint64_t)r * c.vocab, lo, hi, [&](uint32_t i, float v) {
-        const u64 u = w.weight(v);
-        if (u == 0) return;
-        const uint32_t b = first < kBins ? w.bin(v) : 0u;
-        if (b < first) {
-            sum += u >= w.least ? u : 0;
-        } else if (b <= lastP || b == binK) {
-            const uint32_t at = atomicAdd(&row.candidates, 1u);
-            if (at < kList) row.candidate[at] = (u64)rank_key(v) << 32 | (uint32_t)~i;
+    if (w.useP) {
+        // top-p's share is of a weight between zLo and zHi
+        const u64 a0 = limit_of(w.p, zLo), a1 = limit_of(w.p, zHi);
+        find([&](u64 a, u64 b, uint32_t, uint32_t) { return a < a0 && a0 <= b; },
+             [&](uint32_t b, u64 before, u64, uint32_t) {
+                 sBin[1] = b;
+                 sAbove[1] = before;
+             });
+        find([&](u64 a, u64 b, uint32_t, uint32_t) { return a < a1 && a1 <= b; }, [&](uint32_t b, u64, u64, uint32_t) { sBin[2] = b; });
+        __syncthreads();
+        first = sBin[1];
+        lastP = sBin[2];
+    } else {
+        first = lastP = binK;
+    }
+    if (slice == 0 && tid == 0) {
+        row.first = first;
+        row.binK = binK;
+        row.needK = sNeed;
+        row.aboveK = sAbove[0];
+        row.aboveP = sAbove[1];
+        row.total = total;
+        row.lastP = lastP;
+    }
+    const float at = least_at(w);
+    auto put = [&](uint32_t slot, u64 v) {
+        if (slot < kList) row.candidate[slot] = v;
+    };
+    uint32_t found = 0;  // of a thread's eight, a bit each
+    auto collect = [&](uint32_t i0) {
+#pragma unroll 1
+        for (; found; found &= found - 1) {
+            const uint32_t i = i0 + (uint32_t)__ffs((int)found) - 1;
+            const u64 c = (u64)rank_key(T::load(x[i])) << 32 | (uint32_t)~i;
+            const uint32_t n = atomicAdd(&sFound, 1u);
+            if (n < kFound) sList[n] = c;
+            else put(atomicAdd(&row.candidates, 1u), c);
         }
+    };
+    each_logit<T>(x, lo, hi, [&](uint32_t i, uint32_t j, float v) {
+        const uint32_t b = w.bin(v);
+        if ((v > -INFINITY) & (b < first ? least_bin(w, b, at) : (b <= lastP) | (b == binK))) found |= 1u << j;
+        if (j == E - 1 || i + 1 == hi) collect(i - j);
     });
-    sum = wave_sum64(sum);
     __syncthreads();
-    if (lane == 0) sSums[tid >> 6] = sum;
+    // the row's counter is one address for all its blocks: one addition each
+    const uint32_t n = min(sFound, kFound);
+    if (tid == 0) sBase = n ? atomicAdd(&row.candidates, n) : 0;
     __syncthreads();
-    if (tid == 0) row.sliceWeight[slice] = sSums[0] + sSums[1] + sSums[2] + sSums[3];
+    for (uint32_t i = tid; i < n; i += kThreads) put(sBase + i, sList[i]);
 }
 
 struct RowSpace {
     u64 list[kList];
-    u64 sums[kRowWaves], slice[SAMPLE_MAX_SLICES], pick;
-    uint32_t counts[kRowWaves], hist[256], bin;
-    u64 weights[256];
+    u64 sums[kWaves], slice[SAMPLE_MAX_SLICES], pick;
+    u64 weights[kList];
+    uint32_t counts[kWaves], ranks[256], bin;
 };
 
-// Sorts list[0, n), n a power of two, from the greatest.
-__device__ inline void sort_list(u64 *list, uint32_t n) {
+// Sorts list[0, n) from the greatest, by each entry's number of greater ones: n at most 256, all entries distinct.
+__device__ inline void rank_list(RowSpace &s, uint32_t n) {
+    const uint32_t e = threadIdx.x & 255, part = threadIdx.x >> 8;
+    if (threadIdx.x < 256) s.ranks[e] = 0;
+    __syncthreads();
+    u64 mine = 0;
+    if (e < n) {
+        mine = s.list[e];
+        uint32_t greater = 0;
+#pragma unroll 4
+        for (uint32_t j = part; j < n; j += 4) greater += s.list[j] > mine;
+        atomicAdd(&s.ranks[e], greater);
+    }
+    __syncthreads();
+    if (part == 0 && e < n) s.list[s.ranks[e]] = mine;
+    __syncthreads();
+}
+
+// The same for n a power of two of at least 128, by merging. Pairs up to 64
+// apart stay within the 128 entries of one wave, whose LDS accesses are in order.
+__device__ inline void merge_list(u64 *list, uint32_t n) {
+    __syncthreads();
     for (uint32_t size = 2; size <= n; size <<= 1)
         for (uint32_t d = size >> 1; d; d >>= 1) {
-            __syncthreads();
-            for (uint32_t t = threadIdx.x; t < n / 2; t += kRow) {
+            for (uint32_t t = threadIdx.x; t < n / 2; t += kThreads) {
                 const uint32_t i = 2 * t - (t & (d - 1)), j = i + d;
                 const u64 a = list[i], b = list[j];
                 if ((a < b) == ((i & size) == 0)) {
@@ -346,59 +422,56 @@ __device__ inline void sort_list(u64 *list, uint32_t n) {
                     list[j] = a;
                 }
             }
+            if (d > 64 || (d == 1 && size >= 128)) __syncthreads();
+            else asm volatile("" ::: "memory");
         }
     __syncthreads();
 }
 
 // The last token that top-k and top-p keep, of n candidates in the list (in any order): rank key << 32 | ~index.
-__device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_t binK, uint32_t needK, uint32_t lastP, u64 aboveK,
-                                  u64 aboveP, u64 total) {
+// (Tokens of bins before `first` are in the list for min-p's sake, and kept.)
+__device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_t first, uint32_t binK, uint32_t needK, uint32_t lastP,
+                                  u64 aboveK, u64 aboveP, u64 total) {
     const uint32_t tid = threadIdx.x;
-    uint32_t n2 = 64;
-    while (n2 < n) n2 <<= 1;
-    for (uint32_t i = n + tid; i < n2; i += kRow) s.list[i] = 0;
-    sort_list(s.list, n2);
-    constexpr uint32_t P = kList / kRow;  // a thread's candidates, in a row
-    const uint32_t per = (n2 + kRow - 1) / kRow;
-    u64 u[P], mine = 0, all;
-    uint32_t b[P], before = 0, beforeK;
-#pragma unroll
-    for (uint32_t j = 0; j < P; ++j) {
-        const uint32_t i = tid * per + j;
-        const bool in = j < per && i < n;
-        const float v = in ? key_value((uint32_t)(s.list[i] >> 32)) : 0.0f;
-        u[j] = in ? w.weight(v) : 0;
-        b[j] = in ? w.bin(v) : kBins;
-        before += in && b[j] < binK;
+    uint32_t n2 = 256;
+    if (n <= n2) {
+        rank_list(s, n);
+    } else {
+        while (n2 < n) n2 <<= 1;
+        for (uint32_t i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
+        merge_list(s.list, n2);
     }
-    uint32_t kept = n;
+    const uint32_t per = (n2 + kThreads - 1) / kThreads, lo = tid * per, hi = min(lo + per, n);  // a thread's candidates
+    auto value = [&](uint32_t i) { return key_value((uint32_t)(s.list[i] >> 32)); };
+    uint32_t before = 0, kept = n;
+#pragma unroll 1
+    for (uint32_t i = lo; i < hi; ++i) {
+        s.weights[i] = w.weight(value(i));
+        before += w.bin(value(i)) < binK;
+    }
     if (binK < kBins) {
-        (void)block_scan<kRow>(before, s.counts, beforeK);
+        const uint32_t beforeK = block_scan(before, s.counts).total;
         kept = min(n, beforeK + needK);
         u64 part = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < P; ++j) {
-            const uint32_t i = tid * per + j;
-            if (j < per && i >= beforeK && i < kept) part += u[j];
-            if (i >= kept) u[j] = 0;
-        }
-        (void)block_scan<kRow>(part, s.sums, total);
-        total += aboveK;
+#pragma unroll 1
+        for (uint32_t i = max(lo, beforeK); i < min(hi, kept); ++i) part += s.weights[i];
+        total = aboveK + block_scan(part, s.sums).total;
     }
     if (w.useP) {
         const u64 limit = limit_of(w.p, total);
-#pragma unroll
-        for (uint32_t j = 0; j < P; ++j) mine += u[j];
-        u64 run = aboveP + block_scan<kRow>(mine, s.sums, all) - mine;
-        uint32_t keep = 0, sum;
-#pragma unroll
-        for (uint32_t j = 0; j < P; ++j) {
-            const uint32_t i = tid * per + j;
-            keep += j < per && i < kept && b[j] <= lastP && run < limit;
-            run += u[j];
+        const uint32_t end = min(hi, kept);
+        u64 mine = 0;
+#pragma unroll 1
+        for (uint32_t i = lo; i < end; ++i) mine += w.bin(value(i)) < first ? 0 : s.weights[i];
+        u64 run = aboveP + block_scan(mine, s.sums).upto - mine;
+        uint32_t keep = 0;
+#pragma unroll 1
+        for (uint32_t i = lo; i < end; ++i) {
+            const uint32_t b = w.bin(value(i));
+            keep += b < first || (b <= lastP && run < limit);
+            run += b < first ? 0 : s.weights[i];
         }
-        (void)block_scan<kRow>(keep, s.counts, sum);
-        kept = sum;
+        kept = block_scan(keep, s.counts).total;
     }
     __syncthreads();
     return kept ? s.list[kept - 1] : 0;
@@ -418,15 +491,14 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (tid < 256) s.weights[tid] = 0;
             __syncthreads();
-            each_logit<T, kRow>(x, 0, n, [&](uint32_t i, float v) {
+            each_logit<T>(x, 0, n, [&](uint32_t i, uint32_t, float v) {
                 const uint32_t key = rank_key(v);
                 if (shift < 24 && (key >> (shift + 8)) != prefix) return;
                 if (rank(v, i) >= cut) atomicAdd(&s.weights[(key >> shift) & 255u], measure(v));
             });
             __syncthreads();
             // thread t takes digit 255 - t
-            u64 all;
-            const u64 mine = tid < 256 ? s.weights[255 - tid] : 0, run = block_scan<kRow>(mine, s.sums, all);
+            const u64 mine = tid < 256 ? s.weights[255 - tid] : 0, run = block_scan(mine, s.sums).upto;
             if (run - mine < want && want <= run) {
                 s.bin = 255 - tid;
                 s.pick = run - mine;
@@ -437,14 +509,14 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
         }
         // equal logits measure the same: the nth of them in index order
         const u64 each = measure(key_value(prefix)), nth = each ? (want + each - 1) / each : 1;
-        const uint32_t lo = (uint32_t)((uint64_t)n * wave / kRowWaves), hi = (uint32_t)((uint64_t)n * (wave + 1) / kRowWaves);
+        const uint32_t lo = (uint32_t)((uint64_t)n * wave / kWaves), hi = (uint32_t)((uint64_t)n * (wave + 1) / kWaves);
         auto tie = [&](uint32_t i) {
             const float v = T::load(x[min(i, n - 1)]);
             return i < hi && rank_key(v) == prefix && rank(v, i) >= cut;
         };
-        u64 count = 0, all;
+        u64 count = 0;
         for (uint32_t i0 = lo; i0 < hi; i0 += 64) count += __popcll(__ballot(tie(i0 + lane)));
-        u64 before = block_scan<kRow>(lane == 0 ? count : 0, s.sums, all) - count;  // the same in the wave's lanes
+        u64 before = block_scan(lane == 0 ? count : 0, s.sums).upto - count;  // the same in the wave's lanes
         if (before < nth && nth <= before + count) {
             for (uint32_t i0 = lo; i0 < hi; i0 += 64) {
                 const u64 ties = __ballot(tie(i0 + lane)), here = __popcll(ties);
@@ -461,10 +533,9 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
     };
     if (w.useK) move(w.k, [](float) { return (u64)1; });
     if (w.useP) {
-        u64 z = 0, total;
-        each_logit<T, kRow>(x, 0, n, [&](uint32_t i, float v) { z += rank(v, i) >= cut ? w.weight(v) : 0; });
-        (void)block_scan<kRow>(z, s.sums, total);
-        move(limit_of(w.p, total), [&](float v) { return w.weight(v); });
+        u64 z = 0;
+        each_logit<T>(x, 0, n, [&](uint32_t i, uint32_t, float v) { z += rank(v, i) >= cut ? w.weight(v) : 0; });
+        move(limit_of(w.p, block_scan(z, s.sums).total), [&](float v) { return w.weight(v); });
     }
     return cut;
 }
@@ -473,30 +544,38 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
 template <typename T>
 __device__ inline void find_token(RowSpace &s, const typename T::storage *__restrict__ x, const Row &w, u64 cut, uint32_t lo, uint32_t hi,
                                   u64 before, u64 target, int32_t *token) {
-    for (uint32_t i0 = lo; i0 < hi; i0 += kRow * E) {
-        u64 u[E], mine = 0, all;
-#pragma unroll
-        for (uint32_t j = 0; j < E; ++j) u[j] = 0;
+    for (uint32_t i0 = lo; i0 < hi; i0 += kThreads * E) {
         const uint32_t from = i0 + threadIdx.x * E;
+        struct Eight {
+            typename T::storage v[E];
+        } e;
+        if (from + E <= hi) {
+            __builtin_memcpy(&e, x + from, sizeof(e));
+        } else {
 #pragma unroll
-        for (uint32_t j = 0; j < E; ++j)
-            if (from + j < hi) {
-                const float v = T::load(x[from + j]);
-                const u64 m = w.weight(v);
-                u[j] = m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~(from + j)) >= cut ? m : 0;
-                mine += u[j];
-            }
-        u64 run = before + block_scan<kRow>(mine, s.sums, all) - mine;
+            for (uint32_t j = 0; j < E; ++j) e.v[j] = x[min(from + j, hi - 1)];
+        }
+        u64 u[E], mine = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < E; ++j) {
+            const float v = T::load(e.v[j]);
+            const u64 m = w.weight(v);
+            const bool in = (from + j < hi) & (m >= w.least) & (((u64)rank_key(v) << 32 | (uint32_t)~(from + j)) >= cut);
+            u[j] = in ? m : 0;
+            mine += u[j];
+        }
+        const Scan<u64> scan = block_scan(mine, s.sums);
+        u64 run = before + scan.upto - mine;
         if (run <= target && target < run + mine) {
+            uint32_t at = 0;
+#pragma unroll
             for (uint32_t j = 0; j < E; ++j) {
                 run += u[j];
-                if (run > target) {
-                    *token = (int32_t)(from + j);
-                    break;
-                }
+                at += run <= target;
             }
+            *token = (int32_t)(from + at);
         }
-        before += all;
+        before += scan.total;
         if (before > target) return;  // (the same in every thread)
     }
 }
@@ -507,46 +586,70 @@ __device__ inline u64 target_of(float u, u64 z) {
 }
 
 template <typename T>
+__device__ __attribute__((noinline)) void finish_by_digits(RowSpace &s, const typename T::storage *__restrict__ x, Row w, uint32_t n, float u,
+                                                           int32_t *token) {
+    const u64 cut = cut_by_digits<T>(s, x, w, n);
+    u64 z = 0;
+    each_logit<T>(x, 0, n, [&](uint32_t i, uint32_t, float v) {
+        const u64 m = w.weight(v);
+        z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
+    });
+    find_token<T>(s, x, w, cut, 0, n, 0, target_of(u, block_scan(z, s.sums).total), token);
+}
+
+template <typename T>
 __device__ void sample_finish(const typename T::storage *__restrict__ logits, const Options &o, const SampleRow *__restrict__ rows,
-                              int32_t *__restrict__ tokens, const SampleConstants &c) {
+                              const uint64_t *__restrict__ bins, int32_t *__restrict__ tokens, const SampleConstants &c) {
     __shared__ RowSpace s;
-    __shared__ uint32_t sTop[4];
-    const uint32_t r = blockIdx.x, tid = threadIdx.x;
+    const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const SampleRow &row = rows[r];
     const typename T::storage *x = logits + (uint64_t)r * c.vocab;
-    const Row w = row_of(o, r, top_of<kRow>(row, c.slices, sTop), c);
+    const Row w = row_of(o, r, top_of(row, c.slices), c);
     if (!w.live) {
         if (tid == 0) tokens[r] = -1;
         return;
     }
-    if (tid < c.slices) s.slice[tid] = row.sliceWeight[tid];
     u64 cut = 0;
-    if ((w.useK || w.useP) && row.candidates > kList) {
-        cut = cut_by_digits<T>(s, x, w, c.vocab);
-        u64 z = 0, all;
-        each_logit<T, kRow>(x, 0, c.vocab, [&](uint32_t i, float v) {
-            const u64 m = w.weight(v);
-            z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
-        });
-        (void)block_scan<kRow>(z, s.sums, all);
-        find_token<T>(s, x, w, cut, 0, c.vocab, 0, target_of(o.uniforms[r], all), tokens + r);
+    const bool cuts = w.useK || w.useP;
+    if (cuts && row.candidates > kList) {
+        finish_by_digits<T>(s, x, w, c.vocab, o.uniforms[r], tokens + r);
         return;
     }
-    if (w.useK || w.useP) {
-        const uint32_t n = row.candidates;
-        for (uint32_t i = tid; i < n; i += kRow) s.list[i] = row.candidate[i];
+    if (cuts) {
+        const uint32_t n = row.candidates, first = row.first;
+        for (uint32_t i = tid; i < n; i += kThreads) s.list[i] = row.candidate[i];
+        // each slice's weight of the bins that are kept whatever the cuts
+        const float at = least_at(w);
+        for (uint32_t sl = wave; sl < c.slices; sl += kWaves) {
+            const uint64_t *b = bins + ((uint64_t)r * c.slices + sl) * kBins;
+            u64 sum = 0;
+            for (uint32_t i0 = lane; i0 < first; i0 += 512) {
+                u64 v[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) v[j] = b[min(i0 + 64 * j, kBins - 1)];
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) {
+                    const uint32_t i = i0 + 64 * j;
+                    if (i < first && !least_bin(w, i, at) && (float)i < at) sum += v[j];
+                }
+            }
+            sum = wave_sum64(sum);
+            if (lane == 0) s.slice[sl] = sum;
+        }
         __syncthreads();
-        cut = cut_in_list(s, w, n, row.binK, row.needK, row.lastP, row.aboveK, row.aboveP, row.total);
-        for (uint32_t i = tid; i < n; i += kRow)
+        cut = cut_in_list(s, w, n, first, row.binK, row.needK, row.lastP, row.aboveK, row.aboveP, row.total);
+        for (uint32_t i = tid; i < n; i += kThreads)
             if (s.list[i] >= cut) {
                 const u64 m = w.weight(key_value((uint32_t)(s.list[i] >> 32)));
                 if (m >= w.least) atomicAdd(&s.slice[~(uint32_t)s.list[i] / c.sliceLen], m);
             }
+    } else if (tid < c.slices) {
+        s.slice[tid] = row.weight[tid];
     }
     __syncthreads();
-    u64 z;
-    const u64 mine = tid < c.slices ? s.slice[tid] : 0, run = block_scan<kRow>(mine, s.sums, z);
-    const u64 target = target_of(o.uniforms[r], z);
+    const u64 mine = tid < c.slices ? s.slice[tid] : 0;
+    const Scan<u64> scan = block_scan(mine, s.sums);
+    const u64 run = scan.upto, target = target_of(o.uniforms[r], scan.total);
     if (run - mine <= target && target < run) {
         s.bin = tid;
         s.pick = run - mine;
@@ -563,7 +666,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
     const uint32_t r = blockIdx.x, tid = threadIdx.x, n = c.vocab;
     const typename T::storage *x = logits + (uint64_t)r * n;
     uint32_t best = 0;
-    for (uint32_t i = tid; i < n; i += kRow) {
+    for (uint32_t i = tid; i < n; i += kThreads) {
         const uint32_t key = rank_key(T::load(x[i]));
         s.list[i] = (u64)key << 32 | (uint32_t)~i;
         best = max(best, key);
@@ -571,56 +674,52 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
     best = wave_max_u32(best);
     if ((tid & 63) == 0) s.counts[tid >> 6] = best;
     __syncthreads();
-    for (uint32_t v = 0; v < kRowWaves; ++v) best = max(best, s.counts[v]);
+    for (uint32_t v = 0; v < kWaves; ++v) best = max(best, s.counts[v]);
     __syncthreads();
     const Row w = row_of(o, r, best, c);
     if (!w.live) {
         if (tid == 0) tokens[r] = -1;
         return;
     }
-    u64 cut = 0, z = 0, all;
+    u64 cut = 0, z = 0;
     if (w.useK || w.useP) {
-        u64 total = 0;
-        for (uint32_t i = tid; i < n; i += kRow) z += w.weight(T::load(x[i]));
-        (void)block_scan<kRow>(z, s.sums, total);
+        for (uint32_t i = tid; i < n; i += kThreads) z += w.weight(T::load(x[i]));
         // every token a candidate: top-k's bin is then the one that nothing lies before
-        cut = cut_in_list(s, w, n, w.useK ? 0u : kBins, w.k, kBins, 0, 0, total);
+        cut = cut_in_list(s, w, n, 0, w.useK ? 0u : kBins, w.k, kBins, 0, 0, block_scan(z, s.sums).total);
         z = 0;
     }
-    for (uint32_t i = tid; i < n; i += kRow) {
+    for (uint32_t i = tid; i < n; i += kThreads) {
         const float v = T::load(x[i]);
         const u64 m = w.weight(v);
         z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
     }
-    (void)block_scan<kRow>(z, s.sums, all);
-    find_token<T>(s, x, w, cut, 0, n, 0, target_of(o.uniforms[r], all), tokens + r);
+    find_token<T>(s, x, w, cut, 0, n, 0, target_of(o.uniforms[r], block_scan(z, s.sums).total), tokens + r);
 }
 
 }  // namespace
 
-#define SAMPLE(t, T)                                                                                                              \
-    POPCORN_KERNEL void __launch_bounds__(256) sample_top_##t(const T::storage *logits, SampleRow *rows, SampleConstants c) {     \
-        sample_top<T>(logits, rows, c);                                                                                           \
-    }                                                                                                                             \
-    POPCORN_KERNEL void __launch_bounds__(256)                                                                                    \
-        sample_hist_##t(const T::storage *logits, const float *uniforms, const float *temperature, const int32_t *topK,           \
-                        const float *topP, const float *minP, SampleRow *rows, SampleConstants c) {                               \
-        sample_hist<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, c);                                        \
-    }                                                                                                                             \
-    POPCORN_KERNEL void __launch_bounds__(256)                                                                                    \
-        sample_gather_##t(const T::storage *logits, const float *uniforms, const float *temperature, const int32_t *topK,         \
-                          const float *topP, const float *minP, SampleRow *rows, SampleConstants c) {                             \
-        sample_gather<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, c);                                      \
-    }                                                                                                                             \
-    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                   \
-        sample_finish_##t(const T::storage *logits, const float *uniforms, const float *temperature, const int32_t *topK,         \
-                          const float *topP, const float *minP, const SampleRow *rows, int32_t *tokens, SampleConstants c) {      \
-        sample_finish<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, tokens, c);                              \
-    }                                                                                                                             \
-    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                   \
-        sample_small_##t(const T::storage *logits, const float *uniforms, const float *temperature, const int32_t *topK,          \
-                         const float *topP, const float *minP, int32_t *tokens, SampleConstants c) {                              \
-        sample_small<T>(logits, Options{uniforms, temperature, topK, topP, minP}, tokens, c);                                     \
+#define SAMPLE_OPTIONS const float *uniforms, const float *temperature, const int32_t *topK, const float *topP, const float *minP
+#define SAMPLE(t, T)                                                                                                           \
+    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                 \
+        sample_top_##t(const T::storage *logits, SampleRow *rows, SampleConstants c) {                         \
+        sample_top<T>(logits, rows, c);                                                                                  \
+    }                                                                                                                          \
+    POPCORN_KERNEL void __launch_bounds__(1024) sample_hist_##t(const T::storage *logits, SAMPLE_OPTIONS, \
+                                                                SampleRow *rows, uint64_t *bins, SampleConstants c) {          \
+        sample_hist<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, c);                         \
+    }                                                                                                                          \
+    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                 \
+        sample_gather_##t(const T::storage *logits, SAMPLE_OPTIONS, SampleRow *rows, SampleConstants c) { \
+        sample_gather<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, c);                             \
+    }                                                                                                                          \
+    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                \
+        sample_finish_##t(const T::storage *logits, SAMPLE_OPTIONS, const SampleRow *rows,               \
+                          const uint64_t *bins, int32_t *tokens, SampleConstants c) {                                          \
+        sample_finish<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, tokens, c);               \
+    }                                                                                                                          \
+    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                \
+        sample_small_##t(const T::storage *logits, SAMPLE_OPTIONS, int32_t *tokens, SampleConstants c) {                       \
+        sample_small<T>(logits, Options{uniforms, temperature, topK, topP, minP}, tokens, c);                                  \
     }
 
 SAMPLE(f32, pk::F32)

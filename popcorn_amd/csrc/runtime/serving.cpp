@@ -140,14 +140,13 @@ public:
         const int64_t rows = logits.shape[0], vocab = logits.shape[1];
         options_ = {uniforms};
         for (const Tensor *t : {temperature, topK, topP, minP}) options_.push_back(t ? *t : uniforms);  // (not read where absent)
-        sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab, 1};
+        sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab};
         small_ = vocab <= SAMPLE_CANDIDATES;
         if (small_ || rows == 0) return;
-        // slices of 2048 logits or more, about 4 blocks per CU
-        const int64_t slices = std::clamp<int64_t>(cdiv(4 * deviceCUs(), rows), 1, std::min<int64_t>(SAMPLE_MAX_SLICES, cdiv(vocab, 2048)));
+        // slices of 8192 logits or more, about 4 blocks per CU
+        const int64_t slices = std::clamp<int64_t>(cdiv(4 * deviceCUs(), rows), 1, std::min<int64_t>(SAMPLE_MAX_SLICES, cdiv(vocab, 8192)));
         sc_.sliceLen = (uint32_t)cdiv(cdiv(vocab, slices), 8) * 8;
         sc_.slices = (uint32_t)cdiv(vocab, sc_.sliceLen);
-        sc_.histBlocks = (uint32_t)std::clamp<int64_t>(cdiv(2 * deviceCUs(), rows), 1, sc_.slices);
         if (rows * sc_.slices >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("Sample takes fewer rows; got " + logits.shape.str() + ".");
     }
     std::vector<Binding> tensors() const override {
@@ -164,21 +163,22 @@ public:
         if (small_) {
             std::vector<Binding> b = options({{logits_, kRead}});
             b.push_back({tokens_, kWrite});
-            launch(enc, "sample_small_", std::move(b), sc_.rows, 1024);
+            launch(enc, "sample_small_", std::move(b), sc_.rows);
             return;
         }
-        enc.withTemporaryTensor(ScratchSpec{{(int64_t)sc_.rows * (int64_t)sizeof(SampleRow)}, DataType::u8}, [&](Tensor rows) {
-            launch(enc, "sample_top_", {{logits_, kRead}, {rows, kWrite}}, sc_.rows * sc_.slices, 256);
-            auto with = [&](Access a) {
+        const int64_t n = sc_.rows, blocks = n * sc_.slices;
+        const int64_t rowBytes = n * (int64_t)sizeof(SampleRow), binBytes = cuts() ? blocks * SAMPLE_BINS * 8 : 0;
+        enc.withTemporaryTensor(ScratchSpec{{rowBytes + binBytes}, DataType::u8}, [&](Tensor scratch) {
+            const Tensor rows(scratch.data, Shape({rowBytes}), DataType::u8), bins((char *)scratch.data + rowBytes, Shape({binBytes}), DataType::u8);
+            auto with = [&](std::initializer_list<Binding> more) {
                 std::vector<Binding> b = options({{logits_, kRead}});
-                b.push_back({rows, (uint8_t)a});
+                b.insert(b.end(), more);
                 return b;
             };
-            if (cuts()) launch(enc, "sample_hist_", with(kReadWrite), sc_.rows * sc_.histBlocks, 256);
-            launch(enc, "sample_gather_", with(kReadWrite), sc_.rows * sc_.slices, 256);
-            std::vector<Binding> b = with(kRead);
-            b.push_back({tokens_, kWrite});
-            launch(enc, "sample_finish_", std::move(b), sc_.rows, 1024);
+            launch(enc, "sample_top_", {{logits_, kRead}, {rows, kWrite}}, blocks);
+            if (cuts()) launch(enc, "sample_hist_", with({{rows, kReadWrite}, {bins, kWrite}}), blocks);
+            launch(enc, "sample_gather_", with({{rows, kReadWrite}}), blocks);
+            launch(enc, "sample_finish_", with({{rows, kRead}, {bins, kRead}, {tokens_, kWrite}}), n);
         });
     }
 
@@ -189,8 +189,8 @@ private:
         for (const Tensor &t : options_) b.push_back({t, kRead});
         return b;
     }
-    void launch(KernelCommandEncoder &enc, const char *fn, std::vector<Binding> b, uint32_t blocks, unsigned threads) const {
-        enc.encode(*Kernels::Custom(fn + type_, std::move(b), {bytesOf(sc_)}, dim3(blocks, 1, 1), dim3(threads, 1, 1)));
+    void launch(KernelCommandEncoder &enc, const char *fn, std::vector<Binding> b, int64_t blocks) const {
+        enc.encode(*Kernels::Custom(fn + type_, std::move(b), {bytesOf(sc_)}, dim3((unsigned)blocks, 1, 1), dim3(1024, 1, 1)));
     }
 
     Tensor logits_, tokens_;
