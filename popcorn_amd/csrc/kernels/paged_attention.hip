@@ -175,6 +175,7 @@ constexpr int kOutOfRange = (int)0x80000000u;  // past every page: zeros
 typedef __attribute__((address_space(3))) void lds_void;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+using pk::f32x16;
 using pk::u32x2;
 using pk::u32x4;
 
@@ -218,9 +219,81 @@ struct Piece {
 };
 
 // What a worker's last piece leaves to the merge: nothing (pieces 0), or the
-// rows r0 .. r1 - 1 of a unit that it begins and `pieces` workers share.
+// rows r0 .. r1 - 1 of a unit that it begins and `pieces` workers share. Worker
+// w's two states are `rows` rows each, from row base + 2 w rows on.
 struct Shared {
-    uint32_t pieces, start, hkv, r0, r1, pad[3];
+    uint32_t pieces, start, hkv, r0, r1, rows, base, worker;
+};
+
+// Deals a block of NT threads its pieces.
+template <uint32_t NT>
+struct Dealer {
+    const pk::PagedTile *plan;
+    const OwnTile *own;
+    const int32_t *starts, *keyLens;
+    Shared *shared;
+    uint64_t share, x, end;
+    uint32_t tile;
+
+    // `space` is free again afterwards.
+    __device__ inline Dealer(const int32_t *st, const int32_t *kl, const pk::PagedTile *pl, OwnTile *ow, PlanSpace<NT, uint32_t> &space,
+                             Shared *sh, const PagedAttentionConstants &p, const PagedWorkConstants &w)
+        : plan(pl), own(ow), starts(st), keyLens(kl), shared(sh + blockIdx.x) {
+        uint32_t tiles;
+        uint64_t total;
+        if (w.ownPlan) {
+            uint32_t steps;
+            lay_tiles<NT, uint32_t>(starts, keyLens, space, p, w, steps, tiles, [&](uint32_t at, uint32_t before, uint32_t request, uint32_t t) {
+                ow[at] = OwnTile{before, request << 16 | t};
+            });
+            total = (uint64_t)first_lane(steps) * p.Nkv;
+            tiles = first_lane(tiles);
+        } else {
+            total = plan[0].before * p.Nkv;
+            tiles = plan[0].request;
+        }
+        share = pk::paged_share(total, w);
+        x = first_lane64(blockIdx.x * share);
+        end = first_lane64(min(x + share, total));
+        if (x < end) {
+            tile = w.ownPlan ? find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return own[i].before; })
+                             : find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
+        } else if (threadIdx.x == 0) {
+            shared->pieces = 0;
+        }
+    }
+
+    // False at the end of the block's stretch.
+    __device__ inline bool next(Piece &c, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+        while (x < end) {
+            pk::PagedTile t;
+            if (w.ownPlan) {
+                const OwnTile o = own[tile];
+                t = pk::PagedTile{first_lane(o.before), first_lane(o.place >> 16), first_lane(o.place & 0xffffu)};
+            } else {
+                t = plan[1 + tile];
+                t = pk::PagedTile{first_lane64(t.before), first_lane(t.request), first_lane(t.tile)};
+            }
+            c.request = t.request;
+            c.req = pk::paged_request(starts[t.request], starts[t.request + 1], keyLens[t.request], p);
+            c.steps = pk::paged_steps(c.req, t.tile, p, w);
+            const uint64_t in = x - t.before * p.Nkv;  // counted steps before x of this tile's units
+            const uint32_t n = c.steps.n + w.unitSteps;
+            c.hkv = (uint32_t)(in / n);
+            const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * n), hi = (uint32_t)min((uint64_t)n, lo + (end - x));
+            c.lo = max(lo, w.unitSteps) - w.unitSteps;
+            c.hi = max(hi, w.unitSteps) - w.unitSteps;
+            x += hi - lo;
+            if (hi == n && c.hkv + 1 == p.Nkv) ++tile;
+            if (x == end && threadIdx.x == 0) {
+                Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, w.rows, w.stateBase, blockIdx.x};
+                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = (uint32_t)((end + (n - hi) - 1) / share - blockIdx.x) + 1;
+                *shared = sh;
+            }
+            if (c.lo < c.hi) return true;
+        }
+        return false;
+    }
 };
 
 // The result of one row's lane of 4 dims, rounded.
@@ -268,59 +341,9 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     const uint32_t wave = first_lane(threadIdx.x >> 6);
     const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
     const float c2 = p.scale * kLog2e;
-    uint32_t tiles;
-    uint64_t total;
-    if (w.ownPlan) {
-        uint32_t steps;
-        lay_tiles<64 * kWaves, uint32_t>(starts, keyLens, *reinterpret_cast<PlanSpace<64 * kWaves, uint32_t> *>(smem), p, w, steps, tiles,
-                                         [&](uint32_t at, uint32_t before, uint32_t request, uint32_t tile) {
-                                             sm_plan[at] = OwnTile{before, request << 16 | tile};
-                                         });
-        total = (uint64_t)first_lane(steps) * p.Nkv;
-        tiles = first_lane(tiles);
-    } else {
-        total = plan[0].before * p.Nkv;
-        tiles = plan[0].request;
-    }
-    const uint64_t share = pk::paged_share(total, w);
-    uint64_t x = first_lane64(blockIdx.x * share);
-    const uint64_t end = first_lane64(min(x + share, total));
-    if (x >= end) {
-        if (threadIdx.x == 0) shared[blockIdx.x].pieces = 0;
-        return;
-    }
-    uint32_t tile = w.ownPlan ? find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return sm_plan[i].before; })
-                              : find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
-
-    while (x < end) {
-        Piece c;
-        {
-            pk::PagedTile t;
-            if (w.ownPlan) {
-                const OwnTile o = sm_plan[tile];
-                t = pk::PagedTile{first_lane(o.before), first_lane(o.place >> 16), first_lane(o.place & 0xffffu)};
-            } else {
-                t = plan[1 + tile];
-                t = pk::PagedTile{first_lane64(t.before), first_lane(t.request), first_lane(t.tile)};
-            }
-            c.request = t.request;
-            c.req = pk::paged_request(starts[t.request], starts[t.request + 1], keyLens[t.request], p);
-            c.steps = pk::paged_steps(c.req, t.tile, p, w);
-            const uint64_t in = x - t.before * p.Nkv;  // counted steps before x of this tile's units
-            const uint32_t n = c.steps.n + w.unitSteps;
-            c.hkv = (uint32_t)(in / n);
-            const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * n), hi = (uint32_t)min((uint64_t)n, lo + (end - x));
-            c.lo = max(lo, w.unitSteps) - w.unitSteps;
-            c.hi = max(hi, w.unitSteps) - w.unitSteps;
-            x += hi - lo;
-            if (hi == n && c.hkv + 1 == p.Nkv) ++tile;
-            if (x == end && threadIdx.x == 0) {
-                Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, {0, 0, 0}};
-                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = (uint32_t)((end + (n - hi) - 1) / share - blockIdx.x) + 1;
-                shared[blockIdx.x] = sh;
-            }
-            if (c.lo == c.hi) continue;
-        }
+    Dealer<64 * kWaves> dealer(starts, keyLens, plan, sm_plan, *reinterpret_cast<PlanSpace<64 * kWaves, uint32_t> *>(smem), shared, p, w);
+    Piece c;
+    while (dealer.next(c, p, w)) {
         const int32_t *table = tables + (uint64_t)c.request * p.columns;
         const uint32_t keys = (uint32_t)c.req.keys;
         auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
@@ -530,7 +553,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         float *sO = reinterpret_cast<float *>(smem);
         const uint32_t tr = threadIdx.x / 16, td = threadIdx.x % 16 * 4;
         const bool whole = c.lo == 0 && c.hi == c.steps.n;
-        const uint64_t slot = (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * (RT * 16);
+        const uint64_t slot = w.stateBase + (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * (RT * 16);
         auto store = [&](uint32_t r, uint32_t d, const pk::f32x4 &o, float L) {
             if (whole) store4<T>(out + q_row(r) * D + d, o, L);
             else *reinterpret_cast<pk::f32x4 *>(pO + (slot + r - c.steps.r0) * HD + d) = o;
@@ -601,12 +624,294 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     }
 }
 
+// ---- many rows: chunks of prompts --------------------------------------------------------
+// Tiles of 128 rows, 32 to a wave, on v_mfma_f32_32x32x16: S^T = K . Q^T has a
+// row's scores in two lanes (mfma.hpp), so maxima and sums take one lane swap,
+// and a lane's weights are its P^T operand of O^T += V^T . P^T as they are.
+// K and V go from the pages straight into LDS, 16 keys (of one page) to a
+// resource, three steps of 32 keys deep; nothing waits for a copy younger
+// than two steps. K is read by rows, V by ds_read_b64_tr_b16 (four keys of a
+// dim to a lane); 16-byte chunks are swizzled so that the rows of one read
+// fall in different banks.
+// What bounds it: products and softmax take about as long (HD 128: 512 cycles
+// of MFMA and 480 of VALU for 32 keys), so step i + 1's scores are computed
+// beside step i's exponentials, and step i's product with V beside the
+// maximum of step i + 1.
+constexpr int kTileRows = 128, kRing = 3;
+
+template <typename T, int HD>
+__device__ void paged_tile(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
+                           const typename T::storage *__restrict__ V,
+                           const int32_t *__restrict__ tables, const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                           const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
+                           Shared *__restrict__ shared, typename T::storage *__restrict__ out, const PagedAttentionConstants &p,
+                           const PagedWorkConstants &w) {
+    using S = typename T::storage;
+    constexpr int BKV = 32, KS = HD / 16, DT = HD / 32, CH = HD / 8;
+    constexpr int kRowsPer = 64 / CH;      // rows per copy instruction
+    constexpr int kCopies = 8 / kRowsPer;  // instructions for a wave's 8 rows of K (or V) of a step
+    constexpr bool kTwo = std::is_same<T, pk::BF16>::value;  // weights as two bf16, or one f16
+    constexpr float kLead = kTwo ? 0.0f : 4.0f;
+    constexpr uint32_t kTileBytes = BKV * HD * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kRing * kTileBytes];
+    __shared__ OwnTile sm_plan[kOwnTiles];
+    static_assert(sizeof(PlanSpace<256, uint32_t>) <= sizeof(smem), "the plan is laid out where K and V go");
+    uint8_t *sK = smem, *sV = smem + kRing * kTileBytes;
+
+    const uint32_t lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
+    const uint32_t wave = first_lane(threadIdx.x >> 6);
+    const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
+    const float c2 = fabsf(p.scale) * kLog2e;
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;  // -scale K . Q = scale K . -Q
+    auto swzK = [](uint32_t row) { return CH >= 16 ? row % 16u : row / 2u % 8u; };
+    auto swzV = [](uint32_t row) { return CH >= 16 ? row % 4u * 4u : row / 2u % 2u * 4u; };
+
+    Dealer<256> dealer(starts, keyLens, plan, sm_plan, *reinterpret_cast<PlanSpace<256, uint32_t> *>(smem), shared, p, w);
+    Piece c;
+    while (dealer.next(c, p, w)) {
+        const int32_t *table = tables + (uint64_t)c.request * p.columns;
+        const uint32_t keys = (uint32_t)c.req.keys;
+        auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
+        // the wave's rows; those past the tile's last repeat it and are not stored
+        const uint32_t w0 = c.steps.r0 + wave * 32, myRow = w0 + c32, rowAt = min(myRow, c.steps.r1 - 1);
+        const int pos = c.req.pos0 + (int)(rowAt / G);
+        const int posLo = c.req.pos0 + (int)(min(w0, c.steps.r1 - 1) / G), posHi = c.req.pos0 + (int)(min(w0 + 31, c.steps.r1 - 1) / G);
+        u32x4 qf[KS];
+        {
+            const S *row = Q + q_row(rowAt) * D + h * 8;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                qf[s] = s * 16 + h * 8 < D ? *reinterpret_cast<const u32x4 *>(row + s * 16) : u32x4{0u, 0u, 0u, 0u};
+                qf[s] ^= flip;
+            }
+        }
+
+        // Lane l holds page and row in it of group l % 2 of the piece's step held0 + l / 2 (no page: -1).
+        const uint32_t n = c.hi - c.lo;
+        uint32_t held0 = 0, heldPage = 0, heldRow = 0;
+        auto hold = [&](uint32_t i) {
+            const uint32_t at = i + lane / 2;
+            held0 = i;
+            heldPage = ~0u;
+            heldRow = 0;
+            if (at < n) {
+                const uint32_t key = pk::paged_step_key(c.steps, c.lo + at, w) + lane % 2 * 16, column = key / p.pageSize;
+                if (key < keys) {
+                    heldPage = (uint32_t)table[column];
+                    heldRow = key - column * p.pageSize;
+                }
+            }
+        };
+        // Copies step i's K and V into ring place `at`: wave w rows 8 w .. 8 w + 7. Rows that no page holds become zeros.
+        auto copy = [&](uint32_t i, uint32_t at) {
+            const uint32_t from = (i - held0) * 2 + wave / 2;
+            const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)from);
+            const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)heldRow, (int)from);
+            const uint32_t key = pk::paged_step_key(c.steps, c.lo + i, w) + wave / 2 * 16;
+            const bool ok = page < p.pages;
+            const uint64_t off = ok ? (((uint64_t)page * p.Nkv + c.hkv) * p.pageSize + row) * D : 0;
+            const int bytes = ok ? (int)(min(16u, keys - key) * D * 2) : 0;
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(K + off), 0, bytes, 0x00020000);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(V + off), 0, bytes, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const uint32_t r16 = wave % 2 * 8 + j * kRowsPer + lane / CH, r32 = wave * 8 + j * kRowsPer + lane / CH;
+                const uint32_t ck = lane % CH ^ swzK(r32), cv = lane % CH ^ swzV(r32);
+                const uint32_t to = at * kTileBytes + (wave * 8 + j * kRowsPer) * HD * 2;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(sK + to), 16, ck * 8 < D ? (int)((r16 * D + ck * 8) * 2) : kOutOfRange, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(sV + to), 16, cv * 8 < D ? (int)((r16 * D + cv * 8) * 2) : kOutOfRange, 0, 0, 0);
+            }
+        };
+        // Where the keys that a page holds end in the two groups of step i.
+        struct Ends {
+            uint32_t e[2];
+        };
+        auto ends = [&](uint32_t i) {
+            Ends x;
+#pragma unroll
+            for (uint32_t g = 0; g < 2; ++g) {
+                const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)((i - held0) * 2 + g));
+                const uint32_t key = pk::paged_step_key(c.steps, c.lo + i, w) + g * 16;
+                x.e[g] = page < p.pages ? min(key + 16, keys) : key;
+            }
+            return x;
+        };
+
+        f32x16 acc[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
+        float m = -INFINITY, l = 0.0f;
+
+        auto scores = [&](uint32_t at) {
+            f32x16 st;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st[i] = 0.0f;
+            const uint8_t *base = sK + at * kTileBytes + c32 * (HD * 2);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                st = pk::Mma<T>::run(*reinterpret_cast<const u32x4 *>(base + ((2 * s + h) ^ swzK(c32)) * 16), qf[s], st);
+            return st;
+        };
+        // Hides what the rows do not see of step i.
+        auto mask = [&](f32x16 &st, uint32_t i, const Ends &x) {
+            const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + i, w);
+            const bool full = x.e[0] == key0 + 16 && x.e[1] == key0 + 32 &&
+                              (p.maskKind == 2u || ((int)key0 + 31 <= posLo && (p.maskKind == 0u || (int64_t)posHi - key0 < p.slidingWindow ||
+                                                                                key0 + 31 < p.sinks)));
+            if (full) return;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const uint32_t key = key0 + (j >> 2) * 8 + h * 4 + (j & 3);
+                const bool seen = (key < x.e[j / 8]) & pk::paged_sees(pos, (int)key, p);
+                st[j] = seen ? st[j] : -INFINITY;
+            }
+        };
+        auto highest = [&](const f32x16 &st) {
+            float mx = st[0];
+#pragma unroll
+            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, st[j]);
+            return pk::pair32_max(mx) * c2;
+        };
+        // Moves the rows' reference to a maximum that passes it by more than the gap.
+        auto follow = [&](float mx) {
+            const bool move = mx > m + (kRescaleGap + kLead);
+            if (!__ballot(move)) return;
+            float alpha = 1.0f;
+            if (move) {
+                alpha = __builtin_amdgcn_exp2f(m - (mx - kLead));
+                m = mx - kLead;
+            }
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+        };
+
+        hold(0);
+        copy(0, 0);
+        Ends ahead = ends(0), ahead2 = ahead;  // of steps i + 1 and i + 2
+        if (n > 1) {
+            copy(1, 1);
+            ahead2 = ends(1);
+        }
+        wait_vmcnt<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        f32x16 st = scores(0);
+        mask(st, 0, ahead);
+        follow(highest(st));
+        ahead = ahead2;
+        uint32_t at = 0;  // step i's place in the ring
+        for (uint32_t i = 0; i < n; ++i) {
+            const uint32_t at1 = at == kRing - 1 ? 0 : at + 1, at2 = at1 == kRing - 1 ? 0 : at1 + 1;
+            // step i + 1 is in LDS (copied in pass i - 1), and every wave has read what step i + 2 goes over
+            wait_vmcnt<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (i + 2 < n) {
+                if (i + 2 - held0 == 32) hold(i + 2);
+                copy(i + 2, at2);
+                ahead2 = ends(i + 2);
+            }
+            f32x16 sn = st;
+            if (i + 1 < n) sn = scores(at1);
+            u32x4 pf[2], pr[2];
+            const float mref = m == -INFINITY ? 0.0f : m;
+            float ps = 0.0f;
+#pragma unroll
+            for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int e = ks * 8 + 2 * j;
+                    const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e], c2, -mref)), p1 = __builtin_amdgcn_exp2f(fmaf(st[e + 1], c2, -mref));
+                    ps += p0 + p1;
+                    const uint32_t v = pk::pack2<T>(p0, p1);
+                    pf[ks][j] = v;
+                    if constexpr (kTwo) pr[ks][j] = pk::pack2<T>(p0 - __uint_as_float(v << 16), p1 - __uint_as_float(v & 0xffff0000u));
+                }
+            l += pk::pair32_sum(ps);
+            const uint32_t s16 = lane & 15, dimHalf = lane >> 4 & 1;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    auto readV = [&](uint32_t key) {
+                        const uint32_t chunk = (dt * 4 + dimHalf * 2 + (s16 & 3) / 2) ^ swzV(key);
+                        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                             (lds_s16x4 *)(sV + at * kTileBytes + (key * CH + chunk) * 16 + (s16 & 1) * 8)));
+                    };
+                    const u32x2 a = readV(ks * 16 + h * 4 + s16 / 4), b = readV(ks * 16 + 8 + h * 4 + s16 / 4);
+                    const u32x4 va = {a.x, a.y, b.x, b.y};
+                    acc[dt] = pk::Mma<T>::run(va, pf[ks], acc[dt]);
+                    if constexpr (kTwo) acc[dt] = pk::Mma<T>::run(va, pr[ks], acc[dt]);
+                }
+            if (i + 1 < n) {
+                mask(sn, i + 1, ahead);
+                ahead = ahead2;
+                follow(highest(sn));
+                st = sn;
+            }
+            at = at1;
+        }
+        // every wave has read its last tiles before the next piece's copies
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+
+        const bool whole = c.lo == 0 && c.hi == c.steps.n;
+        const uint64_t slot = w.stateBase + (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * kTileRows;
+        auto store = [&](uint32_t r, uint32_t d, const pk::f32x4 &o, float L) {
+            if (whole) store4<T>(out + q_row(r) * D + d, o, L);
+            else *reinterpret_cast<pk::f32x4 *>(pO + (slot + r - c.steps.r0) * HD + d) = o;
+        };
+        bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const uint32_t d = dt * 32 + i4 * 8 + h * 4;
+                const pk::f32x4 o = {acc[dt][4 * i4], acc[dt][4 * i4 + 1], acc[dt][4 * i4 + 2], acc[dt][4 * i4 + 3]};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad |= !(fabsf(o[e]) < INFINITY) & (d < D);
+                if (myRow < c.steps.r1 && d < D) store(myRow, d, o, l);
+            }
+        if (!whole && myRow < c.steps.r1 && h == 0) *reinterpret_cast<float2 *>(pML + 2 * (slot + myRow - c.steps.r0)) = float2{m, l};
+        if (!__ballot(bad)) continue;
+        // as in paged_few: an infinity or NaN in V that a row does not see
+        const uint32_t s0 = min(c.lo, c.steps.sinks), s1 = min(c.hi, c.steps.sinks);
+        const uint32_t t0 = max(c.lo, c.steps.sinks), t1 = max(c.hi, c.steps.sinks);
+        auto key_at = [&](uint32_t k) { return (int)min(k * w.stepKeys, keys); };
+        const uint32_t td = lane % 16 * 4;
+        for (uint32_t r = w0 + lane / 16; r < min(w0 + 32, c.steps.r1); r += 4) {
+            constexpr int NJ = HD / 64;
+            pk::f32x4 qv[NJ], o[NJ];
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                o[j] = qv[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                if (td + 64 * j < D)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) qv[j][e] = T::load(Q[q_row(r) * D + td + 64 * j + e]);
+            }
+            const int rp = c.req.pos0 + (int)(r / G);
+            paged_row<T, NJ, true>(qv, K, V, table, c.hkv, rp, key_at(s0), key_at(s1), p, o, M, L);
+            paged_row<T, NJ, true>(qv, K, V, table, c.hkv, rp, key_at(t0 - c.steps.sinks + c.steps.first),
+                                   key_at(t1 - c.steps.sinks + c.steps.first), p, o, M, L);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                if (td + 64 * j < D) store(r, td + 64 * j, o[j], L);
+            if (!whole && td == 0) *reinterpret_cast<float2 *>(pML + 2 * (slot + r - c.steps.r0)) = float2{M, L};
+        }
+    }
+}
+
 // The units that several workers shared: the first one's state is in its slot
 // 2 w + 1, the following ones' in theirs 2 w'. 16 lanes take a row's dims; with
 // fewer than 16 rows, several groups of lanes share a row's pieces.
 template <typename T, int HD>
 __device__ void paged_merge(const float *__restrict__ pO, const float *__restrict__ pML, const Shared *__restrict__ shared,
-                            typename T::storage *__restrict__ out, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+                            typename T::storage *__restrict__ out, const PagedAttentionConstants &p) {
     constexpr int NJ = HD / 64;
     __shared__ __attribute__((aligned(16))) float sO[16][HD];
     __shared__ float sM[16], sL[16];
@@ -640,7 +945,7 @@ __device__ void paged_merge(const float *__restrict__ pO, const float *__restric
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u) {
                 const uint32_t i = min(i0 + u * each, c.pieces - 1);
-                const uint64_t row = (2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * w.rows + (r - c.r0);
+                const uint64_t row = c.base + (2 * ((uint64_t)c.worker + i) + (i == 0)) * c.rows + (r - c.r0);
                 ml[u] = *reinterpret_cast<const float2 *>(pML + 2 * row);
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) v[u][j] = td + 64 * j < D ? *reinterpret_cast<const pk::f32x4 *>(pO + row * HD + td + 64 * j) : o[j];
@@ -744,10 +1049,17 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
              PagedAttentionConstants p, PagedWorkConstants w) {                                                           \
         paged_few<T, HD, RT>(q, k, v, tables, starts, keyLens, plan, pO, pML, shared, out, p, w);                         \
     }
+#define PAGED_TILE(name, T, HD, PER_CU)                                                                                   \
+    POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                    \
+        name(const T::storage *q, const T::storage *k, const T::storage *v, const int32_t *tables, const int32_t *starts,       \
+             const int32_t *keyLens, const pk::PagedTile *plan, float *pO, float *pML, Shared *shared, T::storage *out,     \
+             PagedAttentionConstants p, PagedWorkConstants w) {                                                           \
+        paged_tile<T, HD>(q, k, v, tables, starts, keyLens, plan, pO, pML, shared, out, p, w);                            \
+    }
 #define PAGED_MERGE(name, T, HD)                                                                                          \
     POPCORN_KERNEL void __launch_bounds__(256) name(const float *pO, const float *pML, const Shared *shared, T::storage *out, \
-                                                    PagedAttentionConstants p, PagedWorkConstants w) {                    \
-        paged_merge<T, HD>(pO, pML, shared, out, p, w);                                                                   \
+                                                    PagedAttentionConstants p) {                                          \
+        paged_merge<T, HD>(pO, pML, shared, out, p);                                                                      \
     }
 #define PAGED_FEW_D(t, T, PER256)                                   \
     PAGED_FEW(paged_attention_few_##t##_d64_r1, T, 64, 1, 4)   \
@@ -765,3 +1077,10 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
 PAGED_FEW_D(f32, F32, 1)
 PAGED_FEW_D(f16, F16, 2)
 PAGED_FEW_D(bf16, BF16, 2)
+
+PAGED_TILE(paged_attention_tile_f16_d64, F16, 64, 2)
+PAGED_TILE(paged_attention_tile_f16_d128, F16, 128, 2)
+PAGED_TILE(paged_attention_tile_f16_d256, F16, 256, 1)
+PAGED_TILE(paged_attention_tile_bf16_d64, BF16, 64, 2)
+PAGED_TILE(paged_attention_tile_bf16_d128, BF16, 128, 2)
+PAGED_TILE(paged_attention_tile_bf16_d256, BF16, 256, 1)

@@ -69,64 +69,103 @@ int deviceCUs() {
     return cachedCUs;
 }
 
-// PagedAttention on the matrix cores (paged_attention.hip): a plan of tiles,
-// the pieces of work, and the merge of what several blocks shared.
+// PagedAttention on the matrix cores (paged_attention.hip): requests of few
+// rows (new tokens x heads of a KV head's group) and of many by a launch each,
+// with plans of tiles where the blocks do not lay them out themselves, and the
+// merge of what several blocks shared.
 class PagedAttentionKernel : public Kernel {
 public:
     PagedAttentionKernel(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &tables, const Tensor &starts, const Tensor &lens,
                          const Tensor &out, const PagedAttentionConstants &pc, int64_t maxQueryLen)
         : q_(q), k_(k), v_(v), tables_(tables), starts_(starts), lens_(lens), out_(out), pc_(pc) {
-        const int64_t G = pc.Nq / pc.Nkv, R = pc.R, T = pc.T;
+        const int64_t G = pc.Nq / pc.Nkv, longest = std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T) * G;
+        const bool f32 = q.dataType == DataType::f32;
         hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
-        const int rt = hdp_ == 512 || (maxQueryLen > 0 && maxQueryLen * G <= 16) ? 1 : 2;
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
-        fn_ = "paged_attention_few_" + type + hd + "_r" + std::to_string(rt);
         merge_ = "paged_attention_merge_" + type + hd;
-        w_.rows = 16 * (uint32_t)rt;
-        w_.stepKeys = q.dataType == DataType::f32 ? 16 : 32;
-        w_.fewRows = 0;
-        w_.manyRows = UINT32_MAX;
-        w_.maxTiles = (uint32_t)(cdiv(T * G, w_.rows) + std::min(R, T));
-        w_.minSteps = 4;
-        // as many as run at once (the kernels' registers)
-        const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && q.dataType != DataType::f32 ? 2 : 1;
-        w_.unitSteps = 12;
-        // no more workers than the longest requests that the tables can name could give work to
-        const double tileSteps = (double)cdiv((int64_t)pc.columns * pc.pageSize + w_.stepKeys, w_.stepKeys) + w_.unitSteps;
-        const double steps = (double)w_.maxTiles * tileSteps;
-        w_.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc.Nkv / w_.minSteps + 1));
-        w_.ownPlan = w_.maxTiles <= 1024 && R <= 1024 && steps < 2147483648.0;
+        // the tile kernel works on the magnitude of the scale (not 0) and 16-bit K and V of up to 256 dims
+        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows;
+        if (!(tiles && pc.R == 1)) {
+            const int rt = hdp_ == 512 || longest <= 16 || tiles ? 1 : 2;
+            // as many blocks as run at once (the kernels' registers)
+            const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
+            add("paged_attention_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);
+        }
+        if (tiles) add("paged_attention_tile_" + type + hd, 128, 32, pc.R == 1 ? 0 : kFewRows, UINT32_MAX, hdp_ == 256 ? 1 : 2);
     }
     std::vector<Binding> tensors() const override {
         return {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {out_, kWrite}};
     }
-    std::string describe() const override { return (w_.ownPlan ? "" : "paged_plan,") + fn_ + "," + merge_; }
+    std::string describe() const override {
+        std::string s;
+        for (const Work &w : work_) s += (w.c.ownPlan ? "" : "paged_plan,") + w.fn + ",";
+        return s + merge_;
+    }
     void encode(KernelCommandEncoder &enc) const override {
-        // one buffer: the states' O, their m and l, what is shared, the plan
-        const int64_t states = 2 * (int64_t)w_.workers * w_.rows;
-        const int64_t o = states * hdp_ * 4, ml = states * 8, shared = (int64_t)w_.workers * 32;
-        const int64_t plan = w_.ownPlan ? 0 : ((int64_t)w_.maxTiles + 1) * 16;
-        enc.withTemporaryTensor(ScratchSpec{{o + ml + shared + plan}, DataType::u8}, [&](Tensor scratch) {
+        // one buffer: the states' O, their m and l, what is shared, the plans
+        int64_t states = 0, workers = 0, tiles = 0;
+        for (const Work &w : work_) {
+            states += 2 * (int64_t)w.c.workers * w.c.rows;
+            workers += w.c.workers;
+            tiles += w.c.ownPlan ? 0 : (int64_t)w.c.maxTiles + 1;
+        }
+        const int64_t o = states * hdp_ * 4, ml = states * 8, shared = workers * 32;
+        enc.withTemporaryTensor(ScratchSpec{{o + ml + shared + tiles * 16}, DataType::u8}, [&](Tensor scratch) {
             auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
-            const Tensor pO = part(0, o), pML = part(o, ml), sh = part(o + ml, shared), pl = part(o + ml + shared, plan);
-            if (!w_.ownPlan) launch(enc, "paged_plan", {{starts_, kRead}, {lens_, kRead}, {pl, kWrite}}, dim3(1, 1, 1), 1024);
-            launch(enc, fn_,
-                   {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {pl, kRead}, {pO, kWrite},
-                    {pML, kWrite}, {sh, kWrite}, {out_, kWrite}},
-                   dim3(w_.workers, 1, 1), 256);
-            launch(enc, merge_, {{pO, kRead}, {pML, kRead}, {sh, kRead}, {out_, kWrite}}, dim3(w_.workers, w_.rows / 16, 1), 256);
+            const Tensor pO = part(0, o), pML = part(o, ml);
+            int64_t at = o + ml, plan = o + ml + shared;
+            for (const Work &w : work_) {
+                const Tensor sh = part(at, (int64_t)w.c.workers * 32), pl = part(plan, ((int64_t)w.c.maxTiles + 1) * 16);
+                const std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_), bytesOf(w.c)};
+                if (!w.c.ownPlan) {
+                    launch(enc, "paged_plan", {{starts_, kRead}, {lens_, kRead}, {pl, kWrite}}, consts, dim3(1, 1, 1), 1024);
+                    plan += ((int64_t)w.c.maxTiles + 1) * 16;
+                }
+                launch(enc, w.fn,
+                       {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {pl, kRead}, {pO, kWrite},
+                        {pML, kWrite}, {sh, kWrite}, {out_, kWrite}},
+                       consts, dim3(w.c.workers, 1, 1), 256);
+                at += (int64_t)w.c.workers * 32;
+            }
+            launch(enc, merge_, {{pO, kRead}, {pML, kRead}, {part(o + ml, shared), kRead}, {out_, kWrite}}, {bytesOf(pc_)},
+                   dim3((unsigned)workers, work_.back().c.rows / 16, 1), 256);
         });
     }
 
 private:
-    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, dim3 grid, unsigned block) const {
-        enc.encode(*Kernels::Custom(fn, std::move(b), {bytesOf(pc_), bytesOf(w_)}, grid, dim3(block, 1, 1)));
+    static constexpr uint32_t kFewRows = 32;
+    struct Work {
+        std::string fn;
+        PagedWorkConstants c;
+    };
+
+    void add(const std::string &fn, uint32_t rows, uint32_t stepKeys, uint32_t few, uint32_t many, int perCU) {
+        const int64_t G = pc_.Nq / pc_.Nkv;
+        PagedWorkConstants w{};
+        w.rows = rows;
+        w.stepKeys = stepKeys;
+        w.fewRows = few;
+        w.manyRows = many;
+        w.maxTiles = (uint32_t)(cdiv((int64_t)pc_.T * G, rows) + std::min(pc_.R, pc_.T));
+        w.minSteps = 4;
+        w.unitSteps = 12;
+        // no more workers than the longest requests that the tables can name could give work to
+        const double tileSteps = (double)cdiv((int64_t)pc_.columns * pc_.pageSize + stepKeys, stepKeys) + w.unitSteps;
+        const double steps = (double)w.maxTiles * tileSteps;
+        w.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc_.Nkv / w.minSteps + 1));
+        w.ownPlan = w.maxTiles <= 1024 && pc_.R <= 1024 && steps < 2147483648.0;
+        w.stateBase = work_.empty() ? 0 : 2 * work_.back().c.workers * work_.back().c.rows;
+        work_.push_back({fn, w});
+    }
+    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, std::vector<std::vector<uint8_t>> consts, dim3 grid,
+                unsigned block) const {
+        enc.encode(*Kernels::Custom(fn, std::move(b), std::move(consts), grid, dim3(block, 1, 1)));
     }
 
     Tensor q_, k_, v_, tables_, starts_, lens_, out_;
     PagedAttentionConstants pc_;
-    PagedWorkConstants w_{};
-    std::string fn_, merge_;
+    std::vector<Work> work_;
+    std::string merge_;
     int64_t hdp_ = 0;
 };
 
