@@ -653,10 +653,11 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
     constexpr bool kTwo = std::is_same<T, pk::BF16>::value;  // weights as two bf16, or one f16
     constexpr float kLead = kTwo ? 0.0f : 4.0f;
     constexpr uint32_t kTileBytes = BKV * HD * 2;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[2 * kRing * kTileBytes];
-    __shared__ OwnTile sm_plan[kOwnTiles];
-    static_assert(sizeof(PlanSpace<256, uint32_t>) <= sizeof(smem), "the plan is laid out where K and V go");
+    // (one array: with two, the compiler has every read of LDS wait for the latest copy into it)
+    __shared__ __attribute__((aligned(256))) uint8_t smem[2 * kRing * kTileBytes + kOwnTiles * sizeof(OwnTile)];
+    static_assert(sizeof(PlanSpace<256, uint32_t>) <= 2 * kRing * kTileBytes, "the plan is laid out where K and V go");
     uint8_t *sK = smem, *sV = smem + kRing * kTileBytes;
+    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 2 * kRing * kTileBytes);
 
     const uint32_t lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
     const uint32_t wave = first_lane(threadIdx.x >> 6);
@@ -744,23 +745,35 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
             for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
-        auto scores = [&](uint32_t at) {
-            f32x16 st;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st[i] = 0.0f;
-            const uint8_t *base = sK + at * kTileBytes + c32 * (HD * 2);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-                st = pk::Mma<T>::run(*reinterpret_cast<const u32x4 *>(base + ((2 * s + h) ^ swzK(c32)) * 16), qf[s], st);
-            return st;
+        // LDS offsets of this lane's K and V, in a ring place: the other fragments' are these with bits 5 to 7 turned over
+        // (a step's 16-byte chunks s and s + 8 are 256 bytes apart), and constant distances. Kept from being computed
+        // once for all fragments (48 registers).
+        const uint32_t kAt = c32 * (HD * 2) + (h ^ swzK(c32)) * 16;
+        const uint32_t s16 = lane & 15, swz4 = CH >= 16 ? s16 / 4 : s16 / 8;
+        const uint32_t vAt = kRing * kTileBytes + (h * 4 + s16 / 4) * (HD * 2) + swz4 * 64 + (lane >> 4 & 1) * 32 + (s16 & 3) * 8;
+        auto in_place = [](uint32_t lane0, uint32_t at) {
+            uint32_t x = lane0 + at * kTileBytes;
+            asm volatile("" : "+v"(x));
+            return x;
+        };
+        auto readK = [&](uint32_t x, int s) { return *reinterpret_cast<const u32x4 *>(smem + ((x ^ (s & 7) * 32u) + (s >> 3) * 256u)); };
+        // fragment ks of dims 32 dt .. + 31: this lane's 4 + 4 keys of one dim
+        auto readV = [&](uint32_t x, int dt, int ks) {
+            const uint32_t y = (x ^ (dt & 3) * 64u) + (dt >> 2) * 256u + ks * (16 * HD * 2);
+            const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(smem + y)));
+            const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(smem + y + 8 * HD * 2)));
+            return u32x4{a.x, a.y, b.x, b.y};
+        };
+        // Whether every row of the wave sees every key of step i.
+        auto all_see = [&](uint32_t i, const Ends &x) {
+            const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + i, w);
+            return x.e[0] == key0 + 16 && x.e[1] == key0 + 32 &&
+                   (p.maskKind == 2u || ((int)key0 + 31 <= posLo &&
+                                         (p.maskKind == 0u || (int64_t)posHi - key0 < p.slidingWindow || key0 + 31 < p.sinks)));
         };
         // Hides what the rows do not see of step i.
         auto mask = [&](f32x16 &st, uint32_t i, const Ends &x) {
             const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + i, w);
-            const bool full = x.e[0] == key0 + 16 && x.e[1] == key0 + 32 &&
-                              (p.maskKind == 2u || ((int)key0 + 31 <= posLo && (p.maskKind == 0u || (int64_t)posHi - key0 < p.slidingWindow ||
-                                                                                key0 + 31 < p.sinks)));
-            if (full) return;
 #pragma unroll
             for (int j = 0; j < 16; ++j) {
                 const uint32_t key = key0 + (j >> 2) * 8 + h * 4 + (j & 3);
@@ -769,9 +782,9 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
             }
         };
         auto highest = [&](const f32x16 &st) {
-            float mx = st[0];
+            float mx = fmaxf(st[0], st[1]);
 #pragma unroll
-            for (int j = 1; j < 16; ++j) mx = fmaxf(mx, st[j]);
+            for (int j = 2; j < 16; ++j) mx = fmaxf(mx, st[j]);
             return pk::pair32_max(mx) * c2;
         };
         // Moves the rows' reference to a maximum that passes it by more than the gap.
@@ -787,73 +800,126 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
         };
+        f32x16 st;
+        u32x4 pf[2], pr[2];
+        float mref = 0.0f, ps = 0.0f;
+        // The weights of two of st's scores, as a word of the P^T operands.
+        auto weigh = [&](int pair) {
+            const int ks = pair / 4, j = pair % 4, e = 2 * pair;
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e], c2, -mref)), p1 = __builtin_amdgcn_exp2f(fmaf(st[e + 1], c2, -mref));
+            ps += p0 + p1;
+            uint32_t v = pk::pack2<T>(p0, p1);
+            if constexpr (kTwo) {
+                uint32_t r = pk::pack2<T>(p0 - __uint_as_float(v << 16), p1 - __uint_as_float(v & 0xffff0000u));
+                asm volatile("" : "+v"(r));
+                pr[ks][j] = r;
+            }
+            asm volatile("" : "+v"(v));  // here, and not where it is used
+            pf[ks][j] = v;
+        };
+        auto start_weights = [&] {
+            mref = m == -INFINITY ? 0.0f : m;
+            ps = 0.0f;
+        };
+        // acc += V^T . P^T of the step at `at`, with `beside(k)` next to the product of fragment k. V is read kAheadV
+        // fragments before its product.
+        constexpr int kFragV = DT * 2, kAheadV = 3;
+        auto multiply = [&](uint32_t at, auto &&beside) {
+            const uint32_t x = in_place(vAt, at);
+            u32x4 va[kAheadV];
+#pragma unroll
+            for (int k = 0; k < kAheadV; ++k) va[k] = readV(x, k / 2, k % 2);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < kFragV; ++k) {
+                const int dt = k / 2, ks = k % 2;
+                acc[dt] = pk::Mma<T>::run(va[k % kAheadV], pf[ks], acc[dt]);
+                if constexpr (kTwo) acc[dt] = pk::Mma<T>::run(va[k % kAheadV], pr[ks], acc[dt]);
+                if (k + kAheadV < kFragV) va[k % kAheadV] = readV(x, (k + kAheadV) / 2, (k + kAheadV) % 2);
+                beside(k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
 
         hold(0);
         copy(0, 0);
-        Ends ahead = ends(0), ahead2 = ahead;  // of steps i + 1 and i + 2
+        Ends ahead = ends(0);
+        bool allSee = all_see(0, ahead);
+        Ends ahead2 = ahead;  // of the step behind `ahead`'s
+        bool allSee2 = allSee;
         if (n > 1) {
             copy(1, 1);
             ahead2 = ends(1);
+            allSee2 = all_see(1, ahead2);
         }
         wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        f32x16 st = scores(0);
-        mask(st, 0, ahead);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[i] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) st = pk::Mma<T>::run(readK(kAt, s), qf[s], st);
+        if (!allSee) mask(st, 0, ahead);
         follow(highest(st));
-        ahead = ahead2;
+        // Pass i: step i + 1's scores beside step i's weights, then step i's product with V beside the maximum of step
+        // i + 1, in chunks that keep their order: products run while the vector instructions behind them issue.
+        auto pass = [&](uint32_t i, uint32_t at, uint32_t at1) {
+            constexpr int kAheadK = KS < 4 ? KS : 4, kChunk = KS >= 8 ? KS / 8 : 1, kPairs = 8 / (KS / kChunk);
+            f32x16 sn;
+            const uint32_t x = in_place(kAt, at1);
+            u32x4 kf[kAheadK];
+#pragma unroll
+            for (int s = 0; s < kAheadK; ++s) kf[s] = readK(x, s);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sn[j] = 0.0f;
+            start_weights();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int s0 = 0; s0 < KS; s0 += kChunk) {
+#pragma unroll
+                for (int s = s0; s < s0 + kChunk; ++s) {
+                    sn = pk::Mma<T>::run(kf[s % kAheadK], qf[s], sn);
+                    if (s + kAheadK < KS) kf[s % kAheadK] = readK(x, s + kAheadK);
+                }
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) weigh(s0 / kChunk * kPairs + j);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (!allSee) mask(sn, i + 1, ahead);
+            float mx = fmaxf(sn[0], sn[1]);
+            multiply(at, [&](int k) {
+                constexpr int kEach = 16 / kFragV > 0 ? 16 / kFragV : 1;
+#pragma unroll
+                for (int j = k * kEach; j < (k + 1) * kEach; ++j)
+                    if (j >= 2 && j < 16) mx = fmaxf(mx, sn[j]);
+            });
+            l += pk::pair32_sum(ps);
+            follow(pk::pair32_max(mx) * c2);
+            st = sn;
+        };
         uint32_t at = 0;  // step i's place in the ring
-        for (uint32_t i = 0; i < n; ++i) {
+        for (uint32_t i = 0; i + 1 < n; ++i) {
             const uint32_t at1 = at == kRing - 1 ? 0 : at + 1, at2 = at1 == kRing - 1 ? 0 : at1 + 1;
             // step i + 1 is in LDS (copied in pass i - 1), and every wave has read what step i + 2 goes over
             wait_vmcnt<0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
+            ahead = ahead2;
+            allSee = allSee2;
             if (i + 2 < n) {
                 if (i + 2 - held0 == 32) hold(i + 2);
                 copy(i + 2, at2);
                 ahead2 = ends(i + 2);
+                allSee2 = all_see(i + 2, ahead2);
             }
-            f32x16 sn = st;
-            if (i + 1 < n) sn = scores(at1);
-            u32x4 pf[2], pr[2];
-            const float mref = m == -INFINITY ? 0.0f : m;
-            float ps = 0.0f;
-#pragma unroll
-            for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int e = ks * 8 + 2 * j;
-                    const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e], c2, -mref)), p1 = __builtin_amdgcn_exp2f(fmaf(st[e + 1], c2, -mref));
-                    ps += p0 + p1;
-                    const uint32_t v = pk::pack2<T>(p0, p1);
-                    pf[ks][j] = v;
-                    if constexpr (kTwo) pr[ks][j] = pk::pack2<T>(p0 - __uint_as_float(v << 16), p1 - __uint_as_float(v & 0xffff0000u));
-                }
-            l += pk::pair32_sum(ps);
-            const uint32_t s16 = lane & 15, dimHalf = lane >> 4 & 1;
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    auto readV = [&](uint32_t key) {
-                        const uint32_t chunk = (dt * 4 + dimHalf * 2 + (s16 & 3) / 2) ^ swzV(key);
-                        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                             (lds_s16x4 *)(sV + at * kTileBytes + (key * CH + chunk) * 16 + (s16 & 1) * 8)));
-                    };
-                    const u32x2 a = readV(ks * 16 + h * 4 + s16 / 4), b = readV(ks * 16 + 8 + h * 4 + s16 / 4);
-                    const u32x4 va = {a.x, a.y, b.x, b.y};
-                    acc[dt] = pk::Mma<T>::run(va, pf[ks], acc[dt]);
-                    if constexpr (kTwo) acc[dt] = pk::Mma<T>::run(va, pr[ks], acc[dt]);
-                }
-            if (i + 1 < n) {
-                mask(sn, i + 1, ahead);
-                ahead = ahead2;
-                follow(highest(sn));
-                st = sn;
-            }
+            pass(i, at, at1);
             at = at1;
         }
+        start_weights();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) weigh(j);
+        l += pk::pair32_sum(ps);
+        multiply(at, [](int) {});
         // every wave has read its last tiles before the next piece's copies
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_s_barrier();
