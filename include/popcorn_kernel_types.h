@@ -460,7 +460,8 @@ typedef struct {
  * unitSteps more than it has (what a unit costs beside its steps). A launch
  * takes the requests of fewRows < rows <= manyRows. ownPlan: every block lays
  * the tiles out by itself (at most 1024, all their steps below 2^31), else
- * paged_plan has. A launch's partial states begin at row stateBase. */
+ * paged_plan has. A launch's partial states begin at row stateBase.
+ * stream: V is read past the caches. */
 typedef struct {
     uint32_t rows;
     uint32_t stepKeys;
@@ -472,6 +473,7 @@ typedef struct {
     uint32_t unitSteps;
     uint32_t ownPlan;
     uint32_t stateBase;
+    uint32_t stream;
 } PagedWorkConstants;
 
 /* sample_*: one token of each row of logits [rows, vocab]; a row is cut into

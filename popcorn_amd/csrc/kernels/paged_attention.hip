@@ -6,6 +6,7 @@
 
 #include "mfma.hpp"
 #include "paged.hpp"
+#include "scan.hpp"
 
 namespace {
 
@@ -82,27 +83,6 @@ __device__ inline uint64_t first_lane64(uint64_t v) {
     return (uint64_t)first_lane((uint32_t)(v >> 32)) << 32 | first_lane((uint32_t)v);
 }
 
-// Inclusive sum of v over the block (`sums`: one entry per wave), and the total.
-template <typename U>
-__device__ inline U block_scan(U v, U *sums, U &total) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const U x = __shfl_up(v, d);
-        if (lane >= d) v += x;
-    }
-    __syncthreads();
-    if (lane == 63) sums[wave] = v;
-    __syncthreads();
-    total = 0;
-    U before = 0;
-    for (uint32_t w = 0; w < blockDim.x / 64; ++w) {
-        if (w == wave) before = total;
-        total += sums[w];
-    }
-    return before + v;
-}
-
 template <uint32_t N, typename U>
 struct PlanSpace {  // of a block of N threads
     U sums[N / 64];
@@ -123,8 +103,8 @@ __device__ inline void lay_tiles(const int32_t *starts, const int32_t *keyLens, 
         if (r < p.R) q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
         const uint32_t rows = (uint32_t)q.n * G;
         const uint32_t mine = rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
-        U total;
-        const U upto = block_scan((U)mine, sp.sums, total);
+        const pk::Scan<U> of = pk::block_scan<N / 64>((U)mine, sp.sums);
+        const U upto = of.upto, total = of.total;
         // overlapping ranges of requests could hold more rows than there are: what passes the plan's room is left out
         const uint32_t here = (uint32_t)min(total, (U)(w.maxTiles - tiles));
         sp.tile[tid] = (uint32_t)min(upto - mine, (U)here);
@@ -139,17 +119,16 @@ __device__ inline void lay_tiles(const int32_t *starts, const int32_t *keyLens, 
                     if (sp.tile[i + d] <= t) i += d;
                 n = pk::paged_steps(sp.req[i], t - sp.tile[i], p, w).n + w.unitSteps;
             }
-            U sum;
-            const U end = block_scan((U)n, sp.sums, sum);
-            if (t < here) put(tiles + t, steps + end - n, base + i, t - sp.tile[i]);
-            steps += sum;
+            const pk::Scan<U> sum = pk::block_scan<N / 64>((U)n, sp.sums);
+            if (t < here) put(tiles + t, steps + sum.upto - n, base + i, t - sp.tile[i]);
+            steps += sum.total;
         }
         tiles += here;
         __syncthreads();
     }
 }
 
-typedef unsigned long long u64;
+typedef uint64_t u64;
 
 }  // namespace
 
@@ -235,6 +214,9 @@ struct Dealer {
     uint64_t share, x, end;
     uint32_t tile;
 
+    // The worker of step at of all units.
+    __device__ inline uint32_t last_of(uint64_t at) const { return (at | share) >> 32 ? (uint32_t)(at / share) : (uint32_t)at / (uint32_t)share; }
+
     // `space` is free again afterwards.
     __device__ inline Dealer(const int32_t *st, const int32_t *kl, const pk::PagedTile *pl, OwnTile *ow, PlanSpace<NT, uint32_t> &space,
                              Shared *sh, const PagedAttentionConstants &p, const PagedWorkConstants &w)
@@ -256,8 +238,8 @@ struct Dealer {
         x = first_lane64(blockIdx.x * share);
         end = first_lane64(min(x + share, total));
         if (x < end) {
-            tile = w.ownPlan ? find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return own[i].before; })
-                             : find_tile(tiles, x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
+            tile = w.ownPlan ? find_tile(tiles, x >> 32 ? x / p.Nkv : (uint32_t)x / p.Nkv, [&](uint32_t i) { return own[i].before; })
+                             : find_tile(tiles, x >> 32 ? x / p.Nkv : (uint32_t)x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
         } else if (threadIdx.x == 0) {
             shared->pieces = 0;
         }
@@ -279,7 +261,7 @@ struct Dealer {
             c.steps = pk::paged_steps(c.req, t.tile, p, w);
             const uint64_t in = x - t.before * p.Nkv;  // counted steps before x of this tile's units
             const uint32_t n = c.steps.n + w.unitSteps;
-            c.hkv = (uint32_t)(in / n);
+            c.hkv = in >> 32 ? (uint32_t)(in / n) : (uint32_t)in / n;  // (64 bits take ten times as long)
             const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * n), hi = (uint32_t)min((uint64_t)n, lo + (end - x));
             c.lo = max(lo, w.unitSteps) - w.unitSteps;
             c.hi = max(hi, w.unitSteps) - w.unitSteps;
@@ -287,7 +269,7 @@ struct Dealer {
             if (hi == n && c.hkv + 1 == p.Nkv) ++tile;
             if (x == end && threadIdx.x == 0) {
                 Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, w.rows, w.stateBase, blockIdx.x};
-                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = (uint32_t)((end + (n - hi) - 1) / share - blockIdx.x) + 1;
+                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = last_of(end + (n - hi) - 1) - blockIdx.x + 1;
                 *shared = sh;
             }
             if (c.lo < c.hi) return true;
@@ -422,7 +404,9 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
                     const uint32_t row = i / kHalves * kRowsPer + (kHalves > 1 ? 0u : lane / CH);
                     const uint32_t chunk = ((i % kHalves) * 64 + lane % CH) ^ swz(row);
                     const int off = chunk * E < D ? (int)((row * D + chunk * E) * sizeof(S)) : kOutOfRange;
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(from[mt].v, (lds_void *)(sV + (mt * 16 / kRowsPer * kHalves + i) * 1024), 16, off, 0, 0, 0);
+                    lds_void *to = (lds_void *)(sV + (mt * 16 / kRowsPer * kHalves + i) * 1024);
+                    if (w.stream) __builtin_amdgcn_raw_ptr_buffer_load_lds(from[mt].v, to, 16, off, 0, 0, 2);  // (not to be kept)
+                    else __builtin_amdgcn_raw_ptr_buffer_load_lds(from[mt].v, to, 16, off, 0, 0, 0);
                 }
         };
 
@@ -511,6 +495,22 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
             }
             wait_vmcnt<(KM * KS < 63 ? KM * KS : 63)>();  // the V copies; the next step's K loads stay in flight
             asm volatile("" ::: "memory");
+            // V's fragments, kAhead of them before their products
+            constexpr int kAhead = HD <= 64 ? 3 : HD <= 128 ? 4 : 0;  // (0: the registers are taken)
+            u32x4 va[kAhead + 1];
+            auto readV = [&](int dt) {
+                auto four = [&](uint32_t key) {
+                    const uint32_t chunk = (2 * dt + (c16 & 3) / 2) ^ swz(key);
+                    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sV + (key * CH + chunk) * 16 + (c16 & 1) * 8)));
+                };
+                const u32x2 a = four(4 * g + c16 / 4), b = four(16 + 4 * g + c16 / 4);
+                return u32x4{a.x, a.y, b.x, b.y};
+            };
+            if constexpr (!kWide && kAhead > 0) {
+#pragma unroll
+                for (int dt = 0; dt < kAhead; ++dt) va[dt] = readV(dt);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 if constexpr (kWide) {
@@ -522,17 +522,12 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
                         for (int rt = 0; rt < RT; ++rt) acc[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(va, pw[rt][e], acc[rt][dt], 0, 0, 0);
                     }
                 } else {
-                    auto readV = [&](uint32_t key) {
-                        const uint32_t chunk = (2 * dt + (c16 & 3) / 2) ^ swz(key);
-                        const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(sV + (key * CH + chunk) * 16 + (c16 & 1) * 8));
-                        return __builtin_bit_cast(u32x2, v);
-                    };
-                    const u32x2 a = readV(4 * g + c16 / 4), b = readV(16 + 4 * g + c16 / 4);
-                    const u32x4 va = {a.x, a.y, b.x, b.y};
+                    if (dt + kAhead < DT) va[(dt + kAhead) % (kAhead + 1)] = readV(dt + kAhead);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                        for (int e = 0; e < kParts; ++e) acc[rt][dt] = pk::Mma16<T>::run(va, pf[rt][e], acc[rt][dt]);
+                        for (int e = 0; e < kParts; ++e) acc[rt][dt] = pk::Mma16<T>::run(va[dt % (kAhead + 1)], pf[rt][e], acc[rt][dt]);
+                    if constexpr (kAhead > 0) __builtin_amdgcn_sched_barrier(0);
                 }
             }
             __builtin_amdgcn_s_waitcnt(0xC07F);  // this wave's reads of its V tile are done before it is overwritten
@@ -628,16 +623,15 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
 // Tiles of 128 rows, 32 to a wave, on v_mfma_f32_32x32x16: S^T = K . Q^T has a
 // row's scores in two lanes (mfma.hpp), so maxima and sums take one lane swap,
 // and a lane's weights are its P^T operand of O^T += V^T . P^T as they are.
-// K and V go from the pages straight into LDS, 16 keys (of one page) to a
-// resource, three steps of 32 keys deep; nothing waits for a copy younger
-// than two steps. K is read by rows, V by ds_read_b64_tr_b16 (four keys of a
-// dim to a lane); 16-byte chunks are swizzled so that the rows of one read
-// fall in different banks.
-// What bounds it: products and softmax take about as long (HD 128: 512 cycles
-// of MFMA and 480 of VALU for 32 keys), so step i + 1's scores are computed
+// Steps are 64 keys; wave w copies group w's 16 keys (of one page) of K and V
+// from the page straight into LDS, K two steps ahead and V one. K is read by
+// rows, V by ds_read_b64_tr_b16 (four keys of a dim to a lane); 16-byte chunks
+// are swizzled so that the rows of one read fall in different banks.
+// What bounds it: products and softmax take about as long (HD 128: 1024 cycles
+// of MFMA and 960 of VALU for a step), so step i + 1's scores are computed
 // beside step i's exponentials, and step i's product with V beside the
 // maximum of step i + 1.
-constexpr int kTileRows = 128, kRing = 3;
+constexpr int kTileRows = 128;
 
 template <typename T, int HD>
 __device__ void paged_tile(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
@@ -647,17 +641,16 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
                            Shared *__restrict__ shared, typename T::storage *__restrict__ out, const PagedAttentionConstants &p,
                            const PagedWorkConstants &w) {
     using S = typename T::storage;
-    constexpr int BKV = 32, KS = HD / 16, DT = HD / 32, CH = HD / 8;
-    constexpr int kRowsPer = 64 / CH;      // rows per copy instruction
-    constexpr int kCopies = 8 / kRowsPer;  // instructions for a wave's 8 rows of K (or V) of a step
+    constexpr int BKV = 64, KS = HD / 16, DT = HD / 32, CH = HD / 8;
+    constexpr int kRowsPer = 64 / CH;       // rows per copy instruction
+    constexpr int kCopies = 16 / kRowsPer;  // instructions for a wave's 16 rows of K (or V) of a step
     constexpr bool kTwo = std::is_same<T, pk::BF16>::value;  // weights as two bf16, or one f16
     constexpr float kLead = kTwo ? 0.0f : 4.0f;
     constexpr uint32_t kTileBytes = BKV * HD * 2;
-    // (one array: with two, the compiler has every read of LDS wait for the latest copy into it)
-    __shared__ __attribute__((aligned(256))) uint8_t smem[2 * kRing * kTileBytes + kOwnTiles * sizeof(OwnTile)];
-    static_assert(sizeof(PlanSpace<256, uint32_t>) <= 2 * kRing * kTileBytes, "the plan is laid out where K and V go");
-    uint8_t *sK = smem, *sV = smem + kRing * kTileBytes;
-    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 2 * kRing * kTileBytes);
+    // K's two places, V's two, the plan (one array: with two, the compiler has every read of LDS wait for the latest copy)
+    __shared__ __attribute__((aligned(256))) uint8_t smem[4 * kTileBytes + kOwnTiles * sizeof(OwnTile)];
+    static_assert(sizeof(PlanSpace<256, uint32_t>) <= 4 * kTileBytes, "the plan is laid out where K and V go");
+    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 4 * kTileBytes);
 
     const uint32_t lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
     const uint32_t wave = first_lane(threadIdx.x >> 6);
@@ -677,67 +670,59 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
         const uint32_t w0 = c.steps.r0 + wave * 32, myRow = w0 + c32, rowAt = min(myRow, c.steps.r1 - 1);
         const int pos = c.req.pos0 + (int)(rowAt / G);
         const int posLo = c.req.pos0 + (int)(min(w0, c.steps.r1 - 1) / G), posHi = c.req.pos0 + (int)(min(w0 + 31, c.steps.r1 - 1) / G);
-        u32x4 qf[KS];
-        {
-            const S *row = Q + q_row(rowAt) * D + h * 8;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                qf[s] = s * 16 + h * 8 < D ? *reinterpret_cast<const u32x4 *>(row + s * 16) : u32x4{0u, 0u, 0u, 0u};
-                qf[s] ^= flip;
-            }
-        }
-
-        // Lane l holds page and row in it of group l % 2 of the piece's step held0 + l / 2 (no page: -1).
+        // Lane l holds, of group l % 4 of the piece's step held0 + l / 4, the bytes from K's (V's) start and the rows that
+        // a page holds (0: none); of the step, all four groups' rows (a byte each) and whether all rows of the wave see all keys.
         const uint32_t n = c.hi - c.lo;
-        uint32_t held0 = 0, heldPage = 0, heldRow = 0;
+        uint32_t held0 = 0, heldLo = 0, heldHi = 0, heldRows = 0, heldAll = 0;
+        uint64_t heldSee = 0;
         auto hold = [&](uint32_t i) {
-            const uint32_t at = i + lane / 2;
+            const uint32_t at = i + lane / 4;
             held0 = i;
-            heldPage = ~0u;
-            heldRow = 0;
-            if (at < n) {
-                const uint32_t key = pk::paged_step_key(c.steps, c.lo + at, w) + lane % 2 * 16, column = key / p.pageSize;
-                if (key < keys) {
-                    heldPage = (uint32_t)table[column];
-                    heldRow = key - column * p.pageSize;
+            uint64_t off = 0;
+            heldRows = 0;
+            const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + at, w), key = key0 + lane % 4 * 16;
+            if (at < n && key < keys) {
+                const uint32_t column = key / p.pageSize, page = (uint32_t)table[column];
+                if (page < p.pages) {
+                    off = (((uint64_t)page * p.Nkv + c.hkv) * p.pageSize + (key - column * p.pageSize)) * (D * 2);
+                    heldRows = min(16u, keys - key);
                 }
             }
+            heldLo = (uint32_t)off;
+            heldHi = (uint32_t)(off >> 32);
+            auto of_quad = [&](auto ctrl) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)heldRows, decltype(ctrl)::value, 0xf, 0xf, false); };
+            heldAll = of_quad(std::integral_constant<int, 0x00>{}) | of_quad(std::integral_constant<int, 0x55>{}) << 8 |
+                      of_quad(std::integral_constant<int, 0xaa>{}) << 16 | of_quad(std::integral_constant<int, 0xff>{}) << 24;
+            const bool see = heldAll == 0x10101010u &&
+                             (p.maskKind == 2u || ((int)key0 + BKV - 1 <= posLo && (p.maskKind == 0u || (int64_t)posHi - key0 < p.slidingWindow ||
+                                                                                    key0 + BKV - 1 < p.sinks)));
+            heldSee = __ballot(see);
         };
-        // Copies step i's K and V into ring place `at`: wave w rows 8 w .. 8 w + 7. Rows that no page holds become zeros.
-        auto copy = [&](uint32_t i, uint32_t at) {
-            const uint32_t from = (i - held0) * 2 + wave / 2;
-            const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)from);
-            const uint32_t row = (uint32_t)__builtin_amdgcn_readlane((int)heldRow, (int)from);
-            const uint32_t key = pk::paged_step_key(c.steps, c.lo + i, w) + wave / 2 * 16;
-            const bool ok = page < p.pages;
-            const uint64_t off = ok ? (((uint64_t)page * p.Nkv + c.hkv) * p.pageSize + row) * D : 0;
-            const int bytes = ok ? (int)(min(16u, keys - key) * D * 2) : 0;
-            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(K + off), 0, bytes, 0x00020000);
-            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(V + off), 0, bytes, 0x00020000);
-#pragma unroll
-            for (int j = 0; j < kCopies; ++j) {
-                const uint32_t r16 = wave % 2 * 8 + j * kRowsPer + lane / CH, r32 = wave * 8 + j * kRowsPer + lane / CH;
-                const uint32_t ck = lane % CH ^ swzK(r32), cv = lane % CH ^ swzV(r32);
-                const uint32_t to = at * kTileBytes + (wave * 8 + j * kRowsPer) * HD * 2;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (lds_void *)(sK + to), 16, ck * 8 < D ? (int)((r16 * D + ck * 8) * 2) : kOutOfRange, 0, 0, 0);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (lds_void *)(sV + to), 16, cv * 8 < D ? (int)((r16 * D + cv * 8) * 2) : kOutOfRange, 0, 0, 0);
-            }
+        // The wave's group of step i of K (V); of a step behind the last, nothing. Rows that no page holds are read as zeros.
+        auto group = [&](const S *from, uint32_t i) {
+            const int at = (int)(((i < n ? i : held0) - held0) * 4 + wave);
+            const uint64_t off = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)heldHi, at) << 32 |
+                                 (uint32_t)__builtin_amdgcn_readlane((int)heldLo, at);
+            const int bytes = i < n ? __builtin_amdgcn_readlane((int)heldRows, at) * (int)(D * 2) : 0;
+            return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<uint8_t *>(const_cast<S *>(from)) + off, 0, bytes, 0x00020000);
         };
-        // Where the keys that a page holds end in the two groups of step i.
-        struct Ends {
-            uint32_t e[2];
+        // Instruction j of kCopies of a group's copy into the place at `to`.
+        auto copy = [&](__amdgpu_buffer_rsrc_t rs, uint32_t to, int j, auto &&swz) {
+            const uint32_t row = j * kRowsPer + lane / CH, chunk = lane % CH ^ swz(row);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(smem + to + (wave * 16 + j * kRowsPer) * HD * 2), 16,
+                                                     chunk * 8 < D ? (int)((row * D + chunk * 8) * 2) : kOutOfRange, 0, 0, 0);
         };
-        auto ends = [&](uint32_t i) {
-            Ends x;
-#pragma unroll
-            for (uint32_t g = 0; g < 2; ++g) {
-                const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)((i - held0) * 2 + g));
-                const uint32_t key = pk::paged_step_key(c.steps, c.lo + i, w) + g * 16;
-                x.e[g] = page < p.pages ? min(key + 16, keys) : key;
-            }
-            return x;
+        auto copyK = [&](__amdgpu_buffer_rsrc_t rs, uint32_t i, int j) { copy(rs, i % 2 * kTileBytes, j, swzK); };
+        auto copyV = [&](__amdgpu_buffer_rsrc_t rs, uint32_t i, int j) { copy(rs, (2 + i % 2) * kTileBytes, j, swzV); };
+        struct Ahead {
+            uint32_t rows;  // a byte per group
+            bool see;
+        };
+        auto ahead_of = [&](uint32_t i) {
+            return Ahead{(uint32_t)__builtin_amdgcn_readlane((int)heldAll, (int)((i - held0) * 4)), (heldSee >> ((i - held0) * 4) & 1) != 0};
         };
 
+        u32x4 qf[KS];
         f32x16 acc[DT];
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -745,50 +730,46 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
             for (int i = 0; i < 16; ++i) acc[dt][i] = 0.0f;
         float m = -INFINITY, l = 0.0f;
 
-        // LDS offsets of this lane's K and V, in a ring place: the other fragments' are these with bits 5 to 7 turned over
-        // (a step's 16-byte chunks s and s + 8 are 256 bytes apart), and constant distances. Kept from being computed
+        // LDS offsets of this lane's K and V, in a place: the other fragments' are these with bits 5 to 7 turned over
+        // (a row's 16-byte chunks s and s + 8 are 256 bytes apart), and constant distances. Kept from being computed
         // once for all fragments (48 registers).
         const uint32_t kAt = c32 * (HD * 2) + (h ^ swzK(c32)) * 16;
         const uint32_t s16 = lane & 15, swz4 = CH >= 16 ? s16 / 4 : s16 / 8;
-        const uint32_t vAt = kRing * kTileBytes + (h * 4 + s16 / 4) * (HD * 2) + swz4 * 64 + (lane >> 4 & 1) * 32 + (s16 & 3) * 8;
-        auto in_place = [](uint32_t lane0, uint32_t at) {
-            uint32_t x = lane0 + at * kTileBytes;
+        const uint32_t vAt = 2 * kTileBytes + (h * 4 + s16 / 4) * (HD * 2) + swz4 * 64 + (lane >> 4 & 1) * 32 + (s16 & 3) * 8;
+        auto in_place = [](uint32_t lane0, uint32_t i) {
+            uint32_t x = lane0 + i % 2 * kTileBytes;
             asm volatile("" : "+v"(x));
             return x;
         };
-        auto readK = [&](uint32_t x, int s) { return *reinterpret_cast<const u32x4 *>(smem + ((x ^ (s & 7) * 32u) + (s >> 3) * 256u)); };
-        // fragment ks of dims 32 dt .. + 31: this lane's 4 + 4 keys of one dim
-        auto readV = [&](uint32_t x, int dt, int ks) {
-            const uint32_t y = (x ^ (dt & 3) * 64u) + (dt >> 2) * 256u + ks * (16 * HD * 2);
+        // fragment f: dims 16 (f % KS) .. + 15 of keys 32 (f / KS) + c32
+        auto readK = [&](uint32_t x, int f) {
+            const int s = f % KS;
+            return *reinterpret_cast<const u32x4 *>(smem + ((x ^ (s & 7) * 32u) + (s >> 3) * 256u + f / KS * (32 * HD * 2)));
+        };
+        // fragment f: this lane's 4 + 4 keys of the 16 from 16 (f % 4) on, one dim of 32 (f / 4) .. + 31
+        auto readV = [&](uint32_t x, int f) {
+            const int dt = f / 4;
+            const uint32_t y = (x ^ (dt & 3) * 64u) + (dt >> 2) * 256u + f % 4 * (16 * HD * 2);
             const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(smem + y)));
             const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(smem + y + 8 * HD * 2)));
             return u32x4{a.x, a.y, b.x, b.y};
         };
-        // Whether every row of the wave sees every key of step i.
-        auto all_see = [&](uint32_t i, const Ends &x) {
-            const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + i, w);
-            return x.e[0] == key0 + 16 && x.e[1] == key0 + 32 &&
-                   (p.maskKind == 2u || ((int)key0 + 31 <= posLo &&
-                                         (p.maskKind == 0u || (int64_t)posHi - key0 < p.slidingWindow || key0 + 31 < p.sinks)));
+        struct Scores {
+            f32x16 half[2];  // of 32 keys each
         };
         // Hides what the rows do not see of step i.
-        auto mask = [&](f32x16 &st, uint32_t i, const Ends &x) {
+        auto mask = [&](Scores &s, uint32_t i, uint32_t rows) {
             const uint32_t key0 = pk::paged_step_key(c.steps, c.lo + i, w);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const uint32_t key = key0 + (j >> 2) * 8 + h * 4 + (j & 3);
-                const bool seen = (key < x.e[j / 8]) & pk::paged_sees(pos, (int)key, p);
-                st[j] = seen ? st[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) {
+                const uint32_t in = (j >> 2) * 8 + h * 4 + (j & 3);  // groups of 16: j / 8
+                const bool seen = (in % 16 < (rows >> j / 8 * 8 & 0xffu)) & pk::paged_sees(pos, (int)(key0 + in), p);
+                s.half[j / 16][j % 16] = seen ? s.half[j / 16][j % 16] : -INFINITY;
             }
         };
-        auto highest = [&](const f32x16 &st) {
-            float mx = fmaxf(st[0], st[1]);
-#pragma unroll
-            for (int j = 2; j < 16; ++j) mx = fmaxf(mx, st[j]);
-            return pk::pair32_max(mx) * c2;
-        };
         // Moves the rows' reference to a maximum that passes it by more than the gap.
-        auto follow = [&](float mx) {
+        auto follow = [&](float highest) {
+            const float mx = pk::pair32_max(highest) * c2;
             const bool move = mx > m + (kRescaleGap + kLead);
             if (!__ballot(move)) return;
             float alpha = 1.0f;
@@ -800,126 +781,145 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
         };
-        f32x16 st;
-        u32x4 pf[2], pr[2];
+        Scores st;
+        u32x4 pf[4], pr[4];
         float mref = 0.0f, ps = 0.0f;
         // The weights of two of st's scores, as a word of the P^T operands.
         auto weigh = [&](int pair) {
-            const int ks = pair / 4, j = pair % 4, e = 2 * pair;
-            const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e], c2, -mref)), p1 = __builtin_amdgcn_exp2f(fmaf(st[e + 1], c2, -mref));
+            const int e = pair % 8 * 2;
+            const f32x16 &x = st.half[pair / 8];
+            const float p0 = __builtin_amdgcn_exp2f(fmaf(x[e], c2, -mref)), p1 = __builtin_amdgcn_exp2f(fmaf(x[e + 1], c2, -mref));
             ps += p0 + p1;
             uint32_t v = pk::pack2<T>(p0, p1);
             if constexpr (kTwo) {
                 uint32_t r = pk::pack2<T>(p0 - __uint_as_float(v << 16), p1 - __uint_as_float(v & 0xffff0000u));
                 asm volatile("" : "+v"(r));
-                pr[ks][j] = r;
+                pr[pair / 4][pair % 4] = r;
             }
             asm volatile("" : "+v"(v));  // here, and not where it is used
-            pf[ks][j] = v;
+            pf[pair / 4][pair % 4] = v;
         };
         auto start_weights = [&] {
             mref = m == -INFINITY ? 0.0f : m;
             ps = 0.0f;
         };
-        // acc += V^T . P^T of the step at `at`, with `beside(k)` next to the product of fragment k. V is read kAheadV
+        // acc += V^T . P^T of step i, with `beside(f)` next to the product of fragment f. V is read kAheadV
         // fragments before its product.
-        constexpr int kFragV = DT * 2, kAheadV = 3;
-        auto multiply = [&](uint32_t at, auto &&beside) {
-            const uint32_t x = in_place(vAt, at);
+        constexpr int kFragV = DT * 4, kAheadV = 4, kFragK = KS * 2, kAheadK = 4;
+        auto multiply = [&](uint32_t i, auto &&beside) {
+            const uint32_t x = in_place(vAt, i);
             u32x4 va[kAheadV];
 #pragma unroll
-            for (int k = 0; k < kAheadV; ++k) va[k] = readV(x, k / 2, k % 2);
+            for (int f = 0; f < kAheadV; ++f) va[f] = readV(x, f);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = 0; k < kFragV; ++k) {
-                const int dt = k / 2, ks = k % 2;
-                acc[dt] = pk::Mma<T>::run(va[k % kAheadV], pf[ks], acc[dt]);
-                if constexpr (kTwo) acc[dt] = pk::Mma<T>::run(va[k % kAheadV], pr[ks], acc[dt]);
-                if (k + kAheadV < kFragV) va[k % kAheadV] = readV(x, (k + kAheadV) / 2, (k + kAheadV) % 2);
-                beside(k);
+            for (int f = 0; f < kFragV; ++f) {
+                acc[f / 4] = pk::Mma<T>::run(va[f % kAheadV], pf[f % 4], acc[f / 4]);
+                if constexpr (kTwo) acc[f / 4] = pk::Mma<T>::run(va[f % kAheadV], pr[f % 4], acc[f / 4]);
+                if (f + kAheadV < kFragV) va[f % kAheadV] = readV(x, f + kAheadV);
+                beside(f);
                 __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        // The scores of step i, with `beside(f)` next to the product of fragment f.
+        auto score = [&](uint32_t i, auto &&beside) {
+            Scores s;
+            const uint32_t x = in_place(kAt, i);
+            u32x4 kf[kAheadK];
+#pragma unroll
+            for (int f = 0; f < kAheadK; ++f) kf[f] = readK(x, f);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s.half[j / 16][j % 16] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int f = 0; f < kFragK; ++f) {
+                s.half[f / KS] = pk::Mma<T>::run(kf[f % kAheadK], qf[f % KS], s.half[f / KS]);
+                if (f + kAheadK < kFragK) kf[f % kAheadK] = readK(x, f + kAheadK);
+                beside(f);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return s;
         };
 
         hold(0);
-        copy(0, 0);
-        Ends ahead = ends(0);
-        bool allSee = all_see(0, ahead);
-        Ends ahead2 = ahead;  // of the step behind `ahead`'s
-        bool allSee2 = allSee;
-        if (n > 1) {
-            copy(1, 1);
-            ahead2 = ends(1);
-            allSee2 = all_see(1, ahead2);
+        {
+            const S *row = Q + q_row(rowAt) * D + h * 8;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) qf[s] = s * 16 + h * 8 < D ? *reinterpret_cast<const u32x4 *>(row + s * 16) : u32x4{0u, 0u, 0u, 0u};
         }
+        {
+            const __amdgpu_buffer_rsrc_t k0 = group(K, 0), v0 = group(V, 0), k1 = group(K, 1);
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                copyK(k0, 0, j);
+                copyV(v0, 0, j);
+                copyK(k1, 1, j);
+            }
+        }
+        Ahead next = ahead_of(0), next2 = n > 1 ? ahead_of(1) : next;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qf[s] ^= flip;
         wait_vmcnt<0>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        st = score(0, [](int) {});
+        if (!next.see) mask(st, 0, next.rows);
+        {
+            float mx = st.half[0][0];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) st[i] = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) st = pk::Mma<T>::run(readK(kAt, s), qf[s], st);
-        if (!allSee) mask(st, 0, ahead);
-        follow(highest(st));
+            for (int j = 1; j < 32; ++j) mx = fmaxf(mx, st.half[j / 16][j % 16]);
+            follow(mx);
+        }
         // Pass i: step i + 1's scores beside step i's weights, then step i's product with V beside the maximum of step
         // i + 1, in chunks that keep their order: products run while the vector instructions behind them issue.
-        auto pass = [&](uint32_t i, uint32_t at, uint32_t at1) {
-            constexpr int kAheadK = KS < 4 ? KS : 4, kChunk = KS >= 8 ? KS / 8 : 1, kPairs = 8 / (KS / kChunk);
-            f32x16 sn;
-            const uint32_t x = in_place(kAt, at1);
-            u32x4 kf[kAheadK];
-#pragma unroll
-            for (int s = 0; s < kAheadK; ++s) kf[s] = readK(x, s);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) sn[j] = 0.0f;
-            start_weights();
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int s0 = 0; s0 < KS; s0 += kChunk) {
-#pragma unroll
-                for (int s = s0; s < s0 + kChunk; ++s) {
-                    sn = pk::Mma<T>::run(kf[s % kAheadK], qf[s], sn);
-                    if (s + kAheadK < KS) kf[s % kAheadK] = readK(x, s + kAheadK);
-                }
-#pragma unroll
-                for (int j = 0; j < kPairs; ++j) weigh(s0 / kChunk * kPairs + j);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            if (!allSee) mask(sn, i + 1, ahead);
-            float mx = fmaxf(sn[0], sn[1]);
-            multiply(at, [&](int k) {
-                constexpr int kEach = 16 / kFragV > 0 ? 16 / kFragV : 1;
-#pragma unroll
-                for (int j = k * kEach; j < (k + 1) * kEach; ++j)
-                    if (j >= 2 && j < 16) mx = fmaxf(mx, sn[j]);
-            });
-            l += pk::pair32_sum(ps);
-            follow(pk::pair32_max(mx) * c2);
-            st = sn;
-        };
-        uint32_t at = 0;  // step i's place in the ring
         for (uint32_t i = 0; i + 1 < n; ++i) {
-            const uint32_t at1 = at == kRing - 1 ? 0 : at + 1, at2 = at1 == kRing - 1 ? 0 : at1 + 1;
-            // step i + 1 is in LDS (copied in pass i - 1), and every wave has read what step i + 2 goes over
+            // K of step i + 1 and V of step i are in LDS (copied in pass i - 1), and every wave has read what is copied over
             wait_vmcnt<0>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            ahead = ahead2;
-            allSee = allSee2;
+            next = next2;
+            const __amdgpu_buffer_rsrc_t rv = group(V, i + 1);
             if (i + 2 < n) {
-                if (i + 2 - held0 == 32) hold(i + 2);
-                copy(i + 2, at2);
-                ahead2 = ends(i + 2);
-                allSee2 = all_see(i + 2, ahead2);
+                if (i + 2 - held0 == 16) hold(i + 2);
+                next2 = ahead_of(i + 2);
             }
-            pass(i, at, at1);
-            at = at1;
+            const __amdgpu_buffer_rsrc_t rk = group(K, i + 2);
+            start_weights();
+            Scores sn = score(i + 1, [&](int f) {
+                // the copies, spread over the products: a CU takes 16 cycles for each, so the four waves' would wait in a row
+                constexpr int kEvery = kFragK / (2 * kCopies);
+                if (f % kEvery == 0) {
+                    const int j = f / kEvery;
+                    if (j < kCopies) copyK(rk, i + 2, j);
+                    else copyV(rv, i + 1, j - kCopies);
+                }
+                // the 16 pairs over the kFragK products
+                if constexpr (kFragK >= 16) {
+                    if (f % (kFragK / 16) == 0) weigh(f / (kFragK / 16));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16 / kFragK; ++j) weigh(f * (16 / kFragK) + j);
+                }
+            });
+            if (!next.see) mask(sn, i + 1, next.rows);
+            float mx = sn.half[0][0];
+            multiply(i, [&](int f) {
+                constexpr int kEach = 32 / kFragV;
+#pragma unroll
+                for (int j = f * kEach; j < (f + 1) * kEach; ++j) mx = fmaxf(mx, sn.half[j / 16][j % 16]);
+            });
+            l += pk::pair32_sum(ps);
+            follow(mx);
+            st = sn;
         }
+        wait_vmcnt<0>();  // V of the last step
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         start_weights();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) weigh(j);
+        for (int j = 0; j < 16; ++j) weigh(j);
         l += pk::pair32_sum(ps);
-        multiply(at, [](int) {});
+        multiply(n - 1, [](int) {});
         // every wave has read its last tiles before the next piece's copies
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_s_barrier();

@@ -1,26 +1,13 @@
 // The paged cache's bookkeeping: page_tables (tables, slots and positions of a
 // step's new tokens from the requests' lengths) and paged_kv_write_* (the new
 // tokens' K and V rows into their slots).
-#include "common.hpp"
+#include "scan.hpp"
 
 namespace {
 
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kPer = 4;                  // requests per thread and pass
 constexpr uint32_t kPass = kThreads * kPer;   // requests per pass
-
-// Inclusive sums over the wave of two counts.
-__device__ inline void wave_scan(uint64_t &a, uint64_t &b) {
-    const uint32_t lane = threadIdx.x & 63;
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint64_t x = __shfl_up((unsigned long long)a, d), y = __shfl_up((unsigned long long)b, d);
-        if (lane >= d) {
-            a += x;
-            b += y;
-        }
-    }
-}
 
 __device__ inline int32_t saturate(uint64_t v) { return v < 0x7fffffffu ? (int32_t)v : 0x7fffffff; }
 
@@ -62,8 +49,7 @@ POPCORN_KERNEL void __launch_bounds__(256)
             a += n[j];
             b += pages[j];
         }
-        uint64_t sa = a, sb = b;
-        wave_scan(sa, sb);
+        const uint64_t sa = pk::wave_scan(a), sb = pk::wave_scan(b);
         __syncthreads();  // the pass before has read the sums and the tables
         if ((tid & 63) == 63) {
             sWave[0][wave] = sa;

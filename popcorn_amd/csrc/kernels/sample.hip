@@ -20,7 +20,7 @@
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
 // More candidates than the list holds (thousands of equal logits at the cut)
 // are counted digit by digit of their logits instead (cut_by_digits).
-#include "common.hpp"
+#include "scan.hpp"
 
 namespace {
 
@@ -30,7 +30,12 @@ constexpr double kOne = 1099511627776.0;                // 2^40
 constexpr uint32_t kBins = SAMPLE_BINS, kList = SAMPLE_CANDIDATES;
 constexpr uint32_t kPerThread = kBins / kThreads;
 constexpr uint32_t kFound = 1024;                       // candidates that a block of sample_gather collects
-typedef unsigned long long u64;
+typedef uint64_t u64;
+using pk::Scan;
+using pk::wave_max_u32;
+using pk::wave_sum64;
+
+__device__ inline void add64(u64 *at, u64 v) { atomicAdd(reinterpret_cast<unsigned long long *>(at), (unsigned long long)v); }
 
 // A logit's place in the ranking: greater for greater logits, 0 for NaN, equal
 // for both zeros.
@@ -115,59 +120,6 @@ __device__ inline u64 limit_of(float p, u64 z) {
     return max(s + more, (u64)1);
 }
 
-// v of the lane that kCtrl names, 0 where there is none or kRows leaves the row out.
-template <int kCtrl, int kRows = 0xf>
-__device__ inline uint32_t moved(uint32_t v) {
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, false);
-}
-template <int kCtrl, int kRows = 0xf>
-__device__ inline u64 moved(u64 v) {
-    return (u64)moved<kCtrl, kRows>((uint32_t)(v >> 32)) << 32 | moved<kCtrl, kRows>((uint32_t)v);
-}
-__device__ inline uint32_t of_lane(uint32_t v, uint32_t lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane); }
-__device__ inline u64 of_lane(u64 v, uint32_t lane) { return (u64)of_lane((uint32_t)(v >> 32), lane) << 32 | of_lane((uint32_t)v, lane); }
-
-// Inclusive sums over a row of 16 lanes, and over the wave, in registers.
-template <typename U>
-__device__ inline U row_scan(U v) {
-    v += moved<0x111>(v);  // row_shr:1, 2, 4, 8
-    v += moved<0x112>(v);
-    v += moved<0x114>(v);
-    return v + moved<0x118>(v);
-}
-template <typename U>
-__device__ inline U wave_scan(U v) {
-    v = row_scan(v);
-    v += moved<0x142, 0xa>(v);         // lane 15 of a row to the odd row behind it
-    return v + moved<0x143, 0xc>(v);   // lane 31 to the upper half
-}
-__device__ inline u64 wave_sum64(u64 v) { return of_lane(wave_scan(v), 63); }
-__device__ inline uint32_t wave_max_u32(uint32_t v) {  // (0 is the least)
-    v = max(v, moved<0x111>(v));
-    v = max(v, moved<0x112>(v));
-    v = max(v, moved<0x114>(v));
-    v = max(v, moved<0x118>(v));
-    v = max(v, moved<0x142, 0xa>(v));
-    return of_lane(max(v, moved<0x143, 0xc>(v)), 63);
-}
-
-template <typename U>
-struct Scan {
-    U upto, total;
-};
-// Inclusive sums over the block of 16 waves, and the total.
-template <typename U>
-__device__ inline Scan<U> block_scan(U v, U *sums) {
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    static_assert(kWaves == 16, "one row of lanes");
-    v = wave_scan(v);
-    __syncthreads();
-    if (lane == 63) sums[wave] = v;
-    __syncthreads();
-    const U run = row_scan(sums[lane & 15]);
-    return {(wave ? of_lane(run, wave - 1) : 0) + v, of_lane(run, 15)};
-}
-
 // f(index, its place among the eight, logit) for this thread's logits of [lo, hi), eight in a row at a time.
 template <typename T, typename F>
 __device__ inline void each_logit(const typename T::storage *__restrict__ x, uint32_t lo, uint32_t hi, F &&f) {
@@ -239,14 +191,14 @@ __device__ void sample_hist(const typename T::storage *__restrict__ logits, cons
         const u64 u = w.weight(v);
         if (u == 0) return;
         const uint32_t b = w.bin(v);
-        atomicAdd(&sWeight[b], u);
+        add64(&sWeight[b], u);
         if (w.useK) atomicAdd(&sCount[b], 1u);
     });
     __syncthreads();
     uint64_t *mine = bins + (uint64_t)blockIdx.x * kBins;
     for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) {
         mine[b] = sWeight[b];
-        if (sWeight[b]) atomicAdd(reinterpret_cast<u64 *>(&row.weight[b]), sWeight[b]);
+        if (sWeight[b]) add64(&row.weight[b], sWeight[b]);
         if (sCount[b]) atomicAdd(&row.count[b], sCount[b]);
     }
 }
@@ -279,7 +231,7 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
             const u64 u = w.weight(v);
             sum += u >= w.least ? u : 0;
         });
-        sum = block_scan(sum, sSums).total;
+        sum = pk::block_scan<kWaves>(sum, sSums).total;
         if (tid == 0) row.weight[slice] = sum;
         return;
     }
@@ -293,9 +245,9 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
         mine += bw[j];
         here += bc[j];
     }
-    const Scan<u64> weights = block_scan(mine, sSums);
+    const Scan<u64> weights = pk::block_scan<kWaves>(mine, sSums);
     const u64 wend = weights.upto, total = weights.total;
-    const uint32_t cend = block_scan(here, sCounts).upto;
+    const uint32_t cend = pk::block_scan<kWaves>(here, sCounts).upto;
     if (tid == 0) {
         sFound = 0;
         sBin[0] = sBin[1] = sBin[2] = kBins;
@@ -450,12 +402,12 @@ __device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_
         before += w.bin(value(i)) < binK;
     }
     if (binK < kBins) {
-        const uint32_t beforeK = block_scan(before, s.counts).total;
+        const uint32_t beforeK = pk::block_scan<kWaves>(before, s.counts).total;
         kept = min(n, beforeK + needK);
         u64 part = 0;
 #pragma unroll 1
         for (uint32_t i = max(lo, beforeK); i < min(hi, kept); ++i) part += s.weights[i];
-        total = aboveK + block_scan(part, s.sums).total;
+        total = aboveK + pk::block_scan<kWaves>(part, s.sums).total;
     }
     if (w.useP) {
         const u64 limit = limit_of(w.p, total);
@@ -463,7 +415,7 @@ __device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_
         u64 mine = 0;
 #pragma unroll 1
         for (uint32_t i = lo; i < end; ++i) mine += w.bin(value(i)) < first ? 0 : s.weights[i];
-        u64 run = aboveP + block_scan(mine, s.sums).upto - mine;
+        u64 run = aboveP + pk::block_scan<kWaves>(mine, s.sums).upto - mine;
         uint32_t keep = 0;
 #pragma unroll 1
         for (uint32_t i = lo; i < end; ++i) {
@@ -471,7 +423,7 @@ __device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_
             keep += b < first || (b <= lastP && run < limit);
             run += b < first ? 0 : s.weights[i];
         }
-        kept = block_scan(keep, s.counts).total;
+        kept = pk::block_scan<kWaves>(keep, s.counts).total;
     }
     __syncthreads();
     return kept ? s.list[kept - 1] : 0;
@@ -494,11 +446,11 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
             each_logit<T>(x, 0, n, [&](uint32_t i, uint32_t, float v) {
                 const uint32_t key = rank_key(v);
                 if (shift < 24 && (key >> (shift + 8)) != prefix) return;
-                if (rank(v, i) >= cut) atomicAdd(&s.weights[(key >> shift) & 255u], measure(v));
+                if (rank(v, i) >= cut) add64(&s.weights[(key >> shift) & 255u], measure(v));
             });
             __syncthreads();
             // thread t takes digit 255 - t
-            const u64 mine = tid < 256 ? s.weights[255 - tid] : 0, run = block_scan(mine, s.sums).upto;
+            const u64 mine = tid < 256 ? s.weights[255 - tid] : 0, run = pk::block_scan<kWaves>(mine, s.sums).upto;
             if (run - mine < want && want <= run) {
                 s.bin = 255 - tid;
                 s.pick = run - mine;
@@ -516,7 +468,7 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
         };
         u64 count = 0;
         for (uint32_t i0 = lo; i0 < hi; i0 += 64) count += __popcll(__ballot(tie(i0 + lane)));
-        u64 before = block_scan(lane == 0 ? count : 0, s.sums).upto - count;  // the same in the wave's lanes
+        u64 before = pk::block_scan<kWaves>(lane == 0 ? count : 0, s.sums).upto - count;  // the same in the wave's lanes
         if (before < nth && nth <= before + count) {
             for (uint32_t i0 = lo; i0 < hi; i0 += 64) {
                 const u64 ties = __ballot(tie(i0 + lane)), here = __popcll(ties);
@@ -535,7 +487,7 @@ __device__ u64 cut_by_digits(RowSpace &s, const typename T::storage *__restrict_
     if (w.useP) {
         u64 z = 0;
         each_logit<T>(x, 0, n, [&](uint32_t i, uint32_t, float v) { z += rank(v, i) >= cut ? w.weight(v) : 0; });
-        move(limit_of(w.p, block_scan(z, s.sums).total), [&](float v) { return w.weight(v); });
+        move(limit_of(w.p, pk::block_scan<kWaves>(z, s.sums).total), [&](float v) { return w.weight(v); });
     }
     return cut;
 }
@@ -564,7 +516,7 @@ __device__ inline void find_token(RowSpace &s, const typename T::storage *__rest
             u[j] = in ? m : 0;
             mine += u[j];
         }
-        const Scan<u64> scan = block_scan(mine, s.sums);
+        const Scan<u64> scan = pk::block_scan<kWaves>(mine, s.sums);
         u64 run = before + scan.upto - mine;
         if (run <= target && target < run + mine) {
             uint32_t at = 0;
@@ -594,7 +546,7 @@ __device__ __attribute__((noinline)) void finish_by_digits(RowSpace &s, const ty
         const u64 m = w.weight(v);
         z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
     });
-    find_token<T>(s, x, w, cut, 0, n, 0, target_of(u, block_scan(z, s.sums).total), token);
+    find_token<T>(s, x, w, cut, 0, n, 0, target_of(u, pk::block_scan<kWaves>(z, s.sums).total), token);
 }
 
 template <typename T>
@@ -641,14 +593,14 @@ __device__ void sample_finish(const typename T::storage *__restrict__ logits, co
         for (uint32_t i = tid; i < n; i += kThreads)
             if (s.list[i] >= cut) {
                 const u64 m = w.weight(key_value((uint32_t)(s.list[i] >> 32)));
-                if (m >= w.least) atomicAdd(&s.slice[~(uint32_t)s.list[i] / c.sliceLen], m);
+                if (m >= w.least) add64(&s.slice[~(uint32_t)s.list[i] / c.sliceLen], m);
             }
     } else if (tid < c.slices) {
         s.slice[tid] = row.weight[tid];
     }
     __syncthreads();
     const u64 mine = tid < c.slices ? s.slice[tid] : 0;
-    const Scan<u64> scan = block_scan(mine, s.sums);
+    const Scan<u64> scan = pk::block_scan<kWaves>(mine, s.sums);
     const u64 run = scan.upto, target = target_of(o.uniforms[r], scan.total);
     if (run - mine <= target && target < run) {
         s.bin = tid;
@@ -685,7 +637,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
     if (w.useK || w.useP) {
         for (uint32_t i = tid; i < n; i += kThreads) z += w.weight(T::load(x[i]));
         // every token a candidate: top-k's bin is then the one that nothing lies before
-        cut = cut_in_list(s, w, n, 0, w.useK ? 0u : kBins, w.k, kBins, 0, 0, block_scan(z, s.sums).total);
+        cut = cut_in_list(s, w, n, 0, w.useK ? 0u : kBins, w.k, kBins, 0, 0, pk::block_scan<kWaves>(z, s.sums).total);
         z = 0;
     }
     for (uint32_t i = tid; i < n; i += kThreads) {
@@ -693,7 +645,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
         const u64 m = w.weight(v);
         z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
     }
-    find_token<T>(s, x, w, cut, 0, n, 0, target_of(o.uniforms[r], block_scan(z, s.sums).total), tokens + r);
+    find_token<T>(s, x, w, cut, 0, n, 0, target_of(o.uniforms[r], pk::block_scan<kWaves>(z, s.sums).total), tokens + r);
 }
 
 }  // namespace
