@@ -1,0 +1,205 @@
+"""GPU tests of the serving operators together, as a step of a server runs them:
+tables from the lengths, the new rows into their slots, attention over the pages,
+a token from the logits; eagerly, from a captured graph, on two streams at once."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import serving_ref as R
+from gpu_util import download, gpu_env, rounded, upload
+
+pytestmark = pytest.mark.gpu
+
+NQ, NKV, HD, PAGE, VOCAB = 8, 2, 128, 16, 5003
+
+
+@pytest.fixture(scope="module")
+def env():
+    return gpu_env()
+
+
+def i32(pa, x):
+    return pa.Tensor.from_numpy(np.asarray(x, np.int32), "i32")
+
+
+class Server:
+    """Caches and tensors of up to `requests` requests and `tokens` new tokens a step, and the step's kernels."""
+
+    def __init__(self, pa, stream, requests, tokens, pages, columns, seed):
+        self.pa, self.stream = pa, stream
+        self.g = np.random.default_rng(seed)
+        self.pages = pages
+        self.host_tables = np.full((requests, columns), -1, np.int64)
+        self.free = list(self.g.permutation(pages))
+        self.past = np.zeros(requests, np.int64)
+        shape = [pages, NKV, PAGE, HD]
+        self.k_cache, self.v_cache = (upload(pa, np.zeros(shape), "bf16") for _ in range(2))
+        self.host = [np.zeros(shape, np.float32) for _ in range(2)]
+        self.d = {n: i32(pa, np.zeros(s)) for n, s in dict(past=requests, new=requests, free=pages, tables=(requests, columns),
+                                                           starts=requests + 1, keys=requests, positions=tokens, slots=tokens,
+                                                           counts=2, tokens=requests).items()}
+        self.d["tables"].copy_from(self.host_tables.astype(np.int32))
+        self.q, self.out = (upload(pa, np.zeros((tokens, NQ, HD)), "bf16") for _ in range(2))
+        self.k, self.v = (upload(pa, np.zeros((tokens, NKV, HD)), "bf16") for _ in range(2))
+        self.logits = upload(pa, np.zeros((requests, VOCAB)), "bf16")
+        self.u = pa.Tensor.from_numpy(np.zeros(requests, np.float32))
+        self.top_p = pa.Tensor.from_numpy(np.full(requests, 0.9, np.float32))
+        self.top_k = i32(pa, np.full(requests, 40))
+        d, K = self.d, pa.Kernels
+        self.kernels = [
+            K.PageTables(d["past"], d["new"], d["free"], d["tables"], page_size=PAGE, query_starts=d["starts"], key_lens=d["keys"],
+                         positions=d["positions"], slots=d["slots"], counts=d["counts"]),
+            K.PagedKVCacheWrite(self.k, self.v, d["slots"], self.k_cache, self.v_cache),
+            K.PagedAttention(self.q, self.k_cache, self.v_cache, d["tables"], d["starts"], d["keys"], self.out, scale=0.09,
+                             mask=pa.AttentionMask.causal_sliding_window(48), sinks=4),
+            K.Sample(self.logits, self.u, d["tokens"], top_k=self.top_k, top_p=self.top_p)]
+
+    def feed(self, new):
+        """The step's inputs; what the step has to give."""
+        g, past, new = self.g, self.past, np.asarray(new)
+        T = self.q.shape[0]
+        free = np.array(self.free + [-1] * (self.pages - len(self.free)))
+        want = R.page_tables(past, new, np.array(self.free), self.host_tables, PAGE, T)
+        x = {n: rounded(g.standard_normal((T, h, HD)), "bf16") for n, h in (("q", NQ), ("k", NKV), ("v", NKV))}
+        logits, u, old = rounded(g.standard_normal((len(past), VOCAB)) * 2, "bf16"), g.random(len(past)), rounded(g.standard_normal((T, NQ, HD)), "bf16")
+        import oracle as O
+
+        s = self.stream
+        for t, a in ((self.q, x["q"]), (self.k, x["k"]), (self.v, x["v"]), (self.logits, logits), (self.out, old)):
+            t.copy_from(O.to_bits(a, O.BF16), s)
+        self.u.copy_from(u.astype(np.float32), s)
+        for n, a in (("past", past), ("new", new), ("free", free)):
+            self.d[n].copy_from(a.astype(np.int32), s)
+        self.host_tables = want[0]
+        for cache, rows in zip(self.host, (x["k"], x["v"])):
+            for t, slot in enumerate(want[4]):
+                if slot >= 0:
+                    cache[slot // PAGE, :, slot % PAGE] = rows[t]
+        att, parts = R.attention(x["q"], *self.host, want[0], want[1], want[2], old, float(np.float32(0.09)), 1, 48, 4)
+        self.free = self.free[want[5][1]:]
+        self.past = past + new
+        return want, att, parts, R.sample(logits, u, top_k=np.full(len(past), 40), top_p=np.full(len(past), 0.9))
+
+    def check(self, expected):
+        want, att, parts, tokens = expected
+        s, d = self.stream, self.d
+        for n, a in zip(("tables", "starts", "keys", "positions", "slots", "counts"), want):
+            np.testing.assert_array_equal(d[n].numpy(s), a)
+        for t, a in zip((self.k_cache, self.v_cache), self.host):
+            np.testing.assert_array_equal(download(t, s), a)
+        got = download(self.out, s)
+        assert (np.abs(got - att) <= R.attention_bound(att, parts, "bf16", HD)).all()
+        np.testing.assert_array_equal(d["tokens"].numpy(s), tokens)
+
+
+STEPS = [[70, 0, 33, 1, 200], [1, 16, 1, 0, 1], [1, 1, 1, 1, 1], [0, 0, 0, 0, 0], [90, 1, 1, 40, 1]]
+
+
+def test_steps(env):
+    pa, lib, stream, enc = env
+    server = Server(pa, stream, 5, 310, 60, 24, seed=1)
+    for new in STEPS:
+        expected = server.feed(new)
+        enc.encode(server.kernels)
+        stream.synchronize()
+        server.check(expected)
+
+
+class Graph:
+    """A capture of `body` on `stream` into an executable graph."""
+
+    def __init__(self, stream, body):
+        self.hip = ctypes.CDLL("libamdhip64.so")
+        self.stream = ctypes.c_void_p(stream.handle)
+        graph, self.exec = ctypes.c_void_p(), ctypes.c_void_p()
+        assert self.hip.hipStreamBeginCapture(self.stream, 0) == 0
+        body()
+        assert self.hip.hipStreamEndCapture(self.stream, ctypes.byref(graph)) == 0
+        assert self.hip.hipGraphInstantiate(ctypes.byref(self.exec), graph, None, None, ctypes.c_size_t(0)) == 0
+        self.hip.hipGraphDestroy(graph)
+
+    def launch(self):
+        assert self.hip.hipGraphLaunch(self.exec, self.stream) == 0
+
+    def close(self):
+        self.hip.hipGraphExecDestroy(self.exec)
+
+
+def test_steps_from_a_graph(env):
+    # captured once, replayed with other lengths, with eager work of another server between the replays
+    pa, lib, _, _ = env
+    stream = pa.Stream()
+    enc = pa.KernelCommandEncoder(lib, stream)
+    server, other = (Server(pa, stream, 5, 310, 60, 24, seed=s) for s in (2, 3))
+    graph = Graph(stream, lambda: enc.encode(server.kernels))
+    for new in STEPS:
+        expected = server.feed(new)
+        graph.launch()
+        stream.synchronize()
+        server.check(expected)
+        expected = other.feed(new[::-1])
+        enc.encode(other.kernels)
+        stream.synchronize()
+        other.check(expected)
+    graph.close()
+
+
+def test_steps_on_two_streams(env):
+    # an encoder (and its scratch) per stream: two servers' steps at once
+    pa, lib, _, _ = env
+    servers = []
+    for seed in (4, 5):
+        stream = pa.Stream()
+        servers.append((Server(pa, stream, 5, 310, 60, 24, seed=seed), pa.KernelCommandEncoder(lib, stream)))
+    for new in STEPS:
+        expected = [s.feed(new if i else new[::-1]) for i, (s, _) in enumerate(servers)]
+        for _ in range(3):  # (a step run again gives the same)
+            for s, enc in servers:
+                enc.encode(s.kernels)
+        for s, _ in servers:
+            s.stream.synchronize()
+        for e, (s, _) in zip(expected, servers):
+            s.check(e)
+
+
+def test_decoding_agrees_with_the_contiguous_cache(env):
+    # one request: FlashAttention over a contiguous cache gives what the pages give
+    pa, lib, stream, enc = env
+    g = np.random.default_rng(6)
+    n, keys = 5, 333
+    k, v = (rounded(g.standard_normal((1, NKV, keys, HD)), "bf16") for _ in range(2))
+    q = rounded(g.standard_normal((n, NQ, HD)), "bf16")
+    pages = -(-keys // PAGE)
+    ids = g.permutation(pages)
+    paged = []
+    for x in (k, v):
+        p = np.zeros((pages, NKV, PAGE, HD), np.float32)
+        for j in range(keys):
+            p[ids[j // PAGE], :, j % PAGE] = x[0, :, j]
+        paged.append(upload(pa, p, "bf16"))
+    o1, o2 = pa.Tensor.empty([1, NQ, n, HD], "bf16"), pa.Tensor.empty([n, NQ, HD], "bf16")
+    enc.encode(pa.Kernels.FlashAttention(upload(pa, q.transpose(1, 0, 2)[None], "bf16"), upload(pa, k, "bf16"), upload(pa, v, "bf16"), out=o1,
+                                         scale=0.09, batch=1, query_heads=NQ, kv_heads=NKV, query_len=n, key_len=keys, head_dim=HD),
+               pa.Kernels.PagedAttention(upload(pa, q, "bf16"), *paged, i32(pa, [ids]), i32(pa, [0, n]), i32(pa, [keys]), o2, scale=0.09))
+    stream.synchronize()
+    a, b = download(o1, stream)[0].transpose(1, 0, 2), download(o2, stream)
+    # two results within half a step of the value each, and near it before: at most a step of bf16 apart, or two at a border
+    assert (np.abs(a - b) <= 2 * 2.0 ** -8 * np.abs(a) + 1e-5).all()
+
+
+def test_scratch_that_is_refused(env):
+    # an allocator with nothing to give: the encode fails with its status, and nothing is left running
+    pa, lib, stream, _ = env
+
+    class Nothing(pa.KernelScratchAllocator):
+        def borrow(self, length):
+            raise MemoryError("none")
+
+    enc = pa.KernelCommandEncoder(lib, stream, Nothing())
+    server = Server(pa, stream, 5, 310, 60, 24, seed=7)
+    for kernel in server.kernels[2:]:
+        with pytest.raises(pa.PopcornError) as e:
+            enc.encode(kernel)
+        assert e.value.code == pa.PopcornError.TENSOR_ALLOCATION_FAILED
+    stream.synchronize()
