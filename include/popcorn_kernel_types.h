@@ -477,7 +477,8 @@ typedef struct {
 } PagedWorkConstants;
 
 /* sample_*: one token of each row of logits [rows, vocab]; a row is cut into
- * `slices` slices of `sliceLen` logits. */
+ * `slices` slices of `sliceLen` logits, which sample_gather takes by `parts`
+ * blocks. */
 typedef struct {
     uint32_t rows;
     uint32_t vocab;
@@ -487,6 +488,7 @@ typedef struct {
     uint32_t hasMinP;
     uint32_t slices;
     uint32_t sliceLen;
+    uint32_t parts;
 } SampleConstants;
 
 /* What the sample_* launches hand on of one row; beside it, the weight of each
@@ -507,8 +509,7 @@ typedef struct {
     uint32_t first;                        /* first bin where top-p, or else top-k, may cut */
     uint32_t binK;                         /* top-k's bin; SAMPLE_BINS: top-k keeps all */
     uint32_t needK;                        /* tokens of binK that top-k keeps */
-    uint32_t lastP;                        /* last bin where top-p may cut */
-    uint32_t pad;
+    uint32_t pad[2];                       /* (the bins of all slices stand behind the rows, read by 16 bytes) */
 } SampleRow;
 
 #ifdef __cplusplus

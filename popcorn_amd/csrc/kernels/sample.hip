@@ -13,7 +13,7 @@
 //  3. sample_gather: the bins in which the cuts must fall, from the bins'
 //     running sums; their tokens (the candidates, a few hundred of a large
 //     vocabulary) go to a list;
-//  4. sample_finish: sorts the candidates, finds the cuts among them, the
+//  4. sample_finish: the cuts among the candidates, by selection, the
 //     slice where the running weight passes the draw, and the token in it.
 // Only the second evaluates the whole row's weights. A row that neither top-k
 // nor top-p cuts has its slices' weights summed by the third instead.
@@ -28,7 +28,7 @@ constexpr uint32_t kThreads = 1024, kWaves = kThreads / 64;
 constexpr uint32_t E = 8;                               // consecutive logits per thread and step
 constexpr double kOne = 1099511627776.0;                // 2^40
 constexpr uint32_t kBins = SAMPLE_BINS, kList = SAMPLE_CANDIDATES;
-constexpr uint32_t kPerThread = kBins / kThreads;
+constexpr uint32_t kPerThread = kBins / kThreads, kEach = kList / kThreads, kFew = 128;
 constexpr uint32_t kFound = 1024;                       // candidates that a block of sample_gather collects
 typedef uint64_t u64;
 using pk::Scan;
@@ -55,6 +55,14 @@ struct Exp2Terms {
     }
 };
 
+// a * b + c of a c that is the same in all lanes, kept in scalar registers (the compiler's own choice adds into c,
+// which takes a copy of each constant first).
+__device__ inline double fma64(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
+
 // One row's options, and its highest logit.
 struct Row {
     float top, bins;  // bins per unit of distance
@@ -66,15 +74,14 @@ struct Row {
 
     __device__ inline u64 weight(float v) const {
         constexpr Exp2Terms terms;
-        if (!(v > -INFINITY)) return 0;
         const double t = ((double)v - (double)top) * rate;
         const double n = __builtin_rint(t), f = t - n;
         double s = terms.c[11];
 #pragma unroll
-        for (int k = 10; k >= 0; --k) s = __builtin_fma(s, f, terms.c[k]);
+        for (int k = 10; k >= 0; --k) s = fma64(s, f, terms.c[k]);
         // adding 2^52 rounds to a whole number and leaves it in the low bits
         const double w = __builtin_ldexp(s, (int)n + 40) + 4503599627370496.0;
-        const u64 u = t > -42.0 ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;  // (a NaN is 0)
+        const u64 u = (t > -42.0) & (v > -INFINITY) ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;  // (a NaN is 0)
         return v == top ? (u64)1 << 40 : u;
     }
     // Grows, if anything, from a logit to the next in the ranking.
@@ -120,9 +127,10 @@ __device__ inline u64 limit_of(float p, u64 z) {
     return max(s + more, (u64)1);
 }
 
-// f(index, its place among the eight, logit) for this thread's logits of [lo, hi), eight in a row at a time.
-template <typename T, typename F>
-__device__ inline void each_logit(const typename T::storage *__restrict__ x, uint32_t lo, uint32_t hi, F &&f) {
+// f(index, its place among the eight, logit) for this thread's logits of [lo, hi), eight in a row at a time;
+// after each eight done(index of the first).
+template <typename T, typename F, typename D>
+__device__ inline void each_logit(const typename T::storage *__restrict__ x, uint32_t lo, uint32_t hi, F &&f, D &&done) {
     struct Eight {
         typename T::storage v[E];
     };
@@ -137,7 +145,12 @@ __device__ inline void each_logit(const typename T::storage *__restrict__ x, uin
 #pragma unroll 1
             for (uint32_t j = i; j < hi; ++j) f(j, j - i, T::load(x[j]));
         }
+        done(i);
     }
+}
+template <typename T, typename F>
+__device__ inline void each_logit(const typename T::storage *__restrict__ x, uint32_t lo, uint32_t hi, F &&f) {
+    each_logit<T>(x, lo, hi, f, [](uint32_t) {});
 }
 
 // Clears what the launches after it add to.
@@ -218,21 +231,23 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
                               const SampleConstants &c) {
     __shared__ u64 sSums[kWaves], sAbove[2], sWith, sList[kFound];
     __shared__ uint32_t sCounts[kWaves], sBin[3], sNeed, sFound, sBase;
-    const uint32_t r = blockIdx.x / c.slices, slice = blockIdx.x % c.slices;
+    const uint32_t r = blockIdx.x / c.parts, part = blockIdx.x % c.parts;
     SampleRow &row = rows[r];
     const uint32_t tid = threadIdx.x;
     const Row w = row_of(o, r, top_of(row, c.slices), c);
     if (!w.live) return;
-    const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
     const typename T::storage *x = logits + (uint64_t)r * c.vocab;
     if (!(w.useK || w.useP)) {
-        u64 sum = 0;
-        each_logit<T>(x, lo, hi, [&](uint32_t, uint32_t, float v) {
-            const u64 u = w.weight(v);
-            sum += u >= w.least ? u : 0;
-        });
-        sum = pk::block_scan<kWaves>(sum, sSums).total;
-        if (tid == 0) row.weight[slice] = sum;
+        for (uint32_t slice = part; slice < c.slices; slice += c.parts) {
+            const uint32_t lo = slice * c.sliceLen, hi = min(lo + c.sliceLen, c.vocab);
+            u64 sum = 0;
+            each_logit<T>(x, lo, hi, [&](uint32_t, uint32_t, float v) {
+                const u64 u = w.weight(v);
+                sum += u >= w.least ? u : 0;
+            });
+            sum = pk::block_scan<kWaves>(sum, sSums).total;
+            if (tid == 0) row.weight[slice] = sum;
+        }
         return;
     }
     // bins before `first` are kept; candidates are the bins first .. lastP and binK
@@ -298,14 +313,13 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
     } else {
         first = lastP = binK;
     }
-    if (slice == 0 && tid == 0) {
+    if (part == 0 && tid == 0) {
         row.first = first;
         row.binK = binK;
         row.needK = sNeed;
         row.aboveK = sAbove[0];
         row.aboveP = sAbove[1];
         row.total = total;
-        row.lastP = lastP;
     }
     const float at = least_at(w);
     auto put = [&](uint32_t slot, u64 v) {
@@ -322,11 +336,15 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
             else put(atomicAdd(&row.candidates, 1u), c);
         }
     };
-    each_logit<T>(x, lo, hi, [&](uint32_t i, uint32_t j, float v) {
-        const uint32_t b = w.bin(v);
-        if ((v > -INFINITY) & (b < first ? least_bin(w, b, at) : (b <= lastP) | (b == binK))) found |= 1u << j;
-        if (j == E - 1 || i + 1 == hi) collect(i - j);
-    });
+    // the part's slices are next to each other
+    const uint32_t per = (c.slices + c.parts - 1) / c.parts * c.sliceLen, lo = min(part * per, c.vocab), hi = min(lo + per, c.vocab);
+    each_logit<T>(
+        x, lo, hi,
+        [&](uint32_t, uint32_t j, float v) {
+            const uint32_t b = w.bin(v);
+            found |= (uint32_t)((v > -INFINITY) & (b < first ? least_bin(w, b, at) : (b <= lastP) | (b == binK))) << j;
+        },
+        collect);
     __syncthreads();
     // the row's counter is one address for all its blocks: one addition each
     const uint32_t n = min(sFound, kFound);
@@ -337,96 +355,116 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
 
 struct RowSpace {
     u64 list[kList];
-    u64 sums[kWaves], slice[SAMPLE_MAX_SLICES], pick;
-    u64 weights[kList];
-    uint32_t counts[kWaves], ranks[256], bin;
+    u64 sums[kWaves], slice[SAMPLE_MAX_SLICES], pick, bits[2];
+    u64 weights[kThreads], few[kFew], measure[kFew];
+    uint32_t counts[kWaves], bin, left;
 };
 
-// Sorts list[0, n) from the greatest, by each entry's number of greater ones: n at most 256, all entries distinct.
-__device__ inline void rank_list(RowSpace &s, uint32_t n) {
-    const uint32_t e = threadIdx.x & 255, part = threadIdx.x >> 8;
-    if (threadIdx.x < 256) s.ranks[e] = 0;
-    __syncthreads();
-    u64 mine = 0;
-    if (e < n) {
-        mine = s.list[e];
-        uint32_t greater = 0;
-#pragma unroll 4
-        for (uint32_t j = part; j < n; j += 4) greater += s.list[j] > mine;
-        atomicAdd(&s.ranks[e], greater);
-    }
-    __syncthreads();
-    if (part == 0 && e < n) s.list[s.ranks[e]] = mine;
-    __syncthreads();
-}
-
-// The same for n a power of two of at least 128, by merging. Pairs up to 64
-// apart stay within the 128 entries of one wave, whose LDS accesses are in order.
-__device__ inline void merge_list(u64 *list, uint32_t n) {
-    __syncthreads();
-    for (uint32_t size = 2; size <= n; size <<= 1)
-        for (uint32_t d = size >> 1; d; d >>= 1) {
-            for (uint32_t t = threadIdx.x; t < n / 2; t += kThreads) {
-                const uint32_t i = 2 * t - (t & (d - 1)), j = i + d;
-                const u64 a = list[i], b = list[j];
-                if ((a < b) == ((i & size) == 0)) {
-                    list[i] = b;
-                    list[j] = a;
+// The entry at which the running measure m, over entries e (all distinct) from the greatest, reaches `want`: at
+// least 1, at most the sum. Entries of measure 0 are not looked at. While more than kFew are left, a pass keeps one
+// of 1024 values of the 10 bits from the highest in which they differ; the few are compared with each other.
+// (A sort by merging made sample_finish 34 us of 64 rows of 256000 bf16 logits, this 20; counting every entry's
+// greater ones made it 14.0 us of one row of 128256 with 100 candidates, this 15.5.)
+__device__ inline u64 select(RowSpace &s, const u64 (&e)[kEach], const u64 (&m)[kEach], u64 want) {
+    const uint32_t tid = threadIdx.x;
+    uint32_t left = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) left |= (uint32_t)(m[j] != 0) << j;
+    while (true) {
+        s.weights[tid] = 0;
+        if (tid < 2) s.bits[tid] = 0;
+        if (tid == 0) s.left = 0;
+        u64 ones = 0, zeros = 0;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j)
+            if (left >> j & 1) {
+                ones |= e[j];
+                zeros |= ~e[j];
+                const uint32_t at = atomicAdd(&s.left, 1u);
+                if (at < kFew) {
+                    s.few[at] = e[j];
+                    s.measure[at] = m[j];
                 }
             }
-            if (d > 64 || (d == 1 && size >= 128)) __syncthreads();
-            else asm volatile("" ::: "memory");
+        if (__ballot(left != 0)) {
+            ones = pk::wave_or64(ones);
+            zeros = pk::wave_or64(zeros);
+            if ((tid & 63) == 0) {
+                atomicOr(reinterpret_cast<unsigned long long *>(&s.bits[0]), (unsigned long long)ones);
+                atomicOr(reinterpret_cast<unsigned long long *>(&s.bits[1]), (unsigned long long)zeros);
+            }
         }
+        __syncthreads();
+        if (s.left <= kFew) break;
+        const int shift = max(63 - __clzll((long long)(s.bits[0] & s.bits[1])) - 9, 0);
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j)
+            if (left >> j & 1) add64(&s.weights[e[j] >> shift & 1023u], m[j]);
+        __syncthreads();
+        const uint32_t digit = 1023 - tid;
+        const u64 mine = s.weights[digit], run = pk::block_scan<kWaves>(mine, s.sums).upto;
+        if (run - mine < want && want <= run) {
+            s.bin = digit;
+            s.pick = run - mine;
+        }
+        __syncthreads();
+        want -= s.pick;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j) left &= ~((uint32_t)((e[j] >> shift & 1023u) != s.bin) << j);
+    }
+    // s.weights, cleared: each of the few's running measure, of a part of the others by each of its threads
+    const uint32_t few = s.left, at = tid % kFew;
+    const u64 mine = at < few ? s.few[at] : ~(u64)0;
+    u64 run = 0;
+#pragma unroll 4
+    for (uint32_t j = tid / kFew; j < few; j += kThreads / kFew) run += s.few[j] >= mine ? s.measure[j] : 0;
+    if (run) add64(&s.weights[at], run);
     __syncthreads();
+    run = s.weights[at];
+    if (tid < few && run - s.measure[at] < want && want <= run) s.pick = mine;
+    __syncthreads();
+    return s.pick;
 }
 
-// The last token that top-k and top-p keep, of n candidates in the list (in any order): rank key << 32 | ~index.
-// (Tokens of bins before `first` are in the list for min-p's sake, and kept.)
-__device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_t first, uint32_t binK, uint32_t needK, uint32_t lastP,
-                                  u64 aboveK, u64 aboveP, u64 total) {
-    const uint32_t tid = threadIdx.x;
-    uint32_t n2 = 256;
-    if (n <= n2) {
-        rank_list(s, n);
-    } else {
-        while (n2 < n) n2 <<= 1;
-        for (uint32_t i = n + tid; i < n2; i += kThreads) s.list[i] = 0;
-        merge_list(s.list, n2);
-    }
-    const uint32_t per = (n2 + kThreads - 1) / kThreads, lo = tid * per, hi = min(lo + per, n);  // a thread's candidates
-    auto value = [&](uint32_t i) { return key_value((uint32_t)(s.list[i] >> 32)); };
-    uint32_t before = 0, kept = n;
-#pragma unroll 1
-    for (uint32_t i = lo; i < hi; ++i) {
-        s.weights[i] = w.weight(value(i));
-        before += w.bin(value(i)) < binK;
+// The last token that top-k and top-p keep, of n candidates in the list (in any order): rank key << 32 | ~index; 0
+// keeps all. (Tokens of bins before `first` are in the list for min-p's sake, and kept.)
+__device__ inline u64 cut_in_list(RowSpace &s, const Row &w, uint32_t n, uint32_t first, uint32_t binK, uint32_t needK, u64 aboveK,
+                                  u64 aboveP, u64 total) {
+    u64 e[kEach], u[kEach], m[kEach], cut = 0, sum = 0;
+    uint32_t bins[kEach], count = 0;
+    __syncthreads();
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
+        const uint32_t i = threadIdx.x + j * kThreads;
+        e[j] = u[j] = m[j] = 0;
+        bins[j] = 0;
+        if (i < n) {
+            e[j] = s.list[i];
+            const float v = key_value((uint32_t)(e[j] >> 32));
+            u[j] = w.weight(v);
+            bins[j] = w.bin(v);
+            m[j] = bins[j] >= binK;
+            count += (uint32_t)m[j];
+        }
     }
     if (binK < kBins) {
-        const uint32_t beforeK = pk::block_scan<kWaves>(before, s.counts).total;
-        kept = min(n, beforeK + needK);
-        u64 part = 0;
-#pragma unroll 1
-        for (uint32_t i = max(lo, beforeK); i < min(hi, kept); ++i) part += s.weights[i];
-        total = aboveK + pk::block_scan<kWaves>(part, s.sums).total;
+        if (pk::block_scan<kWaves>(count, s.counts).total >= needK) cut = select(s, e, m, needK);
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j) sum += m[j] && e[j] >= cut ? u[j] : 0;
+        total = aboveK + pk::block_scan<kWaves>(sum, s.sums).total;
     }
     if (w.useP) {
-        const u64 limit = limit_of(w.p, total);
-        const uint32_t end = min(hi, kept);
-        u64 mine = 0;
-#pragma unroll 1
-        for (uint32_t i = lo; i < end; ++i) mine += w.bin(value(i)) < first ? 0 : s.weights[i];
-        u64 run = aboveP + pk::block_scan<kWaves>(mine, s.sums).upto - mine;
-        uint32_t keep = 0;
-#pragma unroll 1
-        for (uint32_t i = lo; i < end; ++i) {
-            const uint32_t b = w.bin(value(i));
-            keep += b < first || (b <= lastP && run < limit);
-            run += b < first ? 0 : s.weights[i];
+        sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kEach; ++j) {
+            m[j] = bins[j] >= first && e[j] >= cut ? u[j] : 0;
+            sum += m[j];
         }
-        kept = pk::block_scan<kWaves>(keep, s.counts).total;
+        const u64 want = limit_of(w.p, total) - aboveP;
+        if (pk::block_scan<kWaves>(sum, s.sums).total >= want) cut = select(s, e, m, want);
     }
-    __syncthreads();
-    return kept ? s.list[kept - 1] : 0;
+    return cut;
 }
 
 // The same cut for any number of candidates: the running measure over the
@@ -511,9 +549,12 @@ __device__ inline void find_token(RowSpace &s, const typename T::storage *__rest
 #pragma unroll
         for (uint32_t j = 0; j < E; ++j) {
             const float v = T::load(e.v[j]);
-            const u64 m = w.weight(v);
-            const bool in = (from + j < hi) & (m >= w.least) & (((u64)rank_key(v) << 32 | (uint32_t)~(from + j)) >= cut);
-            u[j] = in ? m : 0;
+            const bool in = (from + j < hi) & (((u64)rank_key(v) << 32 | (uint32_t)~(from + j)) >= cut);
+            u[j] = 0;
+            if (__ballot(in)) {  // (top-k leaves most waves none)
+                const u64 m = w.weight(v);
+                u[j] = in & (m >= w.least) ? m : 0;
+            }
             mine += u[j];
         }
         const Scan<u64> scan = pk::block_scan<kWaves>(mine, s.sums);
@@ -575,21 +616,21 @@ __device__ void sample_finish(const typename T::storage *__restrict__ logits, co
         for (uint32_t sl = wave; sl < c.slices; sl += kWaves) {
             const uint64_t *b = bins + ((uint64_t)r * c.slices + sl) * kBins;
             u64 sum = 0;
-            for (uint32_t i0 = lane; i0 < first; i0 += 512) {
-                u64 v[8];
+            for (uint32_t i0 = lane * 2; i0 < first; i0 += 1024) {
+                ulong2 v[8];  // (past the bins' end nothing is read: kBins is a multiple of 1024)
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) v[j] = b[min(i0 + 64 * j, kBins - 1)];
+                for (uint32_t j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const ulong2 *>(b + i0 + 128 * j);
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) {
-                    const uint32_t i = i0 + 64 * j;
-                    if (i < first && !least_bin(w, i, at) && (float)i < at) sum += v[j];
+                for (uint32_t j = 0; j < 16; ++j) {
+                    const uint32_t i = i0 + 128 * (j >> 1) + (j & 1);
+                    if (i < first && !least_bin(w, i, at) && (float)i < at) sum += j & 1 ? v[j >> 1].y : v[j >> 1].x;
                 }
             }
             sum = wave_sum64(sum);
             if (lane == 0) s.slice[sl] = sum;
         }
         __syncthreads();
-        cut = cut_in_list(s, w, n, first, row.binK, row.needK, row.lastP, row.aboveK, row.aboveP, row.total);
+        cut = cut_in_list(s, w, n, first, row.binK, row.needK, row.aboveK, row.aboveP, row.total);
         for (uint32_t i = tid; i < n; i += kThreads)
             if (s.list[i] >= cut) {
                 const u64 m = w.weight(key_value((uint32_t)(s.list[i] >> 32)));
@@ -637,7 +678,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
     if (w.useK || w.useP) {
         for (uint32_t i = tid; i < n; i += kThreads) z += w.weight(T::load(x[i]));
         // every token a candidate: top-k's bin is then the one that nothing lies before
-        cut = cut_in_list(s, w, n, 0, w.useK ? 0u : kBins, w.k, kBins, 0, 0, pk::block_scan<kWaves>(z, s.sums).total);
+        cut = cut_in_list(s, w, n, 0, w.useK ? 0u : kBins, w.k, 0, 0, pk::block_scan<kWaves>(z, s.sums).total);
         z = 0;
     }
     for (uint32_t i = tid; i < n; i += kThreads) {
@@ -660,7 +701,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
                                                                 SampleRow *rows, uint64_t *bins, SampleConstants c) {          \
         sample_hist<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, c);                         \
     }                                                                                                                          \
-    POPCORN_KERNEL void __launch_bounds__(1024)                                                                                 \
+    POPCORN_KERNEL void __launch_bounds__(1024, 8)                                                                              \
         sample_gather_##t(const T::storage *logits, SAMPLE_OPTIONS, SampleRow *rows, SampleConstants c) { \
         sample_gather<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, c);                             \
     }                                                                                                                          \

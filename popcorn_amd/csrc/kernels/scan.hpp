@@ -43,6 +43,14 @@ __device__ inline uint32_t wave_max_u32(uint32_t v) {  // (0 is the least)
     v = max(v, moved<0x142, 0xa>(v));
     return of_lane(max(v, moved<0x143, 0xc>(v)), 63);
 }
+__device__ inline uint64_t wave_or64(uint64_t v) {
+    v |= moved<0x111>(v);
+    v |= moved<0x112>(v);
+    v |= moved<0x114>(v);
+    v |= moved<0x118>(v);
+    v |= moved<0x142, 0xa>(v);
+    return of_lane(v | moved<0x143, 0xc>(v), 63);
+}
 
 template <typename U>
 struct Scan {

@@ -182,13 +182,15 @@ public:
         const int64_t rows = logits.shape[0], vocab = logits.shape[1];
         options_ = {uniforms};
         for (const Tensor *t : {temperature, topK, topP, minP}) options_.push_back(t ? *t : uniforms);  // (not read where absent)
-        sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab};
+        sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab, 1};
         small_ = vocab <= SAMPLE_CANDIDATES;
         if (small_ || rows == 0) return;
         // slices of 8192 logits or more, about 4 blocks per CU
         const int64_t slices = std::clamp<int64_t>(cdiv(4 * deviceCUs(), rows), 1, std::min<int64_t>(SAMPLE_MAX_SLICES, cdiv(vocab, 8192)));
         sc_.sliceLen = (uint32_t)cdiv(cdiv(vocab, slices), 8) * 8;
         sc_.slices = (uint32_t)cdiv(vocab, sc_.sliceLen);
+        // a block of sample_gather reads the row's bins first: no more of them than run at once (2 per CU)
+        sc_.parts = (uint32_t)std::clamp<int64_t>(2 * deviceCUs() / rows, 1, sc_.slices);
         if (rows * sc_.slices >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("Sample takes fewer rows; got " + logits.shape.str() + ".");
     }
     std::vector<Binding> tensors() const override {
@@ -219,7 +221,7 @@ public:
             };
             launch(enc, "sample_top_", {{logits_, kRead}, {rows, kWrite}}, blocks);
             if (cuts()) launch(enc, "sample_hist_", with({{rows, kReadWrite}, {bins, kWrite}}), blocks);
-            launch(enc, "sample_gather_", with({{rows, kReadWrite}}), blocks);
+            launch(enc, "sample_gather_", with({{rows, kReadWrite}}), n * sc_.parts);
             launch(enc, "sample_finish_", with({{rows, kRead}, {bins, kRead}, {tokens_, kWrite}}), n);
         });
     }
