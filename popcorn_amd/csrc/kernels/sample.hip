@@ -364,7 +364,7 @@ struct RowSpace {
 // least 1, at most the sum. Entries of measure 0 are not looked at. While more than kFew are left, a pass keeps one
 // of 1024 values of the 10 bits from the highest in which they differ; the few are compared with each other.
 // (A sort by merging made sample_finish 34 us of 64 rows of 256000 bf16 logits, this 20; counting every entry's
-// greater ones made it 14.0 us of one row of 128256 with 100 candidates, this 15.5.)
+// greater ones made it 14.0 us of one row of 256000 with about 100 candidates, this 15.5.)
 __device__ inline u64 select(RowSpace &s, const u64 (&e)[kEach], const u64 (&m)[kEach], u64 want) {
     const uint32_t tid = threadIdx.x;
     uint32_t left = 0;
