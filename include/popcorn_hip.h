@@ -562,7 +562,8 @@ popcorn_status_t popcorn_kernel_embedding_gather_quantized(const popcorn_tensor_
  * of page s / page_size. Row r of page_tables (i32 [R, columns]) names the
  * pages that hold request r's keys, page_size keys each, in order. All lengths
  * are read on the GPU, so a step captured into a graph is replayed with the
- * lengths that its tensors hold then. */
+ * lengths that its tensors hold then. Outputs that overlap an input or each
+ * other are refused, page tables aside, which PageTables updates in place. */
 
 /* The tables of one step. past_lens[r] keys of request r are in the cache
  * already, new_lens[r] tokens come (i32 [R]; a negative length counts as 0).
@@ -577,7 +578,7 @@ popcorn_status_t popcorn_kernel_embedding_gather_quantized(const popcorn_tensor_
  *   counts i32 [2]: tokens and free pages that the step needs.
  * T is positions' length. Where the free pages or the table's columns run out
  * the entry becomes -1 and the tokens' slots -1; tokens past T are left out.
- * Both show in counts. The outputs must not overlap the inputs. */
+ * Both show in counts. */
 popcorn_status_t popcorn_kernel_page_tables(const popcorn_tensor_t *past_lens, const popcorn_tensor_t *new_lens,
                                             const popcorn_tensor_t *free_pages, const popcorn_tensor_t *page_tables,
                                             int64_t page_size, const popcorn_tensor_t *query_starts,

@@ -38,6 +38,26 @@ void requireShape(const Tensor &t, DataType type, std::initializer_list<int64_t>
     requireTensor(t, what);
 }
 
+// Blocks read the inputs while others write: the outputs lie apart from them, and from each other.
+using Named = std::pair<const Tensor *, const char *>;
+void requireApart(const std::string &op, const std::vector<Named> &outputs, const std::vector<Named> &inputs) {
+    auto apart = [&](const Named &a, const Named &b) {
+        const auto at = reinterpret_cast<uintptr_t>(a.first->data), bt = reinterpret_cast<uintptr_t>(b.first->data);
+        const size_t an = a.first->byteCount(), bn = b.first->byteCount();
+        if (an && bn && at < bt + bn && bt < at + an)
+            throw Error::invalidArgument(op + " " + a.second + " must not overlap " + b.second + ".");
+    };
+    for (size_t i = 0; i < outputs.size(); ++i) {
+        for (size_t j = i + 1; j < outputs.size(); ++j) apart(outputs[i], outputs[j]);
+        for (const Named &in : inputs) apart(outputs[i], in);
+    }
+}
+
+// The runtime counts a grid's threads in 32 bits.
+void requireGrid(int64_t blocks, int64_t threads, const std::string &op, const Tensor &t) {
+    if (blocks > UINT32_MAX / threads) throw Error::tensorShapeMismatch(op + " takes fewer rows in one call; got " + t.shape.str() + ".");
+}
+
 // The caches [pages, Nkv, page size, Hd] of one shape and dtype.
 void requireCaches(const Tensor &k, const Tensor &v, const std::string &op) {
     requireRank(k, 4);
@@ -184,6 +204,7 @@ public:
         for (const Tensor *t : {temperature, topK, topP, minP}) options_.push_back(t ? *t : uniforms);  // (not read where absent)
         sc_ = SampleConstants{(uint32_t)rows, (uint32_t)vocab, temperature != nullptr, topK != nullptr, topP != nullptr, minP != nullptr, 1, (uint32_t)vocab, 1};
         small_ = vocab <= SAMPLE_CANDIDATES;
+        requireGrid(rows, 1024, "Sample", logits);
         if (small_ || rows == 0) return;
         // slices of 8192 logits or more, about 4 blocks per CU
         const int64_t slices = std::clamp<int64_t>(cdiv(4 * deviceCUs(), rows), 1, std::min<int64_t>(SAMPLE_MAX_SLICES, cdiv(vocab, 8192)));
@@ -191,7 +212,6 @@ public:
         sc_.slices = (uint32_t)cdiv(vocab, sc_.sliceLen);
         // a block of sample_gather reads the row's bins first: no more of them than run at once (2 per CU)
         sc_.parts = (uint32_t)std::clamp<int64_t>(2 * deviceCUs() / rows, 1, sc_.slices);
-        if (rows * sc_.slices >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("Sample takes fewer rows; got " + logits.shape.str() + ".");
     }
     std::vector<Binding> tensors() const override {
         std::vector<Binding> b = options({{logits_, kRead}});
@@ -268,6 +288,10 @@ std::unique_ptr<Kernel> PageTables(const Tensor &pastLens, const Tensor &newLens
     requireShape(positions, D::i32, {T}, "PageTables positions");
     requireShape(slots, D::i32, {T}, "PageTables slots");
     requireShape(counts, D::i32, {2}, "PageTables counts");
+    requireApart("PageTables",
+                 {{&pageTables, "page_tables"}, {&queryStarts, "query_starts"}, {&keyLens, "key_lens"}, {&positions, "positions"},
+                  {&slots, "slots"}, {&counts, "counts"}},
+                 {{&pastLens, "past_lens"}, {&newLens, "new_lens"}, {&freePages, "free_pages"}});
     const PageTablesConstants pc{(uint32_t)R, (uint32_t)M, (uint32_t)F, (uint32_t)T, (uint32_t)pageSize};
     const int64_t blocks = std::clamp<int64_t>(cdiv(T, 256), 1, 256);
     return fixed("page_tables",
@@ -296,8 +320,9 @@ std::unique_ptr<Kernel> PagedKVCacheWrite(const Tensor &k, const Tensor &v, cons
     requireShape(slots, D::i32, {T}, "PagedKVCacheWrite slots");
     const int64_t run = 16 / stride(s), perToken = Nkv * cdiv(Hd, run);
     if (perToken >= (int64_t{1} << 30)) throw Error::tensorShapeMismatch("PagedKVCacheWrite rows are too long: " + k.shape.str() + ".");
+    requireApart("PagedKVCacheWrite", {{&kCache, "k_cache"}, {&vCache, "v_cache"}}, {{&k, "k"}, {&v, "v"}, {&slots, "slots"}});
     const int64_t blocks = cdiv(T * perToken, 1024);
-    if (blocks >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("PagedKVCacheWrite holds too many rows: " + k.shape.str() + ".");
+    requireGrid(blocks, 256, "PagedKVCacheWrite", k);
     const PagedKVWriteConstants pc{(uint32_t)T, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page, (uint32_t)kCache.shape[0]};
     return fixed(fn, {{k, kRead}, {v, kRead}, {slots, kRead}, {kCache, kWrite}, {vCache, kWrite}}, bytesOf(pc),
                  dim3((unsigned)blocks, blocks ? 2 : 0, 1), 256);
@@ -335,7 +360,10 @@ std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, co
     requireShape(pageTables, D::i32, {R, M}, "PagedAttention page_tables");
     requireShape(queryStarts, D::i32, {R + 1}, "PagedAttention query_starts");
     requireShape(keyLens, D::i32, {R}, "PagedAttention key_lens");
-    if (T * Nq >= (int64_t{1} << 31)) throw Error::tensorShapeMismatch("PagedAttention takes fewer than 2^31 query rows; got " + q.shape.str() + ".");
+    requireGrid(cdiv(T * Nq, 16), 256, "PagedAttention", q);
+    requireApart("PagedAttention", {{&out, "out"}},
+                 {{&q, "q"}, {&kCache, "k_cache"}, {&vCache, "v_cache"}, {&pageTables, "page_tables"}, {&queryStarts, "query_starts"},
+                  {&keyLens, "key_lens"}});
     const PagedAttentionConstants pc{(uint32_t)T, (uint32_t)R, (uint32_t)Nq, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page,
                                      (uint32_t)kCache.shape[0], (uint32_t)M, mask.kind, mask.window, (uint32_t)sinks, scale};
     // 16-byte rows: the matrix cores
@@ -364,6 +392,10 @@ std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, con
     if (topK) requireShape(*topK, D::i32, {rows}, "Sample top_k");
     if (topP) requireShape(*topP, D::f32, {rows}, "Sample top_p");
     if (minP) requireShape(*minP, D::f32, {rows}, "Sample min_p");
+    std::vector<Named> inputs = {{&logits, "logits"}, {&uniforms, "uniforms"}};
+    for (const Named &n : {Named{temperature, "temperature"}, {topK, "top_k"}, {topP, "top_p"}, {minP, "min_p"}})
+        if (n.first) inputs.push_back(n);
+    requireApart("Sample", {{&tokens, "tokens"}}, inputs);
     return std::make_unique<SampleKernel>(logits, uniforms, temperature, topK, topP, minP, tokens);
 }
 

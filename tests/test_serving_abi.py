@@ -1,6 +1,7 @@
 """CPU tests of the paged-cache and token-draw descriptors: what they refuse, and
 the index arithmetic of the kernels, compiled for the host, over bad lengths."""
 import ctypes
+import itertools
 import os
 import subprocess
 
@@ -11,11 +12,12 @@ import popcorn_amd as pa
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 FAKE = 0x7F0000000000  # never dereferenced: descriptors only validate
+APART = itertools.count(1)  # tensors of up to 2^44 bytes with no byte in common
 E = pa.PopcornError
 
 
-def T(shape, dtype="bf16", ptr=FAKE):
-    return pa.Tensor(ptr, shape, dtype)
+def T(shape, dtype="bf16", ptr=None):
+    return pa.Tensor(FAKE + (next(APART) << 44) if ptr is None else ptr, shape, dtype)
 
 
 def refused(code, fn, *args, **kw):
@@ -65,7 +67,7 @@ def test_paged_write_refusals():
 
 
 def attend(q=(6, 4, 64), cache=(9, 2, 16, 64), vcache=None, table=(3, 5), starts=(4,), lens=(3,), out=None, t="bf16", kt=None, ot=None,
-           it="i32", qptr=FAKE, **kw):
+           it="i32", qptr=None, **kw):
     kw.setdefault("scale", 0.125)
     return pa.Kernels.PagedAttention(T(q, t, qptr), T(cache, kt or t), T(vcache or cache, kt or t), T(table, it), T(starts, "i32"),
                                      T(lens, "i32"), T(out or q, ot or t), **kw)
@@ -112,6 +114,42 @@ def test_sample_refusals():
     refused(E.TENSOR_SHAPE_MISMATCH, draw, logits=(3, 2 ** 22 + 1))
     refused(E.TENSOR_INVALID_RANK, draw, logits=(300,))
     refused(E.INVALID_ARGUMENT, draw, min_p=T([3], "f32", 0))
+
+
+def test_overlaps_are_refused():
+    lens, names = T([3], "i32"), ("past", "new", "free", "table", "query_starts", "key_lens", "positions", "slots", "counts")
+    shapes = dict(past=[3], new=[3], free=[9], table=[3, 4], query_starts=[4], key_lens=[3], positions=[7], slots=[7], counts=[2])
+    for a, b in itertools.combinations(names, 2):
+        kw = {n: T(shapes[n], "i32", lens.ptr) for n in (a, b)}
+        if b in ("new", "free"):  # two inputs
+            tables(**kw)
+        else:
+            refused(E.INVALID_ARGUMENT, tables, **kw)
+    # the last element of one is the first of the other; next to each other is apart
+    refused(E.INVALID_ARGUMENT, tables, past=lens, key_lens=T([3], "i32", lens.ptr + 8))
+    tables(past=lens, key_lens=T([3], "i32", lens.ptr + 12))
+    tables(free=T([0], "i32", lens.ptr), past=lens, positions=T([0], "i32", lens.ptr), slots=T([0], "i32", 0))
+    rows, cache = T([5, 2, 64]), T([7, 2, 16, 64])
+    slots = T([5], "i32")
+    W = pa.Kernels.PagedKVCacheWrite
+    refused(E.INVALID_ARGUMENT, W, rows, rows, slots, cache, cache)
+    refused(E.INVALID_ARGUMENT, W, rows, rows, slots, T([7, 2, 16, 64], ptr=rows.ptr), cache)
+    W(rows, rows, slots, cache, T([7, 2, 16, 64]))
+    q, starts, lens = T([6, 4, 64]), T([4], "i32"), T([3], "i32")
+    for x, k, v, o in ((q, cache, cache, q), (q, cache, cache, T([6, 4, 64], ptr=cache.ptr + 128))):
+        refused(E.INVALID_ARGUMENT, pa.Kernels.PagedAttention, x, k, v, T([3, 5], "i32"), starts, lens, o, scale=1.0)
+    pa.Kernels.PagedAttention(q, cache, cache, T([3, 5], "i32"), starts, lens, T([6, 4, 64]), scale=1.0)
+    k, x = T([3], "i32"), T([3, 100], "f32")
+    for kw in (dict(top_k=k), dict(temperature=T([3], "f32", k.ptr)), dict(top_p=T([3], "f32", k.ptr + 4)), dict(min_p=T([3], "f32", k.ptr))):
+        refused(E.INVALID_ARGUMENT, pa.Kernels.Sample, x, T([3], "f32"), into=k, **kw)
+    refused(E.INVALID_ARGUMENT, pa.Kernels.Sample, x, T([3], "f32"), into=T([3], "i32", x.ptr + 396))
+
+
+def test_too_many_rows_are_refused():
+    n = 2 ** 22
+    refused(E.TENSOR_SHAPE_MISMATCH, pa.Kernels.Sample, T([n, 64], "f16"), T([n], "f32"), into=T([n], "i32"))
+    pa.Kernels.Sample(T([n - 1, 64], "f16"), T([n - 1], "f32"), into=T([n - 1], "i32"))
+    refused(E.TENSOR_SHAPE_MISMATCH, attend, q=(2 ** 26, 4, 64))
 
 
 def test_null_arguments():
