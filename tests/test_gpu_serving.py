@@ -109,8 +109,8 @@ def test_steps(env):
 class Graph:
     """A capture of `body` on `stream` into an executable graph."""
 
-    def __init__(self, stream, body):
-        self.hip = ctypes.CDLL("libamdhip64.so")
+    def __init__(self, pa, stream, body):
+        self.hip = pa.lib()  # the HIP runtime that it is linked to (another package may have loaded one of its own)
         self.stream = ctypes.c_void_p(stream.handle)
         graph, self.exec = ctypes.c_void_p(), ctypes.c_void_p()
         assert self.hip.hipStreamBeginCapture(self.stream, 0) == 0
@@ -132,7 +132,7 @@ def test_steps_from_a_graph(env):
     stream = pa.Stream()
     enc = pa.KernelCommandEncoder(lib, stream)
     server, other = (Server(pa, stream, 5, 310, 60, 24, seed=s) for s in (2, 3))
-    graph = Graph(stream, lambda: enc.encode(server.kernels))
+    graph = Graph(pa, stream, lambda: enc.encode(server.kernels))
     for new in STEPS:
         expected = server.feed(new)
         graph.launch()
