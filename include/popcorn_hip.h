@@ -605,8 +605,8 @@ popcorn_status_t popcorn_kernel_paged_kv_cache_write(const popcorn_tensor_t *k, 
  * is 0; rows outside the requests' ranges are left as they were.
  * q, the caches and out share one dtype (f32, f16, bf16); page_size is a
  * multiple of 16, Hd at most 512. max_query_len (0: unknown) is the longest
- * request's number of new tokens; the kernels are chosen for it, the result
- * does not depend on it. */
+ * request's number of new tokens; the kernels are chosen for it, and with any
+ * value they serve every request. */
 popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
                                                 const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
                                                 const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens,

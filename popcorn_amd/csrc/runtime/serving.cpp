@@ -103,15 +103,26 @@ public:
         hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
         merge_ = "paged_attention_merge_" + type + hd;
-        // the tile kernel works on the magnitude of the scale (not 0) and 16-bit K and V of up to 256 dims
-        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows;
-        if (!(tiles && pc.R == 1)) {
+        // The tile kernel works on the magnitude of the scale (not 0) and 16-bit K and V of up to 256 dims. For requests of up to
+        // 32 rows, or so few rows in all, the tiles' 128 rows cost more than reading keys again: us of the few-row kernel and of
+        // tiles, 4 heads to a KV head, 8 KV heads, 4000 keys: one request of 64 rows 26 and 33 (Hd 128), 34 and 43 (256), of 128
+        // rows 27 and 40, 38 and 46 (but 96 and 67 behind 16000 keys), of 256 rows 33 and 39, 54 and 47.
+        const int tilesPerCU = hdp_ == 256 ? 1 : 2;
+        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows &&
+                           (int64_t)pc.T * G > (hdp_ == 256 ? 64 : 128);
+        // Beside tiles, the requests of few rows have a launch of their own where there are at least as many units as blocks:
+        // 256 requests on 8 KV heads of 128, one of 500 tokens, 81 us and 109 in tiles alone; 64 requests 83 and 87; 24 requests
+        // 99 and 89, 12 requests of few keys 41 and 31.
+        const bool apart = tiles && (int64_t)pc.R * pc.Nkv >= tilesPerCU * deviceCUs();
+        if (!tiles || apart) {
+            // 16 rows per wave or 32: 16 requests of 32 rows, 2000 keys, us: Hd 64 31.1 and 26.5, Hd 256 90 and 60, of 16 rows 22.5
+            // and 25.0, 54 and 56; (Hd 512 leaves no registers for 32)
             const int rt = hdp_ == 512 || longest <= 16 || tiles ? 1 : 2;
             // as many blocks as run at once (the kernels' registers)
             const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
             add("paged_attention_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);
         }
-        if (tiles) add("paged_attention_tile_" + type + hd, 128, 64, pc.R == 1 ? 0 : kFewRows, UINT32_MAX, hdp_ == 256 ? 1 : 2);
+        if (tiles) add("paged_attention_tile_" + type + hd, 128, 64, apart ? kFewRows : 0, UINT32_MAX, tilesPerCU);
     }
     std::vector<Binding> tensors() const override {
         return {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {out_, kWrite}};
@@ -167,6 +178,9 @@ private:
         w.fewRows = few;
         w.manyRows = many;
         w.maxTiles = (uint32_t)(cdiv((int64_t)pc_.T * G, rows) + std::min(pc_.R, pc_.T));
+        // A worker's least work, and what a unit counts beside its steps (its start: about 10 us). One request of 4096 keys, us:
+        // 18.4 with 128 keys at least, 20.1 with 64, 19.9 with 256; 64 requests of 100 to 16000: 136 with 384 keys counted, 146
+        // with none, 142 with 768; chunks of prompts among them: 57 with 384, 94 with none, 62 with 768.
         w.minSteps = 128 / stepKeys;
         w.unitSteps = 384 / stepKeys;
         // Caches of more than the 256 MB of the memory-side cache are read once a step: V past the caches reads 766 MB
@@ -176,6 +190,7 @@ private:
         const double tileSteps = (double)cdiv((int64_t)pc_.columns * pc_.pageSize + stepKeys, stepKeys) + w.unitSteps;
         const double steps = (double)w.maxTiles * tileSteps;
         w.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc_.Nkv / w.minSteps + 1));
+        // (a launch less: one request 18.4 us and 21.3, 256 requests 78 and 81)
         w.ownPlan = w.maxTiles <= 1024 && pc_.R <= 1024 && steps < 2147483648.0;
         w.stateBase = work_.empty() ? 0 : 2 * work_.back().c.workers * work_.back().c.rows;
         work_.push_back({fn, w});

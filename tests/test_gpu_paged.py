@@ -376,3 +376,22 @@ def test_attention_many_requests(env):
     lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 60, 1500), g.integers(0, 3, 1500))]
     for dtype in ("bf16", "f32"):
         Batch(lens, 4, 2, 64, dtype, 16, seed=15, pad=2).check(env)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads,requests", [((16, 8, 128), 66), ((8, 8, 64), 70), ((12, 4, 256), 65), ((2, 1, 128), 520)], ids=str)
+@pytest.mark.parametrize("mask,sinks", [((0, -1), 0), ((1, 40), 3)])
+def test_attention_few_rows_beside_tiles(env, dtype, heads, requests, mask, sinks):
+    # as many units as blocks: requests of few rows and of many in launches of their own, short and long in turn
+    g = np.random.default_rng(16)
+    lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 200, requests), g.integers(0, 5, requests))]
+    lens[0], lens[7], lens[40], lens[-1] = (5, 90), (130, 17), (0, 70), (64, 150)
+    Batch(lens, *heads, dtype, 16, seed=17, pad=2).check(env, mask, sinks)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("heads", [(8, 2, 64), (4, 1, 128), (8, 2, 256)], ids=str)
+@pytest.mark.parametrize("rows", [32, 36, 64, 68, 128, 132])
+def test_attention_one_request_of_few_rows(env, dtype, heads, rows):
+    # either side of the rows at which tiles take over
+    Batch([(700, rows // (heads[0] // heads[1]))], *heads, dtype, 32, seed=rows).check(env)

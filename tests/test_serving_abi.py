@@ -95,6 +95,24 @@ def test_paged_attention_refusals():
     attend(sinks=4, mask=pa.AttentionMask.causal_sliding_window(8))
 
 
+def test_paged_attention_kernels():
+    def kinds(R, T, nq, nkv, hd, hint, t="bf16", scale=0.1):
+        k = attend(q=(T, nq, hd), cache=(9, nkv, 16, hd), table=(R, 5), starts=(R + 1,), lens=(R,), t=t, max_query_len=hint, scale=scale)
+        return {n.split("_")[2] for n in k.function_names if n.split("_")[1] == "attention"} - {"merge"}
+
+    assert kinds(8, 8, 8, 2, 128, 1) == {"few"}  # decode
+    assert kinds(8, 72, 8, 2, 128, 9) == {"tile"}  # 36 rows of one request
+    assert kinds(8, 72, 8, 2, 128, 8) == {"few"}
+    assert kinds(1, 32, 8, 2, 128, 32) == {"few"} and kinds(1, 33, 8, 2, 128, 33) == {"tile"}
+    assert kinds(1, 16, 8, 2, 256, 16) == {"few"} and kinds(1, 17, 8, 2, 256, 17) == {"tile"}
+    assert kinds(256, 300, 8, 2, 128, 40) == {"few", "tile"} and kinds(255, 300, 8, 2, 128, 40) == {"tile"}
+    assert kinds(128, 300, 8, 2, 256, 40) == {"few", "tile"} and kinds(127, 300, 8, 2, 256, 40) == {"tile"}
+    for kw in (dict(t="f32"), dict(scale=0.0), dict(scale=float("nan"))):
+        assert kinds(4, 500, 8, 2, 128, 200, **kw) == {"few"}
+    assert kinds(4, 500, 8, 2, 512, 200) == {"few"}
+    assert kinds(4, 500, 8, 2, 36, 200) == {"plain"}
+
+
 def draw(logits=(3, 100), t="f32", rows=3, ut="f32", kt="i32", **kw):
     o = dict(temperature=T([3], "f32"), top_k=T([3], kt), top_p=T([3], "f32"), min_p=T([3], "f32"))
     o.update(kw)
