@@ -856,6 +856,30 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
                 copyK(k1, 1, j);
             }
         }
+        if (w0 >= c.steps.r1) {  // a wave without rows copies its part of K and V, and leaves LDS and the matrix cores to the others
+            wait_vmcnt<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+#pragma unroll 1
+            for (uint32_t i = 0; i + 1 < n; ++i) {
+                wait_vmcnt<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                const __amdgpu_buffer_rsrc_t rv = group(V, i + 1);
+                if (i + 2 < n && i + 2 - held0 == 16) hold(i + 2);
+                const __amdgpu_buffer_rsrc_t rk = group(K, i + 2);
+#pragma unroll
+                for (int j = 0; j < kCopies; ++j) {
+                    copyK(rk, i + 2, j);
+                    copyV(rv, i + 1, j);
+                }
+            }
+            wait_vmcnt<0>();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            continue;
+        }
         Ahead next = ahead_of(0), next2 = n > 1 ? ahead_of(1) : next;
 #pragma unroll
         for (int s = 0; s < KS; ++s) qf[s] ^= flip;
@@ -944,6 +968,7 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
             }
         if (!whole && myRow < c.steps.r1 && h == 0) *reinterpret_cast<float2 *>(pML + 2 * (slot + myRow - c.steps.r0)) = float2{m, l};
         if (!__ballot(bad)) continue;
+        wait_vmcnt<0>();  // the rows' stores, before other lanes store them again
         // as in paged_few: an infinity or NaN in V that a row does not see
         const uint32_t s0 = min(c.lo, c.steps.sinks), s1 = min(c.hi, c.steps.sinks);
         const uint32_t t0 = max(c.lo, c.steps.sinks), t1 = max(c.hi, c.steps.sinks);
