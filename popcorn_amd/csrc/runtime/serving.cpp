@@ -375,7 +375,7 @@ std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, co
     requireShape(pageTables, D::i32, {R, M}, "PagedAttention page_tables");
     requireShape(queryStarts, D::i32, {R + 1}, "PagedAttention query_starts");
     requireShape(keyLens, D::i32, {R}, "PagedAttention key_lens");
-    requireGrid(cdiv(T * Nq, 16), 256, "PagedAttention", q);
+    requireGrid(T * Nq, 256, "PagedAttention", q);
     requireApart("PagedAttention", {{&out, "out"}},
                  {{&q, "q"}, {&kCache, "k_cache"}, {&vCache, "v_cache"}, {&pageTables, "page_tables"}, {&queryStarts, "query_starts"},
                   {&keyLens, "key_lens"}});
@@ -388,7 +388,7 @@ std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, co
     const int run = 4 * stride(t);
     if (Hd % 4 || !aligned(kCache.data, run) || !aligned(vCache.data, run)) fn += "_any";
     return fixed(fn, {{q, kRead}, {kCache, kRead}, {vCache, kRead}, {pageTables, kRead}, {queryStarts, kRead}, {keyLens, kRead}, {out, kWrite}},
-                 bytesOf(pc), dim3((unsigned)(R ? cdiv(T * Nq, 16) : 0), 1, 1), 256);
+                 bytesOf(pc), dim3((unsigned)(R ? T * Nq : 0), 1, 1), 256);
 }
 
 std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK,

@@ -395,3 +395,23 @@ def test_attention_few_rows_beside_tiles(env, dtype, heads, requests, mask, sink
 def test_attention_one_request_of_few_rows(env, dtype, heads, rows):
     # either side of the rows at which tiles take over
     Batch([(700, rows // (heads[0] // heads[1]))], *heads, dtype, 32, seed=rows).check(env)
+
+
+@pytest.mark.parametrize("dtype,hd", [("bf16", 36), ("f16", 33), ("f32", 62), ("bf16", 500)])
+def test_attention_odd_rows_of_an_empty_cache(env, dtype, hd):
+    # every key on a page that is not there, rows that are no 16-byte runs
+    pa, _, stream, enc = env
+    e = lambda *s: pa.Tensor.empty(s, dtype)
+    q, out = (upload(pa, np.ones((3, 4, hd)), dtype) for _ in range(2))
+    enc.encode(pa.Kernels.PagedAttention(q, e(0, 2, 16, hd), e(0, 2, 16, hd), i32(pa, np.zeros((2, 3))), i32(pa, [0, 1, 2]), i32(pa, [40, 1]),
+                                         out, scale=1.0))
+    stream.synchronize()
+    got = download(out, stream)
+    assert not got[:2].any() and (got[2:] == 1).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("heads", [(4, 2, 33), (2, 1, 250), (3, 3, 510)], ids=str)
+@pytest.mark.parametrize("mask,sinks", [((0, -1), 0), ((2, -1), 0), ((1, 40), 3)])
+def test_attention_odd_rows(env, dtype, heads, mask, sinks):
+    Batch([(500, 1), (0, 1), (0, 7), (30, 2), (15, 0), (64, 33)], *heads, dtype, 16, seed=heads[2], pad=2).check(env, mask, sinks)

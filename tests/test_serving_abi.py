@@ -167,7 +167,7 @@ def test_too_many_rows_are_refused():
     n = 2 ** 22
     refused(E.TENSOR_SHAPE_MISMATCH, pa.Kernels.Sample, T([n, 64], "f16"), T([n], "f32"), into=T([n], "i32"))
     pa.Kernels.Sample(T([n - 1, 64], "f16"), T([n - 1], "f32"), into=T([n - 1], "i32"))
-    refused(E.TENSOR_SHAPE_MISMATCH, attend, q=(2 ** 26, 4, 64))
+    refused(E.TENSOR_SHAPE_MISMATCH, attend, q=(2 ** 22, 4, 64))
 
 
 def test_null_arguments():
