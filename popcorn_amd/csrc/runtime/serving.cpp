@@ -110,10 +110,10 @@ public:
         const int tilesPerCU = hdp_ == 256 ? 1 : 2;
         const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows &&
                            (int64_t)pc.T * G > (hdp_ == 256 ? 64 : 128);
-        // Beside tiles, the requests of few rows have a launch of their own where there are at least as many units as blocks:
-        // 256 requests on 8 KV heads of 128, one of 500 tokens, 81 us and 109 in tiles alone; 64 requests 83 and 87; 24 requests
-        // 99 and 89, 12 requests of few keys 41 and 31.
-        const bool apart = tiles && (int64_t)pc.R * pc.Nkv >= tilesPerCU * deviceCUs();
+        // Beside tiles, the requests of few rows have a launch of their own where there are more units than blocks: one request of
+        // 500 tokens among 256 of up to 1000 keys on 8 KV heads of 128, 80 us and 107 in tiles alone, 128 on 4 of 256 72 and 88;
+        // but as many units as blocks (64 of up to 8000 keys on 8) 81 and 78, 12 requests of few keys 41 and 31.
+        const bool apart = tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU * deviceCUs();
         if (!tiles || apart) {
             // 16 rows per wave or 32: 16 requests of 32 rows, 2000 keys, us: Hd 64 31.1 and 26.5, Hd 256 90 and 60, of 16 rows 22.5
             // and 25.0, 54 and 56; (Hd 512 leaves no registers for 32)

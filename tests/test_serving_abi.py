@@ -105,8 +105,8 @@ def test_paged_attention_kernels():
     assert kinds(8, 72, 8, 2, 128, 8) == {"few"}
     assert kinds(1, 32, 8, 2, 128, 32) == {"few"} and kinds(1, 33, 8, 2, 128, 33) == {"tile"}
     assert kinds(1, 16, 8, 2, 256, 16) == {"few"} and kinds(1, 17, 8, 2, 256, 17) == {"tile"}
-    assert kinds(256, 300, 8, 2, 128, 40) == {"few", "tile"} and kinds(255, 300, 8, 2, 128, 40) == {"tile"}
-    assert kinds(128, 300, 8, 2, 256, 40) == {"few", "tile"} and kinds(127, 300, 8, 2, 256, 40) == {"tile"}
+    assert kinds(257, 300, 8, 2, 128, 40) == {"few", "tile"} and kinds(256, 300, 8, 2, 128, 40) == {"tile"}
+    assert kinds(129, 300, 8, 2, 256, 40) == {"few", "tile"} and kinds(128, 300, 8, 2, 256, 40) == {"tile"}
     for kw in (dict(t="f32"), dict(scale=0.0), dict(scale=float("nan"))):
         assert kinds(4, 500, 8, 2, 128, 200, **kw) == {"few"}
     assert kinds(4, 500, 8, 2, 512, 200) == {"few"}
