@@ -415,3 +415,9 @@ def test_attention_odd_rows_of_an_empty_cache(env, dtype, hd):
 @pytest.mark.parametrize("mask,sinks", [((0, -1), 0), ((2, -1), 0), ((1, 40), 3)])
 def test_attention_odd_rows(env, dtype, heads, mask, sinks):
     Batch([(500, 1), (0, 1), (0, 7), (30, 2), (15, 0), (64, 33)], *heads, dtype, 16, seed=heads[2], pad=2).check(env, mask, sinks)
+
+
+@pytest.mark.parametrize("dtype,heads,mask,sinks", [("bf16", (16, 16, 64), (0, -1), 0), ("f16", (8, 8, 256), (1, 18000), 70)])
+def test_attention_long_keys_in_tiles(env, dtype, heads, mask, sinks):
+    # one new token in a tile beside a chunk, and more steps for a block than it looks up pages for at once
+    Batch([(20000, 1), (19900, 40)], *heads, dtype, 64, seed=18).check(env, mask, sinks)
