@@ -503,6 +503,7 @@ typedef struct {
     uint64_t aboveK;                       /* weight of the bins before top-k's */
     uint64_t aboveP;                       /* weight of the bins before the first where top-p may cut */
     uint64_t total;                        /* weight of the row */
+    uint64_t kept[SAMPLE_MAX_SLICES];      /* weight of the bins that are kept whatever the cuts */
     uint32_t count[SAMPLE_BINS];           /* tokens of each bin */
     uint32_t sliceTop[SAMPLE_MAX_SLICES];  /* highest rank key */
     uint32_t candidates;

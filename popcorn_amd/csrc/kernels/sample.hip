@@ -12,10 +12,12 @@
 //     bins of the distance from the highest, and their sums over the row;
 //  3. sample_gather: the bins in which the cuts must fall, from the bins'
 //     running sums; their tokens (the candidates, a few hundred of a large
-//     vocabulary) go to a list;
+//     vocabulary) go to a list, and of each slice the weight of what lies before;
 //  4. sample_finish: the cuts among the candidates, by selection, the
 //     slice where the running weight passes the draw, and the token in it.
-// Only the second evaluates the whole row's weights. A row that neither top-k
+// Only the second evaluates the whole row's weights, which bounds it (26 us of
+// 64 rows of 256000 bf16 logits, some 35 instructions a logit; the others 8, 18
+// and 18, the last with one block to a row). A row that neither top-k
 // nor top-p cuts has its slices' weights summed by the third instead.
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
 // More candidates than the list holds (thousands of equal logits at the cut)
@@ -228,8 +230,8 @@ __device__ inline float least_at(const Row &w) {
 
 template <typename T>
 __device__ void sample_gather(const typename T::storage *__restrict__ logits, const Options &o, SampleRow *__restrict__ rows,
-                              const SampleConstants &c) {
-    __shared__ u64 sSums[kWaves], sAbove[2], sWith, sList[kFound];
+                              const uint64_t *__restrict__ bins, const SampleConstants &c) {
+    __shared__ u64 sSums[kWaves], sAbove[2], sWith, sList[kFound], sKept[SAMPLE_MAX_SLICES];
     __shared__ uint32_t sCounts[kWaves], sBin[3], sNeed, sFound, sBase;
     const uint32_t r = blockIdx.x / c.parts, part = blockIdx.x % c.parts;
     SampleRow &row = rows[r];
@@ -263,6 +265,7 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
     const Scan<u64> weights = pk::block_scan<kWaves>(mine, sSums);
     const u64 wend = weights.upto, total = weights.total;
     const uint32_t cend = pk::block_scan<kWaves>(here, sCounts).upto;
+    if (tid < SAMPLE_MAX_SLICES) sKept[tid] = 0;
     if (tid == 0) {
         sFound = 0;
         sBin[0] = sBin[1] = sBin[2] = kBins;
@@ -322,6 +325,21 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
         row.total = total;
     }
     const float at = least_at(w);
+    // the part's slices are next to each other
+    const uint32_t each = (c.slices + c.parts - 1) / c.parts, s0 = min(part * each, c.slices), s1 = min(s0 + each, c.slices);
+    // each slice's weight of the bins that are kept whatever the cuts
+    for (uint32_t sl = s0; sl < s1; ++sl) {
+        const uint64_t *b = bins + ((uint64_t)r * c.slices + sl) * kBins + tid * kPerThread;
+        u64 sum = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kPerThread; ++j) {
+            const uint32_t i = tid * kPerThread + j;
+            const u64 v = b[j];
+            sum += (i < first) & !least_bin(w, i, at) & ((float)i < at) ? v : 0;
+        }
+        sum = wave_sum64(sum);
+        if ((tid & 63) == 0) add64(&sKept[sl - s0], sum);
+    }
     auto put = [&](uint32_t slot, u64 v) {
         if (slot < kList) row.candidate[slot] = v;
     };
@@ -336,10 +354,9 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
             else put(atomicAdd(&row.candidates, 1u), c);
         }
     };
-    // the part's slices are next to each other
-    const uint32_t per = (c.slices + c.parts - 1) / c.parts * c.sliceLen, lo = min(part * per, c.vocab), hi = min(lo + per, c.vocab);
+    const uint32_t hi = min(s1 * c.sliceLen, c.vocab);
     each_logit<T>(
-        x, lo, hi,
+        x, s0 * c.sliceLen, hi,
         [&](uint32_t, uint32_t j, float v) {
             const uint32_t b = w.bin(v);
             found |= (uint32_t)((v > -INFINITY) & (b < first ? least_bin(w, b, at) : (b <= lastP) | (b == binK))) << j;
@@ -348,6 +365,7 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
     __syncthreads();
     // the row's counter is one address for all its blocks: one addition each
     const uint32_t n = min(sFound, kFound);
+    if (tid < s1 - s0) row.kept[s0 + tid] = sKept[tid];
     if (tid == 0) sBase = n ? atomicAdd(&row.candidates, n) : 0;
     __syncthreads();
     for (uint32_t i = tid; i < n; i += kThreads) put(sBase + i, sList[i]);
@@ -364,7 +382,7 @@ struct RowSpace {
 // least 1, at most the sum. Entries of measure 0 are not looked at. While more than kFew are left, a pass keeps one
 // of 1024 values of the 10 bits from the highest in which they differ; the few are compared with each other.
 // (A sort by merging made sample_finish 34 us of 64 rows of 256000 bf16 logits, this 20; counting every entry's
-// greater ones made it 14.0 us of one row of 256000 with about 100 candidates, this 15.5.)
+// greater ones was 1.5 us faster for 100 candidates.)
 __device__ inline u64 select(RowSpace &s, const u64 (&e)[kEach], const u64 (&m)[kEach], u64 want) {
     const uint32_t tid = threadIdx.x;
     uint32_t left = 0;
@@ -592,9 +610,9 @@ __device__ __attribute__((noinline)) void finish_by_digits(RowSpace &s, const ty
 
 template <typename T>
 __device__ void sample_finish(const typename T::storage *__restrict__ logits, const Options &o, const SampleRow *__restrict__ rows,
-                              const uint64_t *__restrict__ bins, int32_t *__restrict__ tokens, const SampleConstants &c) {
+                              int32_t *__restrict__ tokens, const SampleConstants &c) {
     __shared__ RowSpace s;
-    const uint32_t r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const uint32_t r = blockIdx.x, tid = threadIdx.x;
     const SampleRow &row = rows[r];
     const typename T::storage *x = logits + (uint64_t)r * c.vocab;
     const Row w = row_of(o, r, top_of(row, c.slices), c);
@@ -609,28 +627,11 @@ __device__ void sample_finish(const typename T::storage *__restrict__ logits, co
         return;
     }
     if (cuts) {
-        const uint32_t n = row.candidates, first = row.first;
+        const uint32_t n = row.candidates;
         for (uint32_t i = tid; i < n; i += kThreads) s.list[i] = row.candidate[i];
-        // each slice's weight of the bins that are kept whatever the cuts
-        const float at = least_at(w);
-        for (uint32_t sl = wave; sl < c.slices; sl += kWaves) {
-            const uint64_t *b = bins + ((uint64_t)r * c.slices + sl) * kBins;
-            u64 sum = 0;
-            for (uint32_t i0 = lane * 2; i0 < first; i0 += 1024) {
-                ulong2 v[8];  // (past the bins' end nothing is read: kBins is a multiple of 1024)
-#pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) v[j] = *reinterpret_cast<const ulong2 *>(b + i0 + 128 * j);
-#pragma unroll
-                for (uint32_t j = 0; j < 16; ++j) {
-                    const uint32_t i = i0 + 128 * (j >> 1) + (j & 1);
-                    if (i < first && !least_bin(w, i, at) && (float)i < at) sum += j & 1 ? v[j >> 1].y : v[j >> 1].x;
-                }
-            }
-            sum = wave_sum64(sum);
-            if (lane == 0) s.slice[sl] = sum;
-        }
+        if (tid < c.slices) s.slice[tid] = row.kept[tid];
         __syncthreads();
-        cut = cut_in_list(s, w, n, first, row.binK, row.needK, row.aboveK, row.aboveP, row.total);
+        cut = cut_in_list(s, w, n, row.first, row.binK, row.needK, row.aboveK, row.aboveP, row.total);
         for (uint32_t i = tid; i < n; i += kThreads)
             if (s.list[i] >= cut) {
                 const u64 m = w.weight(key_value((uint32_t)(s.list[i] >> 32)));
@@ -702,13 +703,12 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
         sample_hist<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, c);                         \
     }                                                                                                                          \
     POPCORN_KERNEL void __launch_bounds__(1024, 8)                                                                              \
-        sample_gather_##t(const T::storage *logits, SAMPLE_OPTIONS, SampleRow *rows, SampleConstants c) { \
-        sample_gather<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, c);                             \
+        sample_gather_##t(const T::storage *logits, SAMPLE_OPTIONS, SampleRow *rows, const uint64_t *bins, SampleConstants c) {    \
+        sample_gather<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, c);                             \
     }                                                                                                                          \
     POPCORN_KERNEL void __launch_bounds__(1024)                                                                                \
-        sample_finish_##t(const T::storage *logits, SAMPLE_OPTIONS, const SampleRow *rows,               \
-                          const uint64_t *bins, int32_t *tokens, SampleConstants c) {                                          \
-        sample_finish<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, bins, tokens, c);               \
+        sample_finish_##t(const T::storage *logits, SAMPLE_OPTIONS, const SampleRow *rows, int32_t *tokens, SampleConstants c) {   \
+        sample_finish<T>(logits, Options{uniforms, temperature, topK, topP, minP}, rows, tokens, c);                           \
     }                                                                                                                          \
     POPCORN_KERNEL void __launch_bounds__(1024)                                                                                \
         sample_small_##t(const T::storage *logits, SAMPLE_OPTIONS, int32_t *tokens, SampleConstants c) {                       \
