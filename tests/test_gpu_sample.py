@@ -134,3 +134,32 @@ def test_sample_no_rows(env):
     z = pa.Tensor.empty([0], "f32")
     enc.encode(pa.Kernels.Sample(pa.Tensor.empty([0, 50], "f32"), z, pa.Tensor.empty([0], "i32")))
     stream.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+def test_sample_special_logits_in_slices(env, dtype):
+    g = np.random.default_rng(20)
+    n = 30001
+    low = {"f32": np.finfo(np.float32).min, "f16": -65504.0, "bf16": -3.3895313892515355e38}[dtype]
+    x = g.standard_normal((9, n)).astype(np.float32)
+    x[0, g.random(n) < 0.99] = -np.inf
+    x[1, g.random(n) < 0.9] = low
+    x[2] = -np.inf
+    x[3] = np.nan
+    x[4, g.random(n) < 0.5] = np.nan
+    x[5, [7, 20000, n - 1]] = np.inf
+    x[6] = -np.inf
+    x[6, n - 1] = low
+    x[7] = low
+    x[8, :2] = np.nan, np.inf
+    for options in (dict(), dict(top_k=[5] * 9, top_p=[0.7] * 9, min_p=[0.05] * 9, temperature=[0.5] * 9), dict(top_k=[n - 3] * 9),
+                    dict(top_k=[n - 10] * 9, top_p=[0.999] * 9), dict(temperature=[0.0] * 9), dict(temperature=[np.inf] * 9, top_p=[0.6] * 9),
+                    dict(temperature=[0.0, 1.0, np.inf] * 3, top_k=[0, 50, n] * 3, top_p=[1.0] * 5 + [0.5] * 4)):
+        got = check(env, x, dtype, g.random(9), **options)
+        assert got[2] == got[3] == -1 and got[6] == n - 1 and got[8] == 1 and got[5] in (7, 20000, n - 1)
+
+
+@pytest.mark.parametrize("dtype,options", [("f32", dict(top_k=[3000], top_p=[0.95])), ("bf16", dict(min_p=[0.001]))])
+def test_sample_longest_row(env, dtype, options):
+    x = np.random.default_rng(21).standard_normal((1, 2 ** 22)).astype(np.float32) * 2
+    check(env, x, dtype, [1.0 - 2.0 ** -24], **options)
