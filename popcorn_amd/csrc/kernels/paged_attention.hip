@@ -349,6 +349,10 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
     __shared__ OwnTile sm_plan[kOwnTiles];
     __shared__ uint32_t sm_bad;
+    // Q of 512 dims in 16 bits is kept in LDS: in registers 60 of 512 spilled (32 requests of 100 to 8000 keys, 8 heads on
+    // 2: 48 us, and 99; 1000 tokens behind as many 148 and 438)
+    constexpr bool kQInLds = HD == 512 && !kWide;
+    __shared__ __attribute__((aligned(16))) u32x4 sm_q[kQInLds ? KS * 64 : 1];
     static_assert(sizeof(PlanSpace<64 * kWaves, uint32_t>) <= sizeof(smem), "the plan is laid out where V goes");
 
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
@@ -363,17 +367,22 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
 
         // rows past the tile's last repeat it and are not stored
-        u32x4 qf[RT][KS];
+        u32x4 qf[RT][kQInLds ? 1 : KS];
         int posQ[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const uint32_t r = min(c.steps.r0 + rt * 16 + c16, c.steps.r1 - 1);
             posQ[rt] = c.req.pos0 + (int)(r / G);
             const S *row = Q + q_row(r) * D + g * E;
+            auto piece = [&](int s) { return s * 4 * E + g * E < D ? *reinterpret_cast<const u32x4 *>(row + s * 4 * E) : u32x4{0u, 0u, 0u, 0u}; };
+            if constexpr (kQInLds) {
+                for (int s = wave; s < KS; s += kWaves) sm_q[s * 64 + lane] = piece(s);
+            } else {
 #pragma unroll
-            for (int s = 0; s < KS; ++s)
-                qf[rt][s] = s * 4 * E + g * E < D ? *reinterpret_cast<const u32x4 *>(row + s * 4 * E) : u32x4{0u, 0u, 0u, 0u};
+                for (int s = 0; s < KS; ++s) qf[rt][s] = piece(s);
+            }
         }
+        if constexpr (kQInLds) __syncthreads();
 
         // The wave's steps are c.lo + wave + kWaves i. Lane l holds page and row in it
         // of group l % KM of the wave's step `page0` + l / KM; a group that no
@@ -460,8 +469,20 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
             bool ok[KM];
 #pragma unroll
             for (int mt = 0; mt < KM; ++mt) ok[mt] = gr[mt].ok;
-            copyV(gr);
+            if constexpr (!kQInLds) copyV(gr);
             pk::f32x4 st[RT][KM];
+            if constexpr (kQInLds) {
+                static_assert(RT == 1, "one tile's rows");
+#pragma unroll
+                for (int mt = 0; mt < KM; ++mt) st[0][mt] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const u32x4 q = sm_q[s * 64 + lane];
+#pragma unroll
+                    for (int mt = 0; mt < KM; ++mt) st[0][mt] = pk::Mma16<T>::run(kf[mt][s], q, st[0][mt]);
+                }
+                copyV(gr);  // (the compiler has a read of LDS wait for copies into it)
+            } else {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -479,6 +500,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
                         }
                     }
                 }
+            }
             __builtin_amdgcn_sched_barrier(0);
             if (i + 1 - page0 == kHeld) hold(i + 1);
             loadK(i + 1, step + kWaves);
