@@ -352,6 +352,8 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     // Q of 512 dims in 16 bits is kept in LDS: in registers 60 of 512 spilled (32 requests of 100 to 8000 keys, 8 heads on
     // 2: 48 us, and 99; 1000 tokens behind as many 148 and 438)
     constexpr bool kQInLds = HD == 512 && !kWide;
+    // and in 32 bits, where LDS has no room for it, read again for each step (the same call 135 us, and 325)
+    constexpr bool kQAgain = HD == 512 && kWide;
     __shared__ __attribute__((aligned(16))) u32x4 sm_q[kQInLds ? KS * 64 : 1];
     static_assert(sizeof(PlanSpace<64 * kWaves, uint32_t>) <= sizeof(smem), "the plan is laid out where V goes");
 
@@ -367,7 +369,8 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         auto q_row = [&](uint32_t r) { return ((uint64_t)(uint32_t)c.req.start + r / G) * p.Nq + c.hkv * G + r % G; };
 
         // rows past the tile's last repeat it and are not stored
-        u32x4 qf[RT][kQInLds ? 1 : KS];
+        u32x4 qf[RT][kQInLds || kQAgain ? 1 : KS];
+        const S *qAgain = Q;
         int posQ[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -377,6 +380,8 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
             auto piece = [&](int s) { return s * 4 * E + g * E < D ? *reinterpret_cast<const u32x4 *>(row + s * 4 * E) : u32x4{0u, 0u, 0u, 0u}; };
             if constexpr (kQInLds) {
                 for (int s = wave; s < KS; s += kWaves) sm_q[s * 64 + lane] = piece(s);
+            } else if constexpr (kQAgain) {
+                qAgain = Q + q_row(r) * D;
             } else {
 #pragma unroll
                 for (int s = 0; s < KS; ++s) qf[rt][s] = piece(s);
@@ -482,6 +487,20 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
                     for (int mt = 0; mt < KM; ++mt) st[0][mt] = pk::Mma16<T>::run(kf[mt][s], q, st[0][mt]);
                 }
                 copyV(gr);  // (the compiler has a read of LDS wait for copies into it)
+            } else if constexpr (kQAgain) {
+                static_assert(RT == 1 && KM == 1, "one tile's rows, 16 keys");
+                st[0][0] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t d0 = g * E;
+                asm volatile("" : "+v"(d0));  // (no load of this is the loop's)
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const uint32_t d = s * 4 * E + d0;
+                    u32x4 q = *reinterpret_cast<const u32x4 *>(qAgain + min(d, D - E));
+                    if (d >= D) q = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        st[0][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[0][s][e]), __uint_as_float(q[e]), st[0][0], 0, 0, 0);
+                }
             } else {
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
