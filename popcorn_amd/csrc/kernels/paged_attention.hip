@@ -1257,7 +1257,6 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
     PAGED_FEW(paged_attention_few_##t##_d128_r1, T, 128, 1, 3) \
     PAGED_FEW(paged_attention_few_##t##_d128_r2, T, 128, 2, 2) \
     PAGED_FEW(paged_attention_few_##t##_d256_r1, T, 256, 1, PER256) \
-    PAGED_FEW(paged_attention_few_##t##_d256_r2, T, 256, 2, 1) \
     PAGED_FEW(paged_attention_few_##t##_d512_r1, T, 512, 1, 1) \
     PAGED_MERGE(paged_attention_merge_##t##_d64, T, 64)        \
     PAGED_MERGE(paged_attention_merge_##t##_d128, T, 128)      \
@@ -1267,6 +1266,8 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
 PAGED_FEW_D(f32, F32, 1)
 PAGED_FEW_D(f16, F16, 2)
 PAGED_FEW_D(bf16, BF16, 2)
+PAGED_FEW(paged_attention_few_f16_d256_r2, F16, 256, 2, 1)
+PAGED_FEW(paged_attention_few_bf16_d256_r2, BF16, 256, 2, 1)
 
 PAGED_TILE(paged_attention_tile_f16_d64, F16, 64, 2)
 PAGED_TILE(paged_attention_tile_f16_d128, F16, 128, 2)

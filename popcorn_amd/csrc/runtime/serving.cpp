@@ -116,8 +116,8 @@ public:
         const bool apart = tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU * deviceCUs();
         if (!tiles || apart) {
             // 16 rows per wave or 32: 16 requests of 32 rows, 2000 keys, us: Hd 64 31.1 and 26.5, Hd 256 90 and 60, of 16 rows 22.5
-            // and 25.0, 54 and 56; (Hd 512 leaves no registers for 32)
-            const int rt = hdp_ == 512 || longest <= 16 || tiles ? 1 : 2;
+            // and 25.0, 54 and 56. Registers for 32 are wanting at Hd 512 and in f32 at 256 (84 and 198 there).
+            const int rt = hdp_ == 512 || (f32 && hdp_ == 256) || longest <= 16 || tiles ? 1 : 2;
             // as many blocks as run at once (the kernels' registers)
             const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
             add("paged_attention_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);

@@ -110,6 +110,9 @@ def test_paged_attention_kernels():
     for kw in (dict(t="f32"), dict(scale=0.0), dict(scale=float("nan"))):
         assert kinds(4, 500, 8, 2, 128, 200, **kw) == {"few"}
     assert kinds(4, 500, 8, 2, 512, 200) == {"few"}
+    for t, hd, rows in (("f32", 256, "r1"), ("f32", 128, "r2"), ("bf16", 256, "r2"), ("f16", 512, "r1")):
+        names = attend(q=(32, 8, hd), cache=(9, 2, 16, hd), table=(4, 5), starts=(5,), lens=(4,), t=t, max_query_len=8).function_names
+        assert names[0].endswith(f"_d{hd}_{rows}")
     assert kinds(4, 500, 8, 2, 36, 200) == {"plain"}
 
 
