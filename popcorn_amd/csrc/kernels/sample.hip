@@ -218,14 +218,14 @@ __device__ void sample_hist(const typename T::storage *__restrict__ logits, cons
     }
 }
 
-// Whether min-p may cut in a bin: the last bins with weights of at least
-// `least`, one to either side for the roundings of bin and weight (a bin's
-// weights span 1.4%).
+// Whether min-p may cut in a bin: the bin where e^-distance is least - 1/2 (from
+// there on a weight is rounded to `least`), and one to either side for the
+// roundings of bin and weight (a bin's weights span 1.4%).
 __device__ inline bool least_bin(const Row &w, uint32_t b, float at) {
     return (w.least != 0) & (fabsf((float)b + 0.5f - at) < 2.0f);
 }
 __device__ inline float least_at(const Row &w) {
-    return w.least ? (40.0f - __log2f((float)w.least)) * (72.0f * 0.69314718f) : 1e9f;
+    return w.least ? (40.0f - __log2f((float)w.least - 0.5f)) * (72.0f * 0.69314718f) : 1e9f;
 }
 
 template <typename T>

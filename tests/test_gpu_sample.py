@@ -163,3 +163,24 @@ def test_sample_special_logits_in_slices(env, dtype):
 def test_sample_longest_row(env, dtype, options):
     x = np.random.default_rng(21).standard_normal((1, 2 ** 22)).astype(np.float32) * 2
     check(env, x, dtype, [1.0 - 2.0 ** -24], **options)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("least", [1, 2, 3, 7, 19, 20, 100])
+def test_sample_min_p_at_its_least_weights(env, dtype, least):
+    # Many tokens whose weights round to the least whole number that min-p keeps, from just below it (min-p's
+    # border in the logits is at least - 1/2), behind one heavy token; top-k is on and cuts nothing.
+    n, many = 250000, 200000
+    x = np.full((3, n), -60.0, np.float32)
+    x[:, 0] = 0.0
+    g = np.random.default_rng(least)
+    at = 1 + g.permutation(n - 1)[:many]
+    x[:, at] = np.log((least - np.array([0.45, 0.3, 0.1]))[:, None] / 2.0 ** 40)
+    if dtype != "f32":  # the nearest logits of the type whose weights are the same
+        steps = {"f16": 2.0 ** -6, "bf16": 2.0 ** -3}[dtype]
+        x[:, at] = np.floor(x[:, at] / steps + 0.5) * steps
+    u = np.array([1.0 - 2.0 ** -24, 1.0 - 2.0 ** -23, 1.0 - 2.0 ** -22])
+    p = [(least - 0.5) / 2.0 ** 40] * 3
+    got = check(env, x, dtype, u, min_p=p, top_k=[n - 1] * 3)
+    if dtype == "f32" and least <= 3:
+        assert got[0] > 0  # (not the heavy token)
