@@ -21,7 +21,8 @@
 // nor top-p cuts has its slices' weights summed by the third instead.
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
 // More candidates than the list holds (thousands of equal logits at the cut)
-// are counted digit by digit of their logits instead (cut_by_digits).
+// are counted digit by digit of their logits instead (cut_by_digits), as is
+// min-p at temperatures that lead the bins out of f32's range.
 #include "scan.hpp"
 
 namespace {
@@ -73,6 +74,7 @@ struct Row {
     float p;
     uint32_t k;
     bool live, useK, useP;
+    bool binned;  // bins are as the definition has them; else they only keep the order
 
     __device__ inline u64 weight(float v) const {
         constexpr Exp2Terms terms;
@@ -108,6 +110,7 @@ __device__ inline Row row_of(const Options &o, uint32_t r, uint32_t topKey, cons
     const bool greedy = !(t > 0.0f);
     w.rate = 1.4426950408889634074 / (greedy ? 1.0 : (double)t);
     w.bins = 72.0f / (greedy ? 1.0f : t);  // weights end at a distance of 28.5 temperatures
+    w.binned = greedy || (t > 3e-37f && t < 1e37f);  // neither 72 / t nor a distance of 28.5 t passes the largest number
     w.k = greedy ? 1u : k > 0 ? (uint32_t)k : 0u;
     w.useK = w.k > 0 && w.k < c.vocab;
     w.useP = p < 1.0f;  // (not where it is NaN)
@@ -250,6 +253,10 @@ __device__ void sample_gather(const typename T::storage *__restrict__ logits, co
             sum = pk::block_scan<kWaves>(sum, sSums).total;
             if (tid == 0) row.weight[slice] = sum;
         }
+        return;
+    }
+    if (w.least && !w.binned) {  // no bin is known to hold min-p's border: the row is counted by digits
+        if (part == 0 && tid == 0) row.candidates = kList + 1;
         return;
     }
     // bins before `first` are kept; candidates are the bins first .. lastP and binK

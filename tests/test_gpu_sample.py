@@ -184,3 +184,23 @@ def test_sample_min_p_at_its_least_weights(env, dtype, least):
     got = check(env, x, dtype, u, min_p=p, top_k=[n - 1] * 3)
     if dtype == "f32" and least <= 3:
         assert got[0] > 0  # (not the heavy token)
+
+
+@pytest.mark.parametrize("temperature,logits", [
+    (1e38, [3e38, 1e38, -1e38, -3e38, -3.4e38]),  # distances past the largest number
+    (3e38, [3.4e38, 0.0, -3.4e38]),
+    (1e-38, [0.0, -4e-39, -1e-38, -2e-38, -1e-37]),  # more bins in a unit than the largest number
+    (1.1e-41, [0.0, -1e-41, -3e-41]),  # numbers below the smallest normal one
+], ids=str)
+@pytest.mark.parametrize("vocab", [1000, 9001])
+def test_sample_min_p_at_extreme_temperatures(env, temperature, logits, vocab):
+    g = np.random.default_rng(vocab)
+    x = np.array(logits, np.float32)[g.integers(0, len(logits), (6, vocab))]
+    x[g.random((6, vocab)) < 0.5] = -np.inf
+    t = [temperature] * 6
+    check(env, x, "f32", g.random(6), temperature=t, min_p=[0.001, 0.05, 0.2, 0.5, 0.9, 1.0], top_k=[vocab - 1] * 6)
+    check(env, x, "f32", g.random(6), temperature=t, min_p=[0.001, 0.05, 0.2, 0.5, 0.9, 1.0], top_p=[0.9999] * 6)
+    # few tokens with weight, so that the candidates fit their list
+    x[g.random((6, vocab)) < 0.9] = -np.inf
+    check(env, x, "f32", g.random(6), temperature=t, min_p=[0.001, 0.05, 0.2, 0.5, 0.9, 1.0], top_k=[vocab - 1] * 6)
+    check(env, x, "f32", g.random(6), temperature=t, top_k=[vocab // 30] * 6)
