@@ -66,6 +66,12 @@ __device__ inline double fma64(double a, double b, double c) {
     return d;
 }
 
+struct Options {
+    const float *uniforms, *temperature;
+    const int32_t *topK;
+    const float *topP, *minP;
+};
+
 // One row's options, and its highest logit.
 struct Row {
     float top, bins;  // bins per unit of distance
@@ -88,16 +94,11 @@ struct Row {
         const u64 u = (t > -42.0) & (v > -INFINITY) ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;  // (a NaN is 0)
         return v == top ? (u64)1 << 40 : u;
     }
+    __device__ inline float uniform(const Options &o, uint32_t r) const { return rate < INFINITY ? o.uniforms[r] : 0.0f; }
     // Grows, if anything, from a logit to the next in the ranking.
     __device__ inline uint32_t bin(float v) const {
         return v == top ? 0u : (uint32_t)fminf((top - v) * bins, (float)(kBins - 1));
     }
-};
-
-struct Options {
-    const float *uniforms, *temperature;
-    const int32_t *topK;
-    const float *topP, *minP;
 };
 
 __device__ inline Row row_of(const Options &o, uint32_t r, uint32_t topKey, const SampleConstants &c) {
@@ -107,15 +108,16 @@ __device__ inline Row row_of(const Options &o, uint32_t r, uint32_t topKey, cons
     const float t = c.hasTemperature ? o.temperature[r] : 1.0f;
     const int32_t k = c.hasTopK ? o.topK[r] : 0;
     const float p = c.hasTopP ? o.topP[r] : 1.0f, least = c.hasMinP ? o.minP[r] : 0.0f;
+    // a temperature of 0 leaves weight to the highest logit alone, of which a uniform of 0 draws the first: no cut
     const bool greedy = !(t > 0.0f);
-    w.rate = 1.4426950408889634074 / (greedy ? 1.0 : (double)t);
-    w.bins = 72.0f / (greedy ? 1.0f : t);  // weights end at a distance of 28.5 temperatures
-    w.binned = greedy || (t > 3e-37f && t < 1e37f);  // neither 72 / t nor a distance of 28.5 t passes the largest number
-    w.k = greedy ? 1u : k > 0 ? (uint32_t)k : 0u;
-    w.useK = w.k > 0 && w.k < c.vocab;
-    w.useP = p < 1.0f;  // (not where it is NaN)
+    w.rate = greedy ? INFINITY : 1.4426950408889634074 / (double)t;
+    w.bins = 72.0f / t;  // weights end at a distance of 28.5 temperatures
+    w.binned = t > 3e-37f && t < 1e37f;  // neither 72 / t nor a distance of 28.5 t passes the largest number
+    w.k = k > 0 ? (uint32_t)k : 0u;
+    w.useK = w.k > 0 && w.k < c.vocab && !greedy;
+    w.useP = p < 1.0f && !greedy;  // (not where it is NaN)
     w.p = fmaxf(p, 0.0f);
-    w.least = least > 0.0f ? (u64)__builtin_ceil((double)fminf(least, 1.0f) * kOne) : 0;
+    w.least = least > 0.0f && !greedy ? (u64)__builtin_ceil((double)fminf(least, 1.0f) * kOne) : 0;
     return w;
 }
 
@@ -630,7 +632,7 @@ __device__ void sample_finish(const typename T::storage *__restrict__ logits, co
     u64 cut = 0;
     const bool cuts = w.useK || w.useP;
     if (cuts && row.candidates > kList) {
-        finish_by_digits<T>(s, x, w, c.vocab, o.uniforms[r], tokens + r);
+        finish_by_digits<T>(s, x, w, c.vocab, w.uniform(o, r), tokens + r);
         return;
     }
     if (cuts) {
@@ -650,7 +652,7 @@ __device__ void sample_finish(const typename T::storage *__restrict__ logits, co
     __syncthreads();
     const u64 mine = tid < c.slices ? s.slice[tid] : 0;
     const Scan<u64> scan = pk::block_scan<kWaves>(mine, s.sums);
-    const u64 run = scan.upto, target = target_of(o.uniforms[r], scan.total);
+    const u64 run = scan.upto, target = target_of(w.uniform(o, r), scan.total);
     if (run - mine <= target && target < run) {
         s.bin = tid;
         s.pick = run - mine;
@@ -694,7 +696,7 @@ __device__ void sample_small(const typename T::storage *__restrict__ logits, con
         const u64 m = w.weight(v);
         z += m >= w.least && ((u64)rank_key(v) << 32 | (uint32_t)~i) >= cut ? m : 0;
     }
-    find_token<T>(s, x, w, cut, 0, n, 0, target_of(o.uniforms[r], pk::block_scan<kWaves>(z, s.sums).total), tokens + r);
+    find_token<T>(s, x, w, cut, 0, n, 0, target_of(w.uniform(o, r), pk::block_scan<kWaves>(z, s.sums).total), tokens + r);
 }
 
 }  // namespace

@@ -265,8 +265,8 @@ public:
     }
 
 private:
-    // A row may be cut: by top-k, by top-p, or by a temperature of 0.
-    bool cuts() const { return sc_.hasTemperature || sc_.hasTopK || sc_.hasTopP; }
+    // A row may be cut, by top-k or top-p.
+    bool cuts() const { return sc_.hasTopK || sc_.hasTopP; }
     std::vector<Binding> options(std::vector<Binding> b) const {
         for (const Tensor &t : options_) b.push_back({t, kRead});
         return b;

@@ -204,3 +204,18 @@ def test_sample_min_p_at_extreme_temperatures(env, temperature, logits, vocab):
     x[g.random((6, vocab)) < 0.9] = -np.inf
     check(env, x, "f32", g.random(6), temperature=t, min_p=[0.001, 0.05, 0.2, 0.5, 0.9, 1.0], top_k=[vocab - 1] * 6)
     check(env, x, "f32", g.random(6), temperature=t, top_k=[vocab // 30] * 6)
+
+
+@pytest.mark.parametrize("vocab", [70, 4096, 4097, 30001])
+def test_sample_greedy_rows_among_others(env, vocab):
+    # a temperature of 0 (or less, or NaN) takes the first of the highest, whatever the other options; beside rows that draw
+    g = np.random.default_rng(vocab)
+    x = g.integers(-5, 3, (8, vocab)).astype(np.float32)
+    x[3], x[5, 9:] = -np.inf, np.nan
+    x[6, [11, 60]] = np.inf
+    t = np.array([0.0, 1.0, -1.0, 0.0, np.nan, 0.0, 0.0, 1e-30], np.float32)
+    u = np.full(8, 1.0 - 2.0 ** -24)
+    for kw in (dict(), dict(min_p=[1.0] * 8), dict(top_k=[7] * 8), dict(top_p=[0.99] * 8), dict(top_k=[40] * 8, top_p=[0.3] * 8, min_p=[0.2] * 8)):
+        got = check(env, x, "f32", u, temperature=t, **kw)
+        want = [int(np.nanargmax(np.where(np.isnan(r), -np.inf, r))) for r in x]
+        assert got[3] == -1 and all(got[r] == want[r] for r in (0, 2, 4, 5, 6))

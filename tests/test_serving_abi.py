@@ -137,6 +137,21 @@ def test_sample_refusals():
     refused(E.INVALID_ARGUMENT, draw, min_p=T([3], "f32", 0))
 
 
+def test_sample_launches():
+    none = dict(temperature=None, top_k=None, top_p=None, min_p=None)
+    t, k = T([3], "f32"), T([3], "i32")
+
+    def names(**kw):
+        return [n.split("_")[1] for n in draw(logits=(3, 50000), **dict(none, **kw)).function_names]
+
+    # the histogram serves top-k and top-p alone
+    for kw in ({}, dict(temperature=t), dict(min_p=t), dict(temperature=t, min_p=T([3], "f32"))):
+        assert names(**kw) == ["top", "gather", "finish"]
+    for kw in (dict(top_k=k), dict(top_p=t), dict(temperature=t, top_k=k)):
+        assert names(**kw) == ["top", "hist", "gather", "finish"]
+    assert draw(logits=(3, 4096)).function_names == ["sample_small_f32"]
+
+
 def test_overlaps_are_refused():
     lens, names = T([3], "i32"), ("past", "new", "free", "table", "query_starts", "key_lens", "positions", "slots", "counts")
     shapes = dict(past=[3], new=[3], free=[9], table=[3, 4], query_starts=[4], key_lens=[3], positions=[7], slots=[7], counts=[2])
