@@ -619,8 +619,9 @@ popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const
  * those before which less than top_p[row] (f32) of their weight lies (the first always), and of
  * these the ones of at least min_p[row] (f32) times the first's weight; the
  * token is drawn among them by weight, in index order.
- * A token's weight is the whole number rint(2^40 exp((logit - highest) /
- * temperature[row])), the sums are exact, and the token is the first kept index
+ * A token's weight is 2^40 exp((logit - highest) / temperature[row]) as a whole
+ * number, at most 0.51 off and the same for the same three numbers wherever they
+ * stand; the sums are exact, and the token is the first kept index
  * whose running weight passes floor(uniform x weight kept), the uniform and top_p taken to 31 bits:
  * the result depends on no order of summation, and two calls agree. Each
  * option may be NULL (off), as are top_k <= 0, top_p >= 1 and min_p <= 0; NULL

@@ -1,9 +1,9 @@
 // One token a row of logits, drawn with a given uniform random number.
 //
-// Tokens rank by logit, ties by index; a token's weight is the whole number
-// rint(2^40 exp((logit - highest) / temperature)), computed in 64 bits, so
-// sums of weights are exact whatever their order, and a vocabulary of up to
-// 2^22 tokens sums below 2^62. Each option keeps a prefix of the ranking, so
+// Tokens rank by logit, ties by index; a token's weight is 2^40 exp((logit -
+// highest) / temperature) as a whole number (sample.hpp), so sums of weights are
+// exact whatever their order, and a vocabulary of up to 2^22 tokens sums below
+// 2^62. Each option keeps a prefix of the ranking, so
 // what is kept is one cut (a logit and an index) and a least weight.
 //
 // Sorting the row is not needed to find the cut. Four launches, a row cut into slices:
@@ -23,6 +23,7 @@
 // More candidates than the list holds (thousands of equal logits at the cut)
 // are counted digit by digit of their logits instead (cut_by_digits), as is
 // min-p at temperatures that lead the bins out of f32's range.
+#include "sample.hpp"
 #include "scan.hpp"
 
 namespace {
@@ -49,23 +50,6 @@ __device__ inline uint32_t rank_key(float v) {
 }
 __device__ inline float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// Coefficients ln(2)^k / k! of 2^f: for |f| <= 1/2 the terms left out are below 2^-47 of it.
-struct Exp2Terms {
-    double c[12];
-    constexpr Exp2Terms() : c() {
-        c[0] = 1.0;
-        for (int k = 1; k < 12; ++k) c[k] = c[k - 1] * 0.69314718055994530942 / k;
-    }
-};
-
-// a * b + c of a c that is the same in all lanes, kept in scalar registers (the compiler's own choice adds into c,
-// which takes a copy of each constant first).
-__device__ inline double fma64(double a, double b, double c) {
-    double d;
-    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
-    return d;
-}
-
 struct Options {
     const float *uniforms, *temperature;
     const int32_t *topK;
@@ -75,25 +59,14 @@ struct Options {
 // One row's options, and its highest logit.
 struct Row {
     float top, bins;  // bins per unit of distance
-    double rate;      // log2(e) / temperature
+    double rate;      // pk::sample_rate
     u64 least;
     float p;
     uint32_t k;
     bool live, useK, useP;
     bool binned;  // bins are as the definition has them; else they only keep the order
 
-    __device__ inline u64 weight(float v) const {
-        constexpr Exp2Terms terms;
-        const double t = ((double)v - (double)top) * rate;
-        const double n = __builtin_rint(t), f = t - n;
-        double s = terms.c[11];
-#pragma unroll
-        for (int k = 10; k >= 0; --k) s = fma64(s, f, terms.c[k]);
-        // adding 2^52 rounds to a whole number and leaves it in the low bits
-        const double w = __builtin_ldexp(s, (int)n + 40) + 4503599627370496.0;
-        const u64 u = (t > -42.0) & (v > -INFINITY) ? __builtin_bit_cast(u64, w) & 0xfffffffffffffull : 0;  // (a NaN is 0)
-        return v == top ? (u64)1 << 40 : u;
-    }
+    __device__ inline u64 weight(float v) const { return pk::sample_weight(v, top, rate); }
     __device__ inline float uniform(const Options &o, uint32_t r) const { return rate < INFINITY ? o.uniforms[r] : 0.0f; }
     // Grows, if anything, from a logit to the next in the ranking.
     __device__ inline uint32_t bin(float v) const {
@@ -110,7 +83,7 @@ __device__ inline Row row_of(const Options &o, uint32_t r, uint32_t topKey, cons
     const float p = c.hasTopP ? o.topP[r] : 1.0f, least = c.hasMinP ? o.minP[r] : 0.0f;
     // a temperature of 0 leaves weight to the highest logit alone, of which a uniform of 0 draws the first: no cut
     const bool greedy = !(t > 0.0f);
-    w.rate = greedy ? INFINITY : 1.4426950408889634074 / (double)t;
+    w.rate = pk::sample_rate(greedy ? 0.0f : t);
     w.bins = 72.0f / t;  // weights end at a distance of 28.5 temperatures
     w.binned = t > 3e-37f && t < 1e37f;  // neither 72 / t nor a distance of 28.5 t passes the largest number
     w.k = k > 0 ? (uint32_t)k : 0u;
