@@ -11,8 +11,8 @@
 //  2. sample_hist: number and weight of the tokens of each slice in 2048
 //     bins of the distance from the highest, and their sums over the row;
 //  3. sample_gather: the bins in which the cuts must fall, from the bins'
-//     running sums; their tokens (the candidates, a few hundred of a large
-//     vocabulary) go to a list, and of each slice the weight of what lies before;
+//     running sums; their tokens (the candidates, a few hundred where a model
+//     has its preferences) go to a list, and of each slice the weight of what lies before;
 //  4. sample_finish: the cuts among the candidates, by selection, the
 //     slice where the running weight passes the draw, and the token in it.
 // Only the second evaluates the whole row's weights, which bounds it (26 us of
@@ -20,9 +20,14 @@
 // and 18, the last with one block to a row). A row that neither top-k
 // nor top-p cuts has its slices' weights summed by the third instead.
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
-// More candidates than the list holds (thousands of equal logits at the cut)
-// are counted digit by digit of their logits instead (cut_by_digits), as is
-// min-p at temperatures that lead the bins out of f32's range.
+// More candidates than the list holds are counted digit by digit of their
+// logits instead (cut_by_digits): thousands of equal logits at the cut, or a flat
+// row, where a bin's 1/72 of a temperature is wide enough for thousands of
+// different ones (256000 normal logits of spread 0.5 at temperature 2 put about
+// 5500 in top-p's bin). So is min-p at temperatures that lead the bins out of
+// f32's range. One block then reads the row 6 to 11 times: 64 such rows of
+// 256000 take 0.65 ms instead of 0.07, 0.90 with top-k too, one 0.47; 64 of equal
+// logits, whose additions all meet in one word, 1.37.
 #include "sample.hpp"
 #include "scan.hpp"
 

@@ -219,3 +219,22 @@ def test_sample_greedy_rows_among_others(env, vocab):
         got = check(env, x, "f32", u, temperature=t, **kw)
         want = [int(np.nanargmax(np.where(np.isnan(r), -np.inf, r))) for r in x]
         assert got[3] == -1 and all(got[r] == want[r] for r in (0, 2, 4, 5, 6))
+
+
+def most_in_a_bin(x, t):
+    """The tokens in the fullest of the bins, 72 to a temperature, that the cuts are looked for in."""
+    return np.bincount(np.minimum((x.max() - x) * (72.0 / t), 2047).astype(np.int64)).max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("options", [dict(top_p=[0.5, 0.6, 0.7]), dict(top_k=[60000, 128000, 150000]),
+                                     dict(top_k=[200000] * 3, top_p=[0.5, 0.7, 0.6], min_p=[0.0, 0.001, 0.3])], ids=lambda o: "-".join(o))
+def test_sample_flat_rows(env, dtype, options):
+    # distinct logits that lie close together: the bin with the cut holds more candidates than their list
+    g = np.random.default_rng(22)
+    x = rounded(g.standard_normal((3, 256000)) * 0.5, dtype)
+    x[:, 0] = x.max()  # rows of one highest logit and one temperature
+    assert all(most_in_a_bin(r, 2.0) > 5000 for r in x)
+    assert dtype == "bf16" or len(np.unique(x[0])) > 250000
+    for u in (g.random(3), [0.0, 0.5, 1.0 - 2.0 ** -24]):
+        check(env, x, dtype, u, temperature=[2.0] * 3, **options)
