@@ -577,8 +577,15 @@ popcorn_status_t popcorn_kernel_embedding_gather_quantized(const popcorn_tensor_
  *     order; entries of pages that hold past keys are read; others stay;
  *   counts i32 [2]: tokens and free pages that the step needs.
  * T is positions' length. Where the free pages or the table's columns run out
- * the entry becomes -1 and the tokens' slots -1; tokens past T are left out.
- * Both show in counts. */
+ * the entry becomes -1 and the tokens' slots -1; tokens past T are left out, with
+ * the entries of pages that they would begin. Both show in counts. T is to hold
+ * the step's tokens: key_lens counts those past T too, so that PagedAttention
+ * takes the kept tokens of the request that T cuts for its last ones. Where
+ * counts[0] passes T that request's rows (and the requests behind it, which have
+ * none) are to be computed by another step. All requests before it are as in a
+ * step with room, and what was written of it stays right: the step can be run
+ * again, from the same lengths and free pages, with a greater T or with fewer
+ * new tokens. */
 popcorn_status_t popcorn_kernel_page_tables(const popcorn_tensor_t *past_lens, const popcorn_tensor_t *new_lens,
                                             const popcorn_tensor_t *free_pages, const popcorn_tensor_t *page_tables,
                                             int64_t page_size, const popcorn_tensor_t *query_starts,

@@ -203,3 +203,59 @@ def test_scratch_that_is_refused(env):
             enc.encode(kernel)
         assert e.value.code == pa.PopcornError.TENSOR_ALLOCATION_FAILED
     stream.synchronize()
+
+
+@pytest.mark.parametrize("room", [15, 3, 0, 26])
+def test_step_without_room_for_its_tokens(env, room):
+    # T cuts a request: those before it are as in a step with room, nothing of another request is written, and the
+    # step run again with room (or with the tokens that had it) gives everything
+    pa, lib, stream, enc = env
+    K = pa.Kernels
+    g = np.random.default_rng(30 + room)
+    past, new, columns, pages = np.array([21, 0, 16, 40, 5]), np.array([3, 20, 9, 5, 0]), 5, 40
+    total = int(new.sum())
+    held = -(-past // PAGE)
+    ids = g.permutation(pages)
+    table = np.full((5, columns), -1)
+    at = 0
+    for r in range(5):
+        table[r, :held[r]] = ids[at:at + held[r]]
+        at += held[r]
+    free = ids[at:]
+    host = [rounded(g.standard_normal((pages, NKV, PAGE, HD)), "bf16") for _ in range(2)]
+    caches = [upload(pa, x, "bf16") for x in host]
+    tables = i32(pa, table)
+    rows = {n: rounded(g.standard_normal((total, h, HD)), "bf16") for n, h in (("q", NQ), ("k", NKV), ("v", NKV))}
+    old = rounded(g.standard_normal((total, NQ, HD)), "bf16")
+
+    def step(T, lens):
+        d = [i32(pa, np.full(n, -77)) for n in (6, 5, T, T, 2)]
+        q, k, v, out = (upload(pa, x[:T], "bf16") for x in (rows["q"], rows["k"], rows["v"], old))
+        enc.encode([K.PageTables(i32(pa, past), i32(pa, lens), i32(pa, free), tables, page_size=PAGE, query_starts=d[0], key_lens=d[1],
+                                 positions=d[2], slots=d[3], counts=d[4]),
+                    K.PagedKVCacheWrite(k, v, d[3], *caches),
+                    K.PagedAttention(q, *caches, tables, d[0], d[1], out, scale=0.09)])
+        stream.synchronize()
+        return [t.numpy(stream) for t in d], download(out, stream), [download(c, stream) for c in caches], tables.numpy(stream)
+
+    def check(T, lens, upto):
+        want = R.page_tables(past, lens, free, table, PAGE, T)
+        d, out, cache, got_table = step(T, lens)
+        np.testing.assert_array_equal(got_table, want[0])
+        for a, b in zip(d, want[1:]):
+            np.testing.assert_array_equal(a, b)
+        assert d[4][0] == lens.sum()  # what the host looks at
+        for x, c, n in zip(host, cache, "kv"):
+            w = x.copy()
+            for t, s in enumerate(want[4]):
+                w[s // PAGE, :, s % PAGE] = rows[n][t]
+            np.testing.assert_array_equal(c, w)
+        filled = [c.copy() for c in cache]
+        att, parts = R.attention(rows["q"][:upto], *filled, want[0], np.minimum(want[1], upto), want[2], old[:upto], float(np.float32(0.09)))
+        assert (np.abs(out[:upto] - att) <= R.attention_bound(att, parts, "bf16", HD)).all()
+
+    starts = np.concatenate([[0], np.cumsum(new)])
+    check(room, new, int(starts[starts <= room].max()))
+    if room:  # the tokens that had room, as a step of their own
+        check(room, np.clip(room - starts[:-1], 0, new), room)
+    check(total, new, total)
