@@ -259,3 +259,52 @@ def test_step_without_room_for_its_tokens(env, room):
     if room:  # the tokens that had room, as a step of their own
         check(room, np.clip(room - starts[:-1], 0, new), room)
     check(total, new, total)
+
+
+def test_step_to_its_tokens_from_a_graph(env):
+    # tables, rows, attention, the last row of each request, logits and tokens in one graph, replayed with other lengths
+    pa, lib, _, _ = env
+    import oracle as O
+
+    stream = pa.Stream()
+    enc = pa.KernelCommandEncoder(lib, stream)
+    K, R_, T, H, vocab = pa.Kernels, 5, 310, NQ * HD, 6000
+    server, other = (Server(pa, stream, R_, T, 60, 24, seed=s) for s in (8, 9))
+    g = np.random.default_rng(10)
+    head = rounded(g.standard_normal((vocab, H)) * 0.5, "bf16")
+    lm_head, hidden = upload(pa, head, "bf16"), upload(pa, np.zeros((T + 1, H)), "bf16")
+    last, logits = pa.Tensor.empty([R_, H], "bf16"), pa.Tensor.empty([R_, vocab], "bf16")
+    u, t, m = (pa.Tensor.from_numpy(np.zeros(R_, np.float32)) for _ in range(3))
+    d = server.d
+    step = [server.kernels[0], server.kernels[1],
+            K.PagedAttention(server.q, server.k_cache, server.v_cache, d["tables"], d["starts"], d["keys"],
+                             hidden.view([T, NQ, HD], offset_elements=H), scale=0.09),
+            K.EmbeddingGather(d["starts"].view([R_], offset_elements=1), hidden, last),
+            K.Matmul(last, lm_head, logits, True),
+            K.Sample(logits, u, d["tokens"], temperature=t, top_k=server.top_k, top_p=server.top_p, min_p=m)]
+    enc.encode(step)  # once before the capture
+    graph = Graph(pa, stream, lambda: enc.encode(step))
+    for new in STEPS:
+        want, _, _, _ = server.feed(new)
+        hidden.copy_from(O.to_bits(np.zeros((T + 1, H), np.float32), O.BF16), stream)
+        uv, tv, mv = g.random(R_).astype(np.float32), g.uniform(0.5, 2, R_).astype(np.float32), g.uniform(0, 0.02, R_).astype(np.float32)
+        for x, a in ((u, uv), (t, tv), (m, mv)):
+            x.copy_from(a, stream)
+        graph.launch()
+        stream.synchronize()
+        np.testing.assert_array_equal(d["starts"].numpy(stream), want[1])
+        rows, x = download(hidden, stream), download(logits, stream)
+        np.testing.assert_array_equal(download(last, stream), rows[want[1][1:]])
+        ends = np.flatnonzero(new)
+        assert rows[want[1][1:]][ends].any(axis=1).all() and not rows[0].any() and not rows[1 + want[1][-1]:].any()
+        exact = rows[want[1][1:]].astype(np.float64) @ head.T.astype(np.float64)
+        # sums of H products of 16-bit values in f32, then one rounding
+        mag = np.abs(rows[want[1][1:]]).astype(np.float64) @ np.abs(head.T).astype(np.float64)
+        assert (np.abs(x - exact) <= 2.0 ** -8 * np.abs(exact) + (H + 1) * 2.0 ** -24 * mag).all()
+        options = dict(temperature=tv, top_k=np.full(R_, 40), top_p=np.full(R_, 0.9), min_p=mv)
+        np.testing.assert_array_equal(d["tokens"].numpy(stream), R.sample(x, uv, **options))
+        expected = other.feed(new[::-1])
+        enc.encode(other.kernels)
+        stream.synchronize()
+        other.check(expected)
+    graph.close()
