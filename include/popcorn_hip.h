@@ -613,7 +613,8 @@ popcorn_status_t popcorn_kernel_paged_kv_cache_write(const popcorn_tensor_t *k, 
  * q, the caches and out share one dtype (f32, f16, bf16); page_size is a
  * multiple of 16, Hd at most 512. max_query_len (0: unknown) is the longest
  * request's number of new tokens; the kernels are chosen for it, and with any
- * value they serve every request. */
+ * value they serve every request. Where it (or T, for 0) allows prompts, steps of
+ * single tokens take 1.1 to 1.3 times as long as with 1. T x Nq is below 2^24. */
 popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
                                                 const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
                                                 const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens,

@@ -724,7 +724,8 @@ class Kernels:
                        key_lens: Tensor, into: Tensor, *, scale: float, mask: AttentionMask = AttentionMask(0),
                        sinks: int = 0, max_query_len: int = 0) -> Kernel:
         """Attention of every request's new tokens q [T, Nq, Hd] over its pages (popcorn_kernel_paged_attention);
-        max_query_len, the longest request's number of new tokens, chooses the kernels."""
+        max_query_len, the longest request's number of new tokens, chooses the kernels: a graph for steps of single
+        tokens is captured with 1."""
         ts = (q, k_cache, v_cache, page_tables, query_starts, key_lens, into)
         return _make(lib().popcorn_kernel_paged_attention, *[_d(t) for t in ts], scale, mask.desc(), sinks,
                      max_query_len, refs=ts)
