@@ -99,4 +99,35 @@ PAGED_FN uint64_t paged_share(uint64_t total, const PagedWorkConstants &w) {
     return q > w.minSteps ? q : w.minSteps;
 }
 
+// The worker of counted step `at` of all units. (A division of 64 bits takes ten times as long as one of 32.)
+PAGED_FN uint32_t paged_worker(uint64_t at, uint64_t share) {
+    return (at | share) >> 32 ? (uint32_t)(at / share) : (uint32_t)at / (uint32_t)share;
+}
+
+// What a worker takes next of a tile's units, one per KV head: steps lo .. hi - 1 of head hkv's, none where it reaches the unit's
+// extra count only. `in`: counted steps of the units before the worker's place; `left`: counted steps to the end of its stretch;
+// n: steps of a unit.
+struct PagedPiece {
+    uint32_t hkv, lo, hi;
+    uint32_t taken, behind;  // counted steps of it, and of the unit behind it
+};
+
+PAGED_FN PagedPiece paged_piece(uint64_t in, uint64_t left, uint32_t n, const PagedWorkConstants &w) {
+    const uint32_t all = n + w.unitSteps;
+    PagedPiece c;
+    c.hkv = in >> 32 ? (uint32_t)(in / all) : (uint32_t)in / all;
+    const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * all), hi = left < all - lo ? lo + (uint32_t)left : all;
+    c.lo = (lo > w.unitSteps ? lo : w.unitSteps) - w.unitSteps;
+    c.hi = (hi > w.unitSteps ? hi : w.unitSteps) - w.unitSteps;
+    c.taken = hi - lo;
+    c.behind = all - hi;
+    return c;
+}
+
+// How many workers share the unit of a worker's last piece, where the piece begins the unit and leaves some of it (its stretch
+// ends at `end`); else 0.
+PAGED_FN uint32_t paged_sharers(const PagedPiece &c, uint32_t n, uint64_t end, uint64_t share, uint32_t worker) {
+    return c.lo == 0 && c.hi > 0 && c.hi < n ? paged_worker(end + c.behind - 1, share) - worker + 1 : 0u;
+}
+
 }  // namespace pk

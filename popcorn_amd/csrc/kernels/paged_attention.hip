@@ -233,9 +233,6 @@ struct Dealer {
     uint64_t share, x, end;
     uint32_t tile;
 
-    // The worker of step at of all units.
-    __device__ inline uint32_t last_of(uint64_t at) const { return (at | share) >> 32 ? (uint32_t)(at / share) : (uint32_t)at / (uint32_t)share; }
-
     // `space` is free again afterwards.
     __device__ inline Dealer(const int32_t *st, const int32_t *kl, const pk::PagedTile *pl, OwnTile *ow, PlanSpace<NT, uint32_t> &space,
                              Shared *sh, const PagedAttentionConstants &p, const PagedWorkConstants &w)
@@ -278,19 +275,15 @@ struct Dealer {
             c.request = t.request;
             c.req = pk::paged_request(starts[t.request], starts[t.request + 1], keyLens[t.request], p);
             c.steps = pk::paged_steps(c.req, t.tile, p, w);
-            const uint64_t in = x - t.before * p.Nkv;  // counted steps before x of this tile's units
-            const uint32_t n = c.steps.n + w.unitSteps;
-            c.hkv = in >> 32 ? (uint32_t)(in / n) : (uint32_t)in / n;  // (64 bits take ten times as long)
-            const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * n), hi = (uint32_t)min((uint64_t)n, lo + (end - x));
-            c.lo = max(lo, w.unitSteps) - w.unitSteps;
-            c.hi = max(hi, w.unitSteps) - w.unitSteps;
-            x += hi - lo;
-            if (hi == n && c.hkv + 1 == p.Nkv) ++tile;
-            if (x == end && threadIdx.x == 0) {
-                Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, w.rows, w.stateBase, blockIdx.x};
-                if (c.lo == 0 && c.hi > 0 && c.hi < c.steps.n) sh.pieces = last_of(end + (n - hi) - 1) - blockIdx.x + 1;
-                *shared = sh;
-            }
+            const pk::PagedPiece piece = pk::paged_piece(x - t.before * p.Nkv, end - x, c.steps.n, w);
+            c.hkv = piece.hkv;
+            c.lo = piece.lo;
+            c.hi = piece.hi;
+            x += piece.taken;
+            if (piece.behind == 0 && c.hkv + 1 == p.Nkv) ++tile;
+            if (x == end && threadIdx.x == 0)
+                *shared = Shared{pk::paged_sharers(piece, c.steps.n, end, share, blockIdx.x), (uint32_t)c.req.start, c.hkv, c.steps.r0,
+                                 c.steps.r1, w.rows, w.stateBase, blockIdx.x};
             if (c.lo < c.hi) return true;
         }
         return false;

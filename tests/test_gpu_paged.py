@@ -421,3 +421,75 @@ def test_attention_odd_rows(env, dtype, heads, mask, sinks):
 def test_attention_long_keys_in_tiles(env, dtype, heads, mask, sinks):
     # one new token in a tile beside a chunk, and more steps for a block than it looks up pages for at once
     Batch([(20000, 1), (19900, 40)], *heads, dtype, 64, seed=18).check(env, mask, sinks)
+
+
+# ---- plans laid out in memory: more tiles or requests than a block lays out by itself ----------------------
+
+
+def launches(b, hint=None):
+    """The kernels of a batch's call, in order."""
+    import popcorn_amd as pa
+
+    fake = lambda i, shape, t: pa.Tensor(0x7F0000000000 + (i << 44), list(shape), t)  # (descriptors only validate)
+    k = pa.Kernels.PagedAttention(fake(1, b.q.shape, b.dtype), fake(2, b.k.shape, b.dtype), fake(3, b.v.shape, b.dtype),
+                                  fake(4, b.table.shape, "i32"), fake(5, [len(b.lens) + 1], "i32"), fake(6, [len(b.lens)], "i32"),
+                                  fake(7, b.q.shape, b.dtype), scale=b.scale,
+                                  max_query_len=max(n for _, n in b.lens) if hint is None else hint)
+    return [n.replace("paged_attention_", "").replace("paged_", "").split("_")[0] for n in k.function_names]
+
+
+@pytest.mark.parametrize("dtype,hd", [("bf16", 64), ("f16", 128), ("bf16", 256)])
+def test_planned_few_and_tiles(env, dtype, hd):
+    # more requests than a block lays out: both launches read plans, each its own
+    g = np.random.default_rng(40)
+    lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 60, 1100), g.integers(0, 3, 1100))]
+    for r, x in ((0, (70, 50)), (500, (0, 90)), (501, (33, 17)), (777, (130, 40)), (1099, (5, 66))):
+        lens[r] = x
+    b = Batch(lens, 4, 2, hd, dtype, 16, seed=41, pad=2)
+    assert launches(b) == ["plan", "few", "plan", "tile", "merge"]
+    b.check(env)
+    b.check(env, (1, 40), 3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_planned_few_beside_tiles_of_the_blocks(env, dtype):
+    # more tiles of 16 rows than a block lays out, fewer of 128 rows: a plan for one launch only
+    g = np.random.default_rng(42)
+    lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 90, 520), g.integers(1, 5, 520))]
+    lens[3], lens[100], lens[519] = (64, 100), (0, 300), (17, 60)
+    b = Batch(lens, 16, 2, 64, dtype, 16, seed=43, pad=1)
+    assert launches(b) == ["plan", "few", "tile", "merge"]
+    b.check(env)
+    b.check(env, (1, 30), 20)
+
+
+@pytest.mark.parametrize("dtype,heads", [("bf16", (16, 1, 64)), ("f16", (16, 1, 64)), ("f16", (16, 1, 128))], ids=str)
+def test_planned_tiles_of_a_long_prompt(env, dtype, heads):
+    # one prompt of more tiles than a block lays out; a window keeps the reference small
+    b = Batch([(20, 8250)], *heads, dtype, 64, seed=44, pad=3)
+    assert launches(b) == ["plan", "tile", "merge"]
+    got = b.run(env, (1, 24), 2)
+    rows = np.r_[0:40, 4000:4030, 8220:8250]
+    want, parts = sampled_rows(b, rows, (1, 24), 2)
+    assert (np.abs(got[rows] - want) <= R.attention_bound(want, parts, dtype, b.hd)).all()
+    np.testing.assert_array_equal(got[8250:], b.old[8250:])
+    assert np.isfinite(got).all()
+
+
+def sampled_rows(b, rows, mask, sinks):
+    """The reference of some new tokens of a batch of one request: each as a request of its own over the same pages."""
+    past, n = b.lens[0]
+    keys = np.array([past + r + 1 for r in rows])
+    return R.attention(b.q[rows], b.k, b.v, np.repeat(b.table, len(rows), 0), np.arange(len(rows) + 1), keys, b.old[rows], b.scale,
+                       mask[0], mask[1], sinks)
+
+
+@pytest.mark.parametrize("dtype,hd", [("bf16", 512), ("f32", 256)])
+def test_planned_few_of_other_kinds(env, dtype, hd):
+    # requests of a row and a prompt without tiles
+    g = np.random.default_rng(45)
+    lens = [(int(p), int(n)) for p, n in zip(g.integers(0, 40, 1060), g.integers(0, 2, 1060))]
+    lens[9] = (30, 70)
+    b = Batch(lens, 4, 2, hd, dtype, 16, seed=46, pad=2)
+    assert launches(b) == ["plan", "few", "merge"]
+    b.check(env)
