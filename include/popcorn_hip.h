@@ -610,6 +610,9 @@ popcorn_status_t popcorn_kernel_paged_kv_cache_write(const popcorn_tensor_t *k, 
  * does not see, and rows of the pages behind the last key, may hold anything. A key whose
  * table entry names no page of the cache is left out. A row that sees no key
  * is 0; rows outside the requests' ranges are left as they were.
+ * Scores, maxima and sums are f32. A weight meets V in f32, as two bf16 (2^-16
+ * off) or as two f16 (2^-22); in f16 as one (2^-11, as the result is rounded) where
+ * requests bring many rows (prompts).
  * q, the caches and out share one dtype (f32, f16, bf16); page_size is a
  * multiple of 16, Hd at most 512. max_query_len (0: unknown) is the longest
  * request's number of new tokens; the kernels are chosen for it, and with any

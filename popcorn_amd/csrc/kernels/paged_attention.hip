@@ -712,7 +712,10 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
     constexpr int BKV = 64, KS = HD / 16, DT = HD / 32, CH = HD / 8;
     constexpr int kRowsPer = 64 / CH;       // rows per copy instruction
     constexpr int kCopies = 16 / kRowsPer;  // instructions for a wave's 16 rows of K (or V) of a step
-    constexpr bool kTwo = std::is_same<T, pk::BF16>::value;  // weights as two bf16, or one f16
+    // The words of a weight in the product with V. One bf16 has 8 bits, so there are two, 2^-16 off. One f16 has 11, as many as
+    // the result: 2048 tokens behind 8192 keys, 8 heads of 256 on 4, are 2.9e-4 off (2-norm, against 64 bits) in 193 us; with two
+    // words 2.1e-4, which the rounding of the result alone makes, in 250 (1000 tokens of 128 dims 70 and 88). As FlashAttention.
+    constexpr bool kTwo = std::is_same<T, pk::BF16>::value;
     constexpr float kLead = kTwo ? 0.0f : 4.0f;
     constexpr uint32_t kTileBytes = BKV * HD * 2;
     // K's two places, V's two, the plan (one array: with two, the compiler has every read of LDS wait for the latest copy)

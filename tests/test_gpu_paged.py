@@ -493,3 +493,57 @@ def test_planned_few_of_other_kinds(env, dtype, hd):
     b = Batch(lens, 4, 2, hd, dtype, 16, seed=46, pad=2)
     assert launches(b) == ["plan", "few", "merge"]
     b.check(env)
+
+
+# ---- the bits of a weight in its product with V ---------------------------------------------
+
+
+def words_of(w, dtype, words):
+    """A weight as the sum of `words` numbers of the type."""
+    left, total = np.array(w, np.float64), 0.0
+    for _ in range(words):
+        part = rounded(left, dtype).astype(np.float64)
+        total, left = total + part, left - part
+    return total
+
+
+def against_each_other(dtype, lens, heads, page, seed):
+    """Keys of two scores in turn, whose weights meet values that take each other away: what a weight loses in its
+    rounding is left, where in a sum of random values the rounding of the result hides it."""
+    b = Batch(lens, *heads, dtype, page, seed=seed)
+    b.scale = 1.0
+    b.q[:], b.q[..., 0] = 0.0, 1.0
+    # the score whose weight has the largest remainder behind one word (the maximum's weight is a power of two)
+    scores = np.arange(1, 129) / 64.0
+    lost = np.abs(words_of(np.exp(-scores), dtype, 1) - np.exp(-scores)) * np.exp(scores)
+    low = -scores[np.argmax(lost)]
+    for r, (p, n) in enumerate(b.lens):
+        for j in range(p + n):
+            at = (b.table[r, j // page], slice(None), j % page)
+            b.k[at] = 0.0
+            b.k[at + (0,)] = low if j % 2 else 0.0
+            b.v[at] = rounded(-np.exp(-low) if j % 2 else 1.0, dtype)
+    return b, low
+
+
+@pytest.mark.parametrize("dtype,lens,heads,kind,words", [
+    ("f16", [(255, 1), (600, 1)], (4, 2, 64), "few", 2), ("f16", [(128, 4)], (8, 2, 128), "few", 2), ("f16", [(201, 1)], (8, 4, 256), "few", 2),
+    ("f16", [(99, 9)], (2, 1, 512), "few", 2), ("bf16", [(255, 1), (600, 1)], (4, 2, 64), "few", 2), ("bf16", [(201, 1)], (8, 4, 256), "few", 2),
+    ("bf16", [(99, 9)], (2, 1, 512), "few", 2), ("bf16", [(128, 72)], (8, 2, 64), "tile", 2), ("bf16", [(100, 60)], (8, 2, 128), "tile", 2),
+    ("bf16", [(64, 90)], (4, 2, 256), "tile", 2), ("f16", [(128, 72)], (8, 2, 64), "tile", 1), ("f16", [(64, 90)], (4, 2, 256), "tile", 1)])
+def test_attention_weights_keep_their_bits(env, dtype, lens, heads, kind, words):
+    b, low = against_each_other(dtype, lens, heads, 16, seed=50)
+    assert launches(b)[0] == kind
+    got = b.run(env)
+    want, (mag, spread, count) = R.attention(b.q, b.k, b.v, b.table, b.starts, b.keys, b.old, b.scale)
+    # as R.attention_bound, with the words of this kernel: 11 bits in an f16, 8 in a bf16, and as many in the second
+    weight = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8}[dtype] ** words
+    eps = 2.0 * ((heads[2] + 3) * 2.0 ** -24 * spread + 2.0 ** -22) + weight + (count + 8) * 2.0 ** -24
+    bound = R.HALF[dtype] * np.abs(want) + R.TINY[dtype] + mag * eps * (1.0 + R.HALF[dtype])
+    assert (np.abs(got - want) <= bound).all()
+    if words == 2:  # a kernel that lost the second word would not pass
+        last = b.starts[1:] - 1
+        n = b.keys // 2
+        w = np.exp(low)
+        lost = n * abs(words_of([w], dtype, 1)[0] - w) * np.exp(-low) / (b.keys - n + n * w)
+        assert (lost > 2 * bound[last].max(axis=(1, 2))).all(), (lost, bound[last].max(axis=(1, 2)))
