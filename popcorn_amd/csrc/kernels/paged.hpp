@@ -112,11 +112,12 @@ struct PagedPiece {
     uint32_t taken, behind;  // counted steps of it, and of the unit behind it
 };
 
+// (hi as it stands: compared in 32 bits it made the few-row kernels 300 instructions longer, 64 requests' decode 137.5 -> 139.6 us.)
 PAGED_FN PagedPiece paged_piece(uint64_t in, uint64_t left, uint32_t n, const PagedWorkConstants &w) {
     const uint32_t all = n + w.unitSteps;
     PagedPiece c;
     c.hkv = in >> 32 ? (uint32_t)(in / all) : (uint32_t)in / all;
-    const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * all), hi = left < all - lo ? lo + (uint32_t)left : all;
+    const uint32_t lo = (uint32_t)(in - (uint64_t)c.hkv * all), hi = (uint32_t)(lo + left < all ? lo + left : all);
     c.lo = (lo > w.unitSteps ? lo : w.unitSteps) - w.unitSteps;
     c.hi = (hi > w.unitSteps ? hi : w.unitSteps) - w.unitSteps;
     c.taken = hi - lo;

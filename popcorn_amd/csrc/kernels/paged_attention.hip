@@ -281,9 +281,11 @@ struct Dealer {
             c.hi = piece.hi;
             x += piece.taken;
             if (piece.behind == 0 && c.hkv + 1 == p.Nkv) ++tile;
-            if (x == end && threadIdx.x == 0)
-                *shared = Shared{pk::paged_sharers(piece, c.steps.n, end, share, blockIdx.x), (uint32_t)c.req.start, c.hkv, c.steps.r0,
-                                 c.steps.r1, w.rows, w.stateBase, blockIdx.x};
+            if (x == end && threadIdx.x == 0) {
+                Shared sh{0, (uint32_t)c.req.start, c.hkv, c.steps.r0, c.steps.r1, w.rows, w.stateBase, blockIdx.x};
+                sh.pieces = pk::paged_sharers(piece, c.steps.n, end, share, blockIdx.x);
+                *shared = sh;
+            }
             if (c.lo < c.hi) return true;
         }
         return false;
