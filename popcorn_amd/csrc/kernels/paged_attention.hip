@@ -344,10 +344,10 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
     __shared__ OwnTile sm_plan[kOwnTiles];
     __shared__ uint32_t sm_bad;
-    // Q of 512 dims in 16 bits is kept in LDS: in registers 60 of 512 spilled (32 requests of 100 to 8000 keys, 8 heads on
-    // 2: 48 us, and 99; 1000 tokens behind as many 148 and 438)
+    // Q of 512 dims in 16 bits is kept in LDS: in registers 60 of 512 spilled, so 4 (32 requests of 100 to 8000 keys, 8 heads
+    // on 2: 48 us, and 99; 1000 tokens behind as many 148 and 438)
     constexpr bool kQInLds = HD == 512 && !kWide;
-    // and in 32 bits, where LDS has no room for it, read again for each step (the same call 135 us, and 325)
+    // and in 32 bits, where LDS has no room for it, read again for each step (19 spilled; the same call 135 us, and 325)
     constexpr bool kQAgain = HD == 512 && kWide;
     __shared__ __attribute__((aligned(16))) u32x4 sm_q[kQInLds ? KS * 64 : 1];
     static_assert(sizeof(PlanSpace<64 * kWaves, uint32_t>) <= sizeof(smem), "the plan is laid out where V goes");
@@ -699,8 +699,10 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
 // of MFMA and 960 of VALU for a step), so step i + 1's scores are computed
 // beside step i's exponentials, and step i's product with V beside the
 // maximum of step i + 1. 2048 tokens behind 8192 keys, 8 heads of 256 in f16:
-// 190 us with the merge, 815 TFLOP/s, where a large product reaches 1250 to 1414;
-// a pass is 3500 cycles, 1500 of them with scores, 1350 with V, 300 at the barrier.
+// 186 to 199 us with the merge, 780 to 830 TFLOP/s, where a large product reaches
+// 1250 to 1414. A pass is 3500 cycles, 1500 of them with scores, 1350 with V (1024
+// of MFMA in each), 300 at the barrier. Counted at 2.04 GHz: a wave lives 321000
+// cycles, 72 passes and 69000 for its starts, states and stores; 148000 (46%) are MFMA.
 constexpr int kTileRows = 128;
 
 template <typename T, int HD>
@@ -1249,6 +1251,9 @@ PAGED_PLAIN(paged_attention_plain_bf16_any, BF16, false)
                                                     PagedAttentionConstants p) {                                          \
         paged_merge<T, HD>(pO, pML, shared, out, p);                                                                      \
     }
+// The blocks per CU limit the registers. Most kernels hold everything in them; of a lane's VGPRs these spill to scratch memory:
+// 11 in tile_bf16_d128 (and 48 bytes of it per lane in all), 2 in tile_f16_d128, 4 in few_f32_d128_r1, 4 in the 16-bit
+// few_d512_r1, 19 in few_f32_d512_r1.
 #define PAGED_FEW_D(t, T, PER256)                                   \
     PAGED_FEW(paged_attention_few_##t##_d64_r1, T, 64, 1, 4)   \
     PAGED_FEW(paged_attention_few_##t##_d64_r2, T, 64, 2, 3)   \

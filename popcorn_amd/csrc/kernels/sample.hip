@@ -15,10 +15,11 @@
 //     has its preferences) go to a list, and of each slice the weight of what lies before;
 //  4. sample_finish: the cuts among the candidates, by selection, the
 //     slice where the running weight passes the draw, and the token in it.
-// Only the second evaluates the whole row's weights, which bounds it (26 us of
-// 64 rows of 256000 bf16 logits, some 35 instructions a logit; the others 8, 18
+// Only the second evaluates the whole row's weights, which bounds it (24 us of
+// 64 rows of 256000 bf16 logits, 49 instructions a logit; the others 8, 18
 // and 18, the last with one block to a row). A row that neither top-k
-// nor top-p cuts has its slices' weights summed by the third instead.
+// nor top-p cuts has its slices' weights summed by the third instead; a call
+// without either has no second launch (64 x 256000 in 40 us).
 // A row of up to 4096 logits is one launch (sample_small): all are candidates.
 // More candidates than the list holds are counted digit by digit of their
 // logits instead (cut_by_digits): thousands of equal logits at the cut, or a flat
