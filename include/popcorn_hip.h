@@ -624,6 +624,72 @@ popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const
                                                 const popcorn_tensor_t *out, float scale, popcorn_attention_mask_t mask,
                                                 int64_t sinks, int64_t max_query_len, popcorn_kernel_t *kernel);
 
+/* PagedAttention of requests that share prefixes. Requests stand in groups that
+ * follow each other: group g's are group_starts[g] .. group_starts[g + 1] - 1
+ * (i32 [groups + 1], ascending), and prefix_lens[g] keys (i32 [groups]) of every one of them lie in
+ * the pages of row g of prefix_tables (i32 [groups, columns]), read once for
+ * the group. A request's own pages hold its keys behind the prefix: key_lens[r]
+ * of them, the new tokens' at the end, at positions prefix_lens[g] + 0, 1, ...
+ * A request of no group has no prefix. A row sees its prefix and its own keys
+ * by the mask, whose window and sinks count positions from the prefix's start; a
+ * prefix lies before every row (of a request with fewer keys than new tokens, the
+ * rows without a key of their own count as the first behind it).
+ * lse (f32 [T, Nq]; NULL: not wanted) gets the natural logarithm of each row's sum of
+ * exp(scale q.k) over the keys it sees: -infinity where it sees none.
+ * prefix_tables, prefix_lens and group_starts may be NULL together: no request has a
+ * prefix, and this is PagedAttention with its lse. Everything else as for PagedAttention; the results
+ * are the same to rounding. Pages that a group shares are read only. */
+popcorn_status_t popcorn_kernel_shared_prefix_attention(
+    const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache, const popcorn_tensor_t *v_cache, const popcorn_tensor_t *prefix_tables,
+    const popcorn_tensor_t *prefix_lens, const popcorn_tensor_t *group_starts, const popcorn_tensor_t *page_tables,
+    const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens, const popcorn_tensor_t *out, const popcorn_tensor_t *lse,
+    float scale, popcorn_attention_mask_t mask, int64_t sinks, int64_t max_query_len, popcorn_kernel_t *kernel);
+
+/* What the new tokens' attention gave each cached key: to weights[r, h, k] (f32
+ * [R, Nkv, columns x page_size], key k of request r for KV head h) is added the sum of exp(scale q.k - lse)
+ * over the request's rows that see the key, in all query heads of the KV head. q, k_cache, tables, starts
+ * and lengths are those of the attention before, lse its logarithms (with a
+ * shared prefix they hold its share too; the prefix's own keys get no weights).
+ * last_rows (0: all): only so many of a request's new tokens count, from its
+ * last one back. The mask is causal or bidirectional: a sliding window's places
+ * are lost once keys have been evicted, so it is refused. Weights of keys that
+ * no counted row sees, and behind the last key, stay as they are; a row with an lse of
+ * -infinity gives nothing. The sums are f32, in an order that the call's lengths alone settle. */
+popcorn_status_t popcorn_kernel_paged_attention_weights(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
+                                                        const popcorn_tensor_t *page_tables, const popcorn_tensor_t *query_starts,
+                                                        const popcorn_tensor_t *key_lens, const popcorn_tensor_t *lse,
+                                                        const popcorn_tensor_t *weights, float scale, popcorn_attention_mask_t mask,
+                                                        int64_t last_rows, int64_t max_query_len, popcorn_kernel_t *kernel);
+
+/* Brings each request's keys down to budgets[r] (i32 [R]; below 0 counts as 0): of its
+ * key_lens[r] keys n = min(key_lens[r], budgets[r]) stay, in each KV head its own: the `first` first
+ * (of n), the `last` last (of the others), and between them those of the highest
+ * weight (f32 [R, Nkv, columns x page_size]; of equal ones the lowest index; NaN ranks lowest). They keep their order and become
+ * keys 0 .. n - 1: kept[r, h, j] (i32, of weights' shape) is the index that key j had,
+ * kept_weights[r, h, j] its weight, 0 from n on (for the next steps' keys); kept behind n,
+ * and cache rows from n on, stay as they were. The keys' rows move within the request's own pages, which
+ * no other request may hold where its kept keys change place (pages of the first
+ * `first` keys may be shared). Rows that no page holds are not moved. weights and
+ * kept_weights change places for the next call. A model's layers share tables and
+ * lengths: this changes neither, ReleasePages does, once, behind the last layer. Keys keep the
+ * rotation of the position they had; new tokens' positions go on from there, past
+ * the number of keys that are left. */
+popcorn_status_t popcorn_kernel_paged_eviction(const popcorn_tensor_t *weights, const popcorn_tensor_t *k_cache,
+                                               const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
+                                               const popcorn_tensor_t *key_lens, const popcorn_tensor_t *budgets,
+                                               const popcorn_tensor_t *kept, const popcorn_tensor_t *kept_weights, int64_t first,
+                                               int64_t last, popcorn_kernel_t *kernel);
+
+/* The lengths behind an eviction, new_lens[r] = min(key_lens[r], budgets[r]) (i32
+ * [R]), for PageTables' past_lens, and the pages that it left empty: the
+ * entries of page_tables (i32 [R, columns]) behind the last kept key's, as they stand there,
+ * request by request from the front of freed (i32 [R x columns]); counts[0]
+ * (i32 [1]) is their number, and freed behind them stays as it was. The tables stay
+ * too: PageTables reads no entry behind a request's past keys before it has written it. */
+popcorn_status_t popcorn_kernel_release_pages(const popcorn_tensor_t *key_lens, const popcorn_tensor_t *budgets,
+                                              const popcorn_tensor_t *page_tables, int64_t page_size, const popcorn_tensor_t *new_lens,
+                                              const popcorn_tensor_t *freed, const popcorn_tensor_t *counts, popcorn_kernel_t *kernel);
+
 /* One token (i32 [rows]) of each row of logits [rows, vocab] (f32, f16, bf16),
  * drawn with the row's uniform random number (f32 [rows], in [0, 1)). Tokens
  * rank by logit, ties by index. Of the first top_k[row] of them (i32) are kept

@@ -476,6 +476,48 @@ typedef struct {
     uint32_t stream;
 } PagedWorkConstants;
 
+/* shared_prefix_*: groups of requests, group g's of groupStarts[g] ..
+ * groupStarts[g + 1] - 1, whose prefix lies in the pages of row g of a table of
+ * `columns`. rows: T x Nq; states: of all partial states, the last 2 x rows of them,
+ * from rowBase on, for units that one block has whole; most: pieces that a unit
+ * may have; parts: waves per row in the merge; windowed: positions are given. */
+typedef struct {
+    uint32_t groups;
+    uint32_t columns;
+    uint32_t windowed;
+    uint32_t hasLse;
+    uint32_t rows;
+    uint32_t states;
+    uint32_t rowBase;
+    uint32_t most;
+    uint32_t parts;
+} SharedPrefixConstants;
+
+/* attention_weights_*: beside PagedAttentionConstants (whose mask is causal or
+ * bidirectional). lastRows: the new tokens of a request that count, from its last
+ * back (0: all); a launch takes the requests of fewRows < rows <= manyRows.
+ * ownPlan: every block sums the requests' keys by itself (at most 1024 requests,
+ * all their groups of 16 keys below 2^32), else attention_weights_plan has. */
+typedef struct {
+    uint32_t lastRows;
+    uint32_t fewRows;
+    uint32_t manyRows;
+    uint32_t ownPlan;
+} AttentionWeightsConstants;
+
+/* evict_*, release_pages: weights [R, Nkv, columns x pageSize]; rowUnits: units
+ * that evict_move_* copies of a cache's row. */
+typedef struct {
+    uint32_t R;
+    uint32_t Nkv;
+    uint32_t columns;
+    uint32_t pageSize;
+    uint32_t pages;
+    uint32_t first;
+    uint32_t last;
+    uint32_t rowUnits;
+} EvictConstants;
+
 /* sample_*: one token of each row of logits [rows, vocab]; a row is cut into
  * `slices` slices of `sliceLen` logits, which sample_gather takes by `parts`
  * blocks. */

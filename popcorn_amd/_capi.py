@@ -190,6 +190,10 @@ PROTOTYPES = {
     "popcorn_kernel_paged_kv_cache_write": (_st, [_T, _T, _T, _T, _T, _K]),
     "popcorn_kernel_paged_attention": (_st, [_T, _T, _T, _T, _T, _T, _T, C.c_float, AttentionMaskDesc, C.c_int64,
                                              C.c_int64, _K]),
+    "popcorn_kernel_shared_prefix_attention": (_st, [_T] * 11 + [C.c_float, AttentionMaskDesc, C.c_int64, C.c_int64, _K]),
+    "popcorn_kernel_paged_attention_weights": (_st, [_T] * 7 + [C.c_float, AttentionMaskDesc, C.c_int64, C.c_int64, _K]),
+    "popcorn_kernel_paged_eviction": (_st, [_T] * 8 + [C.c_int64, C.c_int64, _K]),
+    "popcorn_kernel_release_pages": (_st, [_T, _T, _T, C.c_int64, _T, _T, _T, _K]),
     "popcorn_kernel_sample": (_st, [_T, _T, _T, _T, _T, _T, _T, _K]),
     "popcorn_kernel_custom": (_st, [C.c_char_p, _T, C.POINTER(C.c_uint8), C.c_int32, C.POINTER(C.c_void_p),
                                     C.POINTER(C.c_size_t), C.c_int32, C.POINTER(C.c_uint32),

@@ -1,0 +1,260 @@
+// What a step's attention gives each cached key:
+//   weights[r, hkv, k] += sum of exp(scale q.k - lse) over request r's rows (its last lastRows new tokens, and the query heads
+//   of KV head hkv) that see key k,
+// with the rows' lse from the attention before. K is read once more, V is not, and a key's sum belongs to one
+// wave, so that no order of atomics shows in it.
+#include <type_traits>
+
+#include "mfma.hpp"
+#include "paged.hpp"
+#include "scan.hpp"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kOutOfRange = (int)0x80000000u;
+using pk::u32x4;
+
+__device__ inline uint32_t first_lane(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// A request of the call: the rows that count are tokens start .. start + n - 1, token i at position pos0 + i.
+__device__ inline pk::PagedRequest weights_request(const int32_t *starts, const int32_t *keyLens, uint32_t r, const PagedAttentionConstants &p,
+                                                   const AttentionWeightsConstants &w) {
+    pk::PagedRequest q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
+    if (w.lastRows && (uint32_t)q.n > w.lastRows) {
+        q.pos0 += q.n - (int32_t)w.lastRows;
+        q.start += q.n - (int32_t)w.lastRows;
+        q.n = (int32_t)w.lastRows;
+    }
+    return q;
+}
+
+// Groups of 16 keys that a launch reads of a request, for one KV head.
+__device__ inline uint32_t weights_groups(const pk::PagedRequest &q, const PagedAttentionConstants &p, const AttentionWeightsConstants &w) {
+    const uint32_t rows = (uint32_t)q.n * (p.Nq / p.Nkv);
+    if (rows <= w.fewRows || rows > w.manyRows) return 0;
+    const int32_t last = q.pos0 + q.n - 1;  // (a key behind the last row is nobody's)
+    const int32_t keys = p.maskKind == 2u ? q.keys : min(q.keys, max(last, -1) + 1);
+    return ((uint32_t)keys + 15) / 16;
+}
+
+constexpr uint32_t kOwn = 1024;  // requests that a block sums by itself
+
+}  // namespace
+
+// before[r]: groups of the requests before r; before[R]: of all.
+POPCORN_KERNEL void __launch_bounds__(1024)
+    attention_weights_plan(const int32_t *starts, const int32_t *keyLens, uint64_t *before, PagedAttentionConstants p, AttentionWeightsConstants w) {
+    __shared__ uint64_t sums[16];
+    uint64_t run = 0;
+    for (uint32_t base = 0; base < p.R; base += 1024) {
+        const uint32_t r = base + threadIdx.x;
+        const uint64_t n = r < p.R ? weights_groups(weights_request(starts, keyLens, r, p, w), p, w) : 0u;
+        const pk::Scan<uint64_t> s = pk::block_scan<16>(n, sums);
+        if (r < p.R) before[r] = run + s.upto - n;
+        run += s.total;
+    }
+    if (threadIdx.x == 0) before[p.R] = run;
+}
+
+namespace {
+
+// A few rows: a wave takes a stretch of the groups of all (request, KV head), 16 KM keys at a time: S^T = K . Q^T on 16x16
+// products, so that a key's scores lie in the 16 lanes of a row of lanes, K from memory to fragments a step ahead.
+template <typename T, int HD, int KM>
+__device__ void weights_few(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
+                            const int32_t *__restrict__ tables, const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                            const float *__restrict__ lse, const uint64_t *__restrict__ plan, float *__restrict__ weights,
+                            const PagedAttentionConstants &p, const AttentionWeightsConstants &w) {
+    using S = typename T::storage;
+    constexpr bool kWide = sizeof(S) == 4;
+    constexpr int E = 16 / sizeof(S), KS = HD / (4 * E);
+    __shared__ uint32_t sBefore[kOwn + 1];
+    __shared__ uint32_t sSums[4];
+    const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15, wave = first_lane(threadIdx.x >> 6);
+    const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
+    const float c2 = p.scale * kLog2e;
+    const uint64_t room = (uint64_t)p.columns * p.pageSize;
+    if (w.ownPlan) {
+        uint32_t run = 0;
+        for (uint32_t base = 0; base < p.R; base += 256) {
+            const uint32_t r = base + threadIdx.x;
+            const uint32_t n = r < p.R ? weights_groups(weights_request(starts, keyLens, r, p, w), p, w) : 0u;
+            const pk::Scan<uint32_t> s = pk::block_scan<4>(n, sSums);
+            if (r < p.R) sBefore[r] = run + s.upto - n;
+            run += s.total;
+        }
+        if (threadIdx.x == 0) sBefore[p.R] = run;
+        __syncthreads();
+    }
+    auto before = [&](uint32_t r) { return w.ownPlan ? (uint64_t)sBefore[r] : plan[r]; };
+    const uint64_t total = before(p.R) * p.Nkv, workers = (uint64_t)gridDim.x * 4;
+    // steps of KM groups, so that a wave's stretch begins where a step of the whole does
+    const uint64_t share = ((total + workers - 1) / workers + KM - 1) / KM * KM;
+    uint64_t x = ((uint64_t)blockIdx.x * 4 + wave) * share;
+    const uint64_t end = min(x + share, total);
+    if (x >= end) return;
+    uint32_t r;
+    {
+        uint32_t a = 0, b = p.R;  // the last request that begins at or before x
+        while (b - a > 1) {
+            const uint32_t mid = (a + b) / 2;
+            if (before(mid) * p.Nkv <= x) a = mid;
+            else b = mid;
+        }
+        r = first_lane(a);
+    }
+    while (x < end) {
+        const uint64_t from = before(r) * p.Nkv;
+        const uint32_t groups = first_lane((uint32_t)(before(r + 1) - before(r)));
+        if (groups == 0) {
+            ++r;
+            continue;
+        }
+        const uint32_t in = (uint32_t)(x - from), hkv = first_lane(in / groups), g0 = first_lane(in - hkv * groups);
+        const uint32_t g1 = (uint32_t)min((uint64_t)groups, g0 + (end - x));
+        const pk::PagedRequest q = weights_request(starts, keyLens, r, p, w);
+        const int32_t *table = tables + (uint64_t)r * p.columns;
+        const uint32_t keys = (uint32_t)q.keys, rows = (uint32_t)q.n * G;
+        float *to = weights + ((uint64_t)r * p.Nkv + hkv) * room;
+        for (uint32_t r0 = 0; r0 < rows; r0 += 16) {
+            // this lane's row; those past the last give nothing
+            const uint32_t row = min(r0 + c16, rows - 1);
+            const uint64_t at = ((uint64_t)(uint32_t)q.start + row / G) * p.Nq + hkv * G + row % G;
+            const int pos = q.pos0 + (int)(row / G);
+            const float of = lse[at] * kLog2e;
+            const bool counts = r0 + c16 < rows && of != -INFINITY;
+            u32x4 qf[KS];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint32_t d = (s * 4 + g) * E;
+                qf[s] = d < D ? *reinterpret_cast<const u32x4 *>(Q + at * D + d) : u32x4{0u, 0u, 0u, 0u};
+            }
+            u32x4 kf[KM][KS];
+            float old[KM];
+            bool ok[KM];
+            auto load = [&](uint32_t grp) {
+#pragma unroll
+                for (int m = 0; m < KM; ++m) {
+                    const uint32_t key = (grp + m) * 16, column = key / p.pageSize;
+                    const bool in = grp + m < g1;
+                    const uint32_t page = in ? (uint32_t)table[column] : ~0u;
+                    ok[m] = page < p.pages;
+                    const uint64_t off = ok[m] ? (((uint64_t)page * p.Nkv + hkv) * p.pageSize + (key - column * p.pageSize)) * D : 0;
+                    const int bytes = ok[m] ? (int)(min(16u, keys - key) * D * (uint32_t)sizeof(S)) : 0;
+                    const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(K + off), 0, bytes, 0x00020000);
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        const uint32_t d = (s * 4 + g) * E;
+                        kf[m][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                                                 rs, d < D ? (int)((c16 * D + d) * sizeof(S)) : kOutOfRange, 0, 0));
+                    }
+                    old[m] = 0.0f;
+                    if (in && c16 < 4 && key + 4 * g + c16 < keys) old[m] = to[key + 4 * g + c16];
+                }
+            };
+            load(g0);
+            for (uint32_t grp = g0; grp < g1; grp += KM) {
+                pk::f32x4 st[KM];
+                float was[KM];
+                bool held[KM];
+#pragma unroll
+                for (int m = 0; m < KM; ++m) {
+                    st[m] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) {
+                        if constexpr (kWide) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                st[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[m][s][e]), __uint_as_float(qf[s][e]), st[m], 0, 0, 0);
+                        } else {
+                            st[m] = pk::Mma16<T>::run(kf[m][s], qf[s], st[m]);
+                        }
+                    }
+                    was[m] = old[m];
+                    held[m] = ok[m];
+                }
+                if (grp + KM < g1) load(grp + KM);
+#pragma unroll
+                for (int m = 0; m < KM; ++m) {
+                    const uint32_t key0 = (grp + m) * 16 + 4 * g;
+                    float mine = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const bool seen = counts & (p.maskKind == 2u || (int)(key0 + j) <= pos);
+                        const float sum = pk::row16_sum(seen ? __builtin_amdgcn_exp2f(fmaf(st[m][j], c2, -of)) : 0.0f);
+                        if (c16 == (uint32_t)j) mine = sum;
+                    }
+                    if (held[m] && grp + m < g1 && c16 < 4 && key0 + c16 < keys) to[key0 + c16] = was[m] + mine;
+                }
+            }
+        }
+        x += g1 - g0;
+        if (x >= from + (uint64_t)groups * p.Nkv) ++r;
+    }
+}
+
+// Any head dim and alignment: 16 lanes take a key at a time, for every row in turn.
+template <typename T>
+__device__ void weights_plain(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
+                              const int32_t *__restrict__ tables, const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                              const float *__restrict__ lse, float *__restrict__ weights, const PagedAttentionConstants &p,
+                              const AttentionWeightsConstants &w) {
+    const uint32_t r = blockIdx.x / p.Nkv, hkv = blockIdx.x % p.Nkv, G = p.Nq / p.Nkv, t = threadIdx.x % 16;
+    const float c2 = p.scale * kLog2e;
+    const pk::PagedRequest q = weights_request(starts, keyLens, r, p, w);
+    const uint32_t rows = (uint32_t)q.n * G;
+    if (rows == 0) return;
+    float *to = weights + ((uint64_t)r * p.Nkv + hkv) * ((uint64_t)p.columns * p.pageSize);
+    for (uint64_t k = blockIdx.y * 16 + threadIdx.x / 16; k < (uint32_t)q.keys; k += (uint64_t)gridDim.y * 16) {
+        const uint32_t key = (uint32_t)k, page = (uint32_t)tables[(uint64_t)r * p.columns + key / p.pageSize];
+        if (page >= p.pages) continue;
+        const typename T::storage *kr = K + (((uint64_t)page * p.Nkv + hkv) * p.pageSize + key % p.pageSize) * p.Hd;
+        float sum = 0.0f;
+        for (uint32_t row = 0; row < rows; ++row) {
+            if (p.maskKind != 2u && (int)key > q.pos0 + (int)(row / G)) continue;
+            const uint64_t at = ((uint64_t)(uint32_t)q.start + row / G) * p.Nq + hkv * G + row % G;
+            const float of = lse[at] * kLog2e;
+            if (of == -INFINITY) continue;
+            float s = 0.0f;
+            for (uint32_t d = t; d < p.Hd; d += 16) s = fmaf(T::load(Q[at * p.Hd + d]), T::load(kr[d]), s);
+            sum += __builtin_amdgcn_exp2f(fmaf(pk::row16_sum(s), c2, -of));
+        }
+        if (t == 0) to[key] += sum;
+    }
+}
+
+}  // namespace
+
+#define WEIGHTS_FEW(t, T, HD, KM, PER_CU)                                                                                     \
+    POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                        \
+        attention_weights_few_##t##_d##HD(const T::storage *q, const T::storage *k, const int32_t *tables, const int32_t *starts, \
+                                          const int32_t *keyLens, const float *lse, const uint64_t *plan, float *weights,     \
+                                          PagedAttentionConstants p, AttentionWeightsConstants w) {                           \
+        weights_few<T, HD, KM>(q, k, tables, starts, keyLens, lse, plan, weights, p, w);                                      \
+    }
+#define WEIGHTS_PLAIN(t, T)                                                                                                   \
+    POPCORN_KERNEL void __launch_bounds__(256)                                                                                \
+        attention_weights_plain_##t(const T::storage *q, const T::storage *k, const int32_t *tables, const int32_t *starts,   \
+                                    const int32_t *keyLens, const float *lse, float *weights, PagedAttentionConstants p,      \
+                                    AttentionWeightsConstants w) {                                                            \
+        weights_plain<T>(q, k, tables, starts, keyLens, lse, weights, p, w);                                                  \
+    }
+
+using pk::BF16;
+using pk::F16;
+using pk::F32;
+
+#define WEIGHTS_16(t, T)          \
+    WEIGHTS_FEW(t, T, 64, 4, 4)   \
+    WEIGHTS_FEW(t, T, 128, 4, 3)  \
+    WEIGHTS_FEW(t, T, 256, 2, 2)  \
+    WEIGHTS_FEW(t, T, 512, 1, 2)  \
+    WEIGHTS_PLAIN(t, T)
+WEIGHTS_16(f16, F16)
+WEIGHTS_16(bf16, BF16)
+WEIGHTS_FEW(f32, F32, 64, 4, 3)
+WEIGHTS_FEW(f32, F32, 128, 2, 2)
+WEIGHTS_FEW(f32, F32, 256, 1, 2)
+WEIGHTS_FEW(f32, F32, 512, 1, 1)
+WEIGHTS_PLAIN(f32, F32)

@@ -1,0 +1,204 @@
+// Eviction from a paged cache by weight, and the pages that it leaves empty.
+//   n = min(keys, budget), first' = min(first, n), last' = min(last, n - first'): a KV head of a request keeps its first' first
+//   and last' last keys and, of those between, the n - first' - last' of the highest weight (ties: the lowest index; NaN is
+//   the lowest weight). evict_select says which, in index order, and evict_move brings their rows to the front.
+#include "paged.hpp"
+#include "scan.hpp"
+
+namespace {
+
+// Whole numbers in the order of the weights: NaN 0, then from -infinity on, both zeros alike.
+__device__ inline uint32_t rank_key(float x) {
+    if (x != x) return 0u;
+    const uint32_t b = __float_as_uint(x + 0.0f);  // (-0 + 0 is 0)
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+
+constexpr uint32_t kBins = 2048;
+constexpr uint32_t kTile = 4096;  // weights of a block's pass, four in a row to a thread
+
+}  // namespace
+
+// A block per (request, KV head). The least kept weight by three counts of its bits (11, 11 and 10), then one pass in
+// order that numbers what is kept.
+POPCORN_KERNEL void __launch_bounds__(1024)
+    evict_select(const float *weights, const int32_t *keyLens, const int32_t *budgets, int32_t *kept, float *keptWeights, EvictConstants e) {
+    __shared__ uint32_t bins[kBins], sums[16], found[2];
+    const uint32_t tid = threadIdx.x, r = blockIdx.x / e.Nkv;
+    const uint64_t room = (uint64_t)e.columns * e.pageSize;
+    const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
+    const float *w = weights + blockIdx.x * room;
+    int32_t *to = kept + blockIdx.x * room;
+    float *toW = keptWeights + blockIdx.x * room;
+    for (uint64_t i = k.n + tid; i < room; i += 1024) toW[i] = 0.0f;
+    if (k.n == k.keys) {
+        for (uint32_t i = tid; i < k.n; i += 1024) {
+            to[i] = (int32_t)i;
+            toW[i] = w[i];
+        }
+        return;
+    }
+    const uint32_t lo = k.first, hi = k.keys - k.last;  // between them `need` are kept
+    uint32_t need = k.n - k.first - k.last, least = 0, shift = 32;
+    for (int pass = 0; pass < 3 && need > 0; ++pass) {
+        const uint32_t bits = pass < 2 ? 11u : 10u, above = shift;
+        shift -= bits;
+        for (uint32_t b = tid; b < kBins; b += 1024) bins[b] = 0;
+        __syncthreads();
+        for (uint32_t i = lo + tid; i < hi; i += 1024) {
+            const uint32_t x = rank_key(w[i]);
+            if (above == 32 || x >> above == least >> above) atomicAdd(&bins[x >> shift & ((1u << bits) - 1)], 1u);
+        }
+        __syncthreads();
+        // from the highest bin down: the bin where the need is met
+        const uint32_t a = bins[kBins - 1 - 2 * tid], b = bins[kBins - 2 - 2 * tid];
+        const pk::Scan<uint32_t> s = pk::block_scan<16>(a + b, sums);
+        const uint32_t beforeA = s.upto - a - b, beforeB = beforeA + a;
+        if (beforeA < need && need <= beforeB) {
+            found[0] = kBins - 1 - 2 * tid;
+            found[1] = need - beforeA;
+        }
+        if (beforeB < need && need <= s.upto) {
+            found[0] = kBins - 2 - 2 * tid;
+            found[1] = need - beforeB;
+        }
+        __syncthreads();
+        least |= found[0] << shift;
+        need = found[1];
+        __syncthreads();
+    }
+    // `need` of those at `least` are kept, the lowest indices; where none between is, nothing is above
+    const bool none = k.n == k.first + k.last;
+    uint32_t sure = 0, ties = 0;  // before this pass's tile
+    for (uint32_t base = 0; base < k.keys; base += kTile) {
+        uint32_t count = 0;
+        bool is[4], tie[4];
+        float v[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t i = base + tid * 4 + j;
+            v[j] = i < k.keys ? w[i] : 0.0f;
+            const uint32_t x = rank_key(v[j]);
+            const bool between = i >= lo && i < hi;
+            is[j] = i < k.keys && (!between || (!none && x > least));
+            tie[j] = i < k.keys && between && !none && x == least;
+            count += (uint32_t)is[j] | (uint32_t)tie[j] << 16;
+        }
+        const pk::Scan<uint32_t> s = pk::block_scan<16>(count, sums);
+        uint32_t a = sure + ((s.upto - count) & 0xffffu), b = ties + ((s.upto - count) >> 16);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            if (is[j] || (tie[j] && b < need)) {
+                const uint32_t at = a + min(b, need);
+                to[at] = (int32_t)(base + tid * 4 + j);
+                toW[at] = v[j];
+            }
+            a += is[j];
+            b += tie[j];
+        }
+        sure += s.total & 0xffffu;
+        ties += s.total >> 16;
+    }
+}
+
+namespace {
+
+// A block takes 8 units of U (its slice) of the rows of one (request, KV head) in K or V. Row j becomes row kept[j] >= j, in chunks from
+// the front: a chunk's rows are all read before one of them is written, and what later chunks read lies behind what it
+// writes (kept rises, so kept[j] >= j for them too).
+template <typename U>
+__device__ void evict_move(const int32_t *__restrict__ kept, const int32_t *__restrict__ tables, const int32_t *__restrict__ keyLens,
+                           const int32_t *__restrict__ budgets, U *kCache, U *vCache, const EvictConstants &e) {
+    constexpr uint32_t kUnits = 8, kRows = 1024 / kUnits, kDeep = 8, kChunk = kRows * kDeep;
+    const uint32_t of = blockIdx.x, r = of / e.Nkv, hkv = of % e.Nkv;
+    const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
+    if (k.n == k.keys) return;
+    const uint64_t room = (uint64_t)e.columns * e.pageSize;
+    const int32_t *from = kept + of * room, *table = tables + (uint64_t)r * e.columns;
+    U *cache = blockIdx.z ? vCache : kCache;
+    const uint32_t unit = blockIdx.y * kUnits + threadIdx.x % kUnits, row = threadIdx.x / kUnits;
+    const bool mine = unit < e.rowUnits;
+    auto place = [&](uint32_t i, uint64_t &at) {
+        const uint32_t column = i / e.pageSize, page = (uint32_t)table[column];
+        at = (((uint64_t)page * e.Nkv + hkv) * e.pageSize + (i - column * e.pageSize)) * e.rowUnits + unit;
+        return page < e.pages;
+    };
+    for (uint32_t base = k.first; base < k.n; base += kChunk) {
+        U v[kDeep];
+        uint64_t dst[kDeep];
+        bool moves[kDeep];
+#pragma unroll
+        for (uint32_t d = 0; d < kDeep; ++d) {
+            const uint32_t j = base + d * kRows + row;
+            moves[d] = false;
+            if (j < k.n && mine) {
+                // (what is kept lies at or behind its place; a list that another call has left leads nowhere else)
+                const uint32_t i = min((uint32_t)from[j], k.keys - 1);
+                uint64_t src;
+                moves[d] = i > j && place(i, src) && place(j, dst[d]);
+                if (moves[d]) v[d] = cache[src];
+            }
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the rows have been read
+        __syncthreads();
+#pragma unroll
+        for (uint32_t d = 0; d < kDeep; ++d)
+            if (moves[d]) cache[dst[d]] = v[d];
+    }
+}
+
+}  // namespace
+
+#define EVICT_MOVE(name, U)                                                                                                   \
+    POPCORN_KERNEL void __launch_bounds__(1024) name(const int32_t *kept, const int32_t *tables, const int32_t *keyLens,      \
+                                                     const int32_t *budgets, U *kCache, U *vCache, EvictConstants e) {        \
+        evict_move<U>(kept, tables, keyLens, budgets, kCache, vCache, e);                                                     \
+    }
+EVICT_MOVE(evict_move_b128, pk::u32x4)
+EVICT_MOVE(evict_move_b64, pk::u32x2)
+EVICT_MOVE(evict_move_b32, uint32_t)
+EVICT_MOVE(evict_move_b16, uint16_t)
+
+// The lengths after an eviction, and the pages from ceil(n / pageSize) on of each request that it left empty, in request order.
+// Every block sums what the requests before its own free.
+POPCORN_KERNEL void __launch_bounds__(256)
+    release_pages(const int32_t *keyLens, const int32_t *budgets, const int32_t *tables, int32_t *newLens, int32_t *freed, int32_t *counts,
+                  EvictConstants e) {
+    __shared__ uint32_t sums[4], sBefore[256], sFrom[256], sCount[256];
+    const uint32_t tid = threadIdx.x;
+    const uint32_t lo = (uint32_t)((uint64_t)e.R * blockIdx.x / gridDim.x), hi = (uint32_t)((uint64_t)e.R * (blockIdx.x + 1) / gridDim.x);
+    auto pages = [&](uint32_t keys) { return keys / e.pageSize + (keys % e.pageSize != 0); };
+    uint32_t run = 0;
+    auto wave_total = [&](uint32_t v) {
+        const pk::Scan<uint32_t> s = pk::block_scan<4>(v, sums);
+        return s;
+    };
+    {
+        uint32_t mine = 0;
+        for (uint32_t r = tid; r < lo; r += 256) {
+            const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
+            mine += pages(k.keys) - pages(k.n);
+        }
+        run = wave_total(mine).total;
+    }
+    for (uint32_t base = lo; base < hi; base += 256) {
+        const uint32_t r = base + tid;
+        uint32_t count = 0, from = 0;
+        if (r < hi) {
+            const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
+            from = pages(k.n);
+            count = pages(k.keys) - from;
+            newLens[r] = (int32_t)k.n;
+        }
+        const pk::Scan<uint32_t> s = wave_total(count);
+        sBefore[tid] = run + s.upto - count;
+        sFrom[tid] = from;
+        sCount[tid] = count;
+        __syncthreads();
+        for (uint32_t i = tid / 64; i < min(256u, hi - base); i += 4)
+            for (uint32_t c = tid % 64; c < sCount[i]; c += 64) freed[sBefore[i] + c] = tables[(uint64_t)(base + i) * e.columns + sFrom[i] + c];
+        run += s.total;
+        __syncthreads();
+    }
+    if (blockIdx.x == gridDim.x - 1 && tid == 0) counts[0] = (int32_t)run;
+}

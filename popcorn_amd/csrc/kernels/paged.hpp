@@ -73,18 +73,22 @@ struct PagedSteps {
     uint32_t r0, r1, sinks, first, n;
 };
 
-PAGED_FN PagedSteps paged_steps(const PagedRequest &r, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
-    const uint32_t G = p.Nq / p.Nkv, rows = (uint32_t)r.n * G;
-    PagedSteps s;
-    s.r0 = tile * w.rows;
-    s.r1 = rows - s.r0 < w.rows ? rows : s.r0 + w.rows;
-    const PagedSpan k = paged_span(r.pos0 + (int32_t)(s.r0 / G), r.pos0 + (int32_t)((s.r1 - 1) / G), r.keys, p);
+// The steps of the keys `k`.
+PAGED_FN void paged_cut(PagedSteps &s, const PagedSpan &k, const PagedWorkConstants &w) {
     const uint32_t step = w.stepKeys;
     s.sinks = ((uint32_t)k.sinkEnd + step - 1) / step;
     s.first = (uint32_t)k.lo / step > s.sinks ? (uint32_t)k.lo / step : s.sinks;
     const uint32_t end = k.hi > k.lo ? ((uint32_t)k.hi + step - 1) / step : 0u;
     s.n = s.sinks + (end > s.first ? end - s.first : 0u);
     if (s.n == 0) s.n = 1;
+}
+
+PAGED_FN PagedSteps paged_steps(const PagedRequest &r, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    const uint32_t G = p.Nq / p.Nkv, rows = (uint32_t)r.n * G;
+    PagedSteps s;
+    s.r0 = tile * w.rows;
+    s.r1 = rows - s.r0 < w.rows ? rows : s.r0 + w.rows;
+    paged_cut(s, paged_span(r.pos0 + (int32_t)(s.r0 / G), r.pos0 + (int32_t)((s.r1 - 1) / G), r.keys, p), w);
     return s;
 }
 
@@ -129,6 +133,98 @@ PAGED_FN PagedPiece paged_piece(uint64_t in, uint64_t left, uint32_t n, const Pa
 // ends at `end`); else 0.
 PAGED_FN uint32_t paged_sharers(const PagedPiece &c, uint32_t n, uint64_t end, uint64_t share, uint32_t worker) {
     return c.lo == 0 && c.hi > 0 && c.hi < n ? paged_worker(end + c.behind - 1, share) - worker + 1 : 0u;
+}
+
+// ---- prefixes that requests share ------------------------------------------------------------
+
+// The i with at[i] <= x < at[i + 1], of n + 1 ascending entries; n where there is none.
+PAGED_FN uint32_t paged_span_of(const int32_t *at, uint32_t n, int32_t x) {
+    if (n == 0) return n;
+    uint32_t a = 0, b = n;
+    while (b - a > 1) {
+        const uint32_t mid = (a + b) / 2;
+        if (at[mid] <= x) a = mid;
+        else b = mid;
+    }
+    return at[a] <= x && x < at[a + 1] ? a : n;
+}
+
+PAGED_FN int32_t paged_prefix_keys(int32_t len, const PagedAttentionConstants &p, const SharedPrefixConstants &s) {
+    const int32_t keys = paged_max(len, 0);
+    const uint64_t room = (uint64_t)s.columns * p.pageSize;
+    return (uint64_t)keys < room ? keys : (int32_t)room;
+}
+
+// A unit's rows and keys in a call with prefixes.
+struct SharedRequest : PagedRequest {
+    bool prefix;     // a group's rows against its prefix
+    int32_t before;  // else: keys of the prefix before the request's own
+    int32_t lo;      // of a prefix: no row of it has a lower position
+};
+
+// Group v < groups: the rows of its requests, who follow each other, against its prefix; then the requests. positions: under a
+// window, each token's and then each group's least.
+PAGED_FN SharedRequest paged_shared(uint32_t v, const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
+                                    const int32_t *positions, const PagedAttentionConstants &p, const SharedPrefixConstants &s) {
+    SharedRequest q;
+    q.prefix = v < s.groups;
+    q.before = q.lo = 0;
+    if (q.prefix) {
+        const int32_t a = paged_min(paged_max(groupStarts[v], 0), (int32_t)p.R), b = paged_min(paged_max(groupStarts[v + 1], a), (int32_t)p.R);
+        static_cast<PagedRequest &>(q) = paged_request(starts[a], starts[b], 0, p);
+        q.keys = paged_prefix_keys(prefixLens[v], p, s);
+        if (a == b || q.keys == 0) q.n = 0;
+        q.lo = s.windowed ? positions[p.T + v] : q.keys;
+    } else {
+        const uint32_t r = v - s.groups, g = paged_span_of(groupStarts, s.groups, (int32_t)r);
+        static_cast<PagedRequest &>(q) = paged_request(starts[r], starts[r + 1], keyLens[r], p);
+        if (g < s.groups) q.before = paged_prefix_keys(prefixLens[g], p, s);
+    }
+    return q;
+}
+
+// The constants by which its rows see its keys: a prefix lies before every row; own keys and positions are counted from the
+// prefix's end, and so are the sinks.
+PAGED_FN PagedAttentionConstants paged_shared_mask(const SharedRequest &q, const PagedAttentionConstants &p) {
+    PagedAttentionConstants m = p;
+    if (q.prefix) m.maskKind = p.maskKind == 1u ? 1u : 2u;
+    else m.sinks = p.sinks > (uint32_t)q.before ? p.sinks - (uint32_t)q.before : 0u;
+    return m;
+}
+
+PAGED_FN PagedSteps paged_shared_steps(const SharedRequest &q, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
+    const PagedAttentionConstants m = paged_shared_mask(q, p);
+    if (!q.prefix) return paged_steps(q, tile, m, w);
+    const uint32_t rows = (uint32_t)q.n * (p.Nq / p.Nkv);
+    PagedSteps s;
+    s.r0 = tile * w.rows;
+    s.r1 = rows - s.r0 < w.rows ? rows : s.r0 + w.rows;
+    paged_cut(s, paged_span(q.lo, 0x7fffffff, q.keys, m), w);
+    return s;
+}
+
+// Position of token t of a request (its own keys counted from the prefix's end) in the whole sequence.
+PAGED_FN int32_t paged_place(const PagedRequest &r, int32_t t, int32_t prefix) {
+    const int64_t at = (int64_t)paged_max(r.pos0 + (t - r.start), 0) + prefix;
+    return at < 0x7fffffff ? (int32_t)at : 0x7fffffff;
+}
+
+// ---- eviction -------------------------------------------------------------------------------
+
+// Of a request's keys n stay, the `first` first and the `last` last of them in any case.
+struct EvictKeep {
+    uint32_t keys, n, first, last;
+};
+
+PAGED_FN EvictKeep evict_keep(int32_t keyLen, int32_t budget, const EvictConstants &e) {
+    EvictKeep k;
+    const uint64_t room = (uint64_t)e.columns * e.pageSize;
+    const uint32_t len = (uint32_t)paged_max(keyLen, 0), most = (uint32_t)paged_max(budget, 0);
+    k.keys = len < room ? len : (uint32_t)room;
+    k.n = k.keys < most ? k.keys : most;
+    k.first = e.first < k.n ? e.first : k.n;
+    k.last = e.last < k.n - k.first ? e.last : k.n - k.first;
+    return k;
 }
 
 }  // namespace pk

@@ -848,6 +848,58 @@ popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const
     });
 }
 
+popcorn_status_t popcorn_kernel_shared_prefix_attention(
+    const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache, const popcorn_tensor_t *v_cache, const popcorn_tensor_t *prefix_tables,
+    const popcorn_tensor_t *prefix_lens, const popcorn_tensor_t *group_starts, const popcorn_tensor_t *page_tables,
+    const popcorn_tensor_t *query_starts, const popcorn_tensor_t *key_lens, const popcorn_tensor_t *out, const popcorn_tensor_t *lse,
+    float scale, popcorn_attention_mask_t mask, int64_t sinks, int64_t max_query_len, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        Tensor opt[4];
+        const popcorn_tensor_t *in[4] = {prefix_tables, prefix_lens, group_starts, lse};
+        for (int i = 0; i < 4; ++i)
+            if (in[i]) opt[i] = Tensor::fromC(*in[i]);
+        emit(kernel, Kernels::SharedPrefixAttention(T(q, "q"), T(k_cache, "k_cache"), T(v_cache, "v_cache"), in[0] ? &opt[0] : nullptr,
+                                                    in[1] ? &opt[1] : nullptr, in[2] ? &opt[2] : nullptr, T(page_tables, "page_tables"),
+                                                    T(query_starts, "query_starts"), T(key_lens, "key_lens"), T(out, "out"),
+                                                    in[3] ? &opt[3] : nullptr, scale, AttentionMask{mask.kind, mask.window}, sinks,
+                                                    max_query_len));
+    });
+}
+
+popcorn_status_t popcorn_kernel_paged_attention_weights(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
+                                                        const popcorn_tensor_t *page_tables, const popcorn_tensor_t *query_starts,
+                                                        const popcorn_tensor_t *key_lens, const popcorn_tensor_t *lse,
+                                                        const popcorn_tensor_t *weights, float scale, popcorn_attention_mask_t mask,
+                                                        int64_t last_rows, int64_t max_query_len, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::PagedAttentionWeights(T(q, "q"), T(k_cache, "k_cache"), T(page_tables, "page_tables"),
+                                                    T(query_starts, "query_starts"), T(key_lens, "key_lens"), T(lse, "lse"),
+                                                    T(weights, "weights"), scale, AttentionMask{mask.kind, mask.window}, last_rows,
+                                                    max_query_len));
+    });
+}
+
+popcorn_status_t popcorn_kernel_paged_eviction(const popcorn_tensor_t *weights, const popcorn_tensor_t *k_cache,
+                                               const popcorn_tensor_t *v_cache, const popcorn_tensor_t *page_tables,
+                                               const popcorn_tensor_t *key_lens, const popcorn_tensor_t *budgets,
+                                               const popcorn_tensor_t *kept, const popcorn_tensor_t *kept_weights, int64_t first,
+                                               int64_t last, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::PagedEviction(T(weights, "weights"), T(k_cache, "k_cache"), T(v_cache, "v_cache"), T(page_tables, "page_tables"),
+                                            T(key_lens, "key_lens"), T(budgets, "budgets"), T(kept, "kept"), T(kept_weights, "kept_weights"),
+                                            first, last));
+    });
+}
+
+popcorn_status_t popcorn_kernel_release_pages(const popcorn_tensor_t *key_lens, const popcorn_tensor_t *budgets,
+                                              const popcorn_tensor_t *page_tables, int64_t page_size, const popcorn_tensor_t *new_lens,
+                                              const popcorn_tensor_t *freed, const popcorn_tensor_t *counts, popcorn_kernel_t *kernel) {
+    return guarded([&] {
+        emit(kernel, Kernels::ReleasePages(T(key_lens, "key_lens"), T(budgets, "budgets"), T(page_tables, "page_tables"), page_size,
+                                           T(new_lens, "new_lens"), T(freed, "freed"), T(counts, "counts")));
+    });
+}
+
 popcorn_status_t popcorn_kernel_sample(const popcorn_tensor_t *logits, const popcorn_tensor_t *uniforms,
                                        const popcorn_tensor_t *temperature, const popcorn_tensor_t *top_k,
                                        const popcorn_tensor_t *top_p, const popcorn_tensor_t *min_p,

@@ -467,6 +467,18 @@ std::unique_ptr<Kernel> PagedKVCacheWrite(const Tensor &k, const Tensor &v, cons
 std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
                                        const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, float scale,
                                        AttentionMask mask, int64_t sinks, int64_t maxQueryLen);
+std::unique_ptr<Kernel> SharedPrefixAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor *prefixTables,
+                                              const Tensor *prefixLens, const Tensor *groupStarts, const Tensor &pageTables,
+                                              const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, const Tensor *lse,
+                                              float scale, AttentionMask mask, int64_t sinks, int64_t maxQueryLen);
+std::unique_ptr<Kernel> PagedAttentionWeights(const Tensor &q, const Tensor &kCache, const Tensor &pageTables, const Tensor &queryStarts,
+                                              const Tensor &keyLens, const Tensor &lse, const Tensor &weights, float scale,
+                                              AttentionMask mask, int64_t lastRows, int64_t maxQueryLen);
+std::unique_ptr<Kernel> PagedEviction(const Tensor &weights, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
+                                      const Tensor &keyLens, const Tensor &budgets, const Tensor &kept, const Tensor &keptWeights,
+                                      int64_t first, int64_t last);
+std::unique_ptr<Kernel> ReleasePages(const Tensor &keyLens, const Tensor &budgets, const Tensor &pageTables, int64_t pageSize,
+                                     const Tensor &newLens, const Tensor &freed, const Tensor &counts);
 std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK,
                                const Tensor *topP, const Tensor *minP, const Tensor &tokens);
 

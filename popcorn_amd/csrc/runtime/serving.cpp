@@ -1,5 +1,6 @@
 // Kernels.* descriptors of a batch of requests over a paged cache: page tables,
-// the paged cache write, paged attention, and the draw of the next token.
+// the paged cache write, paged attention, with prefixes that requests share, the
+// weights that it gives the keys, eviction by them, and the draw of the next token.
 // No counterparts in the reference; validation and errors are as for its own
 // operations (kernels.cpp).
 #include <algorithm>
@@ -67,6 +68,61 @@ void requireCaches(const Tensor &k, const Tensor &v, const std::string &op) {
     if (k.shape[2] <= 0) throw Error::tensorShapeMismatch(op + " page size must be positive; got " + k.shape.str() + ".");
     if (k.shape[0] * k.shape[2] >= (int64_t{1} << 31))
         throw Error::tensorShapeMismatch(op + " cache must hold fewer than 2^31 slots; got " + k.shape.str() + ".");
+}
+
+// The sizes of a paged attention call, checked.
+PagedAttentionConstants pagedConstants(const std::string &op, const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
+                                       const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, float scale, AttentionMask mask,
+                                       int64_t sinks, int64_t maxQueryLen) {
+    using D = DataType;
+    const D t = q.dataType;
+    if (!isFloat(t) || kCache.dataType != t || vCache.dataType != t || out.dataType != t)
+        throw Error::unsupportedDataTypeCombination(op + std::string(" needs one floating dtype for q, the caches and out; got ") +
+                                                    name(t) + ", " + name(kCache.dataType) + ", " + name(vCache.dataType) + ", " +
+                                                    name(out.dataType) + ".");
+    if (mask.kind > 2) throw Error::invalidArgument("unknown attention mask kind");
+    if (sinks < 0 || sinks >= (int64_t{1} << 31)) throw Error::invalidArgument(op + " sinks must be at least 0 and below 2^31.");
+    if (sinks > 0 && mask.kind != 1) throw Error::invalidArgument(op + " sinks go with a sliding window.");
+    if (maxQueryLen < 0) throw Error::invalidArgument(op + " max_query_len must not be negative.");
+    requireCaches(kCache, vCache, op);
+    requireRank(q, 3);
+    requireRank(pageTables, 2);
+    const int64_t T = q.shape[0], Nq = q.shape[1], Hd = q.shape[2], Nkv = kCache.shape[1], page = kCache.shape[2];
+    const int64_t R = pageTables.shape[0], M = pageTables.shape[1];
+    if (Nkv <= 0 || Nq <= 0 || Nq % Nkv != 0)
+        throw Error::tensorShapeMismatch(op + " query heads must be divisible by KV heads; got " + std::to_string(Nq) + " and " +
+                                         std::to_string(Nkv) + ".");
+    if (Hd <= 0 || Hd > 512)
+        throw Error::tensorShapeMismatch(op + " head dim must be 1 to 512 (kernel limit); got " + std::to_string(Hd) + ".");
+    if (kCache.shape[3] != Hd)
+        throw Error::tensorShapeMismatch(op + " caches must have q's head dim; got " + q.shape.str() + " and " + kCache.shape.str() + ".");
+    if (page % 16 != 0)
+        throw Error::tensorShapeMismatch(op + " page size must be a multiple of 16; got " + std::to_string(page) + ".");
+    requireShape(q, t, {T, Nq, Hd}, op + " q");
+    requireShape(out, t, {T, Nq, Hd}, op + " out");
+    requireShape(pageTables, D::i32, {R, M}, op + " page_tables");
+    requireShape(queryStarts, D::i32, {R + 1}, op + " query_starts");
+    requireShape(keyLens, D::i32, {R}, op + " key_lens");
+    requireGrid(T * Nq, 256, op, q);
+    return PagedAttentionConstants{(uint32_t)T, (uint32_t)R, (uint32_t)Nq, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page,
+                                   (uint32_t)kCache.shape[0], (uint32_t)M, mask.kind, mask.window, (uint32_t)sinks, scale};
+}
+
+// 16-byte rows: the matrix cores
+bool fastRows(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &out) {
+    return q.shape[2] % (16 / stride(q.dataType)) == 0 && aligned(q.data, 16) && aligned(k.data, 16) && aligned(v.data, 16) && aligned(out.data, 16);
+}
+std::string plainName(const Tensor &q, const Tensor &k, const Tensor &v) {
+    const int run = 4 * stride(q.dataType);
+    return name(q.dataType) + std::string(q.shape[2] % 4 || !aligned(k.data, run) || !aligned(v.data, run) ? "_any" : "");
+}
+
+// Keys that a table's row has room for, counted in 32 bits by the kernels.
+int64_t requireRoom(const std::string &op, int64_t columns, int64_t pageSize) {
+    if (columns >= (int64_t{1} << 31) / pageSize)
+        throw Error::tensorShapeMismatch(op + " tables must hold fewer than 2^31 keys a request; got " + std::to_string(columns) + " pages of " +
+                                         std::to_string(pageSize) + ".");
+    return columns * pageSize;
 }
 
 std::unique_ptr<Kernel> fixed(const std::string &fn, std::vector<Binding> b, std::vector<uint8_t> c, dim3 grid, unsigned block) {
@@ -205,6 +261,202 @@ private:
     std::vector<Work> work_;
     std::string merge_;
     int64_t hdp_ = 0;
+};
+
+// SharedPrefixAttention (shared_prefix.hip): PagedAttention's two kernels over units of groups' rows against their prefixes and of
+// requests' rows against their pages, then a merge of each row's pieces.
+class SharedPrefixKernel : public Kernel {
+public:
+    SharedPrefixKernel(std::vector<Tensor> inputs, const Tensor &out, const Tensor *lse, const PagedAttentionConstants &pc,
+                       const SharedPrefixConstants &sc, int64_t maxQueryLen)
+        : in_(std::move(inputs)), out_(out), lse_(lse ? *lse : out), pc_(pc), sc_(sc) {
+        const Tensor &q = in_[0];
+        const int64_t G = pc.Nq / pc.Nkv, all = (int64_t)pc.T * G;
+        // a group's rows may be all there are
+        const int64_t longest = sc.groups ? all : std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T) * G;
+        const bool f32 = q.dataType == DataType::f32;
+        hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
+        const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
+        merge_ = "shared_prefix_merge_" + type + hd;
+        // the kernels and their limits as for PagedAttention
+        const int tilesPerCU = hdp_ == 256 ? 1 : 2;
+        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows && all > (hdp_ == 256 ? 64 : 128);
+        const bool apart = tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU * deviceCUs();
+        if (!tiles || apart) {
+            const int rt = hdp_ == 512 || (f32 && hdp_ == 256) || longest <= 16 || tiles ? 1 : 2;
+            const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
+            add("shared_prefix_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);
+        }
+        if (tiles) add("shared_prefix_tile_" + type + hd, 128, 64, apart ? kFewRows : 0, UINT32_MAX, tilesPerCU);
+        sc_.rows = pc.T * pc.Nq;
+        sc_.rowBase = work_.back().stateBase + 2 * work_.back().workers * work_.back().rows;
+        sc_.states = sc_.rowBase + 2 * sc_.rows;
+        for (const PagedWorkConstants &w : work_) sc_.most = std::max(sc_.most, w.workers);
+        sc_.parts = sc_.rows < 4096 ? 4 : 1;
+    }
+    std::vector<Binding> tensors() const override {
+        std::vector<Binding> b;
+        for (const Tensor &t : in_) b.push_back({t, kRead});
+        b.push_back({out_, kWrite});
+        if (sc_.hasLse) b.push_back({lse_, kWrite});
+        return b;
+    }
+    std::string describe() const override {
+        std::string s = sc_.windowed ? "shared_prefix_positions," : "";
+        for (size_t i = 0; i < work_.size(); ++i) s += (work_[i].ownPlan ? "" : "shared_prefix_plan,") + fn_[i] + ",";
+        return s + merge_;
+    }
+    void encode(KernelCommandEncoder &enc) const override {
+        // one buffer: the states' O, their m and l, the rows' records, the plans, the positions
+        int64_t tiles = 0;
+        for (const PagedWorkConstants &w : work_) tiles += w.ownPlan ? 0 : (int64_t)w.maxTiles + 1;
+        const int64_t o = (int64_t)sc_.states * hdp_ * 4, ml = cdiv((int64_t)sc_.states * 8, 16) * 16, rec = 2 * (int64_t)sc_.rows * 16;
+        const int64_t positions = sc_.windowed ? ((int64_t)pc_.T + sc_.groups) * 4 : 0;
+        enc.withTemporaryTensor(ScratchSpec{{o + ml + rec + tiles * 16 + positions}, DataType::u8}, [&](Tensor scratch) {
+            auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
+            const Tensor pO = part(0, o), pML = part(o, ml), records = part(o + ml, rec), pos = part(o + ml + rec + tiles * 16, positions);
+            const Tensor &starts = in_[4], &lens = in_[5], &prefixLens = in_[7], &groups = in_[8];
+            if (sc_.windowed)
+                launch(enc, "shared_prefix_positions", {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}, {pos, kWrite}},
+                       {bytesOf(pc_), bytesOf(sc_)}, dim3((unsigned)(cdiv(pc_.T, 256) + sc_.groups), 1, 1), 256);
+            int64_t plan = o + ml + rec;
+            for (size_t i = 0; i < work_.size(); ++i) {
+                const PagedWorkConstants &w = work_[i];
+                const std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_), bytesOf(w), bytesOf(sc_)};
+                const int64_t planBytes = w.ownPlan ? 0 : ((int64_t)w.maxTiles + 1) * 16;
+                const Tensor pl = part(plan, planBytes);
+                if (planBytes)
+                    launch(enc, "shared_prefix_plan",
+                           {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}, {pos, kRead}, {pl, kWrite}}, consts, dim3(1, 1, 1), 1024);
+                plan += planBytes;
+                std::vector<Binding> b;
+                for (const Tensor &t : in_) b.push_back({t, kRead});
+                for (const Binding &x : {Binding{pos, kRead}, {pl, kRead}, {pO, kWrite}, {pML, kWrite}, {records, kWrite}, {out_, kWrite}, {lse_, kWrite}})
+                    b.push_back(x);
+                launch(enc, fn_[i], std::move(b), consts, dim3(w.workers, 1, 1), 256);
+            }
+            launch(enc, merge_,
+                   {{pO, kRead}, {pML, kRead}, {records, kRead}, {starts, kRead}, {prefixLens, kRead}, {groups, kRead}, {out_, kWrite}, {lse_, kWrite}},
+                   {bytesOf(pc_), bytesOf(sc_)}, dim3((unsigned)cdiv(sc_.rows, 4 / sc_.parts), 1, 1), 256);
+        });
+    }
+
+private:
+    static constexpr uint32_t kFewRows = 32;
+
+    void add(const std::string &fn, uint32_t rows, uint32_t stepKeys, uint32_t few, uint32_t many, int perCU) {
+        const int64_t G = pc_.Nq / pc_.Nkv;
+        PagedWorkConstants w{};
+        w.rows = rows;
+        w.stepKeys = stepKeys;
+        w.fewRows = few;
+        w.manyRows = many;
+        const int64_t tiles = cdiv((int64_t)pc_.T * G, rows);
+        w.maxTiles = (uint32_t)(tiles + std::min(pc_.R, pc_.T) + (sc_.groups ? tiles + std::min(sc_.groups, pc_.T) : 0));
+        w.minSteps = 128 / stepKeys;
+        w.unitSteps = 384 / stepKeys;
+        w.stream = in_[1].byteCount() + in_[2].byteCount() > (size_t{256} << 20);
+        const double tileSteps = (double)cdiv((int64_t)std::max(pc_.columns, sc_.columns) * pc_.pageSize + stepKeys, stepKeys) + w.unitSteps;
+        const double steps = (double)w.maxTiles * tileSteps;
+        w.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc_.Nkv / w.minSteps + 1));
+        w.ownPlan = w.maxTiles <= 1024 && pc_.R + sc_.groups <= 1024 && steps < 2147483648.0;
+        w.stateBase = work_.empty() ? 0 : 2 * work_.back().workers * work_.back().rows;
+        work_.push_back(w);
+        fn_.push_back(fn);
+    }
+    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, std::vector<std::vector<uint8_t>> consts, dim3 grid,
+                unsigned block) const {
+        enc.encode(*Kernels::Custom(fn, std::move(b), std::move(consts), grid, dim3(block, 1, 1)));
+    }
+
+    std::vector<Tensor> in_;  // q, k, v, tables, starts, lens, prefix tables, prefix lens, group starts
+    Tensor out_, lse_;
+    PagedAttentionConstants pc_;
+    SharedPrefixConstants sc_;
+    std::vector<PagedWorkConstants> work_;
+    std::vector<std::string> fn_;
+    std::string merge_;
+    int64_t hdp_ = 0;
+};
+
+// PagedAttentionWeights (attention_weights.hip).
+class AttentionWeightsKernel : public Kernel {
+public:
+    AttentionWeightsKernel(std::vector<Tensor> inputs, const Tensor &weights, const PagedAttentionConstants &pc, int64_t lastRows)
+        : in_(std::move(inputs)), weights_(weights), pc_(pc) {
+        const Tensor &q = in_[0];
+        const int64_t groups = cdiv((int64_t)pc.columns * pc.pageSize, 16);
+        const std::string type = name(q.dataType);
+        const int hdp = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
+        fn_ = "attention_weights_few_" + type + "_d" + std::to_string(hdp);
+        wc_ = AttentionWeightsConstants{(uint32_t)std::min<int64_t>(lastRows, pc.T), 0, UINT32_MAX,
+                                        pc.R <= 1024 && (double)groups * pc.R < 4294967296.0};
+        const int perCU = q.dataType == DataType::f32 ? (hdp <= 64 ? 3 : hdp <= 256 ? 2 : 1) : (hdp <= 64 ? 4 : hdp <= 128 ? 3 : 2);
+        blocks_ = (unsigned)std::clamp<double>((double)groups * pc.R * pc.Nkv / 4, 1, (double)perCU * deviceCUs());
+    }
+    std::vector<Binding> tensors() const override {
+        std::vector<Binding> b;
+        for (const Tensor &t : in_) b.push_back({t, kRead});
+        b.push_back({weights_, kReadWrite});
+        return b;
+    }
+    std::string describe() const override { return (wc_.ownPlan ? "" : "attention_weights_plan,") + fn_; }
+    void encode(KernelCommandEncoder &enc) const override {
+        const std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_), bytesOf(wc_)};
+        auto run = [&](const Tensor &plan) {
+            std::vector<Binding> b;
+            for (const Tensor &t : in_) b.push_back({t, kRead});
+            b.push_back({plan, kRead});
+            b.push_back({weights_, kReadWrite});
+            enc.encode(*Kernels::Custom(fn_, std::move(b), consts, dim3(blocks_, 1, 1), dim3(256, 1, 1)));
+        };
+        if (wc_.ownPlan) return run(weights_);  // (not read)
+        enc.withTemporaryTensor(ScratchSpec{{((int64_t)pc_.R + 1) * 8}, DataType::u8}, [&](Tensor plan) {
+            enc.encode(*Kernels::Custom("attention_weights_plan", {{in_[3], kRead}, {in_[4], kRead}, {plan, kWrite}}, consts, dim3(1, 1, 1),
+                                        dim3(1024, 1, 1)));
+            run(plan);
+        });
+    }
+
+private:
+    std::vector<Tensor> in_;  // q, k, tables, starts, lens, lse
+    Tensor weights_;
+    PagedAttentionConstants pc_;
+    AttentionWeightsConstants wc_{};
+    std::string fn_;
+    unsigned blocks_ = 1;
+};
+
+// PagedEviction (evict.hip): the choice, then the moves of K and V.
+class EvictionKernel : public Kernel {
+public:
+    EvictionKernel(const Tensor &weights, const Tensor &k, const Tensor &v, const Tensor &tables, const Tensor &lens, const Tensor &budgets,
+                   const Tensor &kept, const Tensor &keptWeights, const EvictConstants &ec)
+        : weights_(weights), k_(k), v_(v), tables_(tables), lens_(lens), budgets_(budgets), kept_(kept), keptWeights_(keptWeights), ec_(ec) {
+        const int64_t row = k.shape[3] * stride(k.dataType);
+        int unit = 16;
+        while (row % unit || !aligned(k.data, unit) || !aligned(v.data, unit)) unit /= 2;
+        fn_ = "evict_move_b" + std::to_string(unit * 8);
+        ec_.rowUnits = (uint32_t)(row / unit);
+    }
+    std::vector<Binding> tensors() const override {
+        return {{weights_, kRead}, {k_, kReadWrite}, {v_, kReadWrite}, {tables_, kRead}, {lens_, kRead}, {budgets_, kRead}, {kept_, kWrite}, {keptWeights_, kWrite}};
+    }
+    std::string describe() const override { return "evict_select," + fn_; }
+    void encode(KernelCommandEncoder &enc) const override {
+        const unsigned rows = ec_.R * ec_.Nkv;
+        if (rows == 0) return;
+        enc.encode(*Kernels::Custom("evict_select", {{weights_, kRead}, {lens_, kRead}, {budgets_, kRead}, {kept_, kWrite}, {keptWeights_, kWrite}},
+                                    {bytesOf(ec_)}, dim3(rows, 1, 1), dim3(1024, 1, 1)));
+        if (ec_.rowUnits == 0) return;
+        enc.encode(*Kernels::Custom(fn_, {{kept_, kRead}, {tables_, kRead}, {lens_, kRead}, {budgets_, kRead}, {k_, kReadWrite}, {v_, kReadWrite}},
+                                    {bytesOf(ec_)}, dim3(rows, (ec_.rowUnits + 7) / 8, 2), dim3(1024, 1, 1)));
+    }
+
+private:
+    Tensor weights_, k_, v_, tables_, lens_, budgets_, kept_, keptWeights_;
+    EvictConstants ec_;
+    std::string fn_;
 };
 
 // Sample (sample.hip): a row of up to SAMPLE_CANDIDATES logits by one block,
@@ -349,49 +601,137 @@ std::unique_ptr<Kernel> PagedKVCacheWrite(const Tensor &k, const Tensor &v, cons
 std::unique_ptr<Kernel> PagedAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
                                        const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, float scale,
                                        AttentionMask mask, int64_t sinks, int64_t maxQueryLen) {
-    using D = DataType;
-    const D t = q.dataType;
-    if (!isFloat(t) || kCache.dataType != t || vCache.dataType != t || out.dataType != t)
-        throw Error::unsupportedDataTypeCombination(std::string("PagedAttention needs one floating dtype for q, the caches and out; got ") +
-                                                    name(t) + ", " + name(kCache.dataType) + ", " + name(vCache.dataType) + ", " +
-                                                    name(out.dataType) + ".");
-    if (mask.kind > 2) throw Error::invalidArgument("unknown attention mask kind");
-    if (sinks < 0 || sinks >= (int64_t{1} << 31)) throw Error::invalidArgument("PagedAttention sinks must be at least 0 and below 2^31.");
-    if (sinks > 0 && mask.kind != 1) throw Error::invalidArgument("PagedAttention sinks go with a sliding window.");
-    if (maxQueryLen < 0) throw Error::invalidArgument("PagedAttention max_query_len must not be negative.");
-    requireCaches(kCache, vCache, "PagedAttention");
-    requireRank(q, 3);
-    requireRank(pageTables, 2);
-    const int64_t T = q.shape[0], Nq = q.shape[1], Hd = q.shape[2], Nkv = kCache.shape[1], page = kCache.shape[2];
-    const int64_t R = pageTables.shape[0], M = pageTables.shape[1];
-    if (Nkv <= 0 || Nq <= 0 || Nq % Nkv != 0)
-        throw Error::tensorShapeMismatch("PagedAttention query heads must be divisible by KV heads; got " + std::to_string(Nq) + " and " +
-                                         std::to_string(Nkv) + ".");
-    if (Hd <= 0 || Hd > 512)
-        throw Error::tensorShapeMismatch("PagedAttention head dim must be 1 to 512 (kernel limit); got " + std::to_string(Hd) + ".");
-    if (kCache.shape[3] != Hd)
-        throw Error::tensorShapeMismatch("PagedAttention caches must have q's head dim; got " + q.shape.str() + " and " + kCache.shape.str() + ".");
-    if (page % 16 != 0)
-        throw Error::tensorShapeMismatch("PagedAttention page size must be a multiple of 16; got " + std::to_string(page) + ".");
-    requireShape(q, t, {T, Nq, Hd}, "PagedAttention q");
-    requireShape(out, t, {T, Nq, Hd}, "PagedAttention out");
-    requireShape(pageTables, D::i32, {R, M}, "PagedAttention page_tables");
-    requireShape(queryStarts, D::i32, {R + 1}, "PagedAttention query_starts");
-    requireShape(keyLens, D::i32, {R}, "PagedAttention key_lens");
-    requireGrid(T * Nq, 256, "PagedAttention", q);
+    const PagedAttentionConstants pc =
+        pagedConstants("PagedAttention", q, kCache, vCache, pageTables, queryStarts, keyLens, out, scale, mask, sinks, maxQueryLen);
     requireApart("PagedAttention", {{&out, "out"}},
                  {{&q, "q"}, {&kCache, "k_cache"}, {&vCache, "v_cache"}, {&pageTables, "page_tables"}, {&queryStarts, "query_starts"},
                   {&keyLens, "key_lens"}});
-    const PagedAttentionConstants pc{(uint32_t)T, (uint32_t)R, (uint32_t)Nq, (uint32_t)Nkv, (uint32_t)Hd, (uint32_t)page,
-                                     (uint32_t)kCache.shape[0], (uint32_t)M, mask.kind, mask.window, (uint32_t)sinks, scale};
-    // 16-byte rows: the matrix cores
-    if (R && T && Hd % (16 / stride(t)) == 0 && aligned(q.data, 16) && aligned(kCache.data, 16) && aligned(vCache.data, 16) && aligned(out.data, 16))
+    if (pc.R && pc.T && fastRows(q, kCache, vCache, out))
         return std::make_unique<PagedAttentionKernel>(q, kCache, vCache, pageTables, queryStarts, keyLens, out, pc, maxQueryLen);
-    std::string fn = std::string("paged_attention_plain_") + name(t);
-    const int run = 4 * stride(t);
-    if (Hd % 4 || !aligned(kCache.data, run) || !aligned(vCache.data, run)) fn += "_any";
-    return fixed(fn, {{q, kRead}, {kCache, kRead}, {vCache, kRead}, {pageTables, kRead}, {queryStarts, kRead}, {keyLens, kRead}, {out, kWrite}},
-                 bytesOf(pc), dim3((unsigned)(R ? T * Nq : 0), 1, 1), 256);
+    return fixed("paged_attention_plain_" + plainName(q, kCache, vCache), {{q, kRead}, {kCache, kRead}, {vCache, kRead}, {pageTables, kRead}, {queryStarts, kRead}, {keyLens, kRead}, {out, kWrite}},
+                 bytesOf(pc), dim3(pc.R ? pc.T * pc.Nq : 0, 1, 1), 256);
+}
+
+std::unique_ptr<Kernel> SharedPrefixAttention(const Tensor &q, const Tensor &kCache, const Tensor &vCache, const Tensor *prefixTables,
+                                              const Tensor *prefixLens, const Tensor *groupStarts, const Tensor &pageTables,
+                                              const Tensor &queryStarts, const Tensor &keyLens, const Tensor &out, const Tensor *lse,
+                                              float scale, AttentionMask mask, int64_t sinks, int64_t maxQueryLen) {
+    using D = DataType;
+    const std::string op = "SharedPrefixAttention";
+    if (!prefixTables != !prefixLens || !prefixTables != !groupStarts)
+        throw Error::invalidArgument(op + " takes prefix_tables, prefix_lens and group_starts together, or none of them.");
+    const PagedAttentionConstants pc = pagedConstants(op, q, kCache, vCache, pageTables, queryStarts, keyLens, out, scale, mask, sinks, maxQueryLen);
+    std::vector<Named> inputs = {{&q, "q"}, {&kCache, "k_cache"}, {&vCache, "v_cache"}, {&pageTables, "page_tables"},
+                                 {&queryStarts, "query_starts"}, {&keyLens, "key_lens"}};
+    SharedPrefixConstants sc{};
+    if (prefixTables) {
+        requireRank(*prefixTables, 2);
+        const int64_t g = prefixTables->shape[0];
+        if (g >= (int64_t{1} << 31) - 1 - pc.R) throw Error::tensorShapeMismatch(op + " takes fewer groups and requests than 2^31 - 1.");
+        requireShape(*prefixTables, D::i32, {g, prefixTables->shape[1]}, op + " prefix_tables");
+        requireShape(*prefixLens, D::i32, {g}, op + " prefix_lens");
+        requireShape(*groupStarts, D::i32, {g + 1}, op + " group_starts");
+        sc.groups = (uint32_t)g;
+        sc.columns = (uint32_t)prefixTables->shape[1];
+        for (const Named &n : {Named{prefixTables, "prefix_tables"}, {prefixLens, "prefix_lens"}, {groupStarts, "group_starts"}}) inputs.push_back(n);
+    }
+    std::vector<Named> outputs = {{&out, "out"}};
+    if (lse) {
+        requireShape(*lse, D::f32, {q.shape[0], q.shape[1]}, op + " lse");
+        outputs.push_back({lse, "lse"});
+    }
+    requireApart(op, outputs, inputs);
+    sc.hasLse = lse != nullptr;
+    sc.windowed = mask.kind == 1 && sc.groups > 0;
+    const Tensor &none = queryStarts;  // (not read where there is no group)
+    std::vector<Tensor> in = {q, kCache, vCache, pageTables, queryStarts, keyLens, prefixTables ? *prefixTables : none,
+                              prefixLens ? *prefixLens : none, groupStarts ? *groupStarts : none};
+    if (pc.R && pc.T && fastRows(q, kCache, vCache, out)) return std::make_unique<SharedPrefixKernel>(std::move(in), out, lse, pc, sc, maxQueryLen);
+    sc.rows = pc.T * pc.Nq;
+    std::vector<Binding> b;
+    for (const Tensor &t : in) b.push_back({t, kRead});
+    b.push_back({out, kWrite});
+    b.push_back({lse ? *lse : out, kWrite});
+    return Kernels::Custom("shared_prefix_plain_" + plainName(q, kCache, vCache), std::move(b), {bytesOf(pc), bytesOf(sc)},
+                           dim3(pc.R ? pc.T * pc.Nq : 0, 1, 1), dim3(256, 1, 1));
+}
+
+std::unique_ptr<Kernel> PagedAttentionWeights(const Tensor &q, const Tensor &kCache, const Tensor &pageTables, const Tensor &queryStarts,
+                                              const Tensor &keyLens, const Tensor &lse, const Tensor &weights, float scale,
+                                              AttentionMask mask, int64_t lastRows, int64_t maxQueryLen) {
+    using D = DataType;
+    const std::string op = "PagedAttentionWeights";
+    if (mask.kind == 1)
+        throw Error::invalidArgument(op + " takes causal or bidirectional attention: a sliding window's places are lost with the keys that are evicted.");
+    if (lastRows < 0) throw Error::invalidArgument(op + " last_rows must not be negative.");
+    const PagedAttentionConstants pc = pagedConstants(op, q, kCache, kCache, pageTables, queryStarts, keyLens, q, scale, mask, 0, maxQueryLen);
+    requireShape(lse, D::f32, {q.shape[0], q.shape[1]}, op + " lse");
+    requireShape(weights, D::f32, {(int64_t)pc.R, (int64_t)pc.Nkv, (int64_t)pc.columns * pc.pageSize}, op + " weights");
+    requireApart(op, {{&weights, "weights"}},
+                 {{&q, "q"}, {&kCache, "k_cache"}, {&pageTables, "page_tables"}, {&queryStarts, "query_starts"}, {&keyLens, "key_lens"}, {&lse, "lse"}});
+    std::vector<Tensor> in = {q, kCache, pageTables, queryStarts, keyLens, lse};
+    if (pc.R && pc.T && fastRows(q, kCache, kCache, q))
+        return std::make_unique<AttentionWeightsKernel>(std::move(in), weights, pc, lastRows);
+    const AttentionWeightsConstants wc{(uint32_t)std::min<int64_t>(lastRows, pc.T), 0, UINT32_MAX, 0};
+    std::vector<Binding> b;
+    for (const Tensor &t : in) b.push_back({t, kRead});
+    b.push_back({weights, kReadWrite});
+    requireGrid((int64_t)pc.R * pc.Nkv, 256, op, weights);
+    // about 2 blocks per CU, of 16 keys and more
+    const int64_t pairs = std::max<int64_t>((int64_t)pc.R * pc.Nkv, 1);
+    const int64_t parts = std::clamp<int64_t>(2 * deviceCUs() / pairs, 1, std::max<int64_t>(1, cdiv((int64_t)pc.columns * pc.pageSize, 16)));
+    return Kernels::Custom(std::string("attention_weights_plain_") + name(q.dataType), std::move(b), {bytesOf(pc), bytesOf(wc)},
+                           dim3(pc.T ? pc.R * pc.Nkv : 0, (unsigned)parts, 1), dim3(256, 1, 1));
+}
+
+std::unique_ptr<Kernel> PagedEviction(const Tensor &weights, const Tensor &kCache, const Tensor &vCache, const Tensor &pageTables,
+                                      const Tensor &keyLens, const Tensor &budgets, const Tensor &kept, const Tensor &keptWeights,
+                                      int64_t first, int64_t last) {
+    using D = DataType;
+    const std::string op = "PagedEviction";
+    if (!isFloat(kCache.dataType) || vCache.dataType != kCache.dataType)
+        throw Error::unsupportedDataTypeCombination(op + " needs caches of one floating dtype; got " + name(kCache.dataType) + ", " + name(vCache.dataType) + ".");
+    if (first < 0 || last < 0 || first >= (int64_t{1} << 31) || last >= (int64_t{1} << 31))
+        throw Error::invalidArgument(op + " first and last must be at least 0 and below 2^31.");
+    requireCaches(kCache, vCache, op);
+    requireRank(pageTables, 2);
+    const int64_t R = pageTables.shape[0], M = pageTables.shape[1], Nkv = kCache.shape[1], page = kCache.shape[2];
+    const int64_t room = requireRoom(op, M, page);
+    requireShape(pageTables, D::i32, {R, M}, op + " page_tables");
+    requireShape(keyLens, D::i32, {R}, op + " key_lens");
+    requireShape(budgets, D::i32, {R}, op + " budgets");
+    requireShape(weights, D::f32, {R, Nkv, room}, op + " weights");
+    requireShape(kept, D::i32, {R, Nkv, room}, op + " kept");
+    requireShape(keptWeights, D::f32, {R, Nkv, room}, op + " kept_weights");
+    requireGrid(R * Nkv, 1024, op, weights);
+    const int64_t slices = cdiv(kCache.shape[3] * stride(kCache.dataType), 16);
+    if (slices > 65535) throw Error::tensorShapeMismatch(op + " rows are too long: " + kCache.shape.str() + ".");
+    requireApart(op, {{&kCache, "k_cache"}, {&vCache, "v_cache"}, {&kept, "kept"}, {&keptWeights, "kept_weights"}},
+                 {{&weights, "weights"}, {&pageTables, "page_tables"}, {&keyLens, "key_lens"}, {&budgets, "budgets"}});
+    const EvictConstants ec{(uint32_t)R, (uint32_t)Nkv, (uint32_t)M, (uint32_t)page, (uint32_t)kCache.shape[0], (uint32_t)first, (uint32_t)last, 0};
+    return std::make_unique<EvictionKernel>(weights, kCache, vCache, pageTables, keyLens, budgets, kept, keptWeights, ec);
+}
+
+std::unique_ptr<Kernel> ReleasePages(const Tensor &keyLens, const Tensor &budgets, const Tensor &pageTables, int64_t pageSize,
+                                     const Tensor &newLens, const Tensor &freed, const Tensor &counts) {
+    using D = DataType;
+    const std::string op = "ReleasePages";
+    requireRank(pageTables, 2);
+    const int64_t R = pageTables.shape[0], M = pageTables.shape[1];
+    if (pageSize <= 0 || pageSize >= (int64_t{1} << 31)) throw Error::invalidArgument(op + " page size must be positive and below 2^31.");
+    requireShape(pageTables, D::i32, {R, M}, op + " page_tables");
+    requireRoom(op, M, pageSize);
+    requireShape(keyLens, D::i32, {R}, op + " key_lens");
+    requireShape(budgets, D::i32, {R}, op + " budgets");
+    requireShape(newLens, D::i32, {R}, op + " new_lens");
+    requireShape(freed, D::i32, {R * M}, op + " freed");
+    requireShape(counts, D::i32, {1}, op + " counts");
+    requireApart(op, {{&newLens, "new_lens"}, {&freed, "freed"}, {&counts, "counts"}},
+                 {{&keyLens, "key_lens"}, {&budgets, "budgets"}, {&pageTables, "page_tables"}});
+    const EvictConstants ec{(uint32_t)R, 1, (uint32_t)M, (uint32_t)pageSize, 0, 0, 0, 0};
+    const int64_t blocks = std::clamp<int64_t>(cdiv(R, 16), 1, 256);
+    return fixed("release_pages", {{keyLens, kRead}, {budgets, kRead}, {pageTables, kRead}, {newLens, kWrite}, {freed, kWrite}, {counts, kWrite}},
+                 bytesOf(ec), dim3((unsigned)blocks, 1, 1), 256);
 }
 
 std::unique_ptr<Kernel> Sample(const Tensor &logits, const Tensor &uniforms, const Tensor *temperature, const Tensor *topK,

@@ -722,13 +722,56 @@ class Kernels:
     @staticmethod
     def PagedAttention(q: Tensor, k_cache: Tensor, v_cache: Tensor, page_tables: Tensor, query_starts: Tensor,
                        key_lens: Tensor, into: Tensor, *, scale: float, mask: AttentionMask = AttentionMask(0),
-                       sinks: int = 0, max_query_len: int = 0) -> Kernel:
+                       sinks: int = 0, max_query_len: int = 0, lse: Optional[Tensor] = None) -> Kernel:
         """Attention of every request's new tokens q [T, Nq, Hd] over its pages (popcorn_kernel_paged_attention);
         max_query_len, the longest request's number of new tokens, chooses the kernels: a graph for steps of single
-        tokens is captured with 1."""
+        tokens is captured with 1. lse [T, Nq] gets the rows' logarithms (popcorn_kernel_shared_prefix_attention)."""
+        if lse is not None:
+            return Kernels.SharedPrefixAttention(q, k_cache, v_cache, None, None, None, page_tables, query_starts, key_lens,
+                                                 into, scale=scale, mask=mask, sinks=sinks, max_query_len=max_query_len,
+                                                 lse=lse)
         ts = (q, k_cache, v_cache, page_tables, query_starts, key_lens, into)
         return _make(lib().popcorn_kernel_paged_attention, *[_d(t) for t in ts], scale, mask.desc(), sinks,
                      max_query_len, refs=ts)
+
+    @staticmethod
+    def SharedPrefixAttention(q: Tensor, k_cache: Tensor, v_cache: Tensor, prefix_tables: Optional[Tensor],
+                              prefix_lens: Optional[Tensor], group_starts: Optional[Tensor], page_tables: Tensor,
+                              query_starts: Tensor, key_lens: Tensor, into: Tensor, *, scale: float,
+                              mask: AttentionMask = AttentionMask(0), sinks: int = 0, max_query_len: int = 0,
+                              lse: Optional[Tensor] = None) -> Kernel:
+        """PagedAttention of requests that share prefixes (popcorn_kernel_shared_prefix_attention): group g's requests,
+        group_starts[g] .. group_starts[g + 1] - 1, have prefix_lens[g] keys in the pages of prefix_tables[g] before
+        their own; lse [T, Nq] gets the logarithm of each row's sum of exponentials."""
+        ts = (q, k_cache, v_cache, prefix_tables, prefix_lens, group_starts, page_tables, query_starts, key_lens, into, lse)
+        return _make(lib().popcorn_kernel_shared_prefix_attention, *[_d(t) for t in ts], scale, mask.desc(), sinks,
+                     max_query_len, refs=ts)
+
+    @staticmethod
+    def PagedAttentionWeights(q: Tensor, k_cache: Tensor, page_tables: Tensor, query_starts: Tensor, key_lens: Tensor,
+                              lse: Tensor, weights: Tensor, *, scale: float, mask: AttentionMask = AttentionMask(0),
+                              last_rows: int = 0, max_query_len: int = 0) -> Kernel:
+        """What the new tokens' attention gave each key, added to weights [R, Nkv, columns * page_size]
+        (popcorn_kernel_paged_attention_weights); last_rows: of each request only its last new tokens count."""
+        ts = (q, k_cache, page_tables, query_starts, key_lens, lse, weights)
+        return _make(lib().popcorn_kernel_paged_attention_weights, *[_d(t) for t in ts], scale, mask.desc(), last_rows,
+                     max_query_len, refs=ts)
+
+    @staticmethod
+    def PagedEviction(weights: Tensor, k_cache: Tensor, v_cache: Tensor, page_tables: Tensor, key_lens: Tensor,
+                      budgets: Tensor, kept: Tensor, kept_weights: Tensor, *, first: int = 0, last: int = 0) -> Kernel:
+        """Each KV head of a request keeps budgets[r] keys, its first and last ones and the heaviest between, at the
+        front of the request's pages (popcorn_kernel_paged_eviction)."""
+        ts = (weights, k_cache, v_cache, page_tables, key_lens, budgets, kept, kept_weights)
+        return _make(lib().popcorn_kernel_paged_eviction, *[_d(t) for t in ts], first, last, refs=ts)
+
+    @staticmethod
+    def ReleasePages(key_lens: Tensor, budgets: Tensor, page_tables: Tensor, *, page_size: int, new_lens: Tensor,
+                     freed: Tensor, counts: Tensor) -> Kernel:
+        """The lengths behind an eviction and the pages that it left empty (popcorn_kernel_release_pages)."""
+        ts = (key_lens, budgets, page_tables, new_lens, freed, counts)
+        d = [_d(t) for t in ts]
+        return _make(lib().popcorn_kernel_release_pages, *d[:3], page_size, *d[3:], refs=ts)
 
     @staticmethod
     def Sample(logits: Tensor, uniforms: Tensor, into: Tensor, *, temperature: Optional[Tensor] = None,
