@@ -497,12 +497,15 @@ typedef struct {
  * bidirectional). lastRows: the new tokens of a request that count, from its last
  * back (0: all); a launch takes the requests of fewRows < rows <= manyRows.
  * ownPlan: every block sums the requests' keys by itself (at most 1024 requests,
- * all their groups of 16 keys below 2^32), else attention_weights_plan has. */
+ * all their groups of 16 keys below 2^32), else attention_weights_plan has.
+ * everyKey: rows see keys behind them too. The tile kernel's work is dealt as
+ * attention's, with tiles of 256 keys and steps of 64 rows. */
 typedef struct {
     uint32_t lastRows;
     uint32_t fewRows;
     uint32_t manyRows;
     uint32_t ownPlan;
+    uint32_t everyKey;
 } AttentionWeightsConstants;
 
 /* evict_*, release_pages: weights [R, Nkv, columns x pageSize]; rowUnits: units

@@ -3,19 +3,9 @@
 //   of KV head hkv) that see key k,
 // with the rows' lse from the attention before. K is read once more, V is not, and a key's sum belongs to one
 // wave, so that no order of atomics shows in it.
-#include <type_traits>
-
-#include "mfma.hpp"
-#include "paged.hpp"
-#include "scan.hpp"
+#include "paged_attention.hpp"
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kOutOfRange = (int)0x80000000u;
-using pk::u32x4;
-
-__device__ inline uint32_t first_lane(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // A request of the call: the rows that count are tokens start .. start + n - 1, token i at position pos0 + i.
 __device__ inline pk::PagedRequest weights_request(const int32_t *starts, const int32_t *keyLens, uint32_t r, const PagedAttentionConstants &p,
@@ -194,6 +184,221 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
     }
 }
 
+// ---- many rows: prompts -------------------------------------------------------------------
+// A unit is 256 keys of a request for one KV head, 64 to a wave, whose fragments stay in registers, on v_mfma_f32_32x32x16: S^T =
+// K . Q^T has a row's scores in a lane of each half, so a key's sum over rows is added up in its own register, and over the
+// lanes once at the end. Steps are 64 rows of Q, copied straight into LDS, a step ahead. The units' steps
+// in a row are dealt out as for attention; of a unit that several blocks share each leaves 256 partial sums.
+constexpr uint32_t kKeys = 256, kStageRows = 64;
+
+struct WeightsBatch {
+    static constexpr bool kShared = false;
+    using Request = pk::PagedRequest;
+    struct Left {  // a unit that its block shares with others behind it
+        uint32_t pieces, request, hkv, key0;
+    };
+    const int32_t *starts, *keyLens;
+    Left *left;
+    const AttentionWeightsConstants &a;
+
+    __device__ inline uint32_t requests(const PagedAttentionConstants &p) const { return p.R; }
+    __device__ inline Request request(uint32_t r, const PagedAttentionConstants &p) const { return weights_request(starts, keyLens, r, p, a); }
+    __device__ inline uint32_t tiles(const Request &q, uint32_t G, const PagedWorkConstants &w) const {
+        const uint32_t rows = (uint32_t)q.n * G;
+        if (rows <= w.fewRows || rows > w.manyRows) return 0;
+        const int32_t keys = a.everyKey ? q.keys : min(q.keys, max(q.pos0 + q.n - 1, -1) + 1);
+        return ((uint32_t)keys + kKeys - 1) / kKeys;
+    }
+    // Steps of rows from the first that sees a key.
+    __device__ inline pk::PagedSteps steps(const Request &q, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &) const {
+        const uint32_t G = p.Nq / p.Nkv;
+        pk::PagedSteps s{};
+        s.first = a.everyKey ? 0u : (uint32_t)max((int64_t)tile * kKeys - q.pos0, (int64_t)0) * G / kStageRows;
+        s.n = ((uint32_t)q.n * G + kStageRows - 1) / kStageRows - s.first;
+        return s;
+    }
+    __device__ static inline void idle(Left *to) { to->pieces = 0; }
+    __device__ static inline void close(Left *to, const Piece<Request> &c, uint32_t sharers, const PagedWorkConstants &) {
+        *to = Left{sharers, c.request, c.hkv, c.tile * kKeys};
+    }
+};
+
+template <typename T, int HD>
+__device__ void weights_tile(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
+                             const int32_t *__restrict__ tables, const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
+                             const float *__restrict__ lse, const pk::PagedTile *__restrict__ plan, float *__restrict__ partial,
+                             WeightsBatch::Left *__restrict__ left, float *__restrict__ weights, const PagedAttentionConstants &p,
+                             const PagedWorkConstants &w, const AttentionWeightsConstants &a) {
+    using S = typename T::storage;
+    constexpr int KS = HD / 16, CH = HD / 8;
+    constexpr int kRowsPer = 64 / CH;       // rows per copy instruction
+    constexpr int kCopies = 16 / kRowsPer;  // instructions for a wave's 16 rows of a stage
+    constexpr uint32_t kStageBytes = kStageRows * HD * 2;
+    __shared__ __attribute__((aligned(256))) uint8_t smem[2 * kStageBytes + kOwnTiles * sizeof(OwnTile)];
+    using Space = PlanSpace<256, uint32_t, pk::PagedRequest>;
+    static_assert(sizeof(Space) <= 2 * kStageBytes, "the plan is laid out where Q goes");
+    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 2 * kStageBytes);
+    const uint32_t lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31, wave = first_lane(threadIdx.x >> 6);
+    const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
+    const float c2 = p.scale * kLog2e;
+    auto swz = [](uint32_t row) { return CH >= 16 ? row % 16u : row / 2u % 8u; };
+    // row / G: rows are below 2^24 and G at most 256, so that row (ceil(2^32 / G) G - 2^32) stays below 2^32
+    const uint32_t inverse = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
+    auto token_of = [&](uint32_t row) { return G == 1 ? row : __umulhi(row, inverse); };
+    const WeightsBatch batch{starts, keyLens, left, a};
+    Dealer<256, WeightsBatch> dealer(batch, plan, sm_plan, *reinterpret_cast<Space *>(smem), p, w);
+    Piece<pk::PagedRequest> c;
+    while (dealer.next(c, p, w)) {
+        const int32_t *table = tables + (uint64_t)c.request * p.columns;
+        const uint32_t keys = (uint32_t)c.req.keys, rows = (uint32_t)c.req.n * G, key0 = c.tile * kKeys + wave * 64;
+        auto page_of = [&](uint32_t key) { return key < keys ? (uint32_t)table[key / p.pageSize] : ~0u; };
+        // Q's rows of a step; those past the last repeat it and give nothing
+        const uint32_t n = c.hi - c.lo, row0 = (c.steps.first + c.lo) * kStageRows;
+        auto copy = [&](uint32_t i) {
+            const uint32_t first = row0 + i * kStageRows, token = token_of(first);
+            const S *from = Q + (((uint64_t)(uint32_t)c.req.start + token) * p.Nq + c.hkv * G) * D;
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(from), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < kCopies; ++j) {
+                const uint32_t in = wave * 16 + j * kRowsPer + lane / CH, row = min(first + in, rows - 1), chunk = lane % CH ^ swz(in);
+                const uint32_t of = token_of(row), at = ((of - token) * p.Nq + (row - of * G)) * D + chunk * 8;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(smem + i % 2 * kStageBytes + (wave * 16 + j * kRowsPer) * HD * 2), 16,
+                                                         chunk * 8 < D ? (int)(at * 2) : kOutOfRange, 0, 0, 0);
+            }
+        };
+        float next[2];  // the rows' logarithms in base 2; infinity: the row gives nothing
+        auto ahead = [&](uint32_t i) {
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                const uint32_t row = row0 + i * kStageRows + rt * 32 + c32;
+                float x = INFINITY;
+                const uint32_t token = token_of(row);
+                if (row < rows) x = lse[((uint64_t)(uint32_t)c.req.start + token) * p.Nq + c.hkv * G + (row - token * G)];
+                next[rt] = x == -INFINITY ? INFINITY : x * kLog2e;
+            }
+        };
+        copy(0);
+        ahead(0);
+        u32x4 kf[2][KS];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const uint32_t key = key0 + t * 32 + c32, page = page_of(key);
+            const S *row = K + (((uint64_t)(page < p.pages ? page : 0u) * p.Nkv + c.hkv) * p.pageSize + key % p.pageSize) * D;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                const uint32_t d = s * 16 + h * 8;
+                kf[t][s] = page < p.pages && d < D ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0u, 0u, 0u, 0u};
+            }
+        }
+        f32x16 sum[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) sum[t][e] = 0.0f;
+        const uint32_t qAt = c32 * (HD * 2) + (h ^ swz(c32)) * 16;
+        for (uint32_t i = 0; i < n; ++i) {
+            const float of[2] = {next[0], next[1]};
+            wait_vmcnt<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            if (i + 1 < n) {
+                copy(i + 1);
+                ahead(i + 1);
+            }
+            if (key0 >= keys) continue;
+            uint32_t x = qAt + i % 2 * kStageBytes;
+            asm volatile("" : "+v"(x));
+#pragma unroll
+            for (int rt = 0; rt < 2; ++rt) {
+                const uint32_t first = row0 + i * kStageRows + rt * 32;
+                if (first >= rows) break;
+                f32x16 st[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) st[t][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    const u32x4 q = *reinterpret_cast<const u32x4 *>(smem + ((x ^ (s & 7) * 32u) + (s >> 3) * 256u + rt * (32 * HD * 2)));
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) st[t] = pk::Mma<T>::run(kf[t][s], q, st[t]);
+                }
+                const int posLo = c.req.pos0 + (int)token_of(first), pos = c.req.pos0 + (int)token_of(min(first + c32, rows - 1));
+                // a row that gives nothing, or one that does not see all keys
+                const bool hide = __ballot(of[rt] == INFINITY) != 0 || (p.maskKind != 2u && (int)key0 + 63 > posLo);
+                if (hide) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const int key = (int)(key0 + t * 32 + (e >> 2) * 8 + h * 4 + (e & 3));
+                            const bool seen = of[rt] != INFINITY && (p.maskKind == 2u || key <= pos);
+                            const float v = __builtin_amdgcn_exp2f(fmaf(st[t][e], c2, -of[rt]));
+                            sum[t][e] += seen ? v : 0.0f;
+                        }
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) sum[t][e] += __builtin_amdgcn_exp2f(fmaf(st[t][e], c2, -of[rt]));
+                }
+            }
+        }
+        // every wave has read its last rows before the next piece's copies
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        const bool whole = c.lo == 0 && c.hi == c.steps.n;
+        float *to = weights + ((uint64_t)c.request * p.Nkv + c.hkv) * ((uint64_t)p.columns * p.pageSize);
+        float *slot = partial + (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * kKeys + wave * 64;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            float mine = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float v = pk::half32_sum(sum[t][e]);
+                if (c32 == (uint32_t)e) mine = v;
+            }
+            if (c32 < 16) {
+                const uint32_t in = t * 32 + (c32 >> 2) * 8 + h * 4 + (c32 & 3);
+                if (!whole) slot[in] = mine;
+                else if (page_of(key0 + in) < p.pages) to[key0 + in] += mine;
+            }
+        }
+    }
+}
+
+}  // namespace
+
+// The partial sums of the units that several blocks shared, in their order.
+POPCORN_KERNEL void __launch_bounds__(256)
+    attention_weights_join(const int32_t *tables, const int32_t *starts, const int32_t *keyLens, const float *partial,
+                           const WeightsBatch::Left *left, float *weights, PagedAttentionConstants p, AttentionWeightsConstants a) {
+    const WeightsBatch::Left c = left[blockIdx.x];
+    if (c.pieces == 0) return;
+    const pk::PagedRequest q = weights_request(starts, keyLens, c.request, p, a);
+    const uint32_t key = c.key0 + threadIdx.x;
+    if (key >= (uint32_t)q.keys || (uint32_t)tables[(uint64_t)c.request * p.columns + key / p.pageSize] >= p.pages) return;
+    float x = 0.0f;
+    for (uint32_t i = 0; i < c.pieces; ++i) x += partial[(2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * kKeys + threadIdx.x];
+    weights[((uint64_t)c.request * p.Nkv + c.hkv) * ((uint64_t)p.columns * p.pageSize) + key] += x;
+}
+
+POPCORN_KERNEL void __launch_bounds__(1024)
+    attention_weights_tiles(const int32_t *starts, const int32_t *keyLens, pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants w,
+                            AttentionWeightsConstants a) {
+    __shared__ PlanSpace<1024, u64, pk::PagedRequest> space;
+    u64 steps;
+    uint32_t tiles;
+    const WeightsBatch batch{starts, keyLens, nullptr, a};
+    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) {
+        plan[1 + at] = pk::PagedTile{before, request, tile};
+    });
+    if (threadIdx.x == 0) plan[0] = pk::PagedTile{steps, tiles, 0};
+}
+
+namespace {
+
 // Any head dim and alignment: 16 lanes take a key at a time, for every row in turn.
 template <typename T>
 __device__ void weights_plain(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
@@ -233,6 +438,14 @@ __device__ void weights_plain(const typename T::storage *__restrict__ Q, const t
                                           PagedAttentionConstants p, AttentionWeightsConstants w) {                           \
         weights_few<T, HD, KM>(q, k, tables, starts, keyLens, lse, plan, weights, p, w);                                      \
     }
+#define WEIGHTS_TILE(t, T, HD)                                                                                                \
+    POPCORN_KERNEL void __launch_bounds__(256, 2)                                                                             \
+        attention_weights_tile_##t##_d##HD(const T::storage *q, const T::storage *k, const int32_t *tables, const int32_t *starts, \
+                                           const int32_t *keyLens, const float *lse, const pk::PagedTile *plan, float *partial, \
+                                           WeightsBatch::Left *left, float *weights, PagedAttentionConstants p,               \
+                                           PagedWorkConstants w, AttentionWeightsConstants a) {                               \
+        weights_tile<T, HD>(q, k, tables, starts, keyLens, lse, plan, partial, left, weights, p, w, a);                       \
+    }
 #define WEIGHTS_PLAIN(t, T)                                                                                                   \
     POPCORN_KERNEL void __launch_bounds__(256)                                                                                \
         attention_weights_plain_##t(const T::storage *q, const T::storage *k, const int32_t *tables, const int32_t *starts,   \
@@ -250,6 +463,9 @@ using pk::F32;
     WEIGHTS_FEW(t, T, 128, 4, 3)  \
     WEIGHTS_FEW(t, T, 256, 2, 2)  \
     WEIGHTS_FEW(t, T, 512, 1, 2)  \
+    WEIGHTS_TILE(t, T, 64)        \
+    WEIGHTS_TILE(t, T, 128)       \
+    WEIGHTS_TILE(t, T, 256)       \
     WEIGHTS_PLAIN(t, T)
 WEIGHTS_16(f16, F16)
 WEIGHTS_16(bf16, BF16)

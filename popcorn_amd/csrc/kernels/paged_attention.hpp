@@ -112,6 +112,12 @@ struct PlanSpace {  // of a block of N threads
     Request req[N];
 };
 
+// Tiles of a request's rows that a launch takes.
+__device__ inline uint32_t row_tiles(const pk::PagedRequest &q, uint32_t G, const PagedWorkConstants &w) {
+    const uint32_t rows = (uint32_t)q.n * G;
+    return rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
+}
+
 // The tiles of every request, in request order: put(tile, steps before, request, tile of it).
 template <uint32_t N, typename U, typename Batch, typename Put>
 __device__ inline void lay_tiles(const Batch &batch, PlanSpace<N, U, typename Batch::Request> &sp, const PagedAttentionConstants &p,
@@ -123,8 +129,7 @@ __device__ inline void lay_tiles(const Batch &batch, PlanSpace<N, U, typename Ba
         const uint32_t r = base + tid;
         typename Batch::Request q{};
         if (r < requests) q = batch.request(r, p);
-        const uint32_t rows = (uint32_t)q.n * G;
-        const uint32_t mine = rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
+        const uint32_t mine = batch.tiles(q, G, w);
         const pk::Scan<U> of = pk::block_scan<N / 64>((U)mine, sp.sums);
         const U upto = of.upto, total = of.total;
         // overlapping ranges of requests could hold more rows than there are: what passes the plan's room is left out
@@ -203,7 +208,7 @@ template <typename Request>
 struct Piece {
     Request req;
     pk::PagedSteps steps;
-    uint32_t request, hkv, lo, hi;
+    uint32_t request, tile, hkv, lo, hi;
     uint32_t sharers;  // workers of the unit, where this is its first piece and others follow; else 0
 };
 
@@ -229,6 +234,7 @@ struct OwnPages {
     __device__ inline Request request(uint32_t r, const PagedAttentionConstants &p) const {
         return pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
     }
+    __device__ inline uint32_t tiles(const Request &q, uint32_t G, const PagedWorkConstants &w) const { return row_tiles(q, G, w); }
     __device__ inline pk::PagedSteps steps(const Request &r, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) const {
         return pk::paged_steps(r, tile, p, w);
     }
@@ -300,6 +306,7 @@ struct Dealer {
                 t = pk::PagedTile{first_lane64(t.before), first_lane(t.request), first_lane(t.tile)};
             }
             c.request = t.request;
+            c.tile = t.tile;
             c.req = batch.request(t.request, p);
             c.steps = batch.steps(c.req, t.tile, p, w);
             const pk::PagedPiece piece = pk::paged_piece(x - t.before * p.Nkv, end - x, c.steps.n, w);

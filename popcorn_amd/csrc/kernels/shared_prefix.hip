@@ -41,6 +41,7 @@ struct SharedPages {
         return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, more.s);
     }
     __device__ inline PagedAttentionConstants mask(const Request &q, const PagedAttentionConstants &p) const { return pk::paged_shared_mask(q, p); }
+    __device__ inline uint32_t tiles(const Request &q, uint32_t G, const PagedWorkConstants &w) const { return row_tiles(q, G, w); }
     __device__ inline pk::PagedSteps steps(const Request &q, uint32_t tile, const PagedAttentionConstants &p, const PagedWorkConstants &w) const {
         return pk::paged_shared_steps(q, tile, p, w);
     }

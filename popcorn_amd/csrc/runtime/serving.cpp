@@ -382,7 +382,7 @@ private:
 // PagedAttentionWeights (attention_weights.hip).
 class AttentionWeightsKernel : public Kernel {
 public:
-    AttentionWeightsKernel(std::vector<Tensor> inputs, const Tensor &weights, const PagedAttentionConstants &pc, int64_t lastRows)
+    AttentionWeightsKernel(std::vector<Tensor> inputs, const Tensor &weights, const PagedAttentionConstants &pc, int64_t lastRows, int64_t maxQueryLen)
         : in_(std::move(inputs)), weights_(weights), pc_(pc) {
         const Tensor &q = in_[0];
         const int64_t groups = cdiv((int64_t)pc.columns * pc.pageSize, 16);
@@ -390,9 +390,26 @@ public:
         const int hdp = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
         fn_ = "attention_weights_few_" + type + "_d" + std::to_string(hdp);
         wc_ = AttentionWeightsConstants{(uint32_t)std::min<int64_t>(lastRows, pc.T), 0, UINT32_MAX,
-                                        pc.R <= 1024 && (double)groups * pc.R < 4294967296.0};
+                                        pc.R <= 1024 && (double)groups * pc.R < 4294967296.0, pc.maskKind == 2};
         const int perCU = q.dataType == DataType::f32 ? (hdp <= 64 ? 3 : hdp <= 256 ? 2 : 1) : (hdp <= 64 ? 4 : hdp <= 128 ? 3 : 2);
         blocks_ = (unsigned)std::clamp<double>((double)groups * pc.R * pc.Nkv / 4, 1, (double)perCU * deviceCUs());
+        const int64_t G = pc.Nq / pc.Nkv;
+        int64_t longest = std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T);
+        if (lastRows > 0) longest = std::min(longest, lastRows);
+        // 16-bit keys of up to 256 dims, rows divided by G as the kernel does, and a step's rows within reach of one offset
+        if (q.dataType == DataType::f32 || hdp > 256 || longest * G <= kFewRows || G > 256 || (int64_t)64 * pc.Nq * pc.Hd >= (int64_t{1} << 29)) return;
+        tile_ = "attention_weights_tile_" + type + "_d" + std::to_string(hdp);
+        few_ = pc.R > 1;
+        wc_.manyRows = kFewRows;
+        work_.fewRows = few_ ? kFewRows : 0;
+        work_.manyRows = UINT32_MAX;
+        const int64_t blocks = cdiv((int64_t)pc.columns * pc.pageSize, 256);
+        work_.maxTiles = (uint32_t)std::min<int64_t>((int64_t)pc.R * blocks, INT32_MAX);
+        work_.minSteps = 1;
+        work_.unitSteps = 3;
+        const double steps = (double)work_.maxTiles * ((double)cdiv((int64_t)pc.T * G, 64) + work_.unitSteps);
+        work_.workers = (uint32_t)std::max(1.0, std::min(2.0 * deviceCUs(), steps * pc.Nkv));
+        work_.ownPlan = work_.maxTiles <= 1024 && pc.R <= 1024 && steps < 2147483648.0;
     }
     std::vector<Binding> tensors() const override {
         std::vector<Binding> b;
@@ -400,7 +417,12 @@ public:
         b.push_back({weights_, kReadWrite});
         return b;
     }
-    std::string describe() const override { return (wc_.ownPlan ? "" : "attention_weights_plan,") + fn_; }
+    std::string describe() const override {
+        std::string s;
+        if (few_) s = (wc_.ownPlan ? "" : "attention_weights_plan,") + fn_;
+        if (!tile_.empty()) s += (few_ ? "," : "") + std::string(work_.ownPlan ? "" : "attention_weights_tiles,") + tile_ + ",attention_weights_join";
+        return s;
+    }
     void encode(KernelCommandEncoder &enc) const override {
         const std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_), bytesOf(wc_)};
         auto run = [&](const Tensor &plan) {
@@ -410,11 +432,31 @@ public:
             b.push_back({weights_, kReadWrite});
             enc.encode(*Kernels::Custom(fn_, std::move(b), consts, dim3(blocks_, 1, 1), dim3(256, 1, 1)));
         };
-        if (wc_.ownPlan) return run(weights_);  // (not read)
-        enc.withTemporaryTensor(ScratchSpec{{((int64_t)pc_.R + 1) * 8}, DataType::u8}, [&](Tensor plan) {
-            enc.encode(*Kernels::Custom("attention_weights_plan", {{in_[3], kRead}, {in_[4], kRead}, {plan, kWrite}}, consts, dim3(1, 1, 1),
-                                        dim3(1024, 1, 1)));
-            run(plan);
+        if (few_ && wc_.ownPlan) run(weights_);  // (not read)
+        else if (few_)
+            enc.withTemporaryTensor(ScratchSpec{{((int64_t)pc_.R + 1) * 8}, DataType::u8}, [&](Tensor plan) {
+                enc.encode(*Kernels::Custom("attention_weights_plan", {{in_[3], kRead}, {in_[4], kRead}, {plan, kWrite}}, consts, dim3(1, 1, 1),
+                                            dim3(1024, 1, 1)));
+                run(plan);
+            });
+        if (tile_.empty()) return;
+        // the partial sums, what is shared, the plan
+        const int64_t sums = (int64_t)work_.workers * 2 * 256 * 4, shared = (int64_t)work_.workers * 16;
+        const int64_t plan = work_.ownPlan ? 0 : ((int64_t)work_.maxTiles + 1) * 16;
+        enc.withTemporaryTensor(ScratchSpec{{sums + shared + plan}, DataType::u8}, [&](Tensor scratch) {
+            auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
+            const Tensor partial = part(0, sums), left = part(sums, shared), tiles = part(sums + shared, plan);
+            const std::vector<std::vector<uint8_t>> all = {bytesOf(pc_), bytesOf(work_), bytesOf(wc_)};
+            if (plan)
+                enc.encode(*Kernels::Custom("attention_weights_tiles", {{in_[3], kRead}, {in_[4], kRead}, {tiles, kWrite}}, all, dim3(1, 1, 1),
+                                            dim3(1024, 1, 1)));
+            std::vector<Binding> b;
+            for (const Tensor &t : in_) b.push_back({t, kRead});
+            for (const Binding &x : {Binding{tiles, kRead}, {partial, kWrite}, {left, kWrite}, {weights_, kReadWrite}}) b.push_back(x);
+            enc.encode(*Kernels::Custom(tile_, std::move(b), all, dim3(work_.workers, 1, 1), dim3(256, 1, 1)));
+            enc.encode(*Kernels::Custom("attention_weights_join",
+                                        {{in_[2], kRead}, {in_[3], kRead}, {in_[4], kRead}, {partial, kRead}, {left, kRead}, {weights_, kReadWrite}},
+                                        {bytesOf(pc_), bytesOf(wc_)}, dim3(work_.workers, 1, 1), dim3(256, 1, 1)));
         });
     }
 
@@ -423,8 +465,11 @@ private:
     Tensor weights_;
     PagedAttentionConstants pc_;
     AttentionWeightsConstants wc_{};
-    std::string fn_;
+    PagedWorkConstants work_{};
+    std::string fn_, tile_;
+    bool few_ = true;
     unsigned blocks_ = 1;
+    static constexpr int64_t kFewRows = 32;
 };
 
 // PagedEviction (evict.hip): the choice, then the moves of K and V.
@@ -671,8 +716,8 @@ std::unique_ptr<Kernel> PagedAttentionWeights(const Tensor &q, const Tensor &kCa
                  {{&q, "q"}, {&kCache, "k_cache"}, {&pageTables, "page_tables"}, {&queryStarts, "query_starts"}, {&keyLens, "key_lens"}, {&lse, "lse"}});
     std::vector<Tensor> in = {q, kCache, pageTables, queryStarts, keyLens, lse};
     if (pc.R && pc.T && fastRows(q, kCache, kCache, q))
-        return std::make_unique<AttentionWeightsKernel>(std::move(in), weights, pc, lastRows);
-    const AttentionWeightsConstants wc{(uint32_t)std::min<int64_t>(lastRows, pc.T), 0, UINT32_MAX, 0};
+        return std::make_unique<AttentionWeightsKernel>(std::move(in), weights, pc, lastRows, maxQueryLen);
+    const AttentionWeightsConstants wc{(uint32_t)std::min<int64_t>(lastRows, pc.T), 0, UINT32_MAX, 0, 0};
     std::vector<Binding> b;
     for (const Tensor &t : in) b.push_back({t, kRead});
     b.push_back({weights, kReadWrite});
