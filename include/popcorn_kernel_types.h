@@ -509,7 +509,7 @@ typedef struct {
 } AttentionWeightsConstants;
 
 /* evict_*, release_pages: weights [R, Nkv, columns x pageSize]; rowUnits: units
- * that evict_move_* copies of a cache's row. */
+ * that evict_move_* copies of a cache's row, `units` of them (a power of 2) by a block. */
 typedef struct {
     uint32_t R;
     uint32_t Nkv;
@@ -519,6 +519,7 @@ typedef struct {
     uint32_t first;
     uint32_t last;
     uint32_t rowUnits;
+    uint32_t units;
 } EvictConstants;
 
 /* sample_*: one token of each row of logits [rows, vocab]; a row is cut into

@@ -233,18 +233,21 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
     constexpr int KS = HD / 16, CH = HD / 8;
     constexpr int kRowsPer = 64 / CH;       // rows per copy instruction
     constexpr int kCopies = 16 / kRowsPer;  // instructions for a wave's 16 rows of a stage
-    constexpr uint32_t kStageBytes = kStageRows * HD * 2;
-    __shared__ __attribute__((aligned(256))) uint8_t smem[2 * kStageBytes + kOwnTiles * sizeof(OwnTile)];
+    // A step takes less than a copy's latency, so copies run three steps ahead: four places for 64 rows and, for each wave, their
+    // logarithms.
+    constexpr uint32_t kPlaces = 4, kStageBytes = kStageRows * HD * 2, kLse = kPlaces * kStageBytes, kPlan = kLse + kPlaces * 4 * 256;
+    __shared__ __attribute__((aligned(256))) uint8_t smem[kPlan + kOwnTiles * sizeof(OwnTile)];
     using Space = PlanSpace<256, uint32_t, pk::PagedRequest>;
-    static_assert(sizeof(Space) <= 2 * kStageBytes, "the plan is laid out where Q goes");
-    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 2 * kStageBytes);
+    static_assert(sizeof(Space) <= kLse, "the plan is laid out where Q goes");
+    OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + kPlan);
     const uint32_t lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31, wave = first_lane(threadIdx.x >> 6);
     const uint32_t D = p.Hd, G = p.Nq / p.Nkv;
-    const float c2 = p.scale * kLog2e;
+    const float c2 = fabsf(p.scale) * kLog2e;
+    const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;  // -scale K . Q = scale -K . Q
     auto swz = [](uint32_t row) { return CH >= 16 ? row % 16u : row / 2u % 8u; };
     // row / G: rows are below 2^24 and G at most 256, so that row (ceil(2^32 / G) G - 2^32) stays below 2^32
-    const uint32_t inverse = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G);
-    auto token_of = [&](uint32_t row) { return G == 1 ? row : __umulhi(row, inverse); };
+    const uint32_t inverse = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G), single = G == 1 ? ~0u : 0u;
+    auto token_of = [&](uint32_t row) { return __umulhi(row, inverse) + (row & single); };
     const WeightsBatch batch{starts, keyLens, left, a};
     Dealer<256, WeightsBatch> dealer(batch, plan, sm_plan, *reinterpret_cast<Space *>(smem), p, w);
     Piece<pk::PagedRequest> c;
@@ -252,33 +255,43 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
         const int32_t *table = tables + (uint64_t)c.request * p.columns;
         const uint32_t keys = (uint32_t)c.req.keys, rows = (uint32_t)c.req.n * G, key0 = c.tile * kKeys + wave * 64;
         auto page_of = [&](uint32_t key) { return key < keys ? (uint32_t)table[key / p.pageSize] : ~0u; };
-        // Q's rows of a step; those past the last repeat it and give nothing
+        // Q's rows of a step and their logarithms. Those past the request's last give nothing, whatever they hold; those past the
+        // tensor's are zeros. (Always as many instructions.) Where G divides a step its rows lie alike in every step.
         const uint32_t n = c.hi - c.lo, row0 = (c.steps.first + c.lo) * kStageRows;
-        auto copy = [&](uint32_t i) {
-            const uint32_t first = row0 + i * kStageRows, token = token_of(first);
-            const S *from = Q + (((uint64_t)(uint32_t)c.req.start + token) * p.Nq + c.hkv * G) * D;
-            const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(from), 0, 0x7fffffff, 0x00020000);
+        const bool alike = kStageRows % G == 0;
+        uint32_t at[kCopies], lseAt = 0;
+        auto lay = [&](uint32_t first) {
+            const uint32_t token = token_of(first);
+            auto behind = [&](uint32_t row) {  // the first token, in rows of Q
+                const uint32_t of = token_of(row);
+                return (of - token) * p.Nq + (row - of * G);
+            };
 #pragma unroll
             for (int j = 0; j < kCopies; ++j) {
-                const uint32_t in = wave * 16 + j * kRowsPer + lane / CH, row = min(first + in, rows - 1), chunk = lane % CH ^ swz(in);
-                const uint32_t of = token_of(row), at = ((of - token) * p.Nq + (row - of * G)) * D + chunk * 8;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(smem + i % 2 * kStageBytes + (wave * 16 + j * kRowsPer) * HD * 2), 16,
-                                                         chunk * 8 < D ? (int)(at * 2) : kOutOfRange, 0, 0, 0);
+                const uint32_t in = wave * 16 + j * kRowsPer + lane / CH, chunk = lane % CH ^ swz(in);
+                const uint32_t x = (behind(first + in) * D + chunk * 8) * 2;
+                at[j] = chunk * 8 < D ? x : (uint32_t)kOutOfRange;
             }
+            lseAt = behind(first + lane) * 4;
         };
-        float next[2];  // the rows' logarithms in base 2; infinity: the row gives nothing
-        auto ahead = [&](uint32_t i) {
+        lay(row0);
+        auto copy = [&](uint32_t i) {
+            const uint32_t first = row0 + i * kStageRows, place = i % kPlaces;
+            if (!alike) lay(first);
+            const uint64_t at0 = ((uint64_t)(uint32_t)c.req.start + first_lane(token_of(first))) * p.Nq + c.hkv * G, all = (uint64_t)p.T * p.Nq;
+            const uint64_t left = at0 < all ? all - at0 : 0;
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(Q + (at0 < all ? at0 : 0) * D), 0,
+                                                              (int)min(left * D * 2, (uint64_t)0x7fffffff), 0x00020000);
+            const auto ls = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(lse + (at0 < all ? at0 : 0)), 0,
+                                                              (int)min(left * 4, (uint64_t)0x7fffffff), 0x00020000);
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                const uint32_t row = row0 + i * kStageRows + rt * 32 + c32;
-                float x = INFINITY;
-                const uint32_t token = token_of(row);
-                if (row < rows) x = lse[((uint64_t)(uint32_t)c.req.start + token) * p.Nq + c.hkv * G + (row - token * G)];
-                next[rt] = x == -INFINITY ? INFINITY : x * kLog2e;
-            }
+            for (int j = 0; j < kCopies; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(smem + place * kStageBytes + (wave * 16 + j * kRowsPer) * HD * 2), 16,
+                                                         (int)at[j], 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ls, (lds_void *)(smem + kLse + (place * 4 + wave) * 256), 4, (int)lseAt, 0, 0, 0);
         };
-        copy(0);
-        ahead(0);
+#pragma unroll
+        for (uint32_t i = 0; i + 1 < kPlaces; ++i) copy(i);
         u32x4 kf[2][KS];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -287,64 +300,100 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
                 const uint32_t d = s * 16 + h * 8;
-                kf[t][s] = page < p.pages && d < D ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0u, 0u, 0u, 0u};
+                kf[t][s] = (page < p.pages && d < D ? *reinterpret_cast<const u32x4 *>(row + d) : u32x4{0u, 0u, 0u, 0u}) ^ flip;
             }
         }
-        f32x16 sum[2];
+        f32x16 sum[2], st[2][2];  // scores of a step's first and second 32 rows, 32 keys each
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) sum[t][e] = 0.0f;
+            for (int e = 0; e < 16; ++e) {
+                sum[t][e] = 0.0f;
+                st[1][t][e] = -INFINITY;  // (none before the first)
+            }
         const uint32_t qAt = c32 * (HD * 2) + (h ^ swz(c32)) * 16;
+        float ofs[2] = {0.0f, 0.0f};
+        // What scores e and e + 16 j of rows rt give their keys.
+        auto weigh = [&](int rt, int at) {
+            const int t = at / 16, e = at % 16;
+            float v = sum[t][e] + __builtin_amdgcn_exp2f(fmaf(st[rt][t][e], c2, -ofs[rt]));
+            asm volatile("" : "+v"(v));  // here, beside the product
+            sum[t][e] = v;
+        };
+        // The scores of 32 rows, with the weights of the 32 before beside the products.
+        auto score = [&](uint32_t x, int rt) {
+            constexpr int kEach = 32 / (KS * 2) > 0 ? 32 / (KS * 2) : 1, kAhead = 4;
+            u32x4 q[kAhead];
+            auto read = [&](int i) {
+                return *reinterpret_cast<const u32x4 *>(smem + ((x ^ (i & 7) * 32u) + (i >> 3) * 256u + rt * (32 * HD * 2)));
+            };
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i) q[i] = read(i);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st[rt][t][e] = 0.0f;
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    st[rt][t] = pk::Mma<T>::run(kf[t][i], q[i % kAhead], st[rt][t]);
+                    if (t == 1 && i + kAhead < KS) q[i % kAhead] = read(i + kAhead);
+#pragma unroll
+                    for (int j = 0; j < kEach; ++j) weigh(1 - rt, (i * 2 + t) * kEach + j);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        };
+        // Hides what rows do not see, and rows that give nothing.
+        auto mask = [&](int rt, uint32_t first) {
+            const int posLo = c.req.pos0 + (int)token_of(first);
+            if (__ballot(ofs[rt] == INFINITY) == 0 && (p.maskKind == 2u || (int)key0 + 63 <= posLo)) return;
+            const int pos = ofs[rt] == INFINITY ? -1 : p.maskKind == 2u ? 0x7fffffff : c.req.pos0 + (int)token_of(min(first + c32, rows - 1));
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int key = (int)(key0 + t * 32 + (e >> 2) * 8 + h * 4 + (e & 3));
+                    st[rt][t][e] = key <= pos ? st[rt][t][e] : -INFINITY;
+                }
+        };
+        int last = 1;  // the rows whose weights are still to be taken
         for (uint32_t i = 0; i < n; ++i) {
-            const float of[2] = {next[0], next[1]};
-            wait_vmcnt<0>();
+            // this step's rows are in LDS, and every wave has read those that are copied over
+            wait_vmcnt<(int)(kPlaces - 2) * (kCopies + 1)>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            if (i + 1 < n) {
-                copy(i + 1);
-                ahead(i + 1);
-            }
+            copy(i + kPlaces - 1);
             if (key0 >= keys) continue;
-            uint32_t x = qAt + i % 2 * kStageBytes;
+            const uint32_t first = row0 + i * kStageRows, place = i % kPlaces;
+            uint32_t x = qAt + place * kStageBytes;
             asm volatile("" : "+v"(x));
+            // in base 2; infinity: the row gives nothing
+            auto logarithm = [&](int rt) {
+                const float v = *reinterpret_cast<const float *>(smem + kLse + (place * 4 + wave) * 256 + (rt * 32 + c32) * 4);
+                return v == -INFINITY || first + rt * 32 + c32 >= rows ? INFINITY : v * kLog2e;
+            };
+            ofs[0] = logarithm(0);
+            score(x, 0);
+            mask(0, first);
+            last = 0;
+            if (first + 32 >= rows) break;
+            ofs[1] = logarithm(1);
+            score(x, 1);
+            mask(1, first + 32);
+            last = 1;
+        }
+        if (last) {
 #pragma unroll
-            for (int rt = 0; rt < 2; ++rt) {
-                const uint32_t first = row0 + i * kStageRows + rt * 32;
-                if (first >= rows) break;
-                f32x16 st[2];
+            for (int e = 0; e < 32; ++e) weigh(1, e);
+        } else {
 #pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) st[t][e] = 0.0f;
-#pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    const u32x4 q = *reinterpret_cast<const u32x4 *>(smem + ((x ^ (s & 7) * 32u) + (s >> 3) * 256u + rt * (32 * HD * 2)));
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) st[t] = pk::Mma<T>::run(kf[t][s], q, st[t]);
-                }
-                const int posLo = c.req.pos0 + (int)token_of(first), pos = c.req.pos0 + (int)token_of(min(first + c32, rows - 1));
-                // a row that gives nothing, or one that does not see all keys
-                const bool hide = __ballot(of[rt] == INFINITY) != 0 || (p.maskKind != 2u && (int)key0 + 63 > posLo);
-                if (hide) {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int key = (int)(key0 + t * 32 + (e >> 2) * 8 + h * 4 + (e & 3));
-                            const bool seen = of[rt] != INFINITY && (p.maskKind == 2u || key <= pos);
-                            const float v = __builtin_amdgcn_exp2f(fmaf(st[t][e], c2, -of[rt]));
-                            sum[t][e] += seen ? v : 0.0f;
-                        }
-                } else {
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) sum[t][e] += __builtin_amdgcn_exp2f(fmaf(st[t][e], c2, -of[rt]));
-                }
-            }
+            for (int e = 0; e < 32; ++e) weigh(0, e);
         }
         // every wave has read its last rows before the next piece's copies
+        wait_vmcnt<0>();
         __builtin_amdgcn_s_waitcnt(0xC07F);
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -439,7 +488,7 @@ __device__ void weights_plain(const typename T::storage *__restrict__ Q, const t
         weights_few<T, HD, KM>(q, k, tables, starts, keyLens, lse, plan, weights, p, w);                                      \
     }
 #define WEIGHTS_TILE(t, T, HD)                                                                                                \
-    POPCORN_KERNEL void __launch_bounds__(256, 2)                                                                             \
+    POPCORN_KERNEL void __launch_bounds__(256, HD > 128 ? 1 : 2)                                                              \
         attention_weights_tile_##t##_d##HD(const T::storage *q, const T::storage *k, const int32_t *tables, const int32_t *starts, \
                                            const int32_t *keyLens, const float *lse, const pk::PagedTile *plan, float *partial, \
                                            WeightsBatch::Left *left, float *weights, PagedAttentionConstants p,               \

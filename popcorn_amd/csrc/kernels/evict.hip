@@ -16,134 +16,193 @@ __device__ inline uint32_t rank_key(float x) {
 
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kTile = 4096;  // weights of a block's pass, four in a row to a thread
+constexpr uint32_t kHeld = 4;     // passes whose weights a block holds in registers
 
-}  // namespace
+struct SelectSpace {
+    uint32_t bins[kBins], sums[16], found[2];
+};
 
-// A block per (request, KV head). The least kept weight by three counts of its bits (11, 11 and 10), then one pass in
-// order that numbers what is kept.
-POPCORN_KERNEL void __launch_bounds__(1024)
-    evict_select(const float *weights, const int32_t *keyLens, const int32_t *budgets, int32_t *kept, float *keptWeights, EvictConstants e) {
-    __shared__ uint32_t bins[kBins], sums[16], found[2];
-    const uint32_t tid = threadIdx.x, r = blockIdx.x / e.Nkv;
-    const uint64_t room = (uint64_t)e.columns * e.pageSize;
-    const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
-    const float *w = weights + blockIdx.x * room;
-    int32_t *to = kept + blockIdx.x * room;
-    float *toW = keptWeights + blockIdx.x * room;
-    for (uint64_t i = k.n + tid; i < room; i += 1024) toW[i] = 0.0f;
-    if (k.n == k.keys) {
-        for (uint32_t i = tid; i < k.n; i += 1024) {
-            to[i] = (int32_t)i;
-            toW[i] = w[i];
+// HELD: all weights are read once, into registers; else again for each count and for the choice.
+template <bool HELD>
+__device__ inline void select_kept(const float *__restrict__ w, const pk::EvictKeep &k, int32_t *__restrict__ to, float *__restrict__ toW,
+                                   SelectSpace &sp) {
+    const uint32_t tid = threadIdx.x, tiles = (k.keys + kTile - 1) / kTile;
+    struct Four {
+        float v[4];
+    };
+    auto read = [&](uint32_t tile) {
+        const uint32_t i = tile * kTile + tid * 4;
+        Four f{};
+        if (i + 4 <= k.keys) {
+            __builtin_memcpy(&f, w + i, sizeof(f));
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (i + j < k.keys) f.v[j] = w[i + j];
         }
-        return;
+        return f;
+    };
+    Four held[HELD ? kHeld : 1];
+    if constexpr (HELD) {
+#pragma unroll
+        for (uint32_t t = 0; t < kHeld; ++t) held[t] = read(t);
     }
+    auto each = [&](auto &&body) {  // body(tile, its four weights)
+        if constexpr (HELD) {
+#pragma unroll
+            for (uint32_t t = 0; t < kHeld; ++t)
+                if (t < tiles) body(t, held[t]);
+        } else {
+            Four next = read(0);
+            for (uint32_t t = 0; t < tiles; ++t) {
+                const Four f = next;
+                if (t + 1 < tiles) next = read(t + 1);
+                body(t, f);
+            }
+        }
+    };
     const uint32_t lo = k.first, hi = k.keys - k.last;  // between them `need` are kept
     uint32_t need = k.n - k.first - k.last, least = 0, shift = 32;
     for (int pass = 0; pass < 3 && need > 0; ++pass) {
         const uint32_t bits = pass < 2 ? 11u : 10u, above = shift;
         shift -= bits;
-        for (uint32_t b = tid; b < kBins; b += 1024) bins[b] = 0;
+        for (uint32_t b = tid; b < kBins; b += 1024) sp.bins[b] = 0;
         __syncthreads();
-        for (uint32_t i = lo + tid; i < hi; i += 1024) {
-            const uint32_t x = rank_key(w[i]);
-            if (above == 32 || x >> above == least >> above) atomicAdd(&bins[x >> shift & ((1u << bits) - 1)], 1u);
-        }
+        each([&](uint32_t t, const Four &f) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) {
+                const uint32_t i = t * kTile + tid * 4 + j, x = rank_key(f.v[j]);
+                if (i >= lo && i < hi && (above == 32 || x >> above == least >> above)) atomicAdd(&sp.bins[x >> shift & ((1u << bits) - 1)], 1u);
+            }
+        });
         __syncthreads();
         // from the highest bin down: the bin where the need is met
-        const uint32_t a = bins[kBins - 1 - 2 * tid], b = bins[kBins - 2 - 2 * tid];
-        const pk::Scan<uint32_t> s = pk::block_scan<16>(a + b, sums);
+        const uint32_t a = sp.bins[kBins - 1 - 2 * tid], b = sp.bins[kBins - 2 - 2 * tid];
+        const pk::Scan<uint32_t> s = pk::block_scan<16>(a + b, sp.sums);
         const uint32_t beforeA = s.upto - a - b, beforeB = beforeA + a;
         if (beforeA < need && need <= beforeB) {
-            found[0] = kBins - 1 - 2 * tid;
-            found[1] = need - beforeA;
+            sp.found[0] = kBins - 1 - 2 * tid;
+            sp.found[1] = need - beforeA;
         }
         if (beforeB < need && need <= s.upto) {
-            found[0] = kBins - 2 - 2 * tid;
-            found[1] = need - beforeB;
+            sp.found[0] = kBins - 2 - 2 * tid;
+            sp.found[1] = need - beforeB;
         }
         __syncthreads();
-        least |= found[0] << shift;
-        need = found[1];
+        least |= sp.found[0] << shift;
+        need = sp.found[1];
         __syncthreads();
     }
     // `need` of those at `least` are kept, the lowest indices; where none between is, nothing is above
     const bool none = k.n == k.first + k.last;
     uint32_t sure = 0, ties = 0;  // before this pass's tile
-    for (uint32_t base = 0; base < k.keys; base += kTile) {
+    each([&](uint32_t t, const Four &f) {
+        const uint32_t base = t * kTile + tid * 4;
         uint32_t count = 0;
         bool is[4], tie[4];
-        float v[4];
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t i = base + tid * 4 + j;
-            v[j] = i < k.keys ? w[i] : 0.0f;
-            const uint32_t x = rank_key(v[j]);
+            const uint32_t i = base + j, x = rank_key(f.v[j]);
             const bool between = i >= lo && i < hi;
             is[j] = i < k.keys && (!between || (!none && x > least));
-            tie[j] = i < k.keys && between && !none && x == least;
+            tie[j] = between && !none && x == least;
             count += (uint32_t)is[j] | (uint32_t)tie[j] << 16;
         }
-        const pk::Scan<uint32_t> s = pk::block_scan<16>(count, sums);
+        const pk::Scan<uint32_t> s = pk::block_scan<16>(count, sp.sums);
         uint32_t a = sure + ((s.upto - count) & 0xffffu), b = ties + ((s.upto - count) >> 16);
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
             if (is[j] || (tie[j] && b < need)) {
                 const uint32_t at = a + min(b, need);
-                to[at] = (int32_t)(base + tid * 4 + j);
-                toW[at] = v[j];
+                to[at] = (int32_t)(base + j);
+                toW[at] = f.v[j];
             }
             a += is[j];
             b += tie[j];
         }
         sure += s.total & 0xffffu;
         ties += s.total >> 16;
+    });
+}
+
+}  // namespace
+
+// A block per (request, KV head). The least kept weight by three counts of its bits (11, 11 and 10), then one pass in
+// order that numbers what is kept.
+POPCORN_KERNEL void __launch_bounds__(1024, 8)
+    evict_select(const float *weights, const int32_t *keyLens, const int32_t *budgets, int32_t *kept, float *keptWeights, EvictConstants e) {
+    __shared__ SelectSpace space;
+    const uint32_t tid = threadIdx.x, r = blockIdx.x / e.Nkv;
+    const uint64_t room = (uint64_t)e.columns * e.pageSize;
+    const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
+    const float *w = weights + blockIdx.x * room;
+    int32_t *to = kept + blockIdx.x * room;
+    float *toW = keptWeights + blockIdx.x * room;
+    if (k.n == k.keys) {
+        for (uint32_t i = tid; i < k.n; i += 1024) {
+            to[i] = (int32_t)i;
+            toW[i] = w[i];
+        }
+    } else if (k.keys <= kHeld * kTile) {
+        select_kept<true>(w, k, to, toW, space);
+    } else {
+        select_kept<false>(w, k, to, toW, space);
     }
+    for (uint64_t i = k.n + tid; i < room; i += 1024) toW[i] = 0.0f;
 }
 
 namespace {
 
-// A block takes 8 units of U (its slice) of the rows of one (request, KV head) in K or V. Row j becomes row kept[j] >= j, in chunks from
+// A block takes e.units units of U (its slice) of the rows of one (request, KV head) in K or V. Row j becomes row kept[j] >= j, in chunks from
 // the front: a chunk's rows are all read before one of them is written, and what later chunks read lies behind what it
 // writes (kept rises, so kept[j] >= j for them too).
 template <typename U>
 __device__ void evict_move(const int32_t *__restrict__ kept, const int32_t *__restrict__ tables, const int32_t *__restrict__ keyLens,
                            const int32_t *__restrict__ budgets, U *kCache, U *vCache, const EvictConstants &e) {
-    constexpr uint32_t kUnits = 8, kRows = 1024 / kUnits, kDeep = 8, kChunk = kRows * kDeep;
+    constexpr uint32_t kDeep = 4;
+    const uint32_t rows = 1024 / e.units, chunk = rows * kDeep;
     const uint32_t of = blockIdx.x, r = of / e.Nkv, hkv = of % e.Nkv;
     const pk::EvictKeep k = pk::evict_keep(keyLens[r], budgets[r], e);
     if (k.n == k.keys) return;
     const uint64_t room = (uint64_t)e.columns * e.pageSize;
     const int32_t *from = kept + of * room, *table = tables + (uint64_t)r * e.columns;
     U *cache = blockIdx.z ? vCache : kCache;
-    const uint32_t unit = blockIdx.y * kUnits + threadIdx.x % kUnits, row = threadIdx.x / kUnits;
+    const uint32_t unit = blockIdx.y * e.units + threadIdx.x % e.units, row = threadIdx.x / e.units;
     const bool mine = unit < e.rowUnits;
     auto place = [&](uint32_t i, uint64_t &at) {
         const uint32_t column = i / e.pageSize, page = (uint32_t)table[column];
         at = (((uint64_t)page * e.Nkv + hkv) * e.pageSize + (i - column * e.pageSize)) * e.rowUnits + unit;
         return page < e.pages;
     };
-    for (uint32_t base = k.first; base < k.n; base += kChunk) {
+    struct Rows {
         U v[kDeep];
-        uint64_t dst[kDeep];
+        uint64_t to[kDeep];
         bool moves[kDeep];
+    };
+    auto load = [&](uint32_t base, Rows &x) {
 #pragma unroll
         for (uint32_t d = 0; d < kDeep; ++d) {
-            const uint32_t j = base + d * kRows + row;
-            moves[d] = false;
+            const uint32_t j = base + d * rows + row;
+            x.moves[d] = false;
             if (j < k.n && mine) {
                 // (what is kept lies at or behind its place; a list that another call has left leads nowhere else)
                 const uint32_t i = min((uint32_t)from[j], k.keys - 1);
                 uint64_t src;
-                moves[d] = i > j && place(i, src) && place(j, dst[d]);
-                if (moves[d]) v[d] = cache[src];
+                x.moves[d] = i > j && place(i, src) && place(j, x.to[d]);
+                if (x.moves[d]) x.v[d] = cache[src];
             }
         }
+    };
+    Rows now, next;
+    load(k.first, now);
+    for (uint32_t base = k.first; base < k.n; base += chunk) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the rows have been read
         __syncthreads();
+        load(base + chunk, next);
 #pragma unroll
         for (uint32_t d = 0; d < kDeep; ++d)
-            if (moves[d]) cache[dst[d]] = v[d];
+            if (now.moves[d]) cache[now.to[d]] = now.v[d];
+        now = next;
     }
 }
 

@@ -397,7 +397,7 @@ public:
         int64_t longest = std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T);
         if (lastRows > 0) longest = std::min(longest, lastRows);
         // 16-bit keys of up to 256 dims, rows divided by G as the kernel does, and a step's rows within reach of one offset
-        if (q.dataType == DataType::f32 || hdp > 256 || longest * G <= kFewRows || G > 256 || (int64_t)64 * pc.Nq * pc.Hd >= (int64_t{1} << 29)) return;
+        if (q.dataType == DataType::f32 || hdp > 256 || !(pc.scale < 0.0f || pc.scale > 0.0f) || longest * G <= kFewRows || G > 256 || (int64_t)64 * pc.Nq * pc.Hd >= (int64_t{1} << 29)) return;
         tile_ = "attention_weights_tile_" + type + "_d" + std::to_string(hdp);
         few_ = pc.R > 1;
         wc_.manyRows = kFewRows;
@@ -406,9 +406,11 @@ public:
         const int64_t blocks = cdiv((int64_t)pc.columns * pc.pageSize, 256);
         work_.maxTiles = (uint32_t)std::min<int64_t>((int64_t)pc.R * blocks, INT32_MAX);
         work_.minSteps = 1;
-        work_.unitSteps = 3;
+        // A unit's start (its keys, the first rows) takes as long as about 10 steps. A prompt of 4096, 8192 tokens, 32 heads of 128 on 8,
+        // us: 98.9, 319; with 3 steps counted 108.6, 358; with 14 99.9, 311 (8 heads of 256 on 4: 64.9, 177; 67.6, 192; 68.2, 187).
+        work_.unitSteps = 10;
         const double steps = (double)work_.maxTiles * ((double)cdiv((int64_t)pc.T * G, 64) + work_.unitSteps);
-        work_.workers = (uint32_t)std::max(1.0, std::min(2.0 * deviceCUs(), steps * pc.Nkv));
+        work_.workers = (uint32_t)std::max(1.0, std::min((hdp > 128 ? 1.0 : 2.0) * deviceCUs(), steps * pc.Nkv));
         work_.ownPlan = work_.maxTiles <= 1024 && pc.R <= 1024 && steps < 2147483648.0;
     }
     std::vector<Binding> tensors() const override {
@@ -483,6 +485,11 @@ public:
         while (row % unit || !aligned(k.data, unit) || !aligned(v.data, unit)) unit /= 2;
         fn_ = "evict_move_b" + std::to_string(unit * 8);
         ec_.rowUnits = (uint32_t)(row / unit);
+        // A block's slice of the rows is 8 units, 128 bytes; narrower while that gives fewer blocks than CUs (one request of 4 heads of
+        // 256: 12 us, and 23 in slices of 8).
+        const int64_t rows = (int64_t)ec_.R * ec_.Nkv * 2;
+        ec_.units = 8;
+        while (ec_.units > 2 && rows * cdiv(ec_.rowUnits, ec_.units) < deviceCUs()) ec_.units /= 2;
     }
     std::vector<Binding> tensors() const override {
         return {{weights_, kRead}, {k_, kReadWrite}, {v_, kReadWrite}, {tables_, kRead}, {lens_, kRead}, {budgets_, kRead}, {kept_, kWrite}, {keptWeights_, kWrite}};
@@ -495,7 +502,7 @@ public:
                                     {bytesOf(ec_)}, dim3(rows, 1, 1), dim3(1024, 1, 1)));
         if (ec_.rowUnits == 0) return;
         enc.encode(*Kernels::Custom(fn_, {{kept_, kRead}, {tables_, kRead}, {lens_, kRead}, {budgets_, kRead}, {k_, kReadWrite}, {v_, kReadWrite}},
-                                    {bytesOf(ec_)}, dim3(rows, (ec_.rowUnits + 7) / 8, 2), dim3(1024, 1, 1)));
+                                    {bytesOf(ec_)}, dim3(rows, (ec_.rowUnits + ec_.units - 1) / ec_.units, 2), dim3(1024, 1, 1)));
     }
 
 private:
@@ -749,11 +756,11 @@ std::unique_ptr<Kernel> PagedEviction(const Tensor &weights, const Tensor &kCach
     requireShape(kept, D::i32, {R, Nkv, room}, op + " kept");
     requireShape(keptWeights, D::f32, {R, Nkv, room}, op + " kept_weights");
     requireGrid(R * Nkv, 1024, op, weights);
-    const int64_t slices = cdiv(kCache.shape[3] * stride(kCache.dataType), 16);
+    const int64_t slices = cdiv(kCache.shape[3] * stride(kCache.dataType), 4);  // (of 2 units of 2 bytes)
     if (slices > 65535) throw Error::tensorShapeMismatch(op + " rows are too long: " + kCache.shape.str() + ".");
     requireApart(op, {{&kCache, "k_cache"}, {&vCache, "v_cache"}, {&kept, "kept"}, {&keptWeights, "kept_weights"}},
                  {{&weights, "weights"}, {&pageTables, "page_tables"}, {&keyLens, "key_lens"}, {&budgets, "budgets"}});
-    const EvictConstants ec{(uint32_t)R, (uint32_t)Nkv, (uint32_t)M, (uint32_t)page, (uint32_t)kCache.shape[0], (uint32_t)first, (uint32_t)last, 0};
+    const EvictConstants ec{(uint32_t)R, (uint32_t)Nkv, (uint32_t)M, (uint32_t)page, (uint32_t)kCache.shape[0], (uint32_t)first, (uint32_t)last, 0, 8};
     return std::make_unique<EvictionKernel>(weights, kCache, vCache, pageTables, keyLens, budgets, kept, keptWeights, ec);
 }
 
@@ -773,7 +780,7 @@ std::unique_ptr<Kernel> ReleasePages(const Tensor &keyLens, const Tensor &budget
     requireShape(counts, D::i32, {1}, op + " counts");
     requireApart(op, {{&newLens, "new_lens"}, {&freed, "freed"}, {&counts, "counts"}},
                  {{&keyLens, "key_lens"}, {&budgets, "budgets"}, {&pageTables, "page_tables"}});
-    const EvictConstants ec{(uint32_t)R, 1, (uint32_t)M, (uint32_t)pageSize, 0, 0, 0, 0};
+    const EvictConstants ec{(uint32_t)R, 1, (uint32_t)M, (uint32_t)pageSize, 0, 0, 0, 0, 0};
     const int64_t blocks = std::clamp<int64_t>(cdiv(R, 16), 1, 256);
     return fixed("release_pages", {{keyLens, kRead}, {budgets, kRead}, {pageTables, kRead}, {newLens, kWrite}, {freed, kWrite}, {counts, kWrite}},
                  bytesOf(ec), dim3((unsigned)blocks, 1, 1), 256);
