@@ -192,7 +192,7 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
 constexpr uint32_t kKeys = 256, kStageRows = 64;
 
 struct WeightsBatch {
-    static constexpr bool kShared = false;
+    static constexpr bool kShared = false, kPlanned = false;
     using Request = pk::PagedRequest;
     struct Left {  // a unit that its block shares with others behind it
         uint32_t pieces, request, hkv, key0;
@@ -249,7 +249,7 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
     const uint32_t inverse = G == 1 ? 0u : (uint32_t)((0x100000000ull + G - 1) / G), single = G == 1 ? ~0u : 0u;
     auto token_of = [&](uint32_t row) { return __umulhi(row, inverse) + (row & single); };
     const WeightsBatch batch{starts, keyLens, left, a};
-    Dealer<256, WeightsBatch> dealer(batch, plan, sm_plan, *reinterpret_cast<Space *>(smem), p, w);
+    Dealer<256, WeightsBatch> dealer(batch, plan, sm_plan, reinterpret_cast<Space *>(smem), p, w);
     Piece<pk::PagedRequest> c;
     while (dealer.next(c, p, w)) {
         const int32_t *table = tables + (uint64_t)c.request * p.columns;

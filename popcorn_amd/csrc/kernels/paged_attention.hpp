@@ -222,7 +222,8 @@ struct Shared {
 // PagedAttention: every request's new tokens against its own pages. A unit that one worker has whole goes to `out`, of the others
 // the worker that begins one leaves a Shared to the merge.
 struct OwnPages {
-    static constexpr bool kShared = false;
+    static constexpr bool kShared = false;   // states of all units go to records, not to a Shared
+    static constexpr bool kPlanned = false;  // the plan is always in memory, and LDS is the caller's
     using Request = pk::PagedRequest;
     using Left = Shared;
     struct More {};
@@ -256,8 +257,8 @@ struct OwnPages {
     }
 };
 
-// Deals a block of NT threads its pieces.
-template <uint32_t NT, typename Batch>
+// Deals its pieces to a worker: a block of NT threads, or with `Wave` each of its waves.
+template <uint32_t NT, typename Batch, bool Wave = false>
 struct Dealer {
     const Batch batch;
     const pk::PagedTile *plan;
@@ -266,15 +267,23 @@ struct Dealer {
     uint64_t share, x, end;
     uint32_t tile;
 
+    __device__ static inline uint32_t block(const Batch &b) {
+        if constexpr (Batch::kPlanned) return blockIdx.x - b.firstBlock;
+        else return blockIdx.x;
+    }
+    __device__ inline uint32_t worker() const { return Wave ? block(batch) * (NT / 64) + first_lane(threadIdx.x >> 6) : block(batch); }
+
+    using Space = PlanSpace<NT, uint32_t, typename Batch::Request>;
+
     // `space` is free again afterwards.
-    __device__ inline Dealer(const Batch &b, const pk::PagedTile *pl, OwnTile *ow, PlanSpace<NT, uint32_t, typename Batch::Request> &space,
-                             const PagedAttentionConstants &p, const PagedWorkConstants &w)
-        : batch(b), plan(pl), own(ow), left(b.left + blockIdx.x) {
+    __device__ inline Dealer(const Batch &b, const pk::PagedTile *pl, OwnTile *ow, Space *space, const PagedAttentionConstants &p,
+                             const PagedWorkConstants &w)
+        : batch(b), plan(pl), own(ow), left(b.left + worker()) {
         uint32_t tiles;
         uint64_t total;
-        if (w.ownPlan) {
+        if (!Batch::kPlanned && w.ownPlan) {
             uint32_t steps;
-            lay_tiles<NT, uint32_t>(batch, space, p, w, steps, tiles, [&](uint32_t at, uint32_t before, uint32_t request, uint32_t t) {
+            lay_tiles<NT, uint32_t>(batch, *space, p, w, steps, tiles, [&](uint32_t at, uint32_t before, uint32_t request, uint32_t t) {
                 ow[at] = OwnTile{before, request << 16 | t};
             });
             total = (uint64_t)first_lane(steps) * p.Nkv;
@@ -284,10 +293,10 @@ struct Dealer {
             tiles = plan[0].request;
         }
         share = pk::paged_share(total, w);
-        x = first_lane64(blockIdx.x * share);
+        x = first_lane64(worker() * share);
         end = first_lane64(min(x + share, total));
         if (x < end) {
-            tile = w.ownPlan ? find_tile(tiles, x >> 32 ? x / p.Nkv : (uint32_t)x / p.Nkv, [&](uint32_t i) { return own[i].before; })
+            tile = !Batch::kPlanned && w.ownPlan ? find_tile(tiles, x >> 32 ? x / p.Nkv : (uint32_t)x / p.Nkv, [&](uint32_t i) { return own[i].before; })
                              : find_tile(tiles, x >> 32 ? x / p.Nkv : (uint32_t)x / p.Nkv, [&](uint32_t i) { return plan[1 + i].before; });
         } else if (threadIdx.x == 0) {
             if constexpr (!Batch::kShared) batch.idle(left);
@@ -298,7 +307,7 @@ struct Dealer {
     __device__ inline bool next(Piece<typename Batch::Request> &c, const PagedAttentionConstants &p, const PagedWorkConstants &w) {
         while (x < end) {
             pk::PagedTile t;
-            if (w.ownPlan) {
+            if (!Batch::kPlanned && w.ownPlan) {
                 const OwnTile o = own[tile];
                 t = pk::PagedTile{first_lane(o.before), first_lane(o.place >> 16), first_lane(o.place & 0xffffu)};
             } else {
@@ -308,6 +317,7 @@ struct Dealer {
             c.request = t.request;
             c.tile = t.tile;
             c.req = batch.request(t.request, p);
+            if constexpr (Batch::kShared) c.req = Batch::uniform(c.req);
             c.steps = batch.steps(c.req, t.tile, p, w);
             const pk::PagedPiece piece = pk::paged_piece(x - t.before * p.Nkv, end - x, c.steps.n, w);
             c.hkv = piece.hkv;
@@ -316,7 +326,7 @@ struct Dealer {
             x += piece.taken;
             if (piece.behind == 0 && c.hkv + 1 == p.Nkv) ++tile;
             if constexpr (Batch::kShared) {
-                c.sharers = x == end ? pk::paged_sharers(piece, c.steps.n, end, share, blockIdx.x) : 0u;
+                c.sharers = x == end ? pk::paged_sharers(piece, c.steps.n, end, share, worker()) : 0u;
             } else if (x == end && threadIdx.x == 0) {
                 batch.close(left, c, pk::paged_sharers(piece, c.steps.n, end, share, blockIdx.x), w);
             }
@@ -354,13 +364,15 @@ __device__ inline void store4(typename T::storage *dst, const pk::f32x4 &o, floa
 // sides where the kernel is chosen).
 // A piece's partial state goes to one of its worker's two slots: 2 w + 1 if
 // the piece begins its unit, else 2 w.
-template <typename T, int HD, int RT, typename Batch>
+// With WAVES 1 each wave is a worker and takes all steps of its pieces: no wave
+// waits for another one.
+template <typename T, int HD, int RT, typename Batch, int WAVES = kWaves>
 __device__ void paged_few(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
                           const typename T::storage *__restrict__ V, const int32_t *__restrict__ tables,
                           const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
                           const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
                           typename Batch::Left *__restrict__ left, typename T::storage *__restrict__ out, const PagedAttentionConstants &all,
-                          const PagedWorkConstants &w, const typename Batch::More &more) {
+                          const PagedWorkConstants &w, const typename Batch::More &more, uint8_t *lds = nullptr) {
     using S = typename T::storage;
     constexpr bool kWide = sizeof(S) == 4;
     constexpr int KM = kWide ? 1 : 2;          // 16-key groups per step
@@ -373,8 +385,10 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     constexpr int kParts = kWide ? 1 : 2;
     constexpr float kLead = std::is_same<T, pk::F16>::value ? 4.0f : 0.0f;  // max over reference when it moves
     constexpr int LDO = HD + 4;                // merged-state row, in floats
-    constexpr int kStage = kWaves * BKV * HD * (int)sizeof(S), kMerge = kWaves * 16 * LDO * 4;
-    __shared__ __attribute__((aligned(16))) uint8_t smem[kStage > kMerge ? kStage : kMerge];
+    constexpr int kStage = kWaves * BKV * HD * (int)sizeof(S), kMerge = WAVES == 1 ? 0 : kWaves * 16 * LDO * 4;
+    constexpr int kSmem = kStage > kMerge ? kStage : kMerge;
+    __shared__ __attribute__((aligned(16))) uint8_t sm_own[Batch::kPlanned ? 16 : kSmem];
+    uint8_t *const smem = Batch::kPlanned ? lds : sm_own;
     __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
     __shared__ OwnTile sm_plan[kOwnTiles];
     __shared__ uint32_t sm_bad;
@@ -385,14 +399,15 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     constexpr bool kQAgain = HD == 512 && kWide;
     __shared__ __attribute__((aligned(16))) u32x4 sm_q[kQInLds ? KS * 64 : 1];
     using Space = PlanSpace<64 * kWaves, uint32_t, typename Batch::Request>;
-    static_assert(sizeof(Space) <= sizeof(smem), "the plan is laid out where V goes");
+    static_assert(sizeof(Space) <= kSmem, "the plan is laid out where V goes");
+    static_assert(WAVES == kWaves || (WAVES == 1 && !kQInLds), "a worker is a block or a wave");
 
     const uint32_t lane = threadIdx.x & 63, g = lane >> 4, c16 = lane & 15;
-    const uint32_t wave = first_lane(threadIdx.x >> 6);
+    const uint32_t wave = first_lane(threadIdx.x >> 6), member = WAVES == 1 ? 0u : wave;
     const uint32_t D = all.Hd, G = all.Nq / all.Nkv;
     const float c2 = all.scale * kLog2e;
     const Batch batch{tables, starts, keyLens, left, more};
-    Dealer<64 * kWaves, Batch> dealer(batch, plan, sm_plan, *reinterpret_cast<Space *>(smem), all, w);
+    Dealer<64 * kWaves, Batch, WAVES == 1> dealer(batch, plan, sm_plan, reinterpret_cast<Space *>(smem), all, w);
     Piece<typename Batch::Request> c;
     while (dealer.next(c, all, w)) {
         decltype(auto) p = batch.mask(c.req, all);
@@ -421,13 +436,13 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         }
         if constexpr (kQInLds) __syncthreads();
 
-        // The wave's steps are c.lo + wave + kWaves i. Lane l holds page and row in it
+        // The wave's steps are c.lo + member + WAVES i. Lane l holds page and row in it
         // of group l % KM of the wave's step `page0` + l / KM; a group that no
         // page holds has none (-1): its keys are left out and read as zeros.
         constexpr uint32_t kHeld = 64 / KM;
         uint32_t page0 = 0, heldPage = 0, heldRow = 0;
         auto hold = [&](uint32_t i) {
-            const uint32_t step = c.lo + wave + kWaves * (i + lane / KM);
+            const uint32_t step = c.lo + member + WAVES * (i + lane / KM);
             page0 = i;
             heldPage = ~0u;
             heldRow = 0;
@@ -500,8 +515,8 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
 
         hold(0);
         uint32_t i = 0;
-        loadK(0, c.lo + wave);
-        for (uint32_t step = c.lo + wave; step < c.hi; step += kWaves, ++i) {
+        loadK(0, c.lo + member);
+        for (uint32_t step = c.lo + member; step < c.hi; step += WAVES, ++i) {
             const uint32_t k0 = pk::paged_step_key(c.steps, step, w);
             bool ok[KM];
 #pragma unroll
@@ -554,7 +569,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
             }
             __builtin_amdgcn_sched_barrier(0);
             if (i + 1 - page0 == kHeld) hold(i + 1);
-            loadK(i + 1, step + kWaves);
+            loadK(i + 1, step + WAVES);
             __builtin_amdgcn_sched_barrier(0);
             float pw[RT][4 * KM];
             u32x4 pf[RT][kParts];
@@ -640,6 +655,66 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         }
         wait_vmcnt<0>();  // the last K loads (zeros), before their registers go
 
+        if constexpr (WAVES == 1) {  // lane (g, c16): row c16, dims 4 g + 16 dt
+            const bool whole = c.lo == 0 && c.hi == c.steps.n;
+            const uint64_t slot = w.stateBase + (2 * (uint64_t)dealer.worker() + (c.lo == 0)) * (RT * 16);
+            const uint32_t td = lane % 16 * 4;
+            const bool direct = batch.begin(c, whole, q_row, w, dealer.worker(), lane, 64);
+            auto state = [&](uint32_t r) { return whole ? batch.own_row(c.req, q_row(r)) : slot + r - c.steps.r0; };
+            auto store = [&](uint32_t r, uint32_t d, const pk::f32x4 &o, float L) {
+                if (direct) store4<T>(out + q_row(r) * D + d, o, L);
+                else *reinterpret_cast<pk::f32x4 *>(pO + state(r) * HD + d) = o;
+            };
+            auto storeML = [&](uint32_t r, float M, float L) {
+                if (direct) batch.store_lse(q_row(r), M, L);
+                else *reinterpret_cast<float2 *>(pML + 2 * state(r)) = float2{M, L};
+            };
+            bool bad = false;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const uint32_t r = c.steps.r0 + rt * 16 + c16;
+                if (r < c.steps.r1) {
+                    bad |= !(fabsf(l[rt]) < INFINITY);
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+                        if (dt * 16 + g * 4 < D) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) bad |= !(fabsf(acc[rt][dt][e]) < INFINITY);
+                            store(r, dt * 16 + g * 4, acc[rt][dt], l[rt]);
+                        }
+                    if (g == 0) storeML(r, m[rt], l[rt]);
+                }
+            }
+            if (__ballot(bad)) {
+                wait_vmcnt<0>();  // the rows' stores, before other lanes store them again
+                // as below: an infinity or NaN in V that a row does not see
+                const uint32_t s0 = min(c.lo, c.steps.sinks), s1 = min(c.hi, c.steps.sinks);
+                const uint32_t t0 = max(c.lo, c.steps.sinks), t1 = max(c.hi, c.steps.sinks);
+                auto key_at = [&](uint32_t k) { return (int)min(k * w.stepKeys, keys); };
+                for (uint32_t r = c.steps.r0 + lane / 16; r < c.steps.r1; r += 4) {
+                    constexpr int NJ = HD / 64;
+                    pk::f32x4 qv[NJ], o[NJ];
+                    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        o[j] = qv[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (td + 64 * j < D)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) qv[j][e] = T::load(Q[q_row(r) * D + td + 64 * j + e]);
+                    }
+                    const int pos = batch.pos(c.req, r, G);
+                    paged_row<T, NJ, true, 1>(qv, K, V, table, c.hkv, pos, key_at(s0), key_at(s1), p, o, M, L);
+                    paged_row<T, NJ, true, 1>(qv, K, V, table, c.hkv, pos, key_at(t0 - c.steps.sinks + c.steps.first),
+                                           key_at(t1 - c.steps.sinks + c.steps.first), p, o, M, L);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+                        if (td + 64 * j < D) store(r, td + 64 * j, o[j], L);
+                    if (td == 0) storeML(r, M, L);
+                }
+            }
+            continue;
+        }
+
         // merge the waves' states, one tile of 16 rows at a time: O through LDS,
         // thread t takes row t / 16, dims 4 (t % 16) + 64 j
         if (g == 0) {
@@ -655,7 +730,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
         const bool whole = c.lo == 0 && c.hi == c.steps.n;
         const uint64_t slot = w.stateBase + (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * (RT * 16);
         bool direct = whole;
-        if constexpr (Batch::kShared) direct = batch.begin(c, whole, q_row, p, w);
+        if constexpr (Batch::kShared) direct = batch.begin(c, whole, q_row, w, dealer.worker(), threadIdx.x, 256);
         auto state = [&](uint32_t r) {
             if constexpr (Batch::kShared) return whole ? batch.own_row(c.req, q_row(r)) : slot + r - c.steps.r0;
             else return slot + r - c.steps.r0;
@@ -756,7 +831,7 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
                            const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
                            const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
                            typename Batch::Left *__restrict__ left, typename T::storage *__restrict__ out, const PagedAttentionConstants &all,
-                           const PagedWorkConstants &w, const typename Batch::More &more) {
+                           const PagedWorkConstants &w, const typename Batch::More &more, uint8_t *lds = nullptr) {
     using S = typename T::storage;
     constexpr int BKV = 64, KS = HD / 16, DT = HD / 32, CH = HD / 8;
     constexpr int kRowsPer = 64 / CH;       // rows per copy instruction
@@ -768,7 +843,8 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
     constexpr float kLead = kTwo ? 0.0f : 4.0f;
     constexpr uint32_t kTileBytes = BKV * HD * 2;
     // K's two places, V's two, the plan (one array: with two, the compiler has every read of LDS wait for the latest copy)
-    __shared__ __attribute__((aligned(256))) uint8_t smem[4 * kTileBytes + kOwnTiles * sizeof(OwnTile)];
+    __shared__ __attribute__((aligned(256))) uint8_t sm_own[Batch::kPlanned ? 16 : 4 * kTileBytes + kOwnTiles * sizeof(OwnTile)];
+    uint8_t *const smem = Batch::kPlanned ? lds : sm_own;
     using Space = PlanSpace<256, uint32_t, typename Batch::Request>;
     static_assert(sizeof(Space) <= 4 * kTileBytes, "the plan is laid out where K and V go");
     OwnTile *sm_plan = reinterpret_cast<OwnTile *>(smem + 4 * kTileBytes);
@@ -782,7 +858,7 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
     auto swzV = [](uint32_t row) { return CH >= 16 ? row % 4u * 4u : row / 2u % 2u * 4u; };
 
     const Batch batch{tables, starts, keyLens, left, more};
-    Dealer<256, Batch> dealer(batch, plan, sm_plan, *reinterpret_cast<Space *>(smem), all, w);
+    Dealer<256, Batch> dealer(batch, plan, sm_plan, reinterpret_cast<Space *>(smem), all, w);
     Piece<typename Batch::Request> c;
     while (dealer.next(c, all, w)) {
         decltype(auto) p = batch.mask(c.req, all);
@@ -1074,9 +1150,9 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
         asm volatile("" ::: "memory");
 
         const bool whole = c.lo == 0 && c.hi == c.steps.n;
-        const uint64_t slot = w.stateBase + (2 * (uint64_t)blockIdx.x + (c.lo == 0)) * kTileRows;
+        const uint64_t slot = w.stateBase + (2 * (uint64_t)dealer.worker() + (c.lo == 0)) * kTileRows;
         bool direct = whole;
-        if constexpr (Batch::kShared) direct = batch.begin(c, whole, q_row, p, w);
+        if constexpr (Batch::kShared) direct = batch.begin(c, whole, q_row, w, dealer.worker(), threadIdx.x, 256);
         auto state = [&](uint32_t r) {
             if constexpr (Batch::kShared) return whole ? batch.own_row(c.req, q_row(r)) : slot + r - c.steps.r0;
             else return slot + r - c.steps.r0;

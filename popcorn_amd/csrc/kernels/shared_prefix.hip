@@ -22,23 +22,61 @@ __device__ inline uint32_t wave_span_of(const int32_t *at, uint32_t n, int32_t x
     return x < at[a + 1] ? a : n;
 }
 
+// The groups of a call, a lane of every wave for each where there are up to 64 (else read where they are asked for): a unit's
+// group would take loads that wait for each other. Not in LDS: beside another array there the compiler has every read of LDS wait
+// for the latest copy into it (64 requests behind 8192 keys: 95 us, and 65).
+struct HeldGroups {
+    int32_t end, len, first;  // of the lane's group; first: where group 0 begins, in every lane
+    uint32_t n;
+
+    __device__ inline HeldGroups(const int32_t *groupStarts, const int32_t *prefixLens, const SharedPrefixConstants &s) {
+        const uint32_t lane = threadIdx.x & 63;
+        n = s.groups <= 64 ? s.groups : 0u;
+        end = lane < n ? groupStarts[lane + 1] : 0;
+        len = lane < n ? prefixLens[lane] : 0;
+        first = n ? groupStarts[0] : 0;
+    }
+    // Keys of the prefix of request r's group.
+    __device__ inline int32_t before(int32_t r) const {
+        int32_t from = first, keys = 0;
+        for (uint32_t g = 0; g < n; ++g) {
+            const int32_t to = __builtin_amdgcn_readlane(end, (int)g);
+            if (from <= r && r < to) keys = __builtin_amdgcn_readlane(len, (int)g);
+            from = to;
+        }
+        return keys;
+    }
+};
+
+template <bool Planned>
 struct SharedPages {
-    static constexpr bool kShared = true;
+    static constexpr bool kShared = true, kPlanned = Planned;
     using Request = pk::SharedRequest;
     using Left = pk::u32x4;  // the rows' records, of prefixes and then of own keys
     struct More {
         const int32_t *prefixTables, *prefixLens, *groupStarts;
         const int32_t *positions;  // under a window: of each token, then each group's least
         float *lse;
+        const HeldGroups &held;
         const SharedPrefixConstants &s;
+        uint32_t firstBlock;  // of a launch's blocks, the first that takes this work
     };
     const int32_t *tables, *starts, *keyLens;
     Left *left;
     const More &more;
+    const uint32_t firstBlock = more.firstBlock;
 
     __device__ inline uint32_t requests(const PagedAttentionConstants &p) const { return more.s.groups + p.R; }
     __device__ inline Request request(uint32_t v, const PagedAttentionConstants &p) const {
-        return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, more.s);
+        const SharedPrefixConstants &s = more.s;
+        if (s.groups > 64) return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, s);
+        Request q{};
+        q.prefix = v < s.groups;
+        if (q.prefix) return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, s);
+        const uint32_t r = v - s.groups;
+        static_cast<pk::PagedRequest &>(q) = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
+        q.before = pk::paged_prefix_keys(more.held.before((int32_t)r), p, s);
+        return q;
     }
     __device__ inline PagedAttentionConstants mask(const Request &q, const PagedAttentionConstants &p) const { return pk::paged_shared_mask(q, p); }
     __device__ inline uint32_t tiles(const Request &q, uint32_t G, const PagedWorkConstants &w) const { return row_tiles(q, G, w); }
@@ -64,16 +102,30 @@ struct SharedPages {
         hi = (int)first_lane((uint32_t)hi);
     }
 
+    // The same request, in scalar registers. (Where the compiler took its keys for the lanes' own, each load through a descriptor
+    // became a loop over the lanes' descriptors: 256 requests of 20 to 800 own keys 50 us, and KEPT.)
+    __device__ static inline Request uniform(const Request &q) {
+        Request u;
+        u.start = (int32_t)first_lane((uint32_t)q.start);
+        u.n = (int32_t)first_lane((uint32_t)q.n);
+        u.pos0 = (int32_t)first_lane((uint32_t)q.pos0);
+        u.keys = (int32_t)first_lane((uint32_t)q.keys);
+        u.prefix = first_lane(q.prefix) != 0;
+        u.before = (int32_t)first_lane((uint32_t)q.before);
+        u.lo = (int32_t)first_lane((uint32_t)q.lo);
+        return u;
+    }
     // Where a unit's state goes that one worker has whole.
     __device__ inline uint64_t own_row(const Request &q, uint64_t row) const { return more.s.rowBase + (q.prefix ? 0u : more.s.rows) + row; }
     // Of a piece that begins its unit: the rows' records. True where the piece is all that its rows have: they go to `out`.
     template <typename Row>
-    __device__ inline bool begin(const Piece<Request> &c, bool whole, Row &&row, const PagedAttentionConstants &p, const PagedWorkConstants &w) const {
+    __device__ inline bool begin(const Piece<Request> &c, bool whole, Row &&row, const PagedWorkConstants &w, uint32_t worker, uint32_t thread,
+                                 uint32_t threads) const {
         const bool direct = whole && !c.req.prefix && c.req.before == 0;
         if (c.lo != 0) return false;
-        for (uint32_t r = c.steps.r0 + threadIdx.x; r < c.steps.r1; r += 256) {
+        for (uint32_t r = c.steps.r0 + thread; r < c.steps.r1; r += threads) {
             const uint64_t at = row(r);
-            const uint32_t next = w.stateBase + 2 * blockIdx.x * w.rows + (r - c.steps.r0);
+            const uint32_t next = w.stateBase + 2 * worker * w.rows + (r - c.steps.r0);
             left[(c.req.prefix ? 0u : more.s.rows) + at] =
                 whole ? pk::u32x4{(uint32_t)own_row(c.req, at), 0u, 0u, direct ? 0u : 1u} : pk::u32x4{next + w.rows, next, 2 * w.rows, c.sharers};
         }
@@ -84,60 +136,89 @@ struct SharedPages {
     }
 };
 
-}  // namespace
-
-POPCORN_KERNEL void __launch_bounds__(1024)
-    shared_prefix_plan(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
-                       const int32_t *positions, pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants w,
-                       SharedPrefixConstants s) {
-    __shared__ PlanSpace<1024, u64, SharedPages::Request> space;
-    u64 steps;
-    uint32_t tiles;
-    const SharedPages::More more{nullptr, prefixLens, groupStarts, positions, nullptr, s};
-    const SharedPages batch{nullptr, starts, keyLens, nullptr, more};
-    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) {
-        plan[1 + at] = pk::PagedTile{before, request, tile};
-    });
-    if (threadIdx.x == 0) plan[0] = pk::PagedTile{steps, tiles, 0};
-}
-
-// Under a window: each token's position (behind its group's prefix; a token that its request's keys do not hold counts as the
-// first behind it), and behind the tokens each group's least. A block's threads take tokens, or the blocks past them one group.
-POPCORN_KERNEL void __launch_bounds__(256)
-    shared_prefix_positions(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
-                            int32_t *positions, PagedAttentionConstants p, SharedPrefixConstants s) {
-    const uint32_t tokenBlocks = (p.T + 255) / 256;
-    if (blockIdx.x < tokenBlocks) {
-        const uint32_t t = blockIdx.x * 256 + threadIdx.x;
-        if (t >= p.T) return;
-        const uint32_t r = pk::paged_span_of(starts, p.R, (int32_t)t);
-        int32_t pos = 0;
-        if (r < p.R) {
-            const uint32_t g = pk::paged_span_of(groupStarts, s.groups, (int32_t)r);
-            const pk::PagedRequest q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
-            pos = pk::paged_place(q, (int32_t)t, g < s.groups ? pk::paged_prefix_keys(prefixLens[g], p, s) : 0);
-        }
-        positions[t] = pos;
-        return;
-    }
-    __shared__ int32_t sLeast[4];
-    const uint32_t g = blockIdx.x - tokenBlocks;
-    if (g >= s.groups) return;
+// Under a window, a group's least position, by one wave; and a token's position (behind its group's prefix; a token that its
+// request's keys do not hold counts as the first behind it).
+__device__ inline int32_t group_least(uint32_t g, const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
+                                      const PagedAttentionConstants &p, const SharedPrefixConstants &s) {
     const int32_t a = min(max(groupStarts[g], 0), (int32_t)p.R), b = min(max(groupStarts[g + 1], a), (int32_t)p.R);
     int32_t least = 0x7fffffff;
-    for (int32_t r = a + (int32_t)threadIdx.x; r < b; r += 256) {
+    for (int32_t r = a + (int32_t)(threadIdx.x & 63); r < b; r += 64) {
         const pk::PagedRequest q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
         if (q.n > 0) least = min(least, pk::paged_place(q, q.start, pk::paged_prefix_keys(prefixLens[g], p, s)));
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) least = min(least, __shfl_xor(least, d));
-    if ((threadIdx.x & 63) == 0) sLeast[threadIdx.x >> 6] = least;
-    __syncthreads();
-    if (threadIdx.x != 0) return;
-    positions[p.T + g] = min(min(sLeast[0], sLeast[1]), min(sLeast[2], sLeast[3]));
+    return least;
+}
+
+__device__ inline void token_position(uint32_t t, const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens,
+                                      const int32_t *groupStarts, int32_t *positions, const PagedAttentionConstants &p,
+                                      const SharedPrefixConstants &s) {
+    if (t >= p.T) return;
+    const uint32_t r = pk::paged_span_of(starts, p.R, (int32_t)t);
+    int32_t pos = 0;
+    if (r < p.R) {
+        const uint32_t g = pk::paged_span_of(groupStarts, s.groups, (int32_t)r);
+        const pk::PagedRequest q = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
+        pos = pk::paged_place(q, (int32_t)t, g < s.groups ? pk::paged_prefix_keys(prefixLens[g], p, s) : 0);
+    }
+    positions[t] = pos;
+}
+
+}  // namespace
+
+// Block 0 lays out the tiles of many rows, block 1 those of few (of the few-row kernel alone there is just block 0: many is few). Each
+// plan's entry 0: the counted steps, the number of tiles. Under a window both write each group's least position first, behind the
+// tokens' positions, which the blocks behind them write.
+POPCORN_KERNEL void __launch_bounds__(1024)
+    shared_prefix_plan(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts, int32_t *positions,
+                       pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {
+    if (blockIdx.x > 1) {
+        token_position((blockIdx.x - 2) * 1024 + threadIdx.x, starts, keyLens, prefixLens, groupStarts, positions, p, s);
+        return;
+    }
+    __shared__ PlanSpace<1024, u64, pk::SharedRequest> space;
+    if (s.windowed) {
+        for (uint32_t g = threadIdx.x >> 6; g < s.groups; g += 16) {
+            const int32_t least = group_least(g, starts, keyLens, prefixLens, groupStarts, p, s);
+            if ((threadIdx.x & 63) == 0) positions[p.T + g] = least;
+        }
+        __threadfence_block();
+        __syncthreads();
+    }
+    const HeldGroups held(groupStarts, prefixLens, s);
+    using Pages = SharedPages<true>;
+    const Pages::More more{nullptr, prefixLens, groupStarts, positions, nullptr, held, s, 0};
+    const Pages batch{nullptr, starts, keyLens, nullptr, more};
+    u64 steps;
+    uint32_t tiles;
+    const PagedWorkConstants w = blockIdx.x ? few : many;
+    pk::PagedTile *to = plan + (blockIdx.x ? many.maxTiles + 1 : 0u);
+    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles,
+                         [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) { to[1 + at] = pk::PagedTile{before, request, tile}; });
+    if (threadIdx.x == 0) to[0] = pk::PagedTile{steps, tiles, 0};
+}
+
+// The same for the few-row kernel alone, which lays out its plan by itself: blocks take tokens, or those past them four groups.
+POPCORN_KERNEL void __launch_bounds__(256)
+    shared_prefix_positions(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
+                            int32_t *positions, PagedAttentionConstants p, SharedPrefixConstants s) {
+    const uint32_t tokenBlocks = (p.T + 255) / 256;
+    if (blockIdx.x < tokenBlocks) return token_position(blockIdx.x * 256 + threadIdx.x, starts, keyLens, prefixLens, groupStarts, positions, p, s);
+    const uint32_t g = (blockIdx.x - tokenBlocks) * 4 + (threadIdx.x >> 6);
+    if (g >= s.groups) return;
+    const int32_t least = group_least(g, starts, keyLens, prefixLens, groupStarts, p, s);
+    if ((threadIdx.x & 63) == 0) positions[p.T + g] = least;
 }
 
 namespace {
+
+// The launch's blocks are shared out by the counted steps, a wave's counted a quarter of a block's.
+__device__ inline uint32_t tile_blocks(u64 many, u64 few) {
+    const u64 fewSteps = first_lane64((few + 3) / 4), all = first_lane64(many) + fewSteps;
+    const uint32_t blocks = all ? (uint32_t)((gridDim.x * fewSteps + all - 1) / all) : 0u;
+    return first_lane(gridDim.x - (many ? min(blocks, gridDim.x - 1) : blocks));
+}
 
 // A row's pieces, of its prefix and of its own keys, by one wave or the block's four (s.parts): their maximum and sum first,
 // a lane for a piece, then their O, HD / 4 lanes for a piece.
@@ -226,7 +307,7 @@ __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *_
 // keys in turn, of the prefix and then of the row's own.
 template <typename T, bool VEC>
 __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
-                                    const typename T::storage *__restrict__ V, const SharedPages &batch, typename T::storage *__restrict__ out,
+                                    const typename T::storage *__restrict__ V, const SharedPages<false> &batch, typename T::storage *__restrict__ out,
                                     const PagedAttentionConstants &p) {
     constexpr int NJ = 8;
     __shared__ float sO[16][NJ * 64], sM[16], sL[16];
@@ -247,11 +328,11 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
             if (td + 64 * j + i < p.Hd) q[j][i] = T::load(qr[td + 64 * j + i]);
     }
     float m = -INFINITY, l = 0.0f;
-    const SharedPages::Request r = batch.request(s.groups + own, p);
+    const pk::SharedRequest r = batch.request(s.groups + own, p);
     const int pos = r.pos0 + (t - r.start);
     if (r.before > 0) {
         const int32_t *table = batch.table(g, p);
-        SharedPages::Request pre{};
+        pk::SharedRequest pre{};
         pre.prefix = true;
         const PagedAttentionConstants mp = batch.mask(pre, p);
         const int at = pk::paged_place(r, t, r.before);
@@ -293,16 +374,39 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 #define SHARED_PARAMS(T)                                                                                                     \
     const T::storage *q, const T::storage *k, const T::storage *v, const int32_t *tables, const int32_t *starts,             \
         const int32_t *keyLens, const int32_t *prefixTables, const int32_t *prefixLens, const int32_t *groupStarts
-#define SHARED_WORK(name, T, PER_CU, CALL)                                                                                   \
+// Few rows alone.
+#define SHARED_FEW(t, T, HD, RT, PER_CU)                                                                                     \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        name(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, float *pML, pk::u32x4 *records, \
-             T::storage *out, float *lse, PagedAttentionConstants p, PagedWorkConstants w, SharedPrefixConstants s) {        \
-        const SharedPages::More more{prefixTables, prefixLens, groupStarts, positions, lse, s};                              \
-        CALL(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, w, more);                                     \
+        shared_prefix_few_##t##_d##HD##_r##RT(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, \
+                                              float *pML, pk::u32x4 *records, T::storage *out, float *lse,                   \
+                                              PagedAttentionConstants p, PagedWorkConstants w, SharedPrefixConstants s) {    \
+        const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
+        const SharedPages<false>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};              \
+        paged_few<T, HD, RT, SharedPages<false>, HD == 512 ? kWaves : 1>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, \
+                                                                         out, p, w, more);                                   \
     }
-#define SHARED_FEW(t, T, HD, RT, PER_CU) \
-    SHARED_WORK(shared_prefix_few_##t##_d##HD##_r##RT, T, PER_CU, (paged_few<T, HD, RT, SharedPages>))
-#define SHARED_TILE(t, T, HD, PER_CU) SHARED_WORK(shared_prefix_tile_##t##_d##HD, T, PER_CU, (paged_tile<T, HD, SharedPages>))
+// Many rows and few in one launch: the first blocks take tiles of many rows, which the matrix cores bound, the others, a wave each,
+// the requests of few, which memory bounds; so both are busy at once.
+#define SHARED_BOTH(t, T, HD, PER_CU)                                                                                        \
+    POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
+        shared_prefix_both_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, float *pML, \
+                                       pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
+                                       PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {           \
+        __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
+        using Pages = SharedPages<true>;                                                                                     \
+        const pk::PagedTile *planFew = plan + many.maxTiles + 1;                                                             \
+        const uint32_t tileBlocks = tile_blocks(plan[0].before, planFew[0].before);                                          \
+        const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
+        if (blockIdx.x < tileBlocks) {                                                                                       \
+            many.workers = tileBlocks;                                                                                       \
+            const Pages::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};                       \
+            paged_tile<T, HD, Pages>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, many, more, lds);     \
+        } else {                                                                                                             \
+            few.workers = 4 * (gridDim.x - tileBlocks);                                                                      \
+            const Pages::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, tileBlocks};              \
+            paged_few<T, HD, 1, Pages, 1>(q, k, v, tables, starts, keyLens, planFew, pO, pML, records, out, p, few, more, lds); \
+        }                                                                                                                    \
+    }
 #define SHARED_MERGE(t, T, HD)                                                                                               \
     POPCORN_KERNEL void __launch_bounds__(256)                                                                               \
         shared_prefix_merge_##t##_d##HD(const float *pO, const float *pML, const pk::u32x4 *records, const int32_t *starts,  \
@@ -313,8 +417,9 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 #define SHARED_PLAIN(name, T, VEC)                                                                                           \
     POPCORN_KERNEL void __launch_bounds__(256) name(SHARED_PARAMS(T), T::storage *out, float *lse, PagedAttentionConstants p, \
                                                     SharedPrefixConstants s) {                                               \
-        const SharedPages::More more{prefixTables, prefixLens, groupStarts, nullptr, lse, s};                                \
-        shared_prefix_plain<T, VEC>(q, k, v, SharedPages{tables, starts, keyLens, nullptr, more}, out, p);                   \
+        const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
+        const SharedPages<false>::More more{prefixTables, prefixLens, groupStarts, nullptr, lse, held, s, 0};                \
+        shared_prefix_plain<T, VEC>(q, k, v, SharedPages<false>{tables, starts, keyLens, nullptr, more}, out, p);            \
     }
 
 using pk::BF16;
@@ -340,9 +445,9 @@ SHARED_ALL(f16, F16, 2)
 SHARED_ALL(bf16, BF16, 2)
 SHARED_FEW(f16, F16, 256, 2, 1)
 SHARED_FEW(bf16, BF16, 256, 2, 1)
-SHARED_TILE(f16, F16, 64, 2)
-SHARED_TILE(f16, F16, 128, 2)
-SHARED_TILE(f16, F16, 256, 1)
-SHARED_TILE(bf16, BF16, 64, 2)
-SHARED_TILE(bf16, BF16, 128, 2)
-SHARED_TILE(bf16, BF16, 256, 1)
+SHARED_BOTH(f16, F16, 64, 2)
+SHARED_BOTH(f16, F16, 128, 2)
+SHARED_BOTH(f16, F16, 256, 1)
+SHARED_BOTH(bf16, BF16, 64, 2)
+SHARED_BOTH(bf16, BF16, 128, 2)
+SHARED_BOTH(bf16, BF16, 256, 1)

@@ -264,7 +264,8 @@ private:
 };
 
 // SharedPrefixAttention (shared_prefix.hip): PagedAttention's two kernels over units of groups' rows against their prefixes and of
-// requests' rows against their pages, then a merge of each row's pieces.
+// requests' rows against their pages, side by side in one launch behind their plan where there are units of many rows, then a merge
+// of each row's pieces.
 class SharedPrefixKernel : public Kernel {
 public:
     SharedPrefixKernel(std::vector<Tensor> inputs, const Tensor &out, const Tensor *lse, const PagedAttentionConstants &pc,
@@ -279,19 +280,29 @@ public:
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
         merge_ = "shared_prefix_merge_" + type + hd;
         // the kernels and their limits as for PagedAttention
-        const int tilesPerCU = hdp_ == 256 ? 1 : 2;
-        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows && all > (hdp_ == 256 ? 64 : 128);
-        const bool apart = tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU * deviceCUs();
-        if (!tiles || apart) {
-            const int rt = hdp_ == 512 || (f32 && hdp_ == 256) || longest <= 16 || tiles ? 1 : 2;
+        both_ = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows && all > (hdp_ == 256 ? 64 : 128);
+        if (both_) {
+            fn_ = "shared_prefix_both_" + type + hd;
+            blocks_ = (hdp_ == 256 ? 1 : 2) * deviceCUs();
+            many_ = work(128, 64, kFewRows, UINT32_MAX, blocks_, 384);
+            few_ = work(16, 32, 0, kFewRows, 4 * blocks_, 96);
+            few_.stateBase = 2 * many_.workers * many_.rows;
+        } else {
+            const int rt = hdp_ == 512 || (f32 && hdp_ == 256) || longest <= 16 ? 1 : 2;
             const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
-            add("shared_prefix_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);
+            fn_ = "shared_prefix_few_" + type + hd + "_r" + std::to_string(rt);
+            // a worker is a wave, or at 512 dims a block
+            const int team = hdp_ == 512 ? 1 : 4;
+            few_ = work(16 * rt, f32 ? 16 : 32, 0, UINT32_MAX, 0, team == 4 ? 96 : 384);
+            const double steps = (double)few_.maxTiles * tileSteps(few_);
+            blocks_ = (unsigned)std::max(1.0, std::min((double)perCU * deviceCUs(), (steps * pc.Nkv / few_.minSteps + 1) / team));
+            few_.workers = blocks_ * team;
+            few_.ownPlan = few_.maxTiles <= 1024 && pc.R + sc.groups <= 1024 && steps < 2147483648.0;
         }
-        if (tiles) add("shared_prefix_tile_" + type + hd, 128, 64, apart ? kFewRows : 0, UINT32_MAX, tilesPerCU);
         sc_.rows = pc.T * pc.Nq;
-        sc_.rowBase = work_.back().stateBase + 2 * work_.back().workers * work_.back().rows;
+        sc_.rowBase = few_.stateBase + 2 * few_.workers * few_.rows;
         sc_.states = sc_.rowBase + 2 * sc_.rows;
-        for (const PagedWorkConstants &w : work_) sc_.most = std::max(sc_.most, w.workers);
+        sc_.most = std::max(many_.workers, few_.workers);
         sc_.parts = sc_.rows < 4096 ? 4 : 1;
     }
     std::vector<Binding> tensors() const override {
@@ -302,80 +313,83 @@ public:
         return b;
     }
     std::string describe() const override {
-        std::string s = sc_.windowed ? "shared_prefix_positions," : "";
-        for (size_t i = 0; i < work_.size(); ++i) s += (work_[i].ownPlan ? "" : "shared_prefix_plan,") + fn_[i] + ",";
-        return s + merge_;
+        return (both_ ? "shared_prefix_plan," : std::string(sc_.windowed ? "shared_prefix_positions," : "") + (few_.ownPlan ? "" : "shared_prefix_plan,")) +
+               fn_ + "," + merge_;
     }
     void encode(KernelCommandEncoder &enc) const override {
         // one buffer: the states' O, their m and l, the rows' records, the plans, the positions
-        int64_t tiles = 0;
-        for (const PagedWorkConstants &w : work_) tiles += w.ownPlan ? 0 : (int64_t)w.maxTiles + 1;
+        const int64_t tiles = both_ ? (int64_t)many_.maxTiles + few_.maxTiles + 2 : few_.ownPlan ? 0 : (int64_t)few_.maxTiles + 1;
         const int64_t o = (int64_t)sc_.states * hdp_ * 4, ml = cdiv((int64_t)sc_.states * 8, 16) * 16, rec = 2 * (int64_t)sc_.rows * 16;
         const int64_t positions = sc_.windowed ? ((int64_t)pc_.T + sc_.groups) * 4 : 0;
         enc.withTemporaryTensor(ScratchSpec{{o + ml + rec + tiles * 16 + positions}, DataType::u8}, [&](Tensor scratch) {
             auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
-            const Tensor pO = part(0, o), pML = part(o, ml), records = part(o + ml, rec), pos = part(o + ml + rec + tiles * 16, positions);
+            const Tensor pO = part(0, o), pML = part(o, ml), records = part(o + ml, rec), plan = part(o + ml + rec, tiles * 16);
+            const Tensor pos = part(o + ml + rec + tiles * 16, positions);
             const Tensor &starts = in_[4], &lens = in_[5], &prefixLens = in_[7], &groups = in_[8];
-            if (sc_.windowed)
-                launch(enc, "shared_prefix_positions", {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}, {pos, kWrite}},
-                       {bytesOf(pc_), bytesOf(sc_)}, dim3((unsigned)(cdiv(pc_.T, 256) + sc_.groups), 1, 1), 256);
-            int64_t plan = o + ml + rec;
-            for (size_t i = 0; i < work_.size(); ++i) {
-                const PagedWorkConstants &w = work_[i];
-                const std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_), bytesOf(w), bytesOf(sc_)};
-                const int64_t planBytes = w.ownPlan ? 0 : ((int64_t)w.maxTiles + 1) * 16;
-                const Tensor pl = part(plan, planBytes);
-                if (planBytes)
-                    launch(enc, "shared_prefix_plan",
-                           {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}, {pos, kRead}, {pl, kWrite}}, consts, dim3(1, 1, 1), 1024);
-                plan += planBytes;
-                std::vector<Binding> b;
-                for (const Tensor &t : in_) b.push_back({t, kRead});
-                for (const Binding &x : {Binding{pos, kRead}, {pl, kRead}, {pO, kWrite}, {pML, kWrite}, {records, kWrite}, {out_, kWrite}, {lse_, kWrite}})
-                    b.push_back(x);
-                launch(enc, fn_[i], std::move(b), consts, dim3(w.workers, 1, 1), 256);
+            const std::vector<Binding> lengths = {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}};
+            auto with = [](std::vector<Binding> b, std::initializer_list<Binding> more) {
+                b.insert(b.end(), more);
+                return b;
+            };
+            std::vector<std::vector<uint8_t>> consts = {bytesOf(pc_)};
+            if (both_) consts.push_back(bytesOf(many_));
+            consts.push_back(bytesOf(few_));
+            consts.push_back(bytesOf(sc_));
+            if (both_) {
+                launch(enc, "shared_prefix_plan", with(lengths, {{pos, kReadWrite}, {plan, kWrite}}), consts,
+                       2 + (sc_.windowed ? cdiv(pc_.T, 1024) : 0), 1024);
+            } else {
+                if (sc_.windowed)
+                    launch(enc, "shared_prefix_positions", with(lengths, {{pos, kWrite}}), {bytesOf(pc_), bytesOf(sc_)},
+                           cdiv(pc_.T, 256) + cdiv(sc_.groups, 4), 256);
+                if (!few_.ownPlan)  // (writes the groups' least again, the same)
+                    launch(enc, "shared_prefix_plan", with(lengths, {{pos, kReadWrite}, {plan, kWrite}}),
+                           {bytesOf(pc_), bytesOf(few_), bytesOf(few_), bytesOf(sc_)}, 1, 1024);
             }
+            std::vector<Binding> b;
+            for (const Tensor &t : in_) b.push_back({t, kRead});
+            launch(enc, fn_,
+                   with(std::move(b), {{pos, kRead}, {plan, kRead}, {pO, kWrite}, {pML, kWrite}, {records, kWrite}, {out_, kWrite}, {lse_, kWrite}}),
+                   consts, blocks_, 256);
             launch(enc, merge_,
                    {{pO, kRead}, {pML, kRead}, {records, kRead}, {starts, kRead}, {prefixLens, kRead}, {groups, kRead}, {out_, kWrite}, {lse_, kWrite}},
-                   {bytesOf(pc_), bytesOf(sc_)}, dim3((unsigned)cdiv(sc_.rows, 4 / sc_.parts), 1, 1), 256);
+                   {bytesOf(pc_), bytesOf(sc_)}, cdiv(sc_.rows, 4 / sc_.parts), 256);
         });
     }
 
 private:
     static constexpr uint32_t kFewRows = 32;
 
-    void add(const std::string &fn, uint32_t rows, uint32_t stepKeys, uint32_t few, uint32_t many, int perCU) {
-        const int64_t G = pc_.Nq / pc_.Nkv;
+    double tileSteps(const PagedWorkConstants &w) const {
+        return (double)cdiv((int64_t)std::max(pc_.columns, sc_.columns) * pc_.pageSize + w.stepKeys, w.stepKeys) + w.unitSteps;
+    }
+    PagedWorkConstants work(uint32_t rows, uint32_t stepKeys, uint32_t few, uint32_t many, uint32_t workers, uint32_t unitKeys) const {
         PagedWorkConstants w{};
         w.rows = rows;
         w.stepKeys = stepKeys;
         w.fewRows = few;
         w.manyRows = many;
-        const int64_t tiles = cdiv((int64_t)pc_.T * G, rows);
+        w.workers = workers;
+        const int64_t tiles = cdiv((int64_t)pc_.T * (pc_.Nq / pc_.Nkv), rows);
         w.maxTiles = (uint32_t)(tiles + std::min(pc_.R, pc_.T) + (sc_.groups ? tiles + std::min(sc_.groups, pc_.T) : 0));
-        w.minSteps = 128 / stepKeys;
-        w.unitSteps = 384 / stepKeys;
+        w.minSteps = 64 / stepKeys;
+        w.unitSteps = unitKeys / stepKeys;
         w.stream = in_[1].byteCount() + in_[2].byteCount() > (size_t{256} << 20);
-        const double tileSteps = (double)cdiv((int64_t)std::max(pc_.columns, sc_.columns) * pc_.pageSize + stepKeys, stepKeys) + w.unitSteps;
-        const double steps = (double)w.maxTiles * tileSteps;
-        w.workers = (uint32_t)std::max(1.0, std::min((double)perCU * deviceCUs(), steps * pc_.Nkv / w.minSteps + 1));
-        w.ownPlan = w.maxTiles <= 1024 && pc_.R + sc_.groups <= 1024 && steps < 2147483648.0;
-        w.stateBase = work_.empty() ? 0 : 2 * work_.back().workers * work_.back().rows;
-        work_.push_back(w);
-        fn_.push_back(fn);
+        return w;
     }
-    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, std::vector<std::vector<uint8_t>> consts, dim3 grid,
+    void launch(KernelCommandEncoder &enc, const std::string &fn, std::vector<Binding> b, std::vector<std::vector<uint8_t>> consts, int64_t blocks,
                 unsigned block) const {
-        enc.encode(*Kernels::Custom(fn, std::move(b), std::move(consts), grid, dim3(block, 1, 1)));
+        enc.encode(*Kernels::Custom(fn, std::move(b), std::move(consts), dim3((unsigned)blocks, 1, 1), dim3(block, 1, 1)));
     }
 
     std::vector<Tensor> in_;  // q, k, v, tables, starts, lens, prefix tables, prefix lens, group starts
     Tensor out_, lse_;
     PagedAttentionConstants pc_;
     SharedPrefixConstants sc_;
-    std::vector<PagedWorkConstants> work_;
-    std::vector<std::string> fn_;
-    std::string merge_;
+    PagedWorkConstants many_{}, few_{};
+    std::string fn_, merge_;
+    bool both_ = false;
+    unsigned blocks_ = 1;
     int64_t hdp_ = 0;
 };
 

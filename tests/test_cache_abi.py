@@ -50,15 +50,14 @@ def test_shared_prefix_kernels():
         return {n.split("_")[2] for n in k.function_names} - {"merge"}
 
     # a group's rows are one request's: many of them are tiles, whatever the requests bring
-    assert kinds(64, 64, 8, 2, 128) == {"tile"} and kinds(64, 64, 8, 2, 128, groups=False) == {"few"}
-    assert kinds(8, 8, 8, 2, 128) == {"few"} and kinds(33, 33, 8, 2, 128) == {"tile"} and kinds(17, 17, 8, 2, 256) == {"tile"}
-    assert kinds(300, 300, 8, 2, 128) == {"few", "tile"}
+    assert kinds(64, 64, 8, 2, 128) == {"plan", "both"} and kinds(64, 64, 8, 2, 128, groups=False) == {"few"}
+    assert kinds(8, 8, 8, 2, 128) == {"few"} and kinds(33, 33, 8, 2, 128) == {"plan", "both"} and kinds(17, 17, 8, 2, 256) == {"plan", "both"}
     for kw in (dict(t="f32"), dict(scale=0.0), dict(scale=float("nan")), dict()):
         assert kinds(64, 64, 8, 2, 128 if kw else 512, **kw) == {"few"}
     assert kinds(64, 64, 8, 2, 36) == {"plain"}
-    assert kinds(64, 64, 8, 2, 128, mask=WINDOW) == {"positions", "tile"}
+    assert kinds(64, 64, 8, 2, 128, mask=WINDOW) == {"plan", "both"} and kinds(8, 8, 8, 2, 128, mask=WINDOW) == {"positions", "few"}
     assert kinds(64, 64, 8, 2, 128, mask=WINDOW, groups=False) == {"few"}
-    assert "plan" in kinds(1100, 1100, 8, 2, 128)
+    assert kinds(1100, 1100, 8, 2, 128, t="f32") == {"plan", "few"}  # (more than a block lays out)
 
 
 def weigh(q=(6, 4, 64), cache=(9, 2, 16, 64), table=(3, 5), starts=(4,), lens=(3,), lse=(6, 4), weights=(3, 2, 80), t="bf16", kt=None, lt="f32",
