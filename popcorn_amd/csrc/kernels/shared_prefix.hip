@@ -103,7 +103,7 @@ struct SharedPages {
     }
 
     // The same request, in scalar registers. (Where the compiler took its keys for the lanes' own, each load through a descriptor
-    // became a loop over the lanes' descriptors: 256 requests of 20 to 800 own keys 50 us, and KEPT.)
+    // became a loop over the lanes' descriptors: 256 requests of 20 to 800 own keys 50 us, and 49, beside other waves; alone a step 3.3 us, and 2.4.)
     __device__ static inline Request uniform(const Request &q) {
         Request u;
         u.start = (int32_t)first_lane((uint32_t)q.start);
@@ -407,6 +407,18 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
             paged_few<T, HD, 1, Pages, 1>(q, k, v, tables, starts, keyLens, planFew, pO, pML, records, out, p, few, more, lds); \
         }                                                                                                                    \
     }
+// Many rows alone: beside the few-row kernel's code those of 256 dims, which take all registers, spilled 51 to 65 of them (a prompt of
+// 2048 tokens behind 8192 keys, bf16: 332 us, and 251).
+#define SHARED_MANY(t, T, HD, PER_CU)                                                                                        \
+    POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
+        shared_prefix_many_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, float *pML, \
+                                       pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
+                                       PagedWorkConstants w, SharedPrefixConstants s) {                                      \
+        __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
+        const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
+        const SharedPages<true>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};               \
+        paged_tile<T, HD, SharedPages<true>>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, w, more, lds); \
+    }
 #define SHARED_MERGE(t, T, HD)                                                                                               \
     POPCORN_KERNEL void __launch_bounds__(256)                                                                               \
         shared_prefix_merge_##t##_d##HD(const float *pO, const float *pML, const pk::u32x4 *records, const int32_t *starts,  \
@@ -447,7 +459,7 @@ SHARED_FEW(f16, F16, 256, 2, 1)
 SHARED_FEW(bf16, BF16, 256, 2, 1)
 SHARED_BOTH(f16, F16, 64, 2)
 SHARED_BOTH(f16, F16, 128, 2)
-SHARED_BOTH(f16, F16, 256, 1)
+SHARED_MANY(f16, F16, 256, 1)
 SHARED_BOTH(bf16, BF16, 64, 2)
 SHARED_BOTH(bf16, BF16, 128, 2)
-SHARED_BOTH(bf16, BF16, 256, 1)
+SHARED_MANY(bf16, BF16, 256, 1)

@@ -280,12 +280,14 @@ public:
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
         merge_ = "shared_prefix_merge_" + type + hd;
         // the kernels and their limits as for PagedAttention
-        both_ = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows && all > (hdp_ == 256 ? 64 : 128);
+        both_ = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows && all > (sc.groups || hdp_ == 256 ? 64 : 128);
         if (both_) {
-            fn_ = "shared_prefix_both_" + type + hd;
+            // one launch of both kinds of rows, or at 256 dims one after the other
+            fn_ = (hdp_ == 256 ? "shared_prefix_many_" : "shared_prefix_both_") + type + hd;
+            if (hdp_ == 256) before_ = "shared_prefix_few_" + type + hd + "_r1";
             blocks_ = (hdp_ == 256 ? 1 : 2) * deviceCUs();
             many_ = work(128, 64, kFewRows, UINT32_MAX, blocks_, 384);
-            few_ = work(16, 32, 0, kFewRows, 4 * blocks_, 96);
+            few_ = work(16, 32, 0, kFewRows, 4 * 2 * deviceCUs(), 96);
             few_.stateBase = 2 * many_.workers * many_.rows;
         } else {
             const int rt = hdp_ == 512 || (f32 && hdp_ == 256) || longest <= 16 ? 1 : 2;
@@ -314,7 +316,7 @@ public:
     }
     std::string describe() const override {
         return (both_ ? "shared_prefix_plan," : std::string(sc_.windowed ? "shared_prefix_positions," : "") + (few_.ownPlan ? "" : "shared_prefix_plan,")) +
-               fn_ + "," + merge_;
+               (before_.empty() ? "" : before_ + ",") + fn_ + "," + merge_;
     }
     void encode(KernelCommandEncoder &enc) const override {
         // one buffer: the states' O, their m and l, the rows' records, the plans, the positions
@@ -348,9 +350,17 @@ public:
             }
             std::vector<Binding> b;
             for (const Tensor &t : in_) b.push_back({t, kRead});
-            launch(enc, fn_,
-                   with(std::move(b), {{pos, kRead}, {plan, kRead}, {pO, kWrite}, {pML, kWrite}, {records, kWrite}, {out_, kWrite}, {lse_, kWrite}}),
-                   consts, blocks_, 256);
+            auto attend = [&](const std::string &fn, const Tensor &pl, const std::vector<std::vector<uint8_t>> &c, int64_t blocks) {
+                launch(enc, fn, with(b, {{pos, kRead}, {pl, kRead}, {pO, kWrite}, {pML, kWrite}, {records, kWrite}, {out_, kWrite}, {lse_, kWrite}}), c,
+                       blocks, 256);
+            };
+            if (before_.empty()) {
+                attend(fn_, plan, consts, blocks_);
+            } else {
+                const int64_t first = ((int64_t)many_.maxTiles + 1) * 16;
+                attend(before_, part(o + ml + rec + first, tiles * 16 - first), {bytesOf(pc_), bytesOf(few_), bytesOf(sc_)}, few_.workers / 4);
+                attend(fn_, plan, {bytesOf(pc_), bytesOf(many_), bytesOf(sc_)}, blocks_);
+            }
             launch(enc, merge_,
                    {{pO, kRead}, {pML, kRead}, {records, kRead}, {starts, kRead}, {prefixLens, kRead}, {groups, kRead}, {out_, kWrite}, {lse_, kWrite}},
                    {bytesOf(pc_), bytesOf(sc_)}, cdiv(sc_.rows, 4 / sc_.parts), 256);
@@ -387,7 +397,7 @@ private:
     PagedAttentionConstants pc_;
     SharedPrefixConstants sc_;
     PagedWorkConstants many_{}, few_{};
-    std::string fn_, merge_;
+    std::string before_, fn_, merge_;
     bool both_ = false;
     unsigned blocks_ = 1;
     int64_t hdp_ = 0;

@@ -51,7 +51,7 @@ def test_shared_prefix_kernels():
 
     # a group's rows are one request's: many of them are tiles, whatever the requests bring
     assert kinds(64, 64, 8, 2, 128) == {"plan", "both"} and kinds(64, 64, 8, 2, 128, groups=False) == {"few"}
-    assert kinds(8, 8, 8, 2, 128) == {"few"} and kinds(33, 33, 8, 2, 128) == {"plan", "both"} and kinds(17, 17, 8, 2, 256) == {"plan", "both"}
+    assert kinds(8, 8, 8, 2, 128) == {"few"} and kinds(33, 33, 8, 2, 128) == {"plan", "both"} and kinds(17, 17, 8, 2, 256) == {"plan", "few", "many"}
     for kw in (dict(t="f32"), dict(scale=0.0), dict(scale=float("nan")), dict()):
         assert kinds(64, 64, 8, 2, 128 if kw else 512, **kw) == {"few"}
     assert kinds(64, 64, 8, 2, 36) == {"plain"}

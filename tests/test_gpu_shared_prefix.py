@@ -128,7 +128,7 @@ CHUNKS = [(130, [(0, 40), (5, 1), (70, 3)]), (17, [(0, 1), (20, 65)]), (None, [(
 def test_chunks(env, dtype, nq, nkv, hd, page, kind, window, sinks):
     tile = dtype != "f32" and hd <= 256 and hd % 8 == 0
     attend(env, Batch(CHUNKS, nq, nkv, hd, dtype, page, 3 * hd + page, pad=5), hd ** -0.5, kind, window, sinks,
-           kinds={"both"} if tile else {"plain"} if hd == 36 and dtype != "f32" else {"few"})
+           kinds={"few", "many"} if tile and hd == 256 else {"both"} if tile else {"plain"} if hd == 36 and dtype != "f32" else {"few"})
 
 
 @pytest.mark.parametrize("dtype,nq,nkv,hd", [("bf16", 16, 4, 128), ("f16", 8, 4, 256), ("bf16", 4, 2, 64), ("f16", 16, 4, 128)])
@@ -137,7 +137,7 @@ def test_many_rows_many_pieces(env, dtype, nq, nkv, hd, window, sinks):
     # 45 requests' rows fill tiles of 128 and a part of one; the prefix is cut into pieces for most of the blocks
     b = Batch([(2000, [(7 * i % 60, 1) for i in range(45)]), (300, [(3, 1)] * 2)], nq, nkv, hd, dtype, 32, hd, std=2.0)
     attend(env, b, hd ** -0.5, 1 if window else 0, window or -1, sinks, hint=1,
-           kinds={"few"} if nq // nkv * 47 <= 128 and hd < 256 else {"both"})
+           kinds={"few"} if nq // nkv * 47 <= 128 and hd < 256 else {"few", "many"} if hd == 256 else {"both"})
 
 
 def test_requests_of_few_rows_apart(env):
