@@ -241,3 +241,57 @@ def test_release(env, requests):
     np.testing.assert_array_equal(new.numpy(stream), lens_)
     np.testing.assert_array_equal(freed.numpy(stream), freed_)
     assert list(counts.numpy(stream)) == [n]
+
+
+def test_weights_of_starts_out_of_order(env):
+    # within the tensors whatever the lengths say: what lies around the weights is as it was
+    pa, _, stream, enc = env
+    g = np.random.default_rng(17)
+    for i in range(6):
+        for hd, dtype in ((64, "bf16"), (64, "f32"), (36, "f16")):
+            b = Batch(PROMPTS, 4, 2, hd, dtype, 16, 18, pad=4)
+            t, _ = b.tensors(pa)
+            starts = g.permutation(b.starts) if i % 2 else g.integers(-5, 400, b.starts.size)
+            R_, room = len(b.lens), b.table.shape[1] * 16
+            big = f32(pa, np.full((R_ + 2, 2, room), 5.0))
+            w = pa.Tensor(big.ptr + 2 * room * 4, (R_, 2, room), "f32", owner=big)
+            lse = f32(pa, np.full(b.q.shape[:2], 3.0))
+            enc.encode(pa.Kernels.PagedAttentionWeights(t[0], t[1], t[6], i32(pa, starts), i32(pa, g.integers(-9, 900, R_)), lse, w, scale=0.1))
+            stream.synchronize()
+            x = download(big, stream)
+            assert (x[0] == 5.0).all() and (x[-1] == 5.0).all()
+
+
+def test_caches_past_32_bits(env):
+    # the requests' pages lie more than 2^32 elements behind the cache's first
+    pa, _, stream, enc = env
+    nkv, hd, page = 1, 512, 16
+    pages = 2 ** 32 // (nkv * hd * page) + 64
+    b = Batch([(100, [(60, 1), (5, 1)]), (None, [(200, 1), (33, 20)])], 4, nkv, hd, "bf16", page, 19)
+    used = len(b.k)
+    first = pages - used
+    caches = []
+    for x in (b.k, b.v):
+        big = pa.Tensor.empty([pages, nkv, page, hd], "bf16")
+        view = pa.Tensor(big.ptr + first * nkv * page * hd * 2, x.shape, "bf16", owner=big)
+        import oracle as O
+
+        view.copy_from(O.to_bits(x, O.BF16), stream)
+        caches.append((big, view))
+    t, lse = b.tensors(pa)
+    for i, x in ((3, b.prefix_table), (6, b.table)):
+        t[i] = i32(pa, np.where(x >= 0, x + first, -1))
+    t[1], t[2] = caches[0][0], caches[1][0]
+    enc.encode(pa.Kernels.SharedPrefixAttention(*t, scale=0.05, lse=lse))
+    stream.synchronize()
+    b.check(download(t[-1], stream), download(lse, stream), 0.05)
+    weigh(env, b, 0.05, t=t, lse=download(lse, stream).astype(np.float32))
+    lens = b.keys
+    w = np.random.default_rng(3).random((4, nkv, b.table.shape[1] * page)).astype(np.float32)
+    kept, kept_w = i32(pa, np.full(w.shape, -7)), f32(pa, w)
+    enc.encode(pa.Kernels.PagedEviction(f32(pa, w), t[1], t[2], t[6], i32(pa, lens), i32(pa, [20] * 4), kept, kept_w, first=2, last=3))
+    stream.synchronize()
+    ref = C.evict(w, b.k, b.v, b.table, lens, [20] * 4, np.full(w.shape, -7), 2, 3)
+    np.testing.assert_array_equal(kept.numpy(stream), ref[0])
+    for (_, view), x in zip(caches, ref[2:4]):
+        np.testing.assert_array_equal(download(view, stream), x)
