@@ -36,6 +36,13 @@ struct HeldGroups {
         len = lane < n ? prefixLens[lane] : 0;
         first = n ? groupStarts[0] : 0;
     }
+    // Group g's requests and its prefix's keys. (Lanes that ask for a group are among those that hold one, or all ask for the same.)
+    __device__ inline void group(uint32_t g, int32_t &a, int32_t &b, int32_t &keys) const {
+        const int32_t before = __shfl(end, (int)(g ? g - 1 : 0u));
+        a = g ? before : first;
+        b = __shfl(end, (int)g);
+        keys = __shfl(len, (int)g);
+    }
     // Keys of the prefix of request r's group.
     __device__ inline int32_t before(int32_t r) const {
         int32_t from = first, keys = 0;
@@ -70,11 +77,25 @@ struct SharedPages {
     __device__ inline Request request(uint32_t v, const PagedAttentionConstants &p) const {
         const SharedPrefixConstants &s = more.s;
         if (s.groups > 64) return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, s);
+        // The request's own numbers are asked for before the groups' are waited for: cold lines take over a microsecond each.
+        const uint32_t r = v < s.groups ? 0u : v - s.groups;
+        const int32_t from = starts[r], to = starts[r + 1], keys = keyLens[r];
         Request q{};
         q.prefix = v < s.groups;
-        if (q.prefix) return pk::paged_shared(v, starts, keyLens, more.prefixLens, more.groupStarts, more.positions, p, s);
-        const uint32_t r = v - s.groups;
-        static_cast<pk::PagedRequest &>(q) = pk::paged_request(starts[r], starts[r + 1], keyLens[r], p);
+        if (s.groups) {
+            int32_t a, b, len;
+            more.held.group(q.prefix ? v : 0u, a, b, len);
+            if (q.prefix) {
+                a = pk::paged_min(pk::paged_max(a, 0), (int32_t)p.R);
+                b = pk::paged_min(pk::paged_max(b, a), (int32_t)p.R);
+                static_cast<pk::PagedRequest &>(q) = pk::paged_request(starts[a], starts[b], 0, p);
+                q.keys = pk::paged_prefix_keys(len, p, s);
+                if (a == b || q.keys == 0) q.n = 0;
+                q.lo = s.windowed ? more.positions[p.T + v] : q.keys;
+                return q;
+            }
+        }
+        static_cast<pk::PagedRequest &>(q) = pk::paged_request(from, to, keys, p);
         q.before = pk::paged_prefix_keys(more.held.before((int32_t)r), p, s);
         return q;
     }
