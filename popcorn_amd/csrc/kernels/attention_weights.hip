@@ -195,7 +195,7 @@ struct WeightsBatch {
     static constexpr bool kShared = false, kPlanned = false;
     using Request = pk::PagedRequest;
     struct Left {  // a unit that its block shares with others behind it
-        uint32_t pieces, request, hkv, key0;
+        uint32_t pieces, request, hkv, key0, keys, pad[3];
     };
     const int32_t *starts, *keyLens;
     Left *left;
@@ -219,7 +219,7 @@ struct WeightsBatch {
     }
     __device__ static inline void idle(Left *to) { to->pieces = 0; }
     __device__ static inline void close(Left *to, const Piece<Request> &c, uint32_t sharers, const PagedWorkConstants &) {
-        *to = Left{sharers, c.request, c.hkv, c.tile * kKeys};
+        *to = Left{sharers, c.request, c.hkv, c.tile * kKeys, (uint32_t)c.req.keys, {}};
     }
 };
 
@@ -275,20 +275,35 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
             lseAt = behind(first + lane) * 4;
         };
         lay(row0);
-        auto copy = [&](uint32_t i) {
-            const uint32_t first = row0 + i * kStageRows, place = i % kPlaces;
+        struct Rows {
+            __amdgpu_buffer_rsrc_t q, lse;
+            uint32_t place;
+        };
+        auto rows_of = [&](uint32_t i) {
+            const uint32_t first = row0 + i * kStageRows;
             if (!alike) lay(first);
             const uint64_t at0 = ((uint64_t)(uint32_t)c.req.start + first_lane(token_of(first))) * p.Nq + c.hkv * G, all = (uint64_t)p.T * p.Nq;
             const uint64_t left = at0 < all ? all - at0 : 0;
-            const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(Q + (at0 < all ? at0 : 0) * D), 0,
-                                                              (int)min(left * D * 2, (uint64_t)0x7fffffff), 0x00020000);
-            const auto ls = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(lse + (at0 < all ? at0 : 0)), 0,
-                                                              (int)min(left * 4, (uint64_t)0x7fffffff), 0x00020000);
-#pragma unroll
-            for (int j = 0; j < kCopies; ++j)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void *)(smem + place * kStageBytes + (wave * 16 + j * kRowsPer) * HD * 2), 16,
+            Rows r;
+            r.q = __builtin_amdgcn_make_buffer_rsrc(const_cast<S *>(Q + (at0 < all ? at0 : 0) * D), 0, (int)min(left * D * 2, (uint64_t)0x7fffffff),
+                                                    0x00020000);
+            r.lse = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(lse + (at0 < all ? at0 : 0)), 0, (int)min(left * 4, (uint64_t)0x7fffffff),
+                                                      0x00020000);
+            r.place = i % kPlaces;
+            return r;
+        };
+        constexpr int kParts = kCopies + 1;
+        auto copy_part = [&](const Rows &r, int j) {
+            if (j < kCopies)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r.q, (lds_void *)(smem + r.place * kStageBytes + (wave * 16 + j * kRowsPer) * HD * 2), 16,
                                                          (int)at[j], 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ls, (lds_void *)(smem + kLse + (place * 4 + wave) * 256), 4, (int)lseAt, 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r.lse, (lds_void *)(smem + kLse + (r.place * 4 + wave) * 256), 4, (int)lseAt, 0, 0, 0);
+        };
+        auto copy = [&](uint32_t i) {
+            const Rows r = rows_of(i);
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) copy_part(r, j);
         };
 #pragma unroll
         for (uint32_t i = 0; i + 1 < kPlaces; ++i) copy(i);
@@ -321,8 +336,30 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
             sum[t][e] = v;
         };
         // The scores of 32 rows, with the weights of the 32 before beside the products.
-        auto score = [&](uint32_t x, int rt) {
-            constexpr int kEach = 32 / (KS * 2) > 0 ? 32 / (KS * 2) : 1, kAhead = 4;
+        auto score = [&](uint32_t x, int rt, const Rows *ahead) {
+            // Beside product i stand the sum of its scores - 2, the exponential of its scores - 1 and the exponent of its own: in a row of
+            // their own each would wait for the one before it.
+            constexpr int kEach = 32 / (KS * 2), kAhead = 4;
+            float x0[kEach], x1[kEach];
+            auto beside = [&](int i) {
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) {
+                    if (i >= 2) {
+                        const int at = (i - 2) * kEach + j;
+                        float to = sum[at / 16][at % 16] + x1[j];
+                        asm volatile("" : "+v"(to));
+                        sum[at / 16][at % 16] = to;
+                    }
+                    if (i >= 1 && i <= 2 * KS) {
+                        x1[j] = __builtin_amdgcn_exp2f(x0[j]);
+                        asm volatile("" : "+v"(x1[j]));
+                    }
+                    if (i < 2 * KS) {
+                        x0[j] = fmaf(st[1 - rt][(i * kEach + j) / 16][(i * kEach + j) % 16], c2, -ofs[1 - rt]);
+                        asm volatile("" : "+v"(x0[j]));
+                    }
+                }
+            };
             u32x4 q[kAhead];
             auto read = [&](int i) {
                 return *reinterpret_cast<const u32x4 *>(smem + ((x ^ (i & 7) * 32u) + (i >> 3) * 256u + rt * (32 * HD * 2)));
@@ -340,11 +377,15 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
                 for (int t = 0; t < 2; ++t) {
                     st[rt][t] = pk::Mma<T>::run(kf[t][i], q[i % kAhead], st[rt][t]);
                     if (t == 1 && i + kAhead < KS) q[i % kAhead] = read(i + kAhead);
-#pragma unroll
-                    for (int j = 0; j < kEach; ++j) weigh(1 - rt, (i * 2 + t) * kEach + j);
+                    beside(i * 2 + t);
+                    // the copies of a later step between the products: a CU takes 16 cycles for each, so four waves' would wait in a row
+                    constexpr int kEvery = 2 * KS / kParts;
+                    if (ahead && (i * 2 + t) % kEvery == 0 && (i * 2 + t) / kEvery < kParts) copy_part(*ahead, (i * 2 + t) / kEvery);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            beside(2 * KS);
+            beside(2 * KS + 1);
         };
         // Hides what rows do not see, and rows that give nothing.
         auto mask = [&](int rt, uint32_t first) {
@@ -365,8 +406,11 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
             wait_vmcnt<(int)(kPlaces - 2) * (kCopies + 1)>();
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            copy(i + kPlaces - 1);
-            if (key0 >= keys) continue;
+            if (key0 >= keys) {
+                copy(i + kPlaces - 1);
+                continue;
+            }
+            const Rows later = rows_of(i + kPlaces - 1);
             const uint32_t first = row0 + i * kStageRows, place = i % kPlaces;
             uint32_t x = qAt + place * kStageBytes;
             asm volatile("" : "+v"(x));
@@ -376,12 +420,12 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
                 return v == -INFINITY || first + rt * 32 + c32 >= rows ? INFINITY : v * kLog2e;
             };
             ofs[0] = logarithm(0);
-            score(x, 0);
+            score(x, 0, &later);
             mask(0, first);
             last = 0;
             if (first + 32 >= rows) break;
             ofs[1] = logarithm(1);
-            score(x, 1);
+            score(x, 1, nullptr);
             mask(1, first + 32);
             last = 1;
         }
@@ -419,18 +463,25 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
 
 }  // namespace
 
-// The partial sums of the units that several blocks shared, in their order.
+// The partial sums of the units that several blocks shared, in their order. Bound by its launch and two rounds of loads: all that
+// hang on the unit are asked for before any is looked at.
 POPCORN_KERNEL void __launch_bounds__(256)
-    attention_weights_join(const int32_t *tables, const int32_t *starts, const int32_t *keyLens, const float *partial,
-                           const WeightsBatch::Left *left, float *weights, PagedAttentionConstants p, AttentionWeightsConstants a) {
+    attention_weights_join(const int32_t *tables, const float *partial, const WeightsBatch::Left *left, float *weights,
+                           PagedAttentionConstants p) {
     const WeightsBatch::Left c = left[blockIdx.x];
     if (c.pieces == 0) return;
-    const pk::PagedRequest q = weights_request(starts, keyLens, c.request, p, a);
-    const uint32_t key = c.key0 + threadIdx.x;
-    if (key >= (uint32_t)q.keys || (uint32_t)tables[(uint64_t)c.request * p.columns + key / p.pageSize] >= p.pages) return;
-    float x = 0.0f;
-    for (uint32_t i = 0; i < c.pieces; ++i) x += partial[(2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * kKeys + threadIdx.x];
-    weights[((uint64_t)c.request * p.Nkv + c.hkv) * ((uint64_t)p.columns * p.pageSize) + key] += x;
+    const uint32_t key = c.key0 + threadIdx.x, in = min(key, c.keys - 1);  // (a unit has keys)
+    const uint32_t page = (uint32_t)tables[(uint64_t)c.request * p.columns + in / p.pageSize];
+    float *to = weights + ((uint64_t)c.request * p.Nkv + c.hkv) * ((uint64_t)p.columns * p.pageSize) + in;
+    const float old = *to;
+    auto piece = [&](uint32_t i) { return partial[(2 * ((uint64_t)blockIdx.x + i) + (i == 0)) * kKeys + threadIdx.x]; };
+    float x = piece(0), next = piece(1);  // (shared by two at least)
+    for (uint32_t i = 1; i < c.pieces; ++i) {
+        const float v = next;
+        if (i + 1 < c.pieces) next = piece(i + 1);
+        x += v;
+    }
+    if (key < c.keys && page < p.pages) *to = old + x;
 }
 
 POPCORN_KERNEL void __launch_bounds__(1024)

@@ -295,3 +295,16 @@ def test_caches_past_32_bits(env):
     np.testing.assert_array_equal(kept.numpy(stream), ref[0])
     for (_, view), x in zip(caches, ref[2:4]):
         np.testing.assert_array_equal(download(view, stream), x)
+
+
+@pytest.mark.parametrize("dtype,hd,last_rows", [("bf16", 128, 0), ("f16", 256, 0), ("bf16", 64, 40)])
+def test_weights_of_prompts_among_many_single_tokens(env, dtype, hd, last_rows):
+    # a launch for requests of few rows beside the tiles'
+    lens = [(int(p), 1) for p in np.random.default_rng(hd).integers(0, 90, 40)]
+    lens[7], lens[30] = (33, 130), (0, 70)
+    weigh(env, Batch([(None, lens)], 8, 2, hd, dtype, 16, 20), hd ** -0.5, last_rows=last_rows, kinds={"few", "tile", "join"})
+
+
+def test_weights_of_more_tiles_than_a_block_lays_out(env):
+    lens = [(int(p), 1 + 40 * (i % 50 == 0)) for i, p in enumerate(np.random.default_rng(4).integers(0, 60, 1100))]
+    weigh(env, Batch([(None, lens)], 4, 2, 64, "bf16", 16, 21), 0.125, kinds={"few", "tiles", "tile", "join"})
