@@ -478,7 +478,7 @@ typedef struct {
 
 /* shared_prefix_*: groups of requests, group g's of groupStarts[g] ..
  * groupStarts[g + 1] - 1, whose prefix lies in the pages of row g of a table of
- * `columns`. rows: T x Nq; states: of all partial states, the last 2 x rows of them,
+ * `columns`. rows: T x Nq; states: of all partial states, with groups the last 2 x rows of them,
  * from rowBase on, for units that one block has whole; most: pieces that a unit
  * may have; parts: waves per row in the merge; windowed: positions are given. */
 typedef struct {

@@ -187,7 +187,7 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
 // ---- many rows: prompts -------------------------------------------------------------------
 // A unit is 256 keys of a request for one KV head, 64 to a wave, whose fragments stay in registers, on v_mfma_f32_32x32x16: S^T =
 // K . Q^T has a row's scores in a lane of each half, so a key's sum over rows is added up in its own register, and over the
-// lanes once at the end. Steps are 64 rows of Q, copied straight into LDS, a step ahead. The units' steps
+// lanes once at the end. Steps are 64 rows of Q, copied straight into LDS, three steps ahead. The units' steps
 // in a row are dealt out as for attention; of a unit that several blocks share each leaves 256 partial sums.
 constexpr uint32_t kKeys = 256, kStageRows = 64;
 

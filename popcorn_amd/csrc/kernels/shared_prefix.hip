@@ -9,18 +9,16 @@
 // A row has two units, each in one piece or several; a row's record of a unit (u32x4) says
 // where the states of its pieces lie, and the merge adds them all:
 //   O = sum O_i 2^(m_i - M) / L, L = sum l_i 2^(m_i - M), lse = (M + log2 L) ln 2.
+// What bounds it: small calls their chain of dependent reads (lengths, table, keys: 8 us of a kernel) and the merge's launch
+// (5 us): 2 requests behind 777 keys 27 us in all, where their bytes take 1; large batches the cold reads of
+// many short stretches of pages (256 requests behind 4000 keys, 136 MB: 45 us beside 14 for the plan and the merge, 3.0 TB/s, as torch.sum
+// of 111 MB reads); prompts the products, whose weights are two bf16 words (128 requests of 16 new tokens behind 16384 keys: 88 us).
 #include "paged_attention.hpp"
 
 namespace {
 
 constexpr float kLn2 = 0.6931471805599453f;
-
-// A wave's search: its lanes look at 64 entries at once.
-__device__ inline uint32_t wave_span_of(const int32_t *at, uint32_t n, int32_t x) {
-    if (n == 0 || at[0] > x) return n;
-    const uint32_t a = find_tile(n, (uint64_t)(uint32_t)x, [&](uint32_t i) { return at[i] < 0 ? 0u : (uint32_t)at[i]; });
-    return x < at[a + 1] ? a : n;
-}
+constexpr uint32_t kBehindPrefix = 1u << 31;  // in the last word of a row's record of its own keys: it has one of its prefix too
 
 // The groups of a call, a lane of every wave for each where there are up to 64 (else read where they are asked for): a unit's
 // group would take loads that wait for each other. Not in LDS: beside another array there the compiler has every read of LDS wait
@@ -147,8 +145,10 @@ struct SharedPages {
         for (uint32_t r = c.steps.r0 + thread; r < c.steps.r1; r += threads) {
             const uint64_t at = row(r);
             const uint32_t next = w.stateBase + 2 * worker * w.rows + (r - c.steps.r0);
+            const uint32_t behind = !c.req.prefix && c.req.before > 0 ? kBehindPrefix : 0u;
             left[(c.req.prefix ? 0u : more.s.rows) + at] =
-                whole ? pk::u32x4{(uint32_t)own_row(c.req, at), 0u, 0u, direct ? 0u : 1u} : pk::u32x4{next + w.rows, next, 2 * w.rows, c.sharers};
+                whole ? pk::u32x4{(uint32_t)own_row(c.req, at), 0u, 0u, direct ? 0u : 1u | behind}
+                      : pk::u32x4{next + w.rows, next, 2 * w.rows, c.sharers | behind};
         }
         return direct;
     }
@@ -242,11 +242,11 @@ __device__ inline uint32_t tile_blocks(u64 many, u64 few) {
 }
 
 // A row's pieces, of its prefix and of its own keys, by one wave or the block's four (s.parts): their maximum and sum first,
-// a lane for a piece, then their O, HD / 4 lanes for a piece.
+// a lane for a piece, then their O, HD / 4 lanes for a piece. Bound by its launch and two rounds of reads, the records and what they
+// lead to: a row's own record says that there is a prefix's (looked up in starts and groups it took two rounds more: 16 rows 5.0 us, and 4.2; 6000 rows 10, and 9).
 template <typename T, int HD>
 __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *__restrict__ pML, const pk::u32x4 *__restrict__ records,
-                                    const int32_t *__restrict__ starts, const int32_t *__restrict__ prefixLens,
-                                    const int32_t *__restrict__ groupStarts, typename T::storage *__restrict__ out, float *__restrict__ lse,
+                                    const int32_t *__restrict__ starts, typename T::storage *__restrict__ out, float *__restrict__ lse,
                                     const PagedAttentionConstants &p, const SharedPrefixConstants &s) {
     constexpr uint32_t kLanes = HD >= 256 ? 64 : HD / 4, kAtOnce = 64 / kLanes;
     constexpr int NJ = HD > 256 ? HD / 256 : 1;
@@ -255,15 +255,12 @@ __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *_
     const uint32_t lane = threadIdx.x & 63, wave = first_lane(threadIdx.x >> 6);
     const uint32_t part = wave % s.parts, row = blockIdx.x * (4 / s.parts) + wave / s.parts;
     if (row >= s.rows) return;  // (with four parts the whole block)
-    const uint32_t r = wave_span_of(starts, p.R, (int32_t)(row / p.Nq));
-    if (r >= p.R) return;
-    const uint32_t g = wave_span_of(groupStarts, s.groups, (int32_t)r);
-    const bool shared = g < s.groups && pk::paged_prefix_keys(prefixLens[g], p, s) > 0;
-    const pk::u32x4 own = records[s.rows + row];
-    if (!shared && own.w == 0) return;  // its piece has stored it
-    const pk::u32x4 pre = shared ? records[row] : pk::u32x4{0u, 0u, 0u, 0u};
+    const int32_t token = (int32_t)(row / p.Nq), from = starts[0], end = starts[p.R];
+    const pk::u32x4 own = records[s.rows + row], pre = records[row];
+    if (token < from || token >= end) return;  // a row of no request
+    if (own.w == 0) return;                    // its piece has stored it
     // (what lengths out of order could leave here leads to no row past the states)
-    const uint32_t nPre = min(pre.w, s.most), n = nPre + min(own.w, s.most);
+    const uint32_t nPre = own.w & kBehindPrefix ? min(pre.w, s.most) : 0u, n = nPre + min(own.w & ~kBehindPrefix, s.most);
     auto at = [&](uint32_t i) {
         const bool mine = i >= nPre;
         const uint32_t j = mine ? i - nPre : i;
@@ -271,10 +268,25 @@ __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *_
     };
     float m = -INFINITY, l = 0.0f;
     auto weight = [&](float mi, float li, float M) { return mi == -INFINITY && li == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mi - M); };
+    const uint32_t d0 = lane % kLanes * 4, step = s.parts * kAtOnce;
+    pk::f32x4 v[U][NJ];
+    float2 ml[U];
+    auto read = [&](uint32_t i0) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint64_t a = at(min(i0 + u * step, n - 1));
+            ml[u] = *reinterpret_cast<const float2 *>(pML + 2 * a);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+                v[u][j] = d0 + 256 * j < p.Hd ? *reinterpret_cast<const pk::f32x4 *>(pO + a * HD + d0 + 256 * j) : pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+    };
+    uint32_t i0 = part * kAtOnce + lane / kLanes;
+    read(i0);  // the first of them beside the maximum's
     for (uint32_t i = lane; i < n; i += 64) {
-        const float2 ml = *reinterpret_cast<const float2 *>(pML + 2 * at(i));
-        const float mn = fmaxf(m, ml.x);
-        l = (m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mn)) + ml.y * weight(ml.x, ml.y, mn);
+        const float2 x = *reinterpret_cast<const float2 *>(pML + 2 * at(i));
+        const float mn = fmaxf(m, x.x);
+        l = (m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mn)) + x.y * weight(x.x, x.y, mn);
         m = mn;
     }
     const float M = pk::wave_max(m);
@@ -282,17 +294,7 @@ __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *_
     pk::f32x4 o[NJ];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) o[j] = pk::f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t d0 = lane % kLanes * 4, step = s.parts * kAtOnce;
-    for (uint32_t i0 = part * kAtOnce + lane / kLanes; i0 < n; i0 += U * step) {
-        pk::f32x4 v[U][NJ];
-        float2 ml[U];
-#pragma unroll
-        for (uint32_t u = 0; u < U; ++u) {
-            const uint64_t a = at(min(i0 + u * step, n - 1));
-            ml[u] = *reinterpret_cast<const float2 *>(pML + 2 * a);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) v[u][j] = d0 + 256 * j < p.Hd ? *reinterpret_cast<const pk::f32x4 *>(pO + a * HD + d0 + 256 * j) : o[j];
-        }
+    for (; i0 < n;) {
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
             const float w = i0 + u * step < n ? weight(ml[u].x, ml[u].y, M) : 0.0f;
@@ -300,6 +302,8 @@ __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *_
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) o[j] += v[u][j] * w;
         }
+        i0 += U * step;
+        if (i0 < n) read(i0);
     }
     if constexpr (kAtOnce > 1)
 #pragma unroll
@@ -443,9 +447,8 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 #define SHARED_MERGE(t, T, HD)                                                                                               \
     POPCORN_KERNEL void __launch_bounds__(256)                                                                               \
         shared_prefix_merge_##t##_d##HD(const float *pO, const float *pML, const pk::u32x4 *records, const int32_t *starts,  \
-                                        const int32_t *prefixLens, const int32_t *groupStarts, T::storage *out, float *lse,  \
-                                        PagedAttentionConstants p, SharedPrefixConstants s) {                                \
-        shared_prefix_merge<T, HD>(pO, pML, records, starts, prefixLens, groupStarts, out, lse, p, s);                       \
+                                        T::storage *out, float *lse, PagedAttentionConstants p, SharedPrefixConstants s) {   \
+        shared_prefix_merge<T, HD>(pO, pML, records, starts, out, lse, p, s);                                                \
     }
 #define SHARED_PLAIN(name, T, VEC)                                                                                           \
     POPCORN_KERNEL void __launch_bounds__(256) name(SHARED_PARAMS(T), T::storage *out, float *lse, PagedAttentionConstants p, \

@@ -303,7 +303,7 @@ public:
         }
         sc_.rows = pc.T * pc.Nq;
         sc_.rowBase = few_.stateBase + 2 * few_.workers * few_.rows;
-        sc_.states = sc_.rowBase + 2 * sc_.rows;
+        sc_.states = sc_.rowBase + (sc.groups ? 2 * sc_.rows : 0);
         sc_.most = std::max(many_.workers, few_.workers);
         sc_.parts = sc_.rows < 4096 ? 4 : 1;
     }
@@ -362,7 +362,7 @@ public:
                 attend(fn_, plan, {bytesOf(pc_), bytesOf(many_), bytesOf(sc_)}, blocks_);
             }
             launch(enc, merge_,
-                   {{pO, kRead}, {pML, kRead}, {records, kRead}, {starts, kRead}, {prefixLens, kRead}, {groups, kRead}, {out_, kWrite}, {lse_, kWrite}},
+                   {{pO, kRead}, {pML, kRead}, {records, kRead}, {starts, kRead}, {out_, kWrite}, {lse_, kWrite}},
                    {bytesOf(pc_), bytesOf(sc_)}, cdiv(sc_.rows, 4 / sc_.parts), 256);
         });
     }
