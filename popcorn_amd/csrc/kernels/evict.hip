@@ -2,6 +2,9 @@
 //   n = min(keys, budget), first' = min(first, n), last' = min(last, n - first'): a KV head of a request keeps its first' first
 //   and last' last keys and, of those between, the n - first' - last' of the highest weight (ties: the lowest index; NaN is
 //   the lowest weight). evict_select says which, in index order, and evict_move brings their rows to the front.
+// The choice is bound by its passes, the moves by rows of 128 bytes that lie apart. Where: 48 requests of 300 to 8000 keys cut to
+// 1000, 8 heads of 128 in 16 bits: 15 us and 104 (105 MB read, 105 MB written: 2.2 TB/s; the reads alone take 67, the writes alone 41;
+// torch's index_select of as many 256-byte rows has the same rate).
 #include "paged.hpp"
 #include "scan.hpp"
 
@@ -17,12 +20,17 @@ __device__ inline uint32_t rank_key(float x) {
 constexpr uint32_t kBins = 2048;
 constexpr uint32_t kTile = 4096;  // weights of a block's pass, four in a row to a thread
 constexpr uint32_t kHeld = 4;     // passes whose weights a block holds in registers
+// Counters of a bin, the even threads' and the odd ones': additions of a wave to one word take a cycle each. (One request of 4 heads
+// of 8191 weights, uniform in 0 to 1, in 1 to 1.05, all equal: 16, 18 and 23 us with short rows' moves; with one counter 17, 22 and 33;
+// with four 17, 17 and 18, but 48 requests' 8 heads 16 us instead of 15.)
+constexpr uint32_t kCopies = 2, kBinStride = kBins + 8;
 
 struct SelectSpace {
-    uint32_t bins[kBins], sums[16], found[2];
+    __attribute__((aligned(16))) uint32_t bins[kBinStride * kCopies];
+    uint32_t sums[16], found[3][2];
 };
 
-// HELD: all weights are read once, into registers; else again for each count and for the choice.
+// HELD: all weights are read once, into registers, a thread's in a row; else again for each count and for the choice, tile by tile.
 template <bool HELD>
 __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictKeep &k, int32_t *__restrict__ to, float *__restrict__ toW,
                                    SelectSpace &sp) {
@@ -30,8 +38,9 @@ __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictK
     struct Four {
         float v[4];
     };
+    auto first_of = [&](uint32_t tile) { return HELD ? (tid * tiles + tile) * 4 : tile * kTile + tid * 4; };
     auto read = [&](uint32_t tile) {
-        const uint32_t i = tile * kTile + tid * 4;
+        const uint32_t i = first_of(tile);
         Four f{};
         if (i + 4 <= k.keys) {
             __builtin_memcpy(&f, w + i, sizeof(f));
@@ -45,90 +54,129 @@ __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictK
     Four held[HELD ? kHeld : 1];
     if constexpr (HELD) {
 #pragma unroll
-        for (uint32_t t = 0; t < kHeld; ++t) held[t] = read(t);
+        for (uint32_t t = 0; t < kHeld; ++t)
+            if (t < tiles) held[t] = read(t);
     }
-    auto each = [&](auto &&body) {  // body(tile, its four weights)
+    auto each = [&](auto &&body) {  // body(first index, its four weights)
         if constexpr (HELD) {
 #pragma unroll
             for (uint32_t t = 0; t < kHeld; ++t)
-                if (t < tiles) body(t, held[t]);
+                if (t < tiles) body(first_of(t), held[t]);
         } else {
             Four next = read(0);
             for (uint32_t t = 0; t < tiles; ++t) {
                 const Four f = next;
                 if (t + 1 < tiles) next = read(t + 1);
-                body(t, f);
+                body(first_of(t), f);
             }
         }
     };
+    // a thread's two bins, in order from the highest
+    pk::u32x2 *mine2 = reinterpret_cast<pk::u32x2 *>(sp.bins + kBins - 2 - 2 * tid);
+    auto clear = [&] {
+#pragma unroll
+        for (uint32_t c = 0; c < kCopies; ++c) mine2[c * (kBinStride / 2)] = pk::u32x2{0u, 0u};
+    };
     const uint32_t lo = k.first, hi = k.keys - k.last;  // between them `need` are kept
     uint32_t need = k.n - k.first - k.last, least = 0, shift = 32;
+    if (need > 0) {
+        clear();
+        __syncthreads();
+    }
     for (int pass = 0; pass < 3 && need > 0; ++pass) {
         const uint32_t bits = pass < 2 ? 11u : 10u, above = shift;
         shift -= bits;
-        for (uint32_t b = tid; b < kBins; b += 1024) sp.bins[b] = 0;
-        __syncthreads();
-        each([&](uint32_t t, const Four &f) {
+        each([&](uint32_t base, const Four &f) {
 #pragma unroll
             for (uint32_t j = 0; j < 4; ++j) {
-                const uint32_t i = t * kTile + tid * 4 + j, x = rank_key(f.v[j]);
-                if (i >= lo && i < hi && (above == 32 || x >> above == least >> above)) atomicAdd(&sp.bins[x >> shift & ((1u << bits) - 1)], 1u);
+                const uint32_t i = base + j, x = rank_key(f.v[j]);
+                if (i >= lo && i < hi && (above == 32 || x >> above == least >> above))
+                    atomicAdd(&sp.bins[(x >> shift & ((1u << bits) - 1)) + tid % kCopies * kBinStride], 1u);
             }
         });
         __syncthreads();
         // from the highest bin down: the bin where the need is met
-        const uint32_t a = sp.bins[kBins - 1 - 2 * tid], b = sp.bins[kBins - 2 - 2 * tid];
+        uint32_t a = 0, b = 0;
+#pragma unroll
+        for (uint32_t c = 0; c < kCopies; ++c) {
+            const pk::u32x2 x = mine2[c * (kBinStride / 2)];
+            a += x[1];
+            b += x[0];
+        }
+        clear();
         const pk::Scan<uint32_t> s = pk::block_scan<16>(a + b, sp.sums);
         const uint32_t beforeA = s.upto - a - b, beforeB = beforeA + a;
         if (beforeA < need && need <= beforeB) {
-            sp.found[0] = kBins - 1 - 2 * tid;
-            sp.found[1] = need - beforeA;
+            sp.found[pass][0] = kBins - 1 - 2 * tid;
+            sp.found[pass][1] = need - beforeA;
         }
         if (beforeB < need && need <= s.upto) {
-            sp.found[0] = kBins - 2 - 2 * tid;
-            sp.found[1] = need - beforeB;
+            sp.found[pass][0] = kBins - 2 - 2 * tid;
+            sp.found[pass][1] = need - beforeB;
         }
         __syncthreads();
-        least |= sp.found[0] << shift;
-        need = sp.found[1];
-        __syncthreads();
+        least |= sp.found[pass][0] << shift;
+        need = sp.found[pass][1];
     }
     // `need` of those at `least` are kept, the lowest indices; where none between is, nothing is above
     const bool none = k.n == k.first + k.last;
-    uint32_t sure = 0, ties = 0;  // before this pass's tile
-    each([&](uint32_t t, const Four &f) {
-        const uint32_t base = t * kTile + tid * 4;
-        uint32_t count = 0;
-        bool is[4], tie[4];
+    auto is_kept = [&](uint32_t i, float v, bool &sure, bool &tie) {
+        const bool between = i >= lo && i < hi;
+        const uint32_t x = rank_key(v);
+        sure = i < k.keys && (!between || (!none && x > least));
+        tie = between && !none && x == least;
+    };
+    auto count = [&](uint32_t base, const Four &f) {  // of both, 16 bits each (a block's are at most 16384)
+        uint32_t n = 0;
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t i = base + j, x = rank_key(f.v[j]);
-            const bool between = i >= lo && i < hi;
-            is[j] = i < k.keys && (!between || (!none && x > least));
-            tie[j] = between && !none && x == least;
-            count += (uint32_t)is[j] | (uint32_t)tie[j] << 16;
+            bool sure, tie;
+            is_kept(base + j, f.v[j], sure, tie);
+            n += (uint32_t)sure | (uint32_t)tie << 16;
         }
-        const pk::Scan<uint32_t> s = pk::block_scan<16>(count, sp.sums);
-        uint32_t a = sure + ((s.upto - count) & 0xffffu), b = ties + ((s.upto - count) >> 16);
+        return n;
+    };
+    // a, b: of both, those before it
+    auto write = [&](uint32_t base, const Four &f, uint32_t &a, uint32_t &b) {
 #pragma unroll
         for (uint32_t j = 0; j < 4; ++j) {
-            if (is[j] || (tie[j] && b < need)) {
+            bool sure, tie;
+            is_kept(base + j, f.v[j], sure, tie);
+            if (sure || (tie && b < need)) {
                 const uint32_t at = a + min(b, need);
                 to[at] = (int32_t)(base + j);
                 toW[at] = f.v[j];
             }
-            a += is[j];
-            b += tie[j];
+            a += sure;
+            b += tie;
         }
-        sure += s.total & 0xffffu;
-        ties += s.total >> 16;
-    });
+    };
+    if constexpr (HELD) {
+        uint32_t mine = 0;
+        each([&](uint32_t base, const Four &f) { mine += count(base, f); });
+        const uint32_t before = pk::block_scan<16>(mine, sp.sums).upto - mine;
+        uint32_t a = before & 0xffffu, b = before >> 16;
+        each([&](uint32_t base, const Four &f) { write(base, f, a, b); });
+    } else {
+        uint32_t sure = 0, ties = 0;  // before this tile
+        each([&](uint32_t base, const Four &f) {
+            const uint32_t mine = count(base, f);
+            const pk::Scan<uint32_t> s = pk::block_scan<16>(mine, sp.sums);
+            uint32_t a = sure + ((s.upto - mine) & 0xffffu), b = ties + ((s.upto - mine) >> 16);
+            write(base, f, a, b);
+            sure += s.total & 0xffffu;
+            ties += s.total >> 16;
+        });
+    }
 }
 
 }  // namespace
 
 // A block per (request, KV head). The least kept weight by three counts of its bits (11, 11 and 10), then one pass in
-// order that numbers what is kept.
+// order that numbers what is kept: no sort, and no atomics but the counts', so equal weights leave the lowest index whatever
+// the order of waves. Up to 16384 weights stay in registers between the passes (8191 of them: 10 us; read for each pass, 14). One request's
+// 4 heads leave 252 CUs idle; several blocks to a head would have to wait for each other's counts three times (one of 100000 keys, cut to
+// a quarter: 76 us, and the moves 80).
 POPCORN_KERNEL void __launch_bounds__(1024, 8)
     evict_select(const float *weights, const int32_t *keyLens, const int32_t *budgets, int32_t *kept, float *keptWeights, EvictConstants e) {
     __shared__ SelectSpace space;
@@ -153,6 +201,7 @@ POPCORN_KERNEL void __launch_bounds__(1024, 8)
 
 namespace {
 
+// In place, since a step has no spare cache: a kept row only ever moves to the front.
 // A block takes e.units units of U (its slice) of the rows of one (request, KV head) in K or V. Row j becomes row kept[j] >= j, in chunks from
 // the front: a chunk's rows are all read before one of them is written, and what later chunks read lies behind what it
 // writes (kept rises, so kept[j] >= j for them too).

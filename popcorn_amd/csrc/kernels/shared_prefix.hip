@@ -10,7 +10,7 @@
 // where the states of its pieces lie, and the merge adds them all:
 //   O = sum O_i 2^(m_i - M) / L, L = sum l_i 2^(m_i - M), lse = (M + log2 L) ln 2.
 // What bounds it: small calls their chain of dependent reads (lengths, table, keys: 8 us of a kernel) and the merge's launch
-// (5 us): 2 requests behind 777 keys 27 us in all, where their bytes take 1; large batches the cold reads of
+// (4 us): 2 requests behind 777 keys 27 us in all, where their bytes take 1; large batches the cold reads of
 // many short stretches of pages (256 requests behind 4000 keys, 136 MB: 45 us beside 14 for the plan and the merge, 3.0 TB/s, as torch.sum
 // of 111 MB reads); prompts the products, whose weights are two bf16 words (128 requests of 16 new tokens behind 16384 keys: 88 us).
 #include "paged_attention.hpp"
@@ -188,6 +188,8 @@ __device__ inline void token_position(uint32_t t, const int32_t *starts, const i
 
 }  // namespace
 
+// The plan, before a launch that two kinds of work share: 5 to 7 us, four cold reads that wait for each other and the scan. (Each block
+// by itself would take as long, and its lists the LDS of the copies.)
 // Block 0 lays out the tiles of many rows, block 1 those of few (of the few-row kernel alone there is just block 0: many is few). Each
 // plan's entry 0: the counted steps, the number of tiles. Under a window both write each group's least position first, behind the
 // tokens' positions, which the blocks behind them write.
@@ -220,7 +222,8 @@ POPCORN_KERNEL void __launch_bounds__(1024)
     if (threadIdx.x == 0) to[0] = pk::PagedTile{steps, tiles, 0};
 }
 
-// The same for the few-row kernel alone, which lays out its plan by itself: blocks take tokens, or those past them four groups.
+// The same for the few-row kernel alone, which lays out its plan by itself: blocks take tokens, or those past them four groups. A
+// launch (24 requests 4.7 us), since a prefix's rows belong to many requests: a wave would search for each of its rows.
 POPCORN_KERNEL void __launch_bounds__(256)
     shared_prefix_positions(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
                             int32_t *positions, PagedAttentionConstants p, SharedPrefixConstants s) {
@@ -243,7 +246,8 @@ __device__ inline uint32_t tile_blocks(u64 many, u64 few) {
 
 // A row's pieces, of its prefix and of its own keys, by one wave or the block's four (s.parts): their maximum and sum first,
 // a lane for a piece, then their O, HD / 4 lanes for a piece. Bound by its launch and two rounds of reads, the records and what they
-// lead to: a row's own record says that there is a prefix's (looked up in starts and groups it took two rounds more: 16 rows 5.0 us, and 4.2; 6000 rows 10, and 9).
+// lead to: a row's own record says that there is a prefix's. (Looked up in starts and groups it took two rounds more: 16 rows 5.0 us, and
+// 4.2; 6000 rows 10, and 9.) The rest is the states themselves, 20 and more of 512 bytes for each of 2048 rows behind 8192 keys: 9 us.
 template <typename T, int HD>
 __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *__restrict__ pML, const pk::u32x4 *__restrict__ records,
                                     const int32_t *__restrict__ starts, typename T::storage *__restrict__ out, float *__restrict__ lse,
