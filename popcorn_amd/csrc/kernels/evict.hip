@@ -3,7 +3,7 @@
 //   and last' last keys and, of those between, the n - first' - last' of the highest weight (ties: the lowest index; NaN is
 //   the lowest weight). evict_select says which, in index order, and evict_move brings their rows to the front.
 // The choice is bound by its passes, the moves by rows of 128 bytes that lie apart. Where: 48 requests of 300 to 8000 keys cut to
-// 1000, 8 heads of 128 in 16 bits: 15 us and 104 (105 MB read, 105 MB written: 2.2 TB/s; the reads alone take 67, the writes alone 41;
+// 1000, 8 heads of 128 in 16 bits: 15 us and 104 (120 MB read, 115 MB written: 2.3 TB/s; the reads alone take 67, the writes alone 41;
 // torch's index_select of as many 256-byte rows has the same rate).
 #include "paged.hpp"
 #include "scan.hpp"
