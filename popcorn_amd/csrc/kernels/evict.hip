@@ -218,47 +218,41 @@ __device__ void evict_move(const int32_t *__restrict__ kept, const int32_t *__re
     U *cache = blockIdx.z ? vCache : kCache;
     const uint32_t unit = blockIdx.y * e.units + threadIdx.x % e.units, row = threadIdx.x / e.units;
     const bool mine = unit < e.rowUnits;
-    auto place = [&](uint32_t i, uint64_t &at) {
-        const uint32_t column = i / e.pageSize, page = (uint32_t)table[column];
-        at = (((uint64_t)page * e.Nkv + hkv) * e.pageSize + (i - column * e.pageSize)) * e.rowUnits + unit;
-        return page < e.pages;
+    auto page_of = [&](uint32_t i) { return (uint32_t)table[i / e.pageSize]; };
+    auto at = [&](uint32_t page, uint32_t i) {
+        return cache + (((uint64_t)page * e.Nkv + hkv) * e.pageSize + i % e.pageSize) * e.rowUnits + unit;
     };
-    struct Rows {
+    for (uint32_t base = k.first; base < k.n; base += chunk) {
+        // step by step for all kDeep rows, so that their reads stand side by side
         U v[kDeep];
-        uint64_t to[kDeep];
-        bool moves[kDeep];
-    };
-    auto load = [&](uint32_t base, Rows &x) {
+        uint32_t i[kDeep], page[kDeep], to[kDeep];  // `to`: the page; none where the row stays
+#pragma unroll
+        for (uint32_t d = 0; d < kDeep; ++d) i[d] = (uint32_t)from[min(base + d * rows + row, k.n - 1)];
+#pragma unroll
+        for (uint32_t d = 0; d < kDeep; ++d) {
+            // (what is kept lies at or behind its place; a list that another call has left leads nowhere else)
+            i[d] = min(i[d], k.keys - 1);
+            page[d] = page_of(i[d]);
+            to[d] = page_of(min(base + d * rows + row, k.n - 1));
+        }
 #pragma unroll
         for (uint32_t d = 0; d < kDeep; ++d) {
             const uint32_t j = base + d * rows + row;
-            x.moves[d] = false;
-            if (j < k.n && mine) {
-                // (what is kept lies at or behind its place; a list that another call has left leads nowhere else)
-                const uint32_t i = min((uint32_t)from[j], k.keys - 1);
-                uint64_t src;
-                x.moves[d] = i > j && place(i, src) && place(j, x.to[d]);
-                if (x.moves[d]) x.v[d] = cache[src];
-            }
+            if (!(mine && j < k.n && i[d] > j && page[d] < e.pages && to[d] < e.pages)) to[d] = ~0u;
+            if (to[d] != ~0u) v[d] = *at(page[d], i[d]);
         }
-    };
-    Rows now, next;
-    load(k.first, now);
-    for (uint32_t base = k.first; base < k.n; base += chunk) {
         __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the rows have been read
         __syncthreads();
-        load(base + chunk, next);
 #pragma unroll
         for (uint32_t d = 0; d < kDeep; ++d)
-            if (now.moves[d]) cache[now.to[d]] = now.v[d];
-        now = next;
+            if (to[d] != ~0u) *at(to[d], base + d * rows + row) = v[d];
     }
 }
 
 }  // namespace
 
 #define EVICT_MOVE(name, U)                                                                                                   \
-    POPCORN_KERNEL void __launch_bounds__(1024) name(const int32_t *kept, const int32_t *tables, const int32_t *keyLens,      \
+    POPCORN_KERNEL void __launch_bounds__(1024, 8) name(const int32_t *kept, const int32_t *tables, const int32_t *keyLens,      \
                                                      const int32_t *budgets, U *kCache, U *vCache, EvictConstants e) {        \
         evict_move<U>(kept, tables, keyLens, budgets, kCache, vCache, e);                                                     \
     }
