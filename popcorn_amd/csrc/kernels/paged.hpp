@@ -157,9 +157,10 @@ PAGED_FN int32_t paged_prefix_keys(int32_t len, const PagedAttentionConstants &p
 
 // A unit's rows and keys in a call with prefixes.
 struct SharedRequest : PagedRequest {
-    bool prefix;     // a group's rows against its prefix
-    int32_t before;  // else: keys of the prefix before the request's own
-    int32_t lo;      // of a prefix: no row of it has a lower position
+    uint32_t prefix;  // 1: a group's rows against its prefix. (A word: with padding, copies of it went through LDS, by an address that the
+                      // compiler had each block read from the host's memory, 2 to 16 us.)
+    int32_t before;   // else: keys of the prefix before the request's own
+    int32_t lo;       // of a prefix: no row of it has a lower position
 };
 
 // Group v < groups: the rows of its requests, who follow each other, against its prefix; then the requests. positions: under a

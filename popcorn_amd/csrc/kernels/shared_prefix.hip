@@ -129,7 +129,7 @@ struct SharedPages {
         u.n = (int32_t)first_lane((uint32_t)q.n);
         u.pos0 = (int32_t)first_lane((uint32_t)q.pos0);
         u.keys = (int32_t)first_lane((uint32_t)q.keys);
-        u.prefix = first_lane(q.prefix) != 0;
+        u.prefix = first_lane(q.prefix);
         u.before = (int32_t)first_lane((uint32_t)q.before);
         u.lo = (int32_t)first_lane((uint32_t)q.lo);
         return u;
@@ -362,7 +362,7 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
     if (r.before > 0) {
         const int32_t *table = batch.table(g, p);
         pk::SharedRequest pre{};
-        pre.prefix = true;
+        pre.prefix = 1;
         const PagedAttentionConstants mp = batch.mask(pre, p);
         const int at = pk::paged_place(r, t, r.before);
         const pk::PagedSpan k = pk::paged_span(at, at, r.before, mp);
