@@ -198,6 +198,7 @@ constexpr uint32_t kKeys = 256, kStageRows = 64;
 struct WeightsBatch {
     static constexpr bool kShared = false, kPlanned = false;
     using Request = pk::PagedRequest;
+    using Tile = pk::PagedTile;
     struct Left {  // a unit that its block shares with others behind it
         uint32_t pieces, request, hkv, key0, keys, pad[3];
     };
@@ -495,7 +496,7 @@ POPCORN_KERNEL void __launch_bounds__(1024)
     u64 steps;
     uint32_t tiles;
     const WeightsBatch batch{starts, keyLens, nullptr, a};
-    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) {
+    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile, const auto &) {
         plan[1 + at] = pk::PagedTile{before, request, tile};
     });
     if (threadIdx.x == 0) plan[0] = pk::PagedTile{steps, tiles, 0};

@@ -163,6 +163,13 @@ struct SharedRequest : PagedRequest {
     int32_t lo;       // of a prefix: no row of it has a lower position
 };
 
+// An entry of the plan of such a call, with its request: a worker has its next piece by one read.
+struct SharedTile : PagedTile {
+    SharedRequest req;
+    uint32_t pad;
+};
+static_assert(sizeof(SharedTile) == 48, "the runtime's room for it");
+
 // Group v < groups: the rows of its requests, who follow each other, against its prefix; then the requests. positions: under a
 // window, each token's and then each group's least.
 PAGED_FN SharedRequest paged_shared(uint32_t v, const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,

@@ -8,7 +8,7 @@ POPCORN_KERNEL void __launch_bounds__(1024)
     u64 steps;
     uint32_t tiles;
     const OwnPages batch{nullptr, starts, keyLens, nullptr, {}};
-    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) {
+    lay_tiles<1024, u64>(batch, space, p, w, steps, tiles, [&](uint32_t at, u64 before, uint32_t request, uint32_t tile, const auto &) {
         plan[1 + at] = pk::PagedTile{before, request, tile};
     });
     if (threadIdx.x == 0) plan[0] = pk::PagedTile{steps, tiles, 0};

@@ -118,10 +118,10 @@ __device__ inline uint32_t row_tiles(const pk::PagedRequest &q, uint32_t G, cons
     return rows > w.fewRows && rows <= w.manyRows ? (rows + w.rows - 1) / w.rows : 0u;
 }
 
-// The tiles of every request, in request order: put(tile, steps before, request, tile of it).
+// The tiles of every request, in request order: put(tile, steps before, request, tile of it, its record). keep: gets the records of the first 64.
 template <uint32_t N, typename U, typename Batch, typename Put>
 __device__ inline void lay_tiles(const Batch &batch, PlanSpace<N, U, typename Batch::Request> &sp, const PagedAttentionConstants &p,
-                                 const PagedWorkConstants &w, U &steps, uint32_t &tiles, Put &&put) {
+                                 const PagedWorkConstants &w, U &steps, uint32_t &tiles, Put &&put, typename Batch::Request *keep = nullptr) {
     const uint32_t tid = threadIdx.x, G = p.Nq / p.Nkv, requests = batch.requests(p);
     steps = 0;
     tiles = 0;
@@ -136,6 +136,8 @@ __device__ inline void lay_tiles(const Batch &batch, PlanSpace<N, U, typename Ba
         const uint32_t here = (uint32_t)min(total, (U)(w.maxTiles - tiles));
         sp.tile[tid] = (uint32_t)min(upto - mine, (U)here);
         sp.req[tid] = q;
+        if constexpr (Batch::kShared)
+            if (keep && r < 64) keep[r] = q;
         __syncthreads();
         for (uint32_t t0 = 0; t0 < here; t0 += N) {
             const uint32_t t = t0 + tid;
@@ -147,7 +149,7 @@ __device__ inline void lay_tiles(const Batch &batch, PlanSpace<N, U, typename Ba
                 n = batch.steps(sp.req[i], t - sp.tile[i], p, w).n + w.unitSteps;
             }
             const pk::Scan<U> sum = pk::block_scan<N / 64>((U)n, sp.sums);
-            if (t < here) put(tiles + t, steps + sum.upto - n, base + i, t - sp.tile[i]);
+            if (t < here) put(tiles + t, steps + sum.upto - n, base + i, t - sp.tile[i], sp.req[i]);
             steps += sum.total;
         }
         tiles += here;
@@ -225,6 +227,7 @@ struct OwnPages {
     static constexpr bool kShared = false;   // states of all units go to records, not to a Shared
     static constexpr bool kPlanned = false;  // the plan is always in memory, and LDS is the caller's
     using Request = pk::PagedRequest;
+    using Tile = pk::PagedTile;
     using Left = Shared;
     struct More {};
     const int32_t *tables, *starts, *keyLens;
@@ -261,8 +264,9 @@ struct OwnPages {
 template <uint32_t NT, typename Batch, bool Wave = false>
 struct Dealer {
     const Batch batch;
-    const pk::PagedTile *plan;
+    const typename Batch::Tile *plan;
     const OwnTile *own;
+    const typename Batch::Request *keep;  // of up to 64 requests, whose own lines a piece would wait for again
     typename Batch::Left *left;  // (held here: read from the batch it cost the few-row kernels 200 moves of scalar registers)
     uint64_t share, x, end;
     uint32_t tile;
@@ -276,16 +280,16 @@ struct Dealer {
     using Space = PlanSpace<NT, uint32_t, typename Batch::Request>;
 
     // `space` is free again afterwards.
-    __device__ inline Dealer(const Batch &b, const pk::PagedTile *pl, OwnTile *ow, Space *space, const PagedAttentionConstants &p,
-                             const PagedWorkConstants &w)
-        : batch(b), plan(pl), own(ow), left(b.left + worker()) {
+    __device__ inline Dealer(const Batch &b, const typename Batch::Tile *pl, OwnTile *ow, Space *space, const PagedAttentionConstants &p,
+                             const PagedWorkConstants &w, typename Batch::Request *kp = nullptr)
+        : batch(b), plan(pl), own(ow), keep(kp), left(b.left + worker()) {
         uint32_t tiles;
         uint64_t total;
         if (!Batch::kPlanned && w.ownPlan) {
             uint32_t steps;
-            lay_tiles<NT, uint32_t>(batch, *space, p, w, steps, tiles, [&](uint32_t at, uint32_t before, uint32_t request, uint32_t t) {
-                ow[at] = OwnTile{before, request << 16 | t};
-            });
+            lay_tiles<NT, uint32_t>(
+                batch, *space, p, w, steps, tiles,
+                [&](uint32_t at, uint32_t before, uint32_t request, uint32_t t, const auto &) { ow[at] = OwnTile{before, request << 16 | t}; }, kp);
             total = (uint64_t)first_lane(steps) * p.Nkv;
             tiles = first_lane(tiles);
         } else {
@@ -310,14 +314,19 @@ struct Dealer {
             if (!Batch::kPlanned && w.ownPlan) {
                 const OwnTile o = own[tile];
                 t = pk::PagedTile{first_lane(o.before), first_lane(o.place >> 16), first_lane(o.place & 0xffffu)};
+                if constexpr (Batch::kShared) c.req = batch.requests(p) <= 64 ? keep[t.request] : batch.request(t.request, p);
+            } else if constexpr (Batch::kShared) {
+                const typename Batch::Tile e = plan[1 + tile];
+                t = pk::PagedTile{first_lane64(e.before), first_lane(e.request), first_lane(e.tile)};
+                c.req = e.req;
             } else {
                 t = plan[1 + tile];
                 t = pk::PagedTile{first_lane64(t.before), first_lane(t.request), first_lane(t.tile)};
             }
             c.request = t.request;
             c.tile = t.tile;
-            c.req = batch.request(t.request, p);
             if constexpr (Batch::kShared) c.req = Batch::uniform(c.req);
+            else c.req = batch.request(t.request, p);
             c.steps = batch.steps(c.req, t.tile, p, w);
             const pk::PagedPiece piece = pk::paged_piece(x - t.before * p.Nkv, end - x, c.steps.n, w);
             c.hkv = piece.hkv;
@@ -370,7 +379,7 @@ template <typename T, int HD, int RT, typename Batch, int WAVES = kWaves>
 __device__ void paged_few(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
                           const typename T::storage *__restrict__ V, const int32_t *__restrict__ tables,
                           const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
-                          const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
+                          const typename Batch::Tile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
                           typename Batch::Left *__restrict__ left, typename T::storage *__restrict__ out, const PagedAttentionConstants &all,
                           const PagedWorkConstants &w, const typename Batch::More &more, uint8_t *lds = nullptr) {
     using S = typename T::storage;
@@ -391,6 +400,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     uint8_t *const smem = Batch::kPlanned ? lds : sm_own;
     __shared__ float sm_m[kWaves][RT * 16], sm_l[kWaves][RT * 16];
     __shared__ OwnTile sm_plan[kOwnTiles];
+    __shared__ typename Batch::Request sm_req[64];
     __shared__ uint32_t sm_bad;
     // Q of 512 dims in 16 bits is kept in LDS: in registers 60 of 512 spilled, so 4 (32 requests of 100 to 8000 keys, 8 heads
     // on 2: 48 us, and 99; 1000 tokens behind as many 148 and 438)
@@ -407,7 +417,7 @@ __device__ void paged_few(const typename T::storage *__restrict__ Q, const typen
     const uint32_t D = all.Hd, G = all.Nq / all.Nkv;
     const float c2 = all.scale * kLog2e;
     const Batch batch{tables, starts, keyLens, left, more};
-    Dealer<64 * kWaves, Batch, WAVES == 1> dealer(batch, plan, sm_plan, reinterpret_cast<Space *>(smem), all, w);
+    Dealer<64 * kWaves, Batch, WAVES == 1> dealer(batch, plan, sm_plan, reinterpret_cast<Space *>(smem), all, w, sm_req);
     Piece<typename Batch::Request> c;
     while (dealer.next(c, all, w)) {
         decltype(auto) p = batch.mask(c.req, all);
@@ -829,7 +839,7 @@ template <typename T, int HD, typename Batch>
 __device__ void paged_tile(const typename T::storage *__restrict__ Q, const typename T::storage *__restrict__ K,
                            const typename T::storage *__restrict__ V, const int32_t *__restrict__ tables,
                            const int32_t *__restrict__ starts, const int32_t *__restrict__ keyLens,
-                           const pk::PagedTile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
+                           const typename Batch::Tile *__restrict__ plan, float *__restrict__ pO, float *__restrict__ pML,
                            typename Batch::Left *__restrict__ left, typename T::storage *__restrict__ out, const PagedAttentionConstants &all,
                            const PagedWorkConstants &w, const typename Batch::More &more, uint8_t *lds = nullptr) {
     using S = typename T::storage;

@@ -57,6 +57,7 @@ template <bool Planned>
 struct SharedPages {
     static constexpr bool kShared = true, kPlanned = Planned;
     using Request = pk::SharedRequest;
+    using Tile = pk::SharedTile;
     using Left = pk::u32x4;  // the rows' records, of prefixes and then of own keys
     struct More {
         const int32_t *prefixTables, *prefixLens, *groupStarts;
@@ -195,7 +196,7 @@ __device__ inline void token_position(uint32_t t, const int32_t *starts, const i
 // tokens' positions, which the blocks behind them write.
 POPCORN_KERNEL void __launch_bounds__(1024)
     shared_prefix_plan(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts, int32_t *positions,
-                       pk::PagedTile *plan, PagedAttentionConstants p, PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {
+                       pk::SharedTile *plan, PagedAttentionConstants p, PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {
     if (blockIdx.x > 1) {
         token_position((blockIdx.x - 2) * 1024 + threadIdx.x, starts, keyLens, prefixLens, groupStarts, positions, p, s);
         return;
@@ -216,10 +217,12 @@ POPCORN_KERNEL void __launch_bounds__(1024)
     u64 steps;
     uint32_t tiles;
     const PagedWorkConstants w = blockIdx.x ? few : many;
-    pk::PagedTile *to = plan + (blockIdx.x ? many.maxTiles + 1 : 0u);
+    pk::SharedTile *to = plan + (blockIdx.x ? many.maxTiles + 1 : 0u);
     lay_tiles<1024, u64>(batch, space, p, w, steps, tiles,
-                         [&](uint32_t at, u64 before, uint32_t request, uint32_t tile) { to[1 + at] = pk::PagedTile{before, request, tile}; });
-    if (threadIdx.x == 0) to[0] = pk::PagedTile{steps, tiles, 0};
+                         [&](uint32_t at, u64 before, uint32_t request, uint32_t tile, const pk::SharedRequest &req) {
+                             to[1 + at] = pk::SharedTile{{before, request, tile}, req, 0};
+                         });
+    if (threadIdx.x == 0) to[0] = pk::SharedTile{{steps, tiles, 0}, {}, 0};
 }
 
 // The same for the few-row kernel alone, which lays out its plan by itself: blocks take tokens, or those past them four groups. A
@@ -406,7 +409,7 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 // Few rows alone.
 #define SHARED_FEW(t, T, HD, RT, PER_CU)                                                                                     \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        shared_prefix_few_##t##_d##HD##_r##RT(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, \
+        shared_prefix_few_##t##_d##HD##_r##RT(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, \
                                               float *pML, pk::u32x4 *records, T::storage *out, float *lse,                   \
                                               PagedAttentionConstants p, PagedWorkConstants w, SharedPrefixConstants s) {    \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
@@ -418,12 +421,12 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 // the requests of few, which memory bounds; so both are busy at once.
 #define SHARED_BOTH(t, T, HD, PER_CU)                                                                                        \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        shared_prefix_both_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, float *pML, \
+        shared_prefix_both_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
                                        PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {           \
         __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
         using Pages = SharedPages<true>;                                                                                     \
-        const pk::PagedTile *planFew = plan + many.maxTiles + 1;                                                             \
+        const pk::SharedTile *planFew = plan + many.maxTiles + 1;                                                             \
         const uint32_t tileBlocks = tile_blocks(plan[0].before, planFew[0].before);                                          \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
         if (blockIdx.x < tileBlocks) {                                                                                       \
@@ -440,7 +443,7 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 // 2048 tokens behind 8192 keys, bf16: 332 us, and 251).
 #define SHARED_MANY(t, T, HD, PER_CU)                                                                                        \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        shared_prefix_many_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::PagedTile *plan, float *pO, float *pML, \
+        shared_prefix_many_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
                                        PagedWorkConstants w, SharedPrefixConstants s) {                                      \
         __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \

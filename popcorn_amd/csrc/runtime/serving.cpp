@@ -323,10 +323,10 @@ public:
         const int64_t tiles = both_ ? (int64_t)many_.maxTiles + few_.maxTiles + 2 : few_.ownPlan ? 0 : (int64_t)few_.maxTiles + 1;
         const int64_t o = (int64_t)sc_.states * hdp_ * 4, ml = cdiv((int64_t)sc_.states * 8, 16) * 16, rec = 2 * (int64_t)sc_.rows * 16;
         const int64_t positions = sc_.windowed ? ((int64_t)pc_.T + sc_.groups) * 4 : 0;
-        enc.withTemporaryTensor(ScratchSpec{{o + ml + rec + tiles * 16 + positions}, DataType::u8}, [&](Tensor scratch) {
+        enc.withTemporaryTensor(ScratchSpec{{o + ml + rec + tiles * kTile + positions}, DataType::u8}, [&](Tensor scratch) {
             auto part = [&](int64_t at, int64_t bytes) { return Tensor((char *)scratch.data + at, Shape({bytes}), DataType::u8); };
-            const Tensor pO = part(0, o), pML = part(o, ml), records = part(o + ml, rec), plan = part(o + ml + rec, tiles * 16);
-            const Tensor pos = part(o + ml + rec + tiles * 16, positions);
+            const Tensor pO = part(0, o), pML = part(o, ml), records = part(o + ml, rec), plan = part(o + ml + rec, tiles * kTile);
+            const Tensor pos = part(o + ml + rec + tiles * kTile, positions);
             const Tensor &starts = in_[4], &lens = in_[5], &prefixLens = in_[7], &groups = in_[8];
             const std::vector<Binding> lengths = {{starts, kRead}, {lens, kRead}, {prefixLens, kRead}, {groups, kRead}};
             auto with = [](std::vector<Binding> b, std::initializer_list<Binding> more) {
@@ -357,8 +357,8 @@ public:
             if (before_.empty()) {
                 attend(fn_, plan, consts, blocks_);
             } else {
-                const int64_t first = ((int64_t)many_.maxTiles + 1) * 16;
-                attend(before_, part(o + ml + rec + first, tiles * 16 - first), {bytesOf(pc_), bytesOf(few_), bytesOf(sc_)}, few_.workers / 4);
+                const int64_t first = ((int64_t)many_.maxTiles + 1) * kTile;
+                attend(before_, part(o + ml + rec + first, tiles * kTile - first), {bytesOf(pc_), bytesOf(few_), bytesOf(sc_)}, few_.workers / 4);
                 attend(fn_, plan, {bytesOf(pc_), bytesOf(many_), bytesOf(sc_)}, blocks_);
             }
             launch(enc, merge_,
@@ -369,6 +369,7 @@ public:
 
 private:
     static constexpr uint32_t kFewRows = 32;
+    static constexpr int64_t kTile = 48;  // bytes of a plan's entry
 
     double tileSteps(const PagedWorkConstants &w) const {
         return (double)cdiv((int64_t)std::max(pc_.columns, sc_.columns) * pc_.pageSize + w.stepKeys, w.stepKeys) + w.unitSteps;
