@@ -406,12 +406,15 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 #define SHARED_PARAMS(T)                                                                                                     \
     const T::storage *q, const T::storage *k, const T::storage *v, const int32_t *tables, const int32_t *starts,             \
         const int32_t *keyLens, const int32_t *prefixTables, const int32_t *prefixLens, const int32_t *groupStarts
+// (Rows of a tile and keys of a step are the kernels' own, as the plan has them: known here they are shifts, not divisions.)
 // Few rows alone.
 #define SHARED_FEW(t, T, HD, RT, PER_CU)                                                                                     \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
         shared_prefix_few_##t##_d##HD##_r##RT(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, \
                                               float *pML, pk::u32x4 *records, T::storage *out, float *lse,                   \
                                               PagedAttentionConstants p, PagedWorkConstants w, SharedPrefixConstants s) {    \
+        w.rows = 16 * RT;                                                                                                    \
+        w.stepKeys = sizeof(T::storage) == 4 ? 16 : 32;                                                                      \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
         const SharedPages<false>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};              \
         paged_few<T, HD, RT, SharedPages<false>, HD == 512 ? kWaves : 1>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, \
@@ -428,6 +431,10 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
         using Pages = SharedPages<true>;                                                                                     \
         const pk::SharedTile *planFew = plan + many.maxTiles + 1;                                                             \
         const uint32_t tileBlocks = tile_blocks(plan[0].before, planFew[0].before);                                          \
+        many.rows = 128;                                                                                                     \
+        many.stepKeys = 64;                                                                                                  \
+        few.rows = 16;                                                                                                       \
+        few.stepKeys = 32;                                                                                                   \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
         if (blockIdx.x < tileBlocks) {                                                                                       \
             many.workers = tileBlocks;                                                                                       \
@@ -447,6 +454,8 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
                                        PagedWorkConstants w, SharedPrefixConstants s) {                                      \
         __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
+        w.rows = 128;                                                                                                        \
+        w.stepKeys = 64;                                                                                                     \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
         const SharedPages<true>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};               \
         paged_tile<T, HD, SharedPages<true>>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, w, more, lds); \
