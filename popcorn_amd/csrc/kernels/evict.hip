@@ -2,9 +2,8 @@
 //   n = min(keys, budget), first' = min(first, n), last' = min(last, n - first'): a KV head of a request keeps its first' first
 //   and last' last keys and, of those between, the n - first' - last' of the highest weight (ties: the lowest index; NaN is
 //   the lowest weight). evict_select says which, in index order, and evict_move brings their rows to the front.
-// The choice is bound by its passes, the moves by rows of 128 bytes that lie apart. Where: 48 requests of 300 to 8000 keys cut to
-// 1000, 8 heads of 128 in 16 bits: 15 us and 104 (120 MB read, 115 MB written: 2.3 TB/s; the reads alone take 67, the writes alone 41;
-// torch's index_select of as many 256-byte rows has the same rate).
+// The choice is bound by its passes, the moves by rows that lie apart: 48 requests of 300 to 8000 keys cut to 1000, 8 heads of 128 in
+// 16 bits take 14 us and 58 (120 MB read, 115 MB written: 4.1 TB/s, where a copy of 2 GiB reaches 4.85).
 #include "paged.hpp"
 #include "scan.hpp"
 
@@ -22,11 +21,12 @@ constexpr uint32_t kTile = 4096;  // weights of a block's pass, four in a row to
 constexpr uint32_t kHeld = 4;     // passes whose weights a block holds in registers
 // Counters of a bin, the even threads' and the odd ones': additions of a wave to one word take a cycle each. (One request of 4 heads
 // of 8191 weights, uniform in 0 to 1, in 1 to 1.05, all equal: 16, 18 and 23 us with short rows' moves; with one counter 17, 22 and 33;
-// with four 17, 17 and 18, but 48 requests' 8 heads 16 us instead of 15.)
-constexpr uint32_t kCopies = 2, kBinStride = kBins + 8;
+// with four 17, 17 and 18, but 48 requests' 8 heads 16 us instead of 15.) For more weights than a block holds
+// eight: 8 heads of 100000, the choice alone, 78, 78 and 78, and with two 76, 106 and 171.
+constexpr uint32_t kHeldCopies = 2, kLongCopies = 8, kBinStride = kBins + 8;
 
 struct SelectSpace {
-    __attribute__((aligned(16))) uint32_t bins[kBinStride * kCopies];
+    __attribute__((aligned(16))) uint32_t bins[kBinStride * kLongCopies];
     uint32_t sums[16], found[3][2];
 };
 
@@ -34,28 +34,33 @@ struct SelectSpace {
 template <bool HELD>
 __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictKeep &k, int32_t *__restrict__ to, float *__restrict__ toW,
                                    SelectSpace &sp) {
+    constexpr uint32_t kCopies = HELD ? kHeldCopies : kLongCopies;
     const uint32_t tid = threadIdx.x, tiles = (k.keys + kTile - 1) / kTile;
     struct Four {
         float v[4];
     };
     auto first_of = [&](uint32_t tile) { return HELD ? (tid * tiles + tile) * 4 : tile * kTile + tid * 4; };
+    // read without a branch, so that the next read need not wait for it; the last weights, where a thread has fewer than four, again
     auto read = [&](uint32_t tile) {
-        const uint32_t i = first_of(tile);
         Four f{};
-        if (i + 4 <= k.keys) {
-            __builtin_memcpy(&f, w + i, sizeof(f));
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-                if (i + j < k.keys) f.v[j] = w[i + j];
-        }
+        if (k.keys >= 4) __builtin_memcpy(&f, w + min(first_of(tile), k.keys - 4), sizeof(f));
         return f;
+    };
+    auto whole = [&](uint32_t tile, Four &f) {
+        const uint32_t i = first_of(tile);
+        if (i + 4 > k.keys) {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) f.v[j] = i + j < k.keys ? w[i + j] : 0.0f;
+        }
     };
     Four held[HELD ? kHeld : 1];
     if constexpr (HELD) {
 #pragma unroll
         for (uint32_t t = 0; t < kHeld; ++t)
             if (t < tiles) held[t] = read(t);
+#pragma unroll
+        for (uint32_t t = 0; t < kHeld; ++t)
+            if (t < tiles) whole(t, held[t]);
     }
     auto each = [&](auto &&body) {  // body(first index, its four weights)
         if constexpr (HELD) {
@@ -65,8 +70,9 @@ __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictK
         } else {
             Four next = read(0);
             for (uint32_t t = 0; t < tiles; ++t) {
-                const Four f = next;
+                Four f = next;
                 if (t + 1 < tiles) next = read(t + 1);
+                whole(t, f);
                 body(first_of(t), f);
             }
         }
@@ -83,7 +89,10 @@ __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictK
         clear();
         __syncthreads();
     }
-    for (int pass = 0; pass < 3 && need > 0; ++pass) {
+    // (unrolled, so that its shifts are constants: 48 requests' 8 heads 13.7 us, and 15.1)
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+        if (need == 0) break;
         const uint32_t bits = pass < 2 ? 11u : 10u, above = shift;
         shift -= bits;
         each([&](uint32_t base, const Four &f) {
@@ -174,9 +183,9 @@ __device__ inline void select_kept(const float *__restrict__ w, const pk::EvictK
 
 // A block per (request, KV head). The least kept weight by three counts of its bits (11, 11 and 10), then one pass in
 // order that numbers what is kept: no sort, and no atomics but the counts', so equal weights leave the lowest index whatever
-// the order of waves. Up to 16384 weights stay in registers between the passes (8191 of them: 10 us; read for each pass, 14). One request's
+// the order of waves. Up to 16384 weights stay in registers between the passes (8191 of them: 9 us; read for each pass, 14). One request's
 // 4 heads leave 252 CUs idle; several blocks to a head would have to wait for each other's counts three times (one of 100000 keys, cut to
-// a quarter: 76 us, and the moves 80).
+// a quarter: 80 us).
 POPCORN_KERNEL void __launch_bounds__(1024, 8)
     evict_select(const float *weights, const int32_t *keyLens, const int32_t *budgets, int32_t *kept, float *keptWeights, EvictConstants e) {
     __shared__ SelectSpace space;
@@ -223,7 +232,8 @@ __device__ void evict_move(const int32_t *__restrict__ kept, const int32_t *__re
         return cache + (((uint64_t)page * e.Nkv + hkv) * e.pageSize + i % e.pageSize) * e.rowUnits + unit;
     };
     for (uint32_t base = k.first; base < k.n; base += chunk) {
-        // step by step for all kDeep rows, so that their reads stand side by side
+        // step by step for all kDeep rows, so that their reads stand side by side (row by row 69 us, and 58; with the next chunk's rows read
+        // before these are written, in registers that leave a CU one block, 104)
         U v[kDeep];
         uint32_t i[kDeep], page[kDeep], to[kDeep];  // `to`: the page; none where the row stays
 #pragma unroll

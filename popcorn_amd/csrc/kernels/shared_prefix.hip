@@ -9,10 +9,10 @@
 // A row has two units, each in one piece or several; a row's record of a unit (u32x4) says
 // where the states of its pieces lie, and the merge adds them all:
 //   O = sum O_i 2^(m_i - M) / L, L = sum l_i 2^(m_i - M), lse = (M + log2 L) ln 2.
-// What bounds it: small calls their chain of dependent reads (lengths, table, keys: 8 us of a kernel) and the merge's launch
-// (4 us): 2 requests behind 777 keys 27 us in all, where their bytes take 1; large batches the cold reads of
-// many short stretches of pages (256 requests behind 4000 keys, 136 MB: 45 us beside 14 for the plan and the merge, 3.0 TB/s, as torch.sum
-// of 111 MB reads); prompts the products, whose weights are two bf16 words (128 requests of 16 new tokens behind 16384 keys: 88 us).
+// What bounds it: small calls their chain of dependent reads (lengths 3 us, the piece 2, table and q 1, two steps 6, the store 2) and
+// the merge's launch (4): 2 requests behind up to 1024 keys 20 us in all, where their bytes take 1; large batches the cold reads of
+// many short stretches of pages (64 requests of 50 to 1500 own keys behind 8192, 142 MB: 43 us, 3.3 TB/s, beside 14 for the plan and
+// the merge; torch.sum reads 111 MB at 3.0), and in bf16 the products with weights of two words (256 behind 16384, 35 GFLOP: 88 us).
 #include "paged_attention.hpp"
 
 namespace {
@@ -22,7 +22,7 @@ constexpr uint32_t kBehindPrefix = 1u << 31;  // in the last word of a row's rec
 
 // The groups of a call, a lane of every wave for each where there are up to 64 (else read where they are asked for): a unit's
 // group would take loads that wait for each other. Not in LDS: beside another array there the compiler has every read of LDS wait
-// for the latest copy into it (64 requests behind 8192 keys: 95 us, and 65).
+// for the latest copy into it (256 requests behind 16384 keys, the prefix alone: 95 us, and 65).
 struct HeldGroups {
     int32_t end, len, first;  // of the lane's group; first: where group 0 begins, in every lane
     uint32_t n;
@@ -189,7 +189,7 @@ __device__ inline void token_position(uint32_t t, const int32_t *starts, const i
 
 }  // namespace
 
-// The plan, before a launch that two kinds of work share: 5 to 7 us, four cold reads that wait for each other and the scan. (Each block
+// The plan, before a launch that two kinds of work share: 5 us, reads that wait for each other and the scan. (Each block
 // by itself would take as long, and its lists the LDS of the copies.)
 // Block 0 lays out the tiles of many rows, block 1 those of few (of the few-row kernel alone there is just block 0: many is few). Each
 // plan's entry 0: the counted steps, the number of tiles. Under a window both write each group's least position first, behind the
@@ -226,7 +226,7 @@ POPCORN_KERNEL void __launch_bounds__(1024)
 }
 
 // The same for the few-row kernel alone, which lays out its plan by itself: blocks take tokens, or those past them four groups. A
-// launch (24 requests 4.7 us), since a prefix's rows belong to many requests: a wave would search for each of its rows.
+// launch (24 requests 4 us), since a prefix's rows belong to many requests: a wave would search for each of its rows.
 POPCORN_KERNEL void __launch_bounds__(256)
     shared_prefix_positions(const int32_t *starts, const int32_t *keyLens, const int32_t *prefixLens, const int32_t *groupStarts,
                             int32_t *positions, PagedAttentionConstants p, SharedPrefixConstants s) {
@@ -250,7 +250,7 @@ __device__ inline uint32_t tile_blocks(u64 many, u64 few) {
 // A row's pieces, of its prefix and of its own keys, by one wave or the block's four (s.parts): their maximum and sum first,
 // a lane for a piece, then their O, HD / 4 lanes for a piece. Bound by its launch and two rounds of reads, the records and what they
 // lead to: a row's own record says that there is a prefix's. (Looked up in starts and groups it took two rounds more: 16 rows 5.0 us, and
-// 4.2; 6000 rows 10, and 9.) The rest is the states themselves, 20 and more of 512 bytes for each of 2048 rows behind 8192 keys: 9 us.
+// 4.2; 6000 rows 10, and 9.) The rest is the states themselves, of 512 bytes each in 128 dims (2048 rows behind 8192 keys: 9 us).
 template <typename T, int HD>
 __device__ void shared_prefix_merge(const float *__restrict__ pO, const float *__restrict__ pML, const pk::u32x4 *__restrict__ records,
                                     const int32_t *__restrict__ starts, typename T::storage *__restrict__ out, float *__restrict__ lse,
