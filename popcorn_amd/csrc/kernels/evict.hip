@@ -22,7 +22,7 @@ constexpr uint32_t kHeld = 4;     // passes whose weights a block holds in regis
 // Counters of a bin, the even threads' and the odd ones': additions of a wave to one word take a cycle each. (One request of 4 heads
 // of 8191 weights, uniform in 0 to 1, in 1 to 1.05, all equal: 16, 18 and 23 us with short rows' moves; with one counter 17, 22 and 33;
 // with four 17, 17 and 18, but 48 requests' 8 heads 16 us instead of 15.) For more weights than a block holds
-// eight: 8 heads of 100000, the choice alone, 78, 78 and 78, and with two 76, 106 and 171.
+// eight (8 heads of 100000, the choice alone: 78, 80 and 83 us; with two 76, 106 and 171).
 constexpr uint32_t kHeldCopies = 2, kLongCopies = 8, kBinStride = kBins + 8;
 
 struct SelectSpace {
