@@ -124,12 +124,18 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
             u32x4 kf[KM][KS];
             float old[KM];
             bool ok[KM];
+            // lane l holds the page of group held0 + l, so that no read of K waits for its page (54.5 us above, and 53.8)
+            uint32_t held0 = 0, heldPage = 0;
+            auto hold = [&](uint32_t grp) {
+                held0 = grp;
+                heldPage = grp + lane < g1 ? (uint32_t)table[(grp + lane) * 16 / p.pageSize] : ~0u;
+            };
             auto load = [&](uint32_t grp) {
 #pragma unroll
                 for (int m = 0; m < KM; ++m) {
                     const uint32_t key = (grp + m) * 16, column = key / p.pageSize;
                     const bool in = grp + m < g1;
-                    const uint32_t page = in ? (uint32_t)table[column] : ~0u;
+                    const uint32_t page = (uint32_t)__builtin_amdgcn_readlane((int)heldPage, (int)(grp + m - held0));
                     ok[m] = page < p.pages;
                     const uint64_t off = ok[m] ? (((uint64_t)page * p.Nkv + hkv) * p.pageSize + (key - column * p.pageSize)) * D : 0;
                     const int bytes = ok[m] ? (int)(min(16u, keys - key) * D * (uint32_t)sizeof(S)) : 0;
@@ -144,6 +150,7 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
                     if (in && c16 < 4 && key + 4 * g + c16 < keys) old[m] = to[key + 4 * g + c16];
                 }
             };
+            hold(g0);
             load(g0);
             for (uint32_t grp = g0; grp < g1; grp += KM) {
                 pk::f32x4 st[KM];
@@ -165,7 +172,10 @@ __device__ void weights_few(const typename T::storage *__restrict__ Q, const typ
                     was[m] = old[m];
                     held[m] = ok[m];
                 }
-                if (grp + KM < g1) load(grp + KM);
+                if (grp + KM < g1) {
+                    if (grp + KM - held0 == 64) hold(grp + KM);
+                    load(grp + KM);
+                }
 #pragma unroll
                 for (int m = 0; m < KM; ++m) {
                     const uint32_t key0 = (grp + m) * 16 + 4 * g;
