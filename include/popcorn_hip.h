@@ -638,7 +638,8 @@ popcorn_status_t popcorn_kernel_paged_attention(const popcorn_tensor_t *q, const
  * exp(scale q.k) over the keys it sees: -infinity where it sees none.
  * prefix_tables, prefix_lens and group_starts may be NULL together: no request has a
  * prefix, and this is PagedAttention with its lse. Everything else as for PagedAttention; the results
- * are the same to rounding. Pages that a group shares are read only. */
+ * are the same to rounding, with no fewer bits of a weight than PagedAttention has for
+ * the same max_query_len. Pages that a group shares are read only. */
 popcorn_status_t popcorn_kernel_shared_prefix_attention(
     const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache, const popcorn_tensor_t *v_cache, const popcorn_tensor_t *prefix_tables,
     const popcorn_tensor_t *prefix_lens, const popcorn_tensor_t *group_starts, const popcorn_tensor_t *page_tables,

@@ -225,6 +225,7 @@ struct Shared {
 // the worker that begins one leaves a Shared to the merge.
 struct OwnPages {
     static constexpr bool kShared = false;   // states of all units go to records, not to a Shared
+    static constexpr bool kTwoWords = false;  // weights of f16 tiles of many rows in two words
     static constexpr bool kPlanned = false;  // the plan is always in memory, and LDS is the caller's
     using Request = pk::PagedRequest;
     using Tile = pk::PagedTile;
@@ -848,9 +849,10 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
     constexpr int kCopies = 16 / kRowsPer;  // instructions for a wave's 16 rows of K (or V) of a step
     // The words of a weight in the product with V. One bf16 has 8 bits, so there are two, 2^-16 off. One f16 has 11, as many as
     // the result: 2048 tokens behind 8192 keys, 8 heads of 256 on 4, are 2.9e-4 off (2-norm, against 64 bits) in 193 us; with two
-    // words 2.1e-4, which the rounding of the result alone makes, in 250 (1000 tokens of 128 dims 70 and 88). As FlashAttention.
-    constexpr bool kTwo = std::is_same<T, pk::BF16>::value;
-    constexpr float kLead = kTwo ? 0.0f : 4.0f;
+    // words 2.1e-4, which the rounding of the result alone makes, in 250 (1000 tokens of 128 dims 70 and 88). As FlashAttention. But
+    // behind a shared prefix tiles have the rows of decoding requests too, who alone would have two (paged_few): there two.
+    constexpr bool kTwo = std::is_same<T, pk::BF16>::value || Batch::kTwoWords;
+    constexpr float kLead = std::is_same<T, pk::F16>::value ? 4.0f : 0.0f;
     constexpr uint32_t kTileBytes = BKV * HD * 2;
     // K's two places, V's two, the plan (one array: with two, the compiler has every read of LDS wait for the latest copy)
     __shared__ __attribute__((aligned(256))) uint8_t sm_own[Batch::kPlanned ? 16 : 4 * kTileBytes + kOwnTiles * sizeof(OwnTile)];
@@ -1002,7 +1004,7 @@ __device__ void paged_tile(const typename T::storage *__restrict__ Q, const type
             ps += p0 + p1;
             uint32_t v = pk::pack2<T>(p0, p1);
             if constexpr (kTwo) {
-                uint32_t r = pk::pack2<T>(p0 - __uint_as_float(v << 16), p1 - __uint_as_float(v & 0xffff0000u));
+                uint32_t r = pk::pack2<T>(p0 - pk::from_bits16<T>(v & 0xffffu), p1 - pk::from_bits16<T>(v >> 16));  // exact
                 asm volatile("" : "+v"(r));
                 pr[pair / 4][pair % 4] = r;
             }

@@ -11,8 +11,8 @@
 //   O = sum O_i 2^(m_i - M) / L, L = sum l_i 2^(m_i - M), lse = (M + log2 L) ln 2.
 // What bounds it: small calls their chain of dependent reads (lengths 3 us, the piece 2, table and q 1, two steps 6, the store 2) and
 // the merge's launch (4): 2 requests behind up to 1024 keys 20 us in all, where their bytes take 1; large batches the cold reads of
-// many short stretches of pages (64 requests of 50 to 1500 own keys behind 8192, 142 MB: 43 us, 3.3 TB/s, beside 14 for the plan and
-// the merge; torch.sum reads 111 MB at 3.0), and in bf16 the products with weights of two words (256 behind 16384, 35 GFLOP: 88 us).
+// many short stretches of pages (64 requests of 50 to 1500 own keys behind 8192, 142 MB: 46 us, 3.1 TB/s, beside 14 for the plan and
+// the merge; torch.sum reads 111 MB at 3.0), and the products with weights of two words (256 behind 16384, bf16, 35 GFLOP: 88 us).
 #include "paged_attention.hpp"
 
 namespace {
@@ -53,9 +53,9 @@ struct HeldGroups {
     }
 };
 
-template <bool Planned>
+template <bool Planned, bool TwoWords = false>
 struct SharedPages {
-    static constexpr bool kShared = true, kPlanned = Planned;
+    static constexpr bool kShared = true, kPlanned = Planned, kTwoWords = TwoWords;
     using Request = pk::SharedRequest;
     using Tile = pk::SharedTile;
     using Left = pk::u32x4;  // the rows' records, of prefixes and then of own keys
@@ -420,16 +420,17 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
         paged_few<T, HD, RT, SharedPages<false>, HD == 512 ? kWaves : 1>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, \
                                                                          out, p, w, more);                                   \
     }
+// WORDS, TWO: whether weights of the tiles have two words.
 // Many rows and few in one launch: the first blocks take tiles of many rows, which the matrix cores bound, the others, a wave each,
 // the requests of few, which memory bounds; so both are busy at once.
-#define SHARED_BOTH(t, T, HD, PER_CU)                                                                                        \
+#define SHARED_BOTH(t, T, HD, PER_CU, WORDS, TWO)                                                                              \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        shared_prefix_both_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
+        shared_prefix_both_##t##_d##HD##WORDS(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
                                        PagedWorkConstants many, PagedWorkConstants few, SharedPrefixConstants s) {           \
         __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
-        using Pages = SharedPages<true>;                                                                                     \
-        const pk::SharedTile *planFew = plan + many.maxTiles + 1;                                                             \
+        using Pages = SharedPages<true, TWO>;                                                                                \
+        const pk::SharedTile *planFew = plan + many.maxTiles + 1;                                                            \
         const uint32_t tileBlocks = tile_blocks(plan[0].before, planFew[0].before);                                          \
         many.rows = 128;                                                                                                     \
         many.stepKeys = 64;                                                                                                  \
@@ -448,17 +449,17 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
     }
 // Many rows alone: beside the few-row kernel's code those of 256 dims, which take all registers, spilled 51 to 65 of them (a prompt of
 // 2048 tokens behind 8192 keys, bf16: 332 us, and 251).
-#define SHARED_MANY(t, T, HD, PER_CU)                                                                                        \
+#define SHARED_MANY(t, T, HD, PER_CU, WORDS, TWO)                                                                              \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
-        shared_prefix_many_##t##_d##HD(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
+        shared_prefix_many_##t##_d##HD##WORDS(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
                                        PagedWorkConstants w, SharedPrefixConstants s) {                                      \
         __shared__ __attribute__((aligned(256))) uint8_t lds[4 * 64 * HD * 2];                                               \
         w.rows = 128;                                                                                                        \
         w.stepKeys = 64;                                                                                                     \
         const HeldGroups held(groupStarts, prefixLens, s);                                                                   \
-        const SharedPages<true>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};               \
-        paged_tile<T, HD, SharedPages<true>>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, w, more, lds); \
+        const SharedPages<true, TWO>::More more{prefixTables, prefixLens, groupStarts, positions, lse, held, s, 0};          \
+        paged_tile<T, HD, SharedPages<true, TWO>>(q, k, v, tables, starts, keyLens, plan, pO, pML, records, out, p, w, more, lds); \
     }
 #define SHARED_MERGE(t, T, HD)                                                                                               \
     POPCORN_KERNEL void __launch_bounds__(256)                                                                               \
@@ -497,9 +498,12 @@ SHARED_ALL(f16, F16, 2)
 SHARED_ALL(bf16, BF16, 2)
 SHARED_FEW(f16, F16, 256, 2, 1)
 SHARED_FEW(bf16, BF16, 256, 2, 1)
-SHARED_BOTH(f16, F16, 64, 2)
-SHARED_BOTH(f16, F16, 128, 2)
-SHARED_MANY(f16, F16, 256, 1)
-SHARED_BOTH(bf16, BF16, 64, 2)
-SHARED_BOTH(bf16, BF16, 128, 2)
-SHARED_MANY(bf16, BF16, 256, 1)
+SHARED_BOTH(f16, F16, 64, 2, , false)
+SHARED_BOTH(f16, F16, 128, 2, , false)
+SHARED_MANY(f16, F16, 256, 1, , false)
+SHARED_BOTH(f16, F16, 64, 2, _two, true)
+SHARED_BOTH(f16, F16, 128, 2, _two, true)
+SHARED_MANY(f16, F16, 256, 1, _two, true)
+SHARED_BOTH(bf16, BF16, 64, 2, , true)
+SHARED_BOTH(bf16, BF16, 128, 2, , true)
+SHARED_MANY(bf16, BF16, 256, 1, , true)

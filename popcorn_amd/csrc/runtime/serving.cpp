@@ -145,6 +145,30 @@ int deviceCUs() {
     return cachedCUs;
 }
 
+// Rows (new tokens x heads of a KV head's group) up to which a request counts as one of few, and of the longest request.
+constexpr uint32_t kFewRows = 32;
+int64_t longestRows(const PagedAttentionConstants &pc, int64_t maxQueryLen) {
+    return std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T) * (pc.Nq / pc.Nkv);
+}
+int tilesPerCU(int64_t hdp) { return hdp == 256 ? 1 : 2; }
+
+// What PagedAttention uses its tile kernel for: nothing, all requests, or (apart) those of many rows, beside a launch for the others.
+struct TileUse {
+    bool tiles, apart;
+};
+TileUse tileUse(const Tensor &q, const PagedAttentionConstants &pc, int64_t hdp, int64_t longest) {
+    // The tile kernel works on the magnitude of the scale (not 0) and 16-bit K and V of up to 256 dims. For requests of up to
+    // 32 rows, or so few rows in all, the tiles' 128 rows cost more than reading keys again: us of the few-row kernel and of
+    // tiles, 4 heads to a KV head, 8 KV heads, 4000 keys: one request of 64 rows 26 and 33 (Hd 128), 34 and 43 (256), of 128
+    // rows 27 and 40, 38 and 46 (but 96 and 67 behind 16000 keys), of 256 rows 33 and 39, 54 and 47.
+    const bool tiles = q.dataType != DataType::f32 && hdp <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows &&
+                       (int64_t)pc.T * (pc.Nq / pc.Nkv) > (hdp == 256 ? 64 : 128);
+    // Beside tiles, the requests of few rows have a launch of their own where there are more units than blocks: one request of
+    // 500 tokens among 256 of up to 1000 keys on 8 KV heads of 128, 80 us and 107 in tiles alone, 128 on 4 of 256 72 and 88;
+    // but as many units as blocks (64 of up to 8000 keys on 8) 81 and 78, 12 requests of few keys 41 and 31.
+    return {tiles, tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU(hdp) * deviceCUs()};
+}
+
 // PagedAttention on the matrix cores (paged_attention.hip): requests of few
 // rows (new tokens x heads of a KV head's group) and of many by a launch each,
 // with plans of tiles where the blocks do not lay them out themselves, and the
@@ -154,22 +178,12 @@ public:
     PagedAttentionKernel(const Tensor &q, const Tensor &k, const Tensor &v, const Tensor &tables, const Tensor &starts, const Tensor &lens,
                          const Tensor &out, const PagedAttentionConstants &pc, int64_t maxQueryLen)
         : q_(q), k_(k), v_(v), tables_(tables), starts_(starts), lens_(lens), out_(out), pc_(pc) {
-        const int64_t G = pc.Nq / pc.Nkv, longest = std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T) * G;
+        const int64_t longest = longestRows(pc, maxQueryLen);
         const bool f32 = q.dataType == DataType::f32;
         hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
         merge_ = "paged_attention_merge_" + type + hd;
-        // The tile kernel works on the magnitude of the scale (not 0) and 16-bit K and V of up to 256 dims. For requests of up to
-        // 32 rows, or so few rows in all, the tiles' 128 rows cost more than reading keys again: us of the few-row kernel and of
-        // tiles, 4 heads to a KV head, 8 KV heads, 4000 keys: one request of 64 rows 26 and 33 (Hd 128), 34 and 43 (256), of 128
-        // rows 27 and 40, 38 and 46 (but 96 and 67 behind 16000 keys), of 256 rows 33 and 39, 54 and 47.
-        const int tilesPerCU = hdp_ == 256 ? 1 : 2;
-        const bool tiles = !f32 && hdp_ <= 256 && pc.scale != 0.0f && pc.scale == pc.scale && longest > kFewRows &&
-                           (int64_t)pc.T * G > (hdp_ == 256 ? 64 : 128);
-        // Beside tiles, the requests of few rows have a launch of their own where there are more units than blocks: one request of
-        // 500 tokens among 256 of up to 1000 keys on 8 KV heads of 128, 80 us and 107 in tiles alone, 128 on 4 of 256 72 and 88;
-        // but as many units as blocks (64 of up to 8000 keys on 8) 81 and 78, 12 requests of few keys 41 and 31.
-        const bool apart = tiles && (int64_t)pc.R * pc.Nkv > tilesPerCU * deviceCUs();
+        const auto [tiles, apart] = tileUse(q, pc, hdp_, longest);
         if (!tiles || apart) {
             // 16 rows per wave or 32: 16 requests of 32 rows, 2000 keys, us: Hd 64 31.1 and 26.5, Hd 256 90 and 60, of 16 rows 22.5
             // and 25.0, 54 and 56. Registers for 32 are wanting at Hd 512 and in f32 at 256 (84 and 198 there).
@@ -178,7 +192,7 @@ public:
             const int perCU = hdp_ == 64 ? 5 - rt : hdp_ == 128 ? 4 - rt : hdp_ == 256 && rt == 1 && !f32 ? 2 : 1;
             add("paged_attention_few_" + type + hd + "_r" + std::to_string(rt), 16 * rt, f32 ? 16 : 32, 0, tiles ? kFewRows : UINT32_MAX, perCU);
         }
-        if (tiles) add("paged_attention_tile_" + type + hd, 128, 64, apart ? kFewRows : 0, UINT32_MAX, tilesPerCU);
+        if (tiles) add("paged_attention_tile_" + type + hd, 128, 64, apart ? kFewRows : 0, UINT32_MAX, tilesPerCU(hdp_));
     }
     std::vector<Binding> tensors() const override {
         return {{q_, kRead}, {k_, kRead}, {v_, kRead}, {tables_, kRead}, {starts_, kRead}, {lens_, kRead}, {out_, kWrite}};
@@ -220,7 +234,6 @@ public:
     }
 
 private:
-    static constexpr uint32_t kFewRows = 32;
     struct Work {
         std::string fn;
         PagedWorkConstants c;
@@ -274,7 +287,7 @@ public:
         const Tensor &q = in_[0];
         const int64_t G = pc.Nq / pc.Nkv, all = (int64_t)pc.T * G;
         // a group's rows may be all there are
-        const int64_t longest = sc.groups ? all : std::min<int64_t>(maxQueryLen > 0 ? maxQueryLen : pc.T, pc.T) * G;
+        const int64_t longest = sc.groups ? all : longestRows(pc, maxQueryLen);
         const bool f32 = q.dataType == DataType::f32;
         hdp_ = pc.Hd <= 64 ? 64 : pc.Hd <= 128 ? 128 : pc.Hd <= 256 ? 256 : 512;
         const std::string type = name(q.dataType), hd = "_d" + std::to_string(hdp_);
@@ -284,6 +297,12 @@ public:
         if (both_) {
             // one launch of both kinds of rows, or at 256 dims one after the other
             fn_ = (hdp_ == 256 ? "shared_prefix_many_" : "shared_prefix_both_") + type + hd;
+            // No row's weights have fewer bits than PagedAttention gives them for the same max_query_len: f16 tiles have two words
+            // where its few-row kernel would take some of the rows that share them here. (64 requests, a token each, behind 8192 keys, 2-norm
+            // against 64 bits: 2.1e-4, the result's rounding, and 2.8e-4 with one word; 60.5 us and 56.8. But 2048 tokens of one
+            // request behind as many, 32 heads of 128 on 8, 560 us and 415; 8 of 256 on 4 273 and 240.)
+            const TileUse alone = tileUse(q, pc, hdp_, longestRows(pc, maxQueryLen));
+            if (q.dataType == DataType::f16 && sc.groups && (!alone.tiles || alone.apart)) fn_ += "_two";
             if (hdp_ == 256) before_ = "shared_prefix_few_" + type + hd + "_r1";
             blocks_ = (hdp_ == 256 ? 1 : 2) * deviceCUs();
             many_ = work(128, 64, kFewRows, UINT32_MAX, blocks_, 384);
@@ -368,7 +387,6 @@ public:
     }
 
 private:
-    static constexpr uint32_t kFewRows = 32;
     static constexpr int64_t kTile = 48;  // bytes of a plan's entry
 
     double tileSteps(const PagedWorkConstants &w) const {
@@ -499,7 +517,6 @@ private:
     std::string fn_, tile_;
     bool few_ = true;
     unsigned blocks_ = 1;
-    static constexpr int64_t kFewRows = 32;
 };
 
 // PagedEviction (evict.hip): the choice, then the moves of K and V.
