@@ -655,7 +655,7 @@ popcorn_status_t popcorn_kernel_shared_prefix_attention(
  * last one back. The mask is causal or bidirectional: a sliding window's places
  * are lost once keys have been evicted, so it is refused. Weights of keys that
  * no counted row sees, and behind the last key, stay as they are; a row with an lse of
- * -infinity gives nothing. The sums are f32, in an order that the call's lengths alone settle. */
+ * -infinity gives nothing, one of NaN a NaN to the keys that it sees. The sums are f32, in an order that the call's lengths alone settle. */
 popcorn_status_t popcorn_kernel_paged_attention_weights(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
                                                         const popcorn_tensor_t *page_tables, const popcorn_tensor_t *query_starts,
                                                         const popcorn_tensor_t *key_lens, const popcorn_tensor_t *lse,

@@ -405,6 +405,14 @@ __device__ void weights_tile(const typename T::storage *__restrict__ Q, const ty
         // Hides what rows do not see, and rows that give nothing.
         auto mask = [&](int rt, uint32_t first) {
             const int posLo = c.req.pos0 + (int)token_of(first);
+            if (__ballot(ofs[rt] != ofs[rt])) {  // a NaN is its row's scores, so that keys which the row does not see can be told from them
+                const bool nan = ofs[rt] != ofs[rt];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) st[rt][t][e] = nan ? __builtin_nanf("") : st[rt][t][e];
+                ofs[rt] = nan ? 0.0f : ofs[rt];
+            }
             if (__ballot(ofs[rt] == INFINITY) == 0 && (p.maskKind == 2u || (int)key0 + 63 <= posLo)) return;
             const int pos = ofs[rt] == INFINITY ? -1 : p.maskKind == 2u ? 0x7fffffff : c.req.pos0 + (int)token_of(min(first + c32, rows - 1));
 #pragma unroll
