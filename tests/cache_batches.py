@@ -9,40 +9,55 @@ def scores(q, k, scale):
     return q @ k.T * scale, np.abs(q) @ np.abs(k).T * abs(scale)
 
 
+def part(q, k, v, see, scale):
+    """Of rows q and keys k: the highest score, the sum of exponentials from it, those times v and times |v|, the largest magnitude and
+    how many keys are seen (0 and no score where none is)."""
+    s, size = scores(q, k, scale)
+    s[~see], size[~see] = -np.inf, 0.0
+    top = s.max(1, keepdims=True, initial=-np.inf)
+    s -= np.where(np.isneginf(top), 0.0, top)
+    w = np.exp(s, out=s)
+    return top, w.sum(1, keepdims=True), w @ v, w @ np.abs(v), size.max(1, keepdims=True, initial=0.0), see.sum(1, keepdims=True)
+
+
 def shared_attention(q, k_cache, v_cache, prefix_tables, prefix_lens, group_starts, tables, starts, key_lens, out, lse, scale, kind=0,
                      window=-1, sinks=0):
     """C.shared_attention for lengths in order, finite values and rows that see a key."""
-    T, Nq, _ = q.shape
-    nkv = k_cache.shape[1]
+    T, Nq, hd = q.shape
+    nkv, G = k_cache.shape[1], Nq // k_cache.shape[1]
     out, lse = out.astype(np.float64).copy(), lse.astype(np.float64).copy()
     mag, spread, count = np.zeros_like(out), np.zeros((T, Nq, 1)), np.ones((T, Nq, 1))
-    held = {}
-    for r in range(len(tables)):
-        a, n, length, g = starts[r], starts[r + 1] - starts[r], key_lens[r], C.group_of(r, group_starts)
-        if n == 0:
+    inside = [C.group_of(r, group_starts) for r in range(len(tables))]
+    groups = [(g, [r for r, x in enumerate(inside) if x == g]) for g in range(len(prefix_lens))]
+    groups += [(None, [r]) for r, x in enumerate(inside) if x is None]
+    for g, rs in groups:
+        if not rs:
             continue
+        a, b = starts[rs[0]], starts[rs[-1] + 1]
         first = 0 if g is None else prefix_lens[g]
-        if g is not None and g not in held:
-            held = {g: [C.rows_of(c, prefix_tables[g], first)[0] for c in (k_cache, v_cache)]}
-        own = [C.rows_of(c, tables[r], length)[0] for c in (k_cache, v_cache)]
-        k, v = own if g is None else (np.concatenate(x, 1) for x in zip(held[g], own))
-        at, o = np.arange(first + length), (length - n + np.arange(n))[:, None]
-        see = np.full((n, first + length), kind == 2) | (at < first) | (at - first <= o)
-        if kind == 1:
-            see &= (first + np.maximum(o, 0) - at < window) | (at < sinks)
-        rows = slice(a, a + n)
-        for h in range(Nq):
-            kv = h // (Nq // nkv)
-            s, size = scores(q[rows, h].astype(np.float64), k[kv], scale)
-            s = np.where(see, s, -np.inf)
-            top = s.max(1, keepdims=True)
-            w = np.exp(s - top)
-            total = w.sum(1, keepdims=True)
-            lse[rows, h] = (top + np.log(total))[:, 0]
-            w /= total
-            out[rows, h], mag[rows, h] = w @ v[kv], w @ np.abs(v[kv])
-            spread[rows, h, 0] = np.where(see, size, 0.0).max(1)
-            count[rows, h, 0] = see.sum(1)
+        pk, pv = (C.rows_of(c, [] if g is None else prefix_tables[g], first)[0] for c in (k_cache, v_cache))
+        own = [[C.rows_of(c, tables[r], key_lens[r])[0] for c in (k_cache, v_cache)] for r in rs]
+        o = np.concatenate([key_lens[r] - (starts[r + 1] - starts[r]) + np.arange(starts[r + 1] - starts[r]) for r in rs])[:, None]
+
+        def sees(o, at, behind):  # keys `at` of the whole sequence, `behind` the prefix or in it
+            see = np.full((len(o), len(at)), kind == 2) | ((at - first <= o) if behind else True)
+            return see & ((first + np.maximum(o, 0) - at < window) | (at < sinks)) if kind == 1 else see
+
+        for kv in range(nkv):
+            rows = q[a:b, kv * G:(kv + 1) * G].astype(np.float64).reshape(-1, hd)
+            parts = [part(rows, pk[kv], pv[kv], np.repeat(sees(o, np.arange(first), False), G, 0), scale)]
+            mine = []
+            for r, (k, v) in zip(rs, own):
+                x, y = starts[r] - a, starts[r + 1] - a
+                mine.append(part(rows[x * G:y * G], k[kv], v[kv], np.repeat(sees(o[x:y], first + np.arange(key_lens[r]), True), G, 0), scale))
+            parts.append([np.concatenate(x) for x in zip(*mine)])
+            top = np.maximum(parts[0][0], parts[1][0])
+            total, up, size = (sum(x[i] * np.exp(x[0] - top) for x in parts) for i in (1, 2, 3))
+            heads = lambda x: x.reshape(b - a, G, -1)  # noqa: E731
+            at = (slice(a, b), slice(kv * G, (kv + 1) * G))
+            lse[at] = heads(top + np.log(total))[..., 0]
+            out[at], mag[at] = heads(up / total), heads(size / total)
+            spread[at], count[at] = heads(np.maximum(parts[0][4], parts[1][4])), heads(parts[0][5] + parts[1][5])
     return out, lse, (mag, spread, count)
 
 
