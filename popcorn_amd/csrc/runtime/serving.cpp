@@ -442,10 +442,16 @@ public:
         // 16-bit keys of up to 256 dims, rows divided by G as the kernel does, and a step's rows within reach of one offset
         if (q.dataType == DataType::f32 || hdp > 256 || !(pc.scale < 0.0f || pc.scale > 0.0f) || longest * G <= kFewRows || G > 256 || (int64_t)64 * pc.Nq * pc.Hd >= (int64_t{1} << 29)) return;
         tile_ = "attention_weights_tile_" + type + "_d" + std::to_string(hdp);
-        // Requests of few rows have a launch of their own where there are enough of them. us with and without it: 6 requests of 32 rows,
-        // 2 KV heads 24.7 and 17.5; 12 requests, 4 heads, two of them prompts 32.0 and 32.9; 48, 4 heads, 6 prompts 63.8 and 70.7; 48,
-        // 8 heads, one prompt 84 and 131.
-        few_ = (int64_t)pc.R * pc.Nkv > 64;
+        // Requests of few rows have a launch of their own where there are many of them, or where their keys may be: a tile's start is
+        // as long as 10 of its steps, for 256 keys that a single token's row reads in one. us with the launch and without:
+        //   6 requests of 32 rows, 2 KV heads 20.3 and 18.5; 48, 4 heads, 6 prompts 63.8 and 70.7; 48, 8 heads, one prompt 84 and 131
+        //   (but 24, 4 heads, 3 prompts among 500 keys 31.3 and 25.0, 40, 4 heads, 800 keys 41.1 and 40.2);
+        //   8, 8 heads of 128, a prompt of 500, the others 1000, 2000, 4000, 30000 keys 26.6 and 23.5, 28.6 and 29.0, 34 and 39,
+        //   119 and 222; of 64 dims 28.4 and 21.9, 29.3 and 29.4, 32 and 37; of 256, 500 to 4000 keys, 28.7 and 30.5, 32 and 38,
+        //   36 and 48, 50 and 81 (4 heads, 1000 keys 32.0 and 29.1); 16 tokens behind 20000 keys, 4 heads, 84 and 148.
+        // Where the tables have room for more than there is, the launch takes 2 for nothing (8 prompts of 300 35.5 and 33.5).
+        const double room = (double)pc.R * pc.Nkv * pc.columns * pc.pageSize;
+        few_ = (int64_t)pc.R * pc.Nkv > 64 || (pc.R > 1 && room > (hdp > 128 ? 1 << 15 : 1 << 17));
         wc_.manyRows = kFewRows;
         work_.fewRows = few_ ? kFewRows : 0;
         work_.manyRows = UINT32_MAX;

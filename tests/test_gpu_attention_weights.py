@@ -121,3 +121,12 @@ def test_blocks_that_take_several_units(env, dtype, nq, nkv, hd, requests, last_
     share, units = tile_share(b, nq, nkv, hd, 0, last_rows, 32)
     assert share > 1.5 * (np.mean(units) + 10)
     weigh_loose(env, b, dtype, 0, last_rows, kinds={"few", "tile", "join"})
+
+
+@pytest.mark.parametrize("dtype,nq,nkv,hd,keys", [("f16", 16, 8, 128, 9000), ("bf16", 8, 2, 256, 9000), ("bf16", 8, 4, 64, 9000)])
+def test_long_caches_of_single_tokens_beside_a_prompt(env, dtype, nq, nkv, hd, keys):
+    # few requests, whose keys are read by the kernel that streams them and not by tiles
+    b = Loose([(0, 300)] + [(keys - 500 * i, 1) for i in range(7)], nq, nkv, hd, dtype, 16, hd)
+    weigh_loose(env, b, dtype, kinds={"few", "tile", "join"})
+    b = Loose([(0, 300)] + [(300 - 50 * i, 1) for i in range(5)], nq, nkv, hd, dtype, 16, hd)
+    weigh_loose(env, b, dtype, kinds={"tile", "join"})
