@@ -655,7 +655,9 @@ popcorn_status_t popcorn_kernel_shared_prefix_attention(
  * last one back. The mask is causal or bidirectional: a sliding window's places
  * are lost once keys have been evicted, so it is refused. Weights of keys that
  * no counted row sees, and behind the last key, stay as they are; a row with an lse of
- * -infinity gives nothing, one of NaN a NaN to the keys that it sees. The sums are f32, in an order that the call's lengths alone settle. */
+ * -infinity gives nothing, one of NaN a NaN to the keys that it sees. The sums are f32: the same call with the same lengths gives the same bits on
+ * a device, but their order is not the lengths' alone (max_query_len, the padded sizes of q and the tables and the number of CUs choose
+ * the kernels and where their stretches end). */
 popcorn_status_t popcorn_kernel_paged_attention_weights(const popcorn_tensor_t *q, const popcorn_tensor_t *k_cache,
                                                         const popcorn_tensor_t *page_tables, const popcorn_tensor_t *query_starts,
                                                         const popcorn_tensor_t *key_lens, const popcorn_tensor_t *lse,
@@ -669,8 +671,8 @@ popcorn_status_t popcorn_kernel_paged_attention_weights(const popcorn_tensor_t *
  * keys 0 .. n - 1: kept[r, h, j] (i32, of weights' shape) is the index that key j had,
  * kept_weights[r, h, j] its weight, 0 from n on (for the next steps' keys); kept behind n,
  * and cache rows from n on, stay as they were. The keys' rows move within the request's own pages, which
- * no other request may hold where its kept keys change place (pages of the first
- * `first` keys may be shared). Rows that no page holds are not moved. weights and
+ * no other request may hold where its kept keys change place (pages whose keys
+ * are all among the `first` first may be shared). Rows that no page holds are not moved. weights and
  * kept_weights change places for the next call. A model's layers share tables and
  * lengths: this changes neither, ReleasePages does, once, behind the last layer. Keys keep the
  * rotation of the position they had; new tokens' positions go on from there, past
@@ -685,7 +687,9 @@ popcorn_status_t popcorn_kernel_paged_eviction(const popcorn_tensor_t *weights, 
  * [R]), for PageTables' past_lens, and the pages that it left empty: the
  * entries of page_tables (i32 [R, columns]) behind the last kept key's, as they stand there,
  * request by request from the front of freed (i32 [R x columns]); counts[0]
- * (i32 [1]) is their number, and freed behind them stays as it was. The tables stay
+ * (i32 [1]) is their number, and freed behind them stays as it was. A page that several
+ * requests hold (one of `first` keys, where a budget is below `first`) is listed by each of them that leaves it: who shares pages counts
+ * their holders before they are free. The tables stay
  * too: PageTables reads no entry behind a request's past keys before it has written it. */
 popcorn_status_t popcorn_kernel_release_pages(const popcorn_tensor_t *key_lens, const popcorn_tensor_t *budgets,
                                               const popcorn_tensor_t *page_tables, int64_t page_size, const popcorn_tensor_t *new_lens,

@@ -11,8 +11,8 @@
 //   O = sum O_i 2^(m_i - M) / L, L = sum l_i 2^(m_i - M), lse = (M + log2 L) ln 2.
 // What bounds it: small calls their chain of dependent reads (lengths 3 us, the piece 2, table and q 1, two steps 6, the store 2) and
 // the merge's launch (4): 2 requests behind up to 1024 keys 20 us in all, where their bytes take 1; large batches the cold reads of
-// many short stretches of pages (64 requests of 50 to 1500 own keys behind 8192, 142 MB: 46 us, 3.1 TB/s, beside 14 for the plan and
-// the merge; torch.sum reads 111 MB at 3.0), and the products with weights of two words (256 behind 16384, bf16, 35 GFLOP: 88 us).
+// many short stretches of pages (64 requests of 50 to 1500 own keys behind 8192, 142 MB: 47 us, 3.0 TB/s, beside 14 for the plan and
+// the merge; torch.sum reads 111 MB at 3.0), and the products with weights of two words (256 behind 16384, bf16, 35 GFLOP: 80 to 90 us).
 #include "paged_attention.hpp"
 
 namespace {
