@@ -423,7 +423,7 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
 // WORDS, TWO: whether weights of the tiles have two words.
 // Many rows and few in one launch: the first blocks take tiles of many rows, which the matrix cores bound, the others, a wave each,
 // the requests of few, which memory bounds; so both are busy at once.
-#define SHARED_BOTH(t, T, HD, PER_CU, WORDS, TWO)                                                                              \
+#define SHARED_BOTH(t, T, HD, PER_CU, WORDS, TWO)                                                                            \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
         shared_prefix_both_##t##_d##HD##WORDS(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
@@ -449,7 +449,7 @@ __device__ void shared_prefix_plain(const typename T::storage *__restrict__ Q, c
     }
 // Many rows alone: beside the few-row kernel's code those of 256 dims, which take all registers, spilled 51 to 65 of them (a prompt of
 // 2048 tokens behind 8192 keys, bf16: 332 us, and 251).
-#define SHARED_MANY(t, T, HD, PER_CU, WORDS, TWO)                                                                              \
+#define SHARED_MANY(t, T, HD, PER_CU, WORDS, TWO)                                                                            \
     POPCORN_KERNEL void __launch_bounds__(256, PER_CU)                                                                       \
         shared_prefix_many_##t##_d##HD##WORDS(SHARED_PARAMS(T), const int32_t *positions, const pk::SharedTile *plan, float *pO, float *pML, \
                                        pk::u32x4 *records, T::storage *out, float *lse, PagedAttentionConstants p,           \
